@@ -119,8 +119,8 @@ _SIGNATURES = {
 
 
 def declared_symbols():
-    from . import gguf as _gguf, llama as _llama, window as _window
-    return sorted(list(_SIGNATURES) + list(_llama.SIGNATURES) + list(_gguf.SIGNATURES) + list(_window.SIGNATURES))
+    from . import gguf as _gguf, llama as _llama, paged as _paged, window as _window
+    return sorted(list(_SIGNATURES) + list(_llama.SIGNATURES) + list(_gguf.SIGNATURES) + list(_window.SIGNATURES) + list(_paged.SIGNATURES))
 
 
 def lib():
@@ -135,10 +135,11 @@ def lib():
             fn = getattr(_lib, name)
             fn.restype = C.c_uint32
             fn.argtypes = args
-        from . import gguf as _gguf, llama as _llama, window as _window
+        from . import gguf as _gguf, llama as _llama, paged as _paged, window as _window
         _llama.register(_lib)
         _gguf.register(_lib)
         _window.register(_lib)
+        _paged.register(_lib)
     return _lib
 
 
@@ -397,6 +398,27 @@ class Backend:
         """Causal attention of `batch` prompt tokens over the f16 cache; device pointers, token-fastest q / dst."""
         return self._ret(lib().emelb_flash_attn_batch(self._h, q_dev, k_dev, v_dev, dst_dev, head_dim, heads, kv_heads, batch,
                                                       pos0, cache_head_stride, scale))
+
+    # -- many requests over one 4-bit paged cache (requests: emel_cpp_b200.paged)
+    def kv_plan(self, request) -> bool:
+        """Page tables, slots and running sums of a step."""
+        return self._ret(lib().emelb_kv_plan(self._h, request))
+
+    def kv_store(self, request) -> bool:
+        """Keys and values into their slots."""
+        return self._ret(lib().emelb_kv_store(self._h, request))
+
+    def kv_load(self, request) -> bool:
+        """Rows of the cache as the values that it keeps."""
+        return self._ret(lib().emelb_kv_load(self._h, request))
+
+    def kv_attend(self, request) -> bool:
+        """Each request's newest query rows over its pages."""
+        return self._ret(lib().emelb_kv_attend(self._h, request))
+
+    def attend_packed(self, request) -> bool:
+        """Packed prompts of different lengths over 16-bit keys and values."""
+        return self._ret(lib().emelb_attend_packed(self._h, request))
 
     def quantize(self, src: View, dst: View) -> bool:
         return self._ret(lib().emelb_quantize(self._h, C.byref(src), C.byref(dst)))

@@ -47,6 +47,10 @@ SOURCES = {
     "gguf.cu": [],
     "upload.cu": [],
     "window.cu": [],
+    "kv_pages.cu": ["-fmad=false"],
+    "kv_attend.cu": [],
+    "attend_packed.cu": [],
+    "paged_api.cu": [],
     "api.cu": [],
 }
 
@@ -77,6 +81,7 @@ def build(verbose: bool = False, force: bool = False) -> str:
     headers.append(os.path.join(os.path.dirname(HERE), "include", "emelb_llama.h"))
     headers.append(os.path.join(os.path.dirname(HERE), "include", "emelb_gguf.h"))
     headers.append(os.path.join(os.path.dirname(HERE), "include", "emelb_window.h"))
+    headers.append(os.path.join(os.path.dirname(HERE), "include", "emelb_paged.h"))
     headers = [h for h in headers if os.path.exists(h)]
     nccl_inc, nccl_lib = _nccl_paths()
     objs = []

@@ -407,16 +407,20 @@ uint32_t emelb_destroy(emelb_ctx* c) {
 uint32_t emelb_sync(emelb_ctx* c) {
   if (!c) return EMELB_INVALID_REQUEST;
   if (!cuda_ok(c, cudaStreamSynchronize(c->stream))) return EMELB_INTERNAL_ERROR;
-  // a kernel whose bounded wait ran out leaves 1 in the status word
-  int status = 0;
-  if (!cuda_ok(c, cudaMemcpy(&status, c->status_word(), sizeof(int), cudaMemcpyDeviceToHost))) return EMELB_INTERNAL_ERROR;
-  if (status != 0) {
+  // a kernel whose bounded wait ran out leaves 1 in the status word, one that skipped values out of range in the word behind it
+  int status[2] = {0, 0};
+  if (!cuda_ok(c, cudaMemcpy(status, c->status_word(), sizeof(status), cudaMemcpyDeviceToHost))) return EMELB_INTERNAL_ERROR;
+  if (status[0] != 0) {
     // a kernel that gave up leaves task and arrival counters half-way
     cudaMemset(c->gemv_sched, 0, (2 * kSchedSlots + 2) * sizeof(int));
     cudaMemset(c->grp_cnt, 0, c->grp_cnt_ints * sizeof(int));
     cudaMemset(c->token_bar, 0, 4 * sizeof(unsigned));
     cudaMemset(c->token_cnt, 0, emelb_ctx::kTokenCounters * sizeof(int));
     return EMELB_INTERNAL_ERROR;
+  }
+  if (status[1] != 0) {
+    cudaMemset(c->bad_word(), 0, sizeof(int));
+    return EMELB_INVALID_REQUEST;
   }
   return EMELB_OK;
 }

@@ -85,6 +85,8 @@ struct emelb_ctx {
   int pdl = 0;  // launch decode-chain kernels with programmatic stream serialization
   int* next_sched() { int* p = gemv_sched + 2 * sched_next; sched_next = (sched_next + 1) % emelb::kSchedSlots; return p; }
   int* status_word() { return gemv_sched + 2 * emelb::kSchedSlots; }
+  // behind it: raised by a paged operator that met a length, page or slot out of range
+  int* bad_word() { return status_word() + 1; }
   // scratch of the whole-token decode kernel's products: block values per row (rows whose K spans several
   // chunk pairs are completed through it) and row-group arrival counters, zero between launches
   float* bv_table = nullptr;

@@ -1,0 +1,117 @@
+"""The paged operators' checks of their requests, and the cache's sizes.  CPU only: nothing is launched and no pointer followed."""
+import ctypes as C
+
+import pytest
+
+import emel_cpp_b200 as eb
+from emel_cpp_b200 import paged
+
+MB = 1 << 20
+
+
+def at(n):
+    """An address in a region of its own."""
+    return 0x7000_0000_0000 + n * 64 * MB
+
+
+def cache(**kw):
+    a = dict(data=at(0), count=100, page_tokens=16, kv_heads=2, head_dim=64)
+    a.update(kw)
+    return paged.pages(a["data"], a["count"], a["page_tokens"], a["kv_heads"], a["head_dim"])
+
+
+def test_page_bytes():
+    for dim in (32, 64, 96, 128):
+        for heads in (1, 3, 8):
+            for page in (16, 32, 64, 128, 256):
+                assert paged.page_bytes(dim, heads, page) == 2 * heads * page * dim * 18 // 32
+    for dim, heads, page in ((0, 1, 16), (40, 1, 16), (160, 1, 16), (64, 0, 16), (64, 1, 8), (64, 1, 48), (64, 1, 512), (-64, 1, 16)):
+        assert paged.page_bytes(dim, heads, page) == 0
+
+
+def test_null_requests_and_contexts():
+    lib = eb.lib()
+    for name, t in paged._REQUESTS.items():
+        assert getattr(lib, f"emelb_{name}_can_run")(None) == eb.INVALID_REQUEST
+        assert getattr(lib, f"emelb_{name}")(None, C.byref(t())) == eb.INVALID_REQUEST
+        assert paged.can_run(t()) == eb.INVALID_REQUEST
+
+
+PLAN = dict(cached=at(1), fresh=at(2), table=at(3), table_width=40, free_pages=at(4), pages=500, free_count=at(5), free_left=at(6), lengths=at(7),
+            query_begin=at(8), key_begin=at(9), slots=at(10), positions=at(11), shortage=at(12), requests=7, page_tokens=16, token_capacity=64)
+
+
+@pytest.mark.parametrize("change,why", [
+    ({}, eb.OK), (dict(lengths=at(1)), eb.OK), (dict(free_left=at(5)), eb.OK), (dict(lengths=at(1), free_left=at(5)), eb.OK),
+    (dict(table_stride=50), eb.OK), (dict(requests=8192), eb.OK), (dict(page_tokens=256), eb.OK),
+    (dict(requests=0), eb.INVALID_REQUEST), (dict(requests=8193), eb.UNSUPPORTED_OP), (dict(table_width=0), eb.INVALID_REQUEST),
+    (dict(table_stride=39), eb.INVALID_REQUEST), (dict(pages=0), eb.INVALID_REQUEST), (dict(token_capacity=0), eb.INVALID_REQUEST),
+    (dict(page_tokens=0), eb.INVALID_REQUEST), (dict(page_tokens=8), eb.UNSUPPORTED_OP), (dict(page_tokens=48), eb.UNSUPPORTED_OP),
+    (dict(page_tokens=512), eb.UNSUPPORTED_OP), (dict(cached=0), eb.INVALID_REQUEST), (dict(fresh=at(2) + 2), eb.INVALID_REQUEST),
+    (dict(slots=at(10) + 4), eb.INVALID_REQUEST), (dict(slots=0), eb.INVALID_REQUEST), (dict(shortage=0), eb.INVALID_REQUEST),
+    (dict(lengths=at(1) + 4), eb.INVALID_REQUEST), (dict(lengths=at(2)), eb.INVALID_REQUEST), (dict(free_left=at(1)), eb.INVALID_REQUEST),
+    (dict(positions=at(10) + 8), eb.INVALID_REQUEST), (dict(table=at(4) + 1996), eb.INVALID_REQUEST), (dict(key_begin=at(8) + 28), eb.INVALID_REQUEST),
+    (dict(key_begin=at(8) + 32), eb.OK),
+])
+def test_plan_requests(change, why):
+    assert paged.can_run(paged.plan_request(**{**PLAN, **change})) == why
+
+
+@pytest.mark.parametrize("kw,change,why", [
+    ({}, {}, eb.OK), (dict(head_dim=96, page_tokens=128), {}, eb.OK), ({}, dict(type=99), eb.UNSUPPORTED_OP), ({}, dict(type=eb.Q4_0), eb.UNSUPPORTED_OP),
+    (dict(head_dim=80), {}, eb.UNSUPPORTED_OP), (dict(head_dim=0), {}, eb.INVALID_REQUEST), (dict(page_tokens=24), {}, eb.UNSUPPORTED_OP),
+    (dict(kv_heads=0), {}, eb.INVALID_REQUEST), (dict(kv_heads=65536), {}, eb.UNSUPPORTED_OP), (dict(count=0), {}, eb.INVALID_REQUEST),
+    (dict(data=at(0) + 8), {}, eb.INVALID_REQUEST), (dict(data=0), {}, eb.INVALID_REQUEST), ({}, dict(tokens=0), eb.INVALID_REQUEST),
+    ({}, dict(tokens=-1), eb.INVALID_REQUEST), ({}, dict(k=0), eb.INVALID_REQUEST), ({}, dict(v=at(2) + 1), eb.INVALID_REQUEST),
+    ({}, dict(v=at(2) + 2), eb.OK), ({}, dict(slots=at(3) + 4), eb.INVALID_REQUEST), ({}, dict(k_strides=(127, 64)), eb.OK),
+    ({}, dict(k_strides=(63, 64)), eb.INVALID_REQUEST), ({}, dict(k_strides=(128, 63)), eb.INVALID_REQUEST),
+    ({}, dict(v_strides=(-128, 64)), eb.INVALID_REQUEST), ({}, dict(v_strides=(64, 64 * 9)), eb.OK), ({}, dict(k=at(0) + 1024), eb.INVALID_REQUEST),
+    ({}, dict(slots=at(0)), eb.INVALID_REQUEST), ({}, dict(k_strides=(1 << 41, 64)), eb.INVALID_REQUEST),
+])
+def test_store_requests(kw, change, why):
+    a = dict(k=at(1), v=at(2), type="f16", slots=at(3), tokens=9)
+    assert paged.can_run(paged.store_request(cache(**kw), **{**a, **change})) == why
+
+
+@pytest.mark.parametrize("kw,change,why", [
+    ({}, {}, eb.OK), ({}, dict(first=at(6)), eb.OK), ({}, dict(type="f32"), eb.OK), ({}, dict(type=7), eb.UNSUPPORTED_OP),
+    (dict(head_dim=48), {}, eb.UNSUPPORTED_OP), ({}, dict(rows=0), eb.INVALID_REQUEST), ({}, dict(requests=0), eb.INVALID_REQUEST),
+    ({}, dict(table_stride=3), eb.INVALID_REQUEST), ({}, dict(first=at(6) + 1), eb.INVALID_REQUEST), ({}, dict(lengths=0), eb.INVALID_REQUEST),
+    ({}, dict(k_strides=(64, 64)), eb.INVALID_REQUEST),                      # a row's heads on the next row's
+    ({}, dict(k_strides=(64, 640)), eb.OK), ({}, dict(v=at(1)), eb.INVALID_REQUEST), ({}, dict(v=at(1) + 64), eb.INVALID_REQUEST),
+    ({}, dict(v=at(1) + 256, k_strides=(256, 64), v_strides=(256, 64)), eb.OK),   # keys and values side by side in a row
+    ({}, dict(v=at(1) + 128, k_strides=(256, 128), v_strides=(256, 128)), eb.INVALID_REQUEST),
+    ({}, dict(k=at(0)), eb.INVALID_REQUEST), ({}, dict(v=at(3)), eb.INVALID_REQUEST), ({}, dict(k=at(4) - 8), eb.INVALID_REQUEST),
+])
+def test_load_requests(kw, change, why):
+    a = dict(k=at(1), v=at(2), type="bf16", table=at(3), table_width=4, lengths=at(4), row_begin=at(5), requests=3, rows=10)
+    assert paged.can_run(paged.load_request(cache(**kw), **{**a, **change})) == why
+
+
+@pytest.mark.parametrize("kw,change,why", [
+    ({}, {}, eb.OK), ({}, dict(query_begin=at(5), queries=20, max_queries=8), eb.OK), ({}, dict(type="f32"), eb.OK), ({}, dict(type=3), eb.UNSUPPORTED_OP),
+    ({}, dict(heads=5), eb.INVALID_REQUEST), ({}, dict(heads=128), eb.OK), ({}, dict(heads=130), eb.UNSUPPORTED_OP), ({}, dict(heads=0), eb.INVALID_REQUEST),
+    ({}, dict(scale=0.0), eb.INVALID_REQUEST), ({}, dict(scale=-1.0), eb.INVALID_REQUEST), ({}, dict(scale=float("nan")), eb.INVALID_REQUEST),
+    ({}, dict(scale=float("inf")), eb.INVALID_REQUEST), ({}, dict(queries=2), eb.INVALID_REQUEST), ({}, dict(max_queries=0), eb.INVALID_REQUEST),
+    ({}, dict(requests=8193, queries=8193), eb.UNSUPPORTED_OP), ({}, dict(out=at(1)), eb.INVALID_REQUEST), ({}, dict(out=at(0)), eb.INVALID_REQUEST),
+    ({}, dict(out_strides=(64, 64)), eb.INVALID_REQUEST), ({}, dict(q_strides=(512, 64)), eb.OK), ({}, dict(table_stride=1), eb.INVALID_REQUEST),
+    (dict(head_dim=160), {}, eb.UNSUPPORTED_OP), (dict(page_tokens=17), {}, eb.UNSUPPORTED_OP), ({}, dict(lengths=at(4) + 2), eb.INVALID_REQUEST),
+])
+def test_attend_requests(kw, change, why):
+    a = dict(q=at(1), out=at(2), type="f16", table=at(3), table_width=4, lengths=at(4), requests=3, heads=4, queries=3)
+    assert paged.can_run(paged.attend_request(cache(**kw), **{**a, **change})) == why
+
+
+@pytest.mark.parametrize("change,why", [
+    ({}, eb.OK), (dict(causal=False), eb.OK), (dict(head_dim=8), eb.OK), (dict(head_dim=72), eb.OK), (dict(keys=0), eb.OK), (dict(type="bf16"), eb.OK),
+    (dict(type="f32"), eb.UNSUPPORTED_OP), (dict(head_dim=68), eb.UNSUPPORTED_OP), (dict(head_dim=136), eb.UNSUPPORTED_OP),
+    (dict(head_dim=0), eb.INVALID_REQUEST), (dict(heads=3), eb.INVALID_REQUEST), (dict(heads=256), eb.OK), (dict(heads=258), eb.UNSUPPORTED_OP),
+    (dict(queries=0), eb.INVALID_REQUEST), (dict(keys=-1), eb.INVALID_REQUEST), (dict(requests=0), eb.INVALID_REQUEST), (dict(scale=0.0), eb.INVALID_REQUEST),
+    (dict(q=at(0) + 2), eb.UNSUPPORTED_OP), (dict(q=at(0) + 1), eb.INVALID_REQUEST), (dict(k_strides=(132, 64)), eb.UNSUPPORTED_OP),
+    (dict(k_strides=(136, 64)), eb.OK), (dict(v_strides=(64, 1280)), eb.OK), (dict(out=at(0)), eb.INVALID_REQUEST), (dict(out=at(2) + 16), eb.INVALID_REQUEST),
+    (dict(out_strides=(64, 64)), eb.INVALID_REQUEST), (dict(query_begin=at(4) + 2), eb.INVALID_REQUEST), (dict(max_queries=0), eb.INVALID_REQUEST),
+])
+def test_packed_requests(change, why):
+    a = dict(q=at(0), k=at(1), v=at(2), out=at(3), type="f16", query_begin=at(4), key_begin=at(5), requests=3, heads=4, kv_heads=2, head_dim=64, queries=20,
+             keys=30)
+    assert paged.can_run(paged.packed_request(**{**a, **change})) == why
