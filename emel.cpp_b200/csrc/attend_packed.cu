@@ -1,99 +1,466 @@
-// Attention of packed prompts of different lengths.
+// Attention of packed prompts of different lengths, on the Blackwell tensor cores.
+//
+// Per request and key / value head, the query rows of the head's group stand behind one another, token after token, so that a
+// short prompt fills tiles of rows too.  A CTA takes 256 of them as two tiles of 128 and walks the keys in tiles of 128:
+//   S = Q K^T       tcgen05.mma, operands in shared memory, K by TMA; S {128 rows, 128 keys} in TMEM, a row a lane
+//   P = exp2(S - m) a thread a row: 128 scores out of TMEM, running maximum and sum, P as 16-bit values back over S
+//   O += P V        tcgen05.mma, P as the A operand out of TMEM, V by TMA as it lies in memory (its dims are contiguous: MN-major)
+// While the warps of one tile take the exponentials, the tensor cores work for the other.  The running maximum a row's weights are
+// taken against follows the true one only when that has passed it by 2^8: only then does O, in TMEM, have to be rescaled.
+//
+// Two matrix products of 128 x 128 x head_dim and 128 x 128 exponentials a tile: at head_dim 128 both take the same time (4096
+// products, 16 exponentials a cycle and SM), at 64 the exponentials bound it.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "common.cuh"
 #include "paged.h"
+#include "tc_common.cuh"
 
 namespace emelb {
 namespace {
 
 constexpr unsigned kAll = 0xffffffffu;
+constexpr int kTileRows = 128, kTileKeys = 128, kTiles = 2;   // tiles of a CTA
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kThreads = 384;
+constexpr float kLowest = -3.0e38f;
+constexpr float kSlack = 8.0f;
+constexpr int kTmemCols = 512;
 
-struct PackedArgs {
-  emelb_attend_packed_request r;
-  int group;
-  float scale_log2;
-  int* bad;
+struct __align__(64) Map {
+  unsigned char bytes[128];
 };
 
-template <class E>
-__device__ __forceinline__ float value_of(E x);
-template <>
-__device__ __forceinline__ float value_of<__half>(__half x) { return __half2float(x); }
-template <>
-__device__ __forceinline__ float value_of<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <class E>
-__device__ __forceinline__ E elem_of(float x);
-template <>
-__device__ __forceinline__ __half elem_of<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 elem_of<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+struct PackedArgs {
+  const void* q;
+  void* out;
+  const int32_t *query_begin, *key_begin;
+  int64_t qs, qh, os, oh;
+  int requests, kv_heads, group, head_dim, queries, keys, max_queries, causal;
+  float scale_log2;
+  int *bad, *status;
+};
 
-// a warp to a (query row, head): 32 keys a turn, a key a lane, then the dims of the mix across the lanes
-template <class E>
-__global__ void __launch_bounds__(128) attend_packed_rows_kernel(const __grid_constant__ PackedArgs a) {
-  const emelb_attend_packed_request& r = a.r;
-  __shared__ float query[4][128];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y, row = blockIdx.x * 4 + warp, D = r.head_dim;
-  if (row >= r.queries || row < r.query_begin[0] || row >= r.query_begin[r.requests]) return;
-  int lo = 0, hi = r.requests - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (r.query_begin[mid] <= row) lo = mid;
-    else hi = mid - 1;
+template <int DP>
+struct Smem {
+  static constexpr int kHalf = kTileKeys * 128;          // 64 dims of 128 rows
+  static constexpr int kTile = DP / 64 * kHalf;
+  static constexpr int kStages = DP == 128 ? 5 : 10;     // of K and V tiles in turn
+  static constexpr int kQ = kTiles * kTile;
+  static constexpr int kBytes = kQ + kStages * kTile + 1024;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if (kBf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
+               "r"(x), "r"(y), "r"(z), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                 "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+                 "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+                 "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+               : "r"(taddr));
+}
+// values that were loaded are used behind this
+template <int N>
+__device__ __forceinline__ void wait_ld(uint32_t (&v)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
+}
+
+// both operands in shared memory, or A in TMEM
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// V {keys, dims} as the B operand: 8 keys of 64 dims an atom, 16 keys further 2048 bytes, the next 64 dims kTileKeys * 128
+__device__ __forceinline__ uint64_t value_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | (uint64_t)(kTileKeys * 128 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)2 << 61;
+}
+
+// Row tiles of request b stand in slots first_slot(b) .. first_slot(b + 1) - 1, of which it may leave one empty: rows before it / 256
+// + b is known from query_begin alone, without a sum over the requests in front.
+__device__ __forceinline__ int64_t first_slot(const PackedArgs& a, int b) {
+  return (int64_t)(a.query_begin[b] - a.query_begin[0]) * a.group / (kTiles * kTileRows) + b;
+}
+
+template <int DP, bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1)
+    attend_packed_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ Map k_map, const __grid_constant__ Map v_map) {
+  using S = Smem<DP>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t bars[2 * kStages + 4 * kTiles + 2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int gave_up;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t smem = (tc::smem_u32(raw) + 1023u) & ~1023u;
+  const uint32_t bar0 = tc::smem_u32(bars);
+  auto full = [&](int s) { return bar0 + 8 * s; };
+  auto empty = [&](int s) { return bar0 + 8 * (kStages + s); };
+  auto q_ready = [&](int t) { return bar0 + 8 * (2 * kStages + t); };
+  auto s_ready = [&](int t) { return bar0 + 8 * (2 * kStages + kTiles + t); };
+  auto p_ready = [&](int t) { return bar0 + 8 * (2 * kStages + 2 * kTiles + t); };
+  auto o_ready = [&](int t) { return bar0 + 8 * (2 * kStages + 3 * kTiles + t); };
+  const uint32_t raw_bar = bar0 + 8 * (2 * kStages + 4 * kTiles), drain_bar = raw_bar + 8;
+
+  // ---- which rows
+  const int head = blockIdx.x % a.kv_heads;
+  const int64_t slot = blockIdx.x / a.kv_heads;
+  int lo = 0, hi = a.requests;          // first_slot(lo) <= slot, first_slot(hi) > slot (or hi = requests)
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, b = lo + lane * step;
+    const unsigned before = __ballot_sync(kAll, b < hi && first_slot(a, b) <= slot);
+    const int last = before ? 31 - __clz(before) : 0;
+    hi = min(hi, lo + (last + 1) * step);
+    lo = lo + last * step;
   }
-  const int q0 = r.query_begin[lo], q1 = r.query_begin[lo + 1], k0 = r.key_begin[lo], k1 = r.key_begin[lo + 1];
-  if (q0 < 0 || q1 > r.queries || row >= q1 || q1 - q0 > r.max_queries || k0 < 0 || k1 < k0 || k1 > r.keys) {
-    *a.bad = 1;
+  const int b = lo;
+  const int q0 = a.query_begin[b], nq = a.query_begin[b + 1] - q0, k0 = a.key_begin[b], nk = a.key_begin[b + 1] - k0;
+  if (a.query_begin[0] < 0 || q0 < 0 || nq < 0 || nq > a.max_queries || q0 > a.queries - nq || k0 < 0 || nk < 0 || k0 > a.keys - nk) {
+    if (tid == 0) *a.bad = 1;
     return;
   }
-  const int sees = r.causal ? min(k1 - k0, k1 - k0 - (q1 - q0) + (row - q0) + 1) : k1 - k0;
-  const E* q = static_cast<const E*>(r.q) + row * r.q_token_stride + head * r.q_head_stride;
-  const E* k = static_cast<const E*>(r.k) + k0 * r.k_token_stride + head / a.group * r.k_head_stride;
-  const E* v = static_cast<const E*>(r.v) + k0 * r.v_token_stride + head / a.group * r.v_head_stride;
-  for (int d = lane; d < D; d += 32) query[warp][d] = value_of<E>(q[d]);
-  __syncwarp();
-  float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int j0 = 0; j0 < sees; j0 += 32) {
-    const int j = j0 + lane;
-    float s = -INFINITY;
-    if (j < sees) {
-      float dot = 0.0f;
-      for (int d = 0; d < D; ++d) dot = fmaf(query[warp][d], value_of<E>(k[j * r.k_token_stride + d]), dot);
-      s = dot * a.scale_log2;
+  const int64_t rows = (int64_t)nq * a.group;
+  const int64_t tiles = (rows + kTiles * kTileRows - 1) / (kTiles * kTileRows), local = slot - first_slot(a, b);
+  if (local < 0 || local >= tiles) return;
+  const int64_t row0 = (tiles - 1 - local) * (kTiles * kTileRows);   // long walks first
+  // keys that a row of the request sees; row tiles of this CTA walk turns(t) key tiles
+  auto sees = [&](int64_t row) { return a.causal ? max(0, min(nk, nk - nq + (int)(row / a.group) + 1)) : nk; };
+  auto turns = [&](int t) {
+    const int64_t r = row0 + t * kTileRows;
+    return r >= rows ? 0 : (sees(min(rows, r + kTileRows) - 1) + kTileKeys - 1) / kTileKeys;
+  };
+  const int n0 = turns(0), n1 = turns(1), n = max(n0, n1);
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      tc::mbar_init(full(s), 1);
+      tc::mbar_init(empty(s), 1);
     }
-    float top = s;
-#pragma unroll
-    for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, w));
-    top = fmaxf(top, m);
-    const float base = top == -INFINITY ? 0.0f : top, keep = exp2f(m - base), p = exp2f(s - base);
-    l = l * keep + warp_sum(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] *= keep;
-    for (int jj = 0; jj < min(32, sees - j0); ++jj) {
-      const float pj = __shfl_sync(kAll, p, jj);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (lane + 32 * i < D) o[i] = fmaf(pj, value_of<E>(v[(j0 + jj) * r.v_token_stride + lane + 32 * i]), o[i]);
+    for (int t = 0; t < kTiles; ++t) {
+      tc::mbar_init(q_ready(t), kTileRows);
+      tc::mbar_init(s_ready(t), 1);
+      tc::mbar_init(p_ready(t), kTileRows);
+      tc::mbar_init(o_ready(t), 1);
     }
-    m = top;
+    tc::mbar_init(raw_bar, 1);
+    tc::mbar_init(drain_bar, 1);
+    gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  E* out = static_cast<E*>(r.out) + row * r.out_token_stride + head * r.out_head_stride;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&tmem_slot)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = tmem_slot;
+  int loaded = 0;          // loader: tiles asked for
+  int used = 0;            // MMA warp: tiles waited for
+
+  if (warp == kLoadWarp) {
+    // K tile, V tile, K tile, ... of the walk
+    bool alive = true;
+    for (; alive && loaded < 2 * n; ++loaded) {
+      const int s = loaded % kStages, j = loaded >> 1;
+      if (loaded >= kStages) alive = tc::mbar_wait(empty(s), (loaded / kStages - 1) & 1, &gave_up);
+      if (!__all_sync(kAll, alive)) break;
+      const bool values = loaded & 1;
+      const int left = nk - j * kTileKeys;
+      // behind the last key stand other rows, of which P = 0 would make NaN where they hold one: zeroed before anyone reads them
+      const bool ragged = values && left < kTileKeys;
+      const uint32_t dst = smem + S::kQ + s * S::kTile, bar = ragged ? raw_bar : full(s);
+      if (lane == 0) {
+        tc::mbar_arrive_expect_tx(bar, S::kTile);
+        for (int h = 0; h < DP / 64; ++h) tma_load_3d(dst + h * S::kHalf, values ? &v_map : &k_map, 64 * h, head, k0 + j * kTileKeys, bar);
+      }
+      if (ragged) {
+        __syncwarp();
+        alive = tc::mbar_wait(raw_bar, 0, &gave_up);
+        for (int i = left * 8 + lane; i < kTileKeys * 8; i += 32)
+          for (int h = 0; h < DP / 64; ++h)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + h * S::kHalf + i * 16), "r"(0) : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(full(s));
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (tc::elect_one()) {
+      constexpr uint32_t type = kBf16 ? 1u : 0u;
+      constexpr uint32_t common = 1u << 4 | type << 7 | type << 10 | (uint32_t)(kTileRows >> 4) << 24;
+      constexpr uint32_t idesc_s = common | (uint32_t)(kTileKeys >> 3) << 17;
+      constexpr uint32_t idesc_o = common | 1u << 16 | (uint32_t)(DP >> 3) << 17;
+      auto stage = [&](int e) { return smem + S::kQ + e % kStages * S::kTile; };
+      auto scores = [&](int t, int e) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i < D) out[lane + 32 * i] = elem_of<E>(o[i] * inv);
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint32_t off = kk / 4 * S::kHalf + kk % 4 * 32;
+          mma_ss(tmem + t * 128, tc::operand_desc(smem + t * S::kTile + off, 1024), tc::operand_desc(stage(e) + off, 1024), idesc_s, kk > 0);
+        }
+        tc::mma_commit(s_ready(t));
+      };
+      auto wait_tile = [&](int e) {
+        if (e < used) return true;
+        used = e + 1;
+        return tc::mbar_wait(full(e % kStages), e / kStages & 1, &gave_up);
+      };
+      bool alive = true;
+      const int n_of[2] = {n0, n1};
+      for (int j = -1; alive && j < n; ++j) {
+        for (int t = 0; t < kTiles && alive; ++t) {
+          if (j >= 0 && j < n_of[t]) {
+            alive = wait_tile(2 * j + 1) && tc::mbar_wait(p_ready(t), j & 1, &gave_up);
+            if (!alive) break;
+            tc::fence_after();
+#pragma unroll
+            for (int kk = 0; kk < kTileKeys / 16; ++kk)
+              tc::mma_f16(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, value_desc(stage(2 * j + 1) + kk * 2048), idesc_o, j > 0 || kk > 0);
+            if (j + 1 == n_of[t]) tc::mma_commit(o_ready(t));
+          }
+          if (j + 1 < n_of[t]) {
+            alive = wait_tile(2 * j + 2) && (j >= 0 || tc::mbar_wait(q_ready(t), 0, &gave_up));
+            if (!alive) break;
+            tc::fence_after();
+            scores(t, 2 * j + 2);
+          }
+        }
+        // the tiles of this turn are free once everything issued so far is done
+        if (alive && j >= 0) tc::mma_commit(empty((2 * j + 1) % kStages));
+        if (alive && j + 1 < n) tc::mma_commit(empty((2 * j + 2) % kStages));
+      }
+      if (!alive) {
+        // let what was issued end
+        volatile int own = 0;
+        tc::mma_commit(drain_bar);
+        tc::mbar_wait(drain_bar, 0, &own);
+      }
+    }
+    __syncwarp();
+  } else if (warp < kLoadWarp) {
+    const int t = warp >> 2, r = tid & 127, n_mine = t ? n1 : n0;
+    const int64_t row = row0 + t * kTileRows + r;
+    const bool live = row < rows;
+    const int64_t first = row0 + t * kTileRows;
+    if (n_mine > 0) {
+      // queries: 16-byte pieces of rows into the swizzled K-major layout, zeros behind the last row and the last dim
+      constexpr int kPieces = DP / 8;
+#pragma unroll 4
+      for (int i = r; i < kTileRows * kPieces; i += kTileRows) {
+        const int rr = i / kPieces, c = i % kPieces;
+        const int64_t g_row = first + rr;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (g_row < rows && c * 8 < a.head_dim) {
+          const int tok = (int)(g_row / a.group), h = (int)(g_row - (int64_t)tok * a.group);
+          v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (q0 + tok) * a.qs + (int64_t)(head * a.group + h) * a.qh + c * 8);
+        }
+        const uint32_t dst = smem + t * S::kTile + c / 8 * S::kHalf + rr * 128 + ((c % 8) ^ (rr & 7)) * 16;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc::mbar_arrive(q_ready(t));
+    }
+    const int see = sees(live ? row : rows - 1), see_all = n_mine > 0 ? sees(first) : 0;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_col = tmem + t * 128 + lanes, o_col = tmem + 256 + t * 128 + lanes;
+    const tc::f2 scale2 = tc::pack2(a.scale_log2, a.scale_log2);
+    float m = kLowest;
+    tc::f2 sum2 = tc::pack2(0.0f, 0.0f);
+    bool alive = true;
+    for (int j = 0; j < n_mine; ++j) {
+      alive = tc::mbar_wait(s_ready(t), j & 1, &gave_up);
+      if (!__all_sync(kAll, alive)) {
+        alive = false;
+        break;
+      }
+      tc::fence_after();
+      uint32_t s[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_col + 32 * c, s + 32 * c);
+      wait_ld(s);
+      if ((j + 1) * kTileKeys > see_all) {
+        const int in_tile = see - j * kTileKeys;
+#pragma unroll
+        for (int i = 0; i < 128; ++i)
+          if (i >= in_tile) s[i] = __float_as_uint(-INFINITY);
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 128; i += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(__uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1])));
+      const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+      if (__any_sync(kAll, now > m + kSlack)) {
+        const float next = fmaxf(m, now), f = exp2_fast(m - next);
+        m = next;
+        sum2 = tc::mul2(sum2, tc::pack2(f, f));
+        // the mix so far: its last product was issued before these scores, so it is done
+        if (j > 0) {
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_col + c, o);
+            wait_ld(o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tc::tmem_st32(o_col + c, o);
+          }
+        }
+      }
+      const tc::f2 minus_m = tc::pack2(-m, -m);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t p[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const tc::f2 x = tc::fma2(tc::pack2u(s[64 * c + 2 * i], s[64 * c + 2 * i + 1]), scale2, minus_m);
+          const float2 xy = tc::unpack2(x);
+          const float e0 = exp2_fast(xy.x), e1 = exp2_fast(xy.y);
+          sum2 = tc::add2(sum2, tc::pack2(e0, e1));
+          p[i] = pack16<kBf16>(e0, e1);
+        }
+        tc::tmem_st32(s_col + 32 * c, p);
+      }
+      tc::tmem_wait_st();
+      tc::fence_before();
+      tc::mbar_arrive(p_ready(t));
+    }
+    if (alive && n_mine > 0) alive = tc::mbar_wait(o_ready(t), 0, &gave_up);
+    alive = __all_sync(kAll, alive);
+    if (alive) {
+      tc::fence_after();
+      const float2 two = tc::unpack2(sum2);
+      const float sum = two.x + two.y, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const int tok = (int)((live ? row : 0) / a.group), h = (int)((live ? row : 0) - (int64_t)tok * a.group);
+      uint16_t* out = static_cast<uint16_t*>(a.out) + (q0 + tok) * a.os + (int64_t)(head * a.group + h) * a.oh;
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        if (n_mine > 0) {
+          tmem_ld32(o_col + c, o);
+          wait_ld(o);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = __uint_as_float(o[8 * i + 2 * e]) * inv, y = __uint_as_float(o[8 * i + 2 * e + 1]) * inv;
+            w[e] = inv == 0.0f ? 0u : pack16<kBf16>(x, y);
+          }
+          if (live && c + 8 * i < a.head_dim) *reinterpret_cast<uint4*>(out + c + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+  }
+  // a wait that ran out: copies in flight end before the CTA does
+  __syncwarp();
+  if (gave_up) {
+    if (tid == 0) *a.status = 1;
+    if (warp == kLoadWarp) {
+      volatile int own = 0;
+      for (int e = max(0, loaded - kStages); e < loaded; ++e) {
+        own = 0;
+        tc::mbar_wait(full(e % kStages), e / kStages & 1, &own);
+      }
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+// rows {keys, kv_heads, head_dim} for boxes of 128 keys of one head, 64 dims wide
+bool encode_rows(Map* map, const void* base, bool bf16, int head_dim, int heads, int keys, int64_t token_stride, int64_t head_stride) {
+  static_assert(sizeof(CUtensorMap) == sizeof(Map), "tensor map size");
+  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess) {
+      cudaGetLastError();
+      fn = nullptr;
+    }
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  }();
+  if (!encode) return false;
+  // a stride that no second row or head uses may be anything in the request
+  if (heads == 1) head_stride = head_dim;
+  if (keys <= 1) token_stride = (int64_t)head_dim * heads;
+  const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)(keys > 0 ? keys : 1)};
+  const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
+  const cuuint32_t box[3] = {64, 1, kTileKeys}, steps[3] = {1, 1, 1};
+  return encode(reinterpret_cast<CUtensorMap*>(map), bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
+                dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DP, bool kBf16>
+cudaError_t launch_one(const PackedArgs& a, const Map& k, const Map& v, cudaStream_t st) {
+  const int smem = Smem<DP>::kBytes;
+  cudaError_t e = cudaFuncSetAttribute(attend_packed_kernel<DP, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const int64_t slots = (int64_t)a.queries * a.group / (kTiles * kTileRows) + a.requests;
+  if (slots * a.kv_heads > 0x7fffffff) return cudaErrorInvalidValue;
+  attend_packed_kernel<DP, kBf16><<<(unsigned)(slots * a.kv_heads), kThreads, smem, st>>>(a, k, v);
+  return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int sm_count, int* bad, int* status, cudaStream_t st) {
-  PackedArgs a{r, r.heads / r.kv_heads, r.scale * 1.44269504088896340736f, bad};
-  const dim3 grid((r.queries + 3) / 4, r.heads);
-  if (r.type == EMELB_F16) attend_packed_rows_kernel<__half><<<grid, 128, 0, st>>>(a);
-  else attend_packed_rows_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(a);
-  return cudaGetLastError();
+  PackedArgs a{};
+  a.q = r.q;
+  a.out = r.out;
+  a.query_begin = r.query_begin;
+  a.key_begin = r.key_begin;
+  a.qs = r.q_token_stride;
+  a.qh = r.q_head_stride;
+  a.os = r.out_token_stride;
+  a.oh = r.out_head_stride;
+  a.requests = r.requests;
+  a.kv_heads = r.kv_heads;
+  a.group = r.heads / r.kv_heads;
+  a.head_dim = r.head_dim;
+  a.queries = r.queries;
+  a.keys = r.keys;
+  a.max_queries = r.max_queries;
+  a.causal = r.causal != 0;
+  a.scale_log2 = r.scale * 1.44269504088896340736f;
+  a.bad = bad;
+  a.status = status;
+  const bool bf16 = r.type == EMELB_BF16;
+  Map k, v;
+  if (!encode_rows(&k, r.k, bf16, r.head_dim, r.kv_heads, r.keys, r.k_token_stride, r.k_head_stride) ||
+      !encode_rows(&v, r.v, bf16, r.head_dim, r.kv_heads, r.keys, r.v_token_stride, r.v_head_stride))
+    return cudaErrorInvalidValue;
+  if (r.head_dim <= 64) return bf16 ? launch_one<64, true>(a, k, v, st) : launch_one<64, false>(a, k, v, st);
+  return bf16 ? launch_one<128, true>(a, k, v, st) : launch_one<128, false>(a, k, v, st);
 }
 
 }  // namespace emelb
