@@ -3,12 +3,12 @@
 // The cache is read once: 18 bytes for 32 values, so HBM bounds it, with about 25 instructions of a warp to each token of a head
 // at that rate.  What keeps it under them: the cache is the A operand of mma.sync.m16n8k16 (16 tokens, or 16 dims, a side), the query
 // rows of a group of heads the other (8 of them, none of a tile wasted on a group of 8), so tokens and not heads fill the
-// tiles; quants become f16 by one lop3 a pair (64 + q; the scores' accumulators start at -72 times the queries' sums, values
-// are centred by one addition, since a sum over tokens would not survive the difference); a key's scale multiplies its sum of
-// 32 products in f32, a value's scale joins the softmax weight; weights turn from accumulators into operands by movmatrix.
+// tiles; quants become f16 by one lop3 a pair, as a power of two + q, and what that is above q - 8 leaves the scores through the
+// tensor cores too (one tf32 product a tile), the values by an addition, since sums over tokens would not survive it; a key's scale multiplies its sum of 32 products in f32, a value's scale joins the softmax weight;
+// weights turn from accumulators into operands by movmatrix.
 //
-// All tiles of 16 tokens of all (request, key / value head, 8 rows) stand in one line, which the units share evenly, whatever the
-// requests' lengths.  A unit is a team of 1 to 8 warps, each with a ring of tiles of its own that bulk copies fill; the team
+// All steps of 32 tokens of all (request, key / value head, 8 rows) stand in one line, which the units share evenly, whatever the
+// requests' lengths.  A unit is a team of 1 to 12 warps, each with a ring of tiles of its own that asynchronous copies fill; the team
 // takes every tile in turn and joins its warps' results in shared memory.  What a unit has of a (request, head) that others
 // share goes to scratch, and the last to arrive joins the parts in the units' order, so results do not depend on timing.
 #include <cuda_bf16.h>
@@ -24,10 +24,12 @@ namespace {
 using kv::Tile;
 typedef long long i64;
 constexpr unsigned kAll = 0xffffffffu;
-constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr float kLowest = -3.0e38f;   // running maximum before the first token: finite, below every score
 constexpr float kSlack = 3.0f;        // a score may pass the running maximum by this (log2) before sums are rescaled
-constexpr int kMinShare = 2;          // tiles a warp, below which fewer units share the work
+constexpr int kMinShare = 1;          // steps a warp, below which fewer units share the work
+constexpr int kJoinSteps = 5;         // what joining the parts of units costs, in steps of a warp
+constexpr int kMostParts = 6;             // parts of a (head, row tile) up to which a team may be smaller
+constexpr int kStep = 32;             // tokens a warp takes at a time: two tiles
 
 struct AttendArgs {
   const uint8_t* data;
@@ -35,21 +37,22 @@ struct AttendArgs {
   void* out;
   const int32_t *table, *lengths, *query_begin;
   int64_t table_stride, qs, qh, os, oh, page_bytes;
-  int requests, table_width, kv_heads, group, queries, max_queries, pages, page_tokens, page_shift, type, q_vec;
+  int requests, table_width, kv_heads, group, queries, max_queries, pages, page_tokens, page_shift, type, q_vec, out_pairs;
   float scale_log2;
   float *acc, *stats;
   int* arrived;
   int most_units;
-  int *bad, *status;
+  int* bad;
 };
 
-template <int D, int NT>
+template <int D, int NT, bool kExact>
 struct Shape {
+  static constexpr int kWarps = NT == 1 && !kExact ? 12 : 8;   // one CTA an SM: 168 registers a thread, or 255
   static constexpr int kRows = 8 * NT;
-  static constexpr int kStages = D == 128 ? 4 : D == 96 ? 5 : D == 64 ? 8 : 12;
-  static constexpr int kRing = kStages * Tile<D>::kBytes;
-  static constexpr int kJoinLd = D + 2;
-  static constexpr int kSmem = kWarps * kRing + kWarps * kRows * kJoinLd * 4;
+  static constexpr int kStages = D == 128 ? 2 : D == 32 ? 4 : 3;
+  static constexpr int kStage = 2 * Tile<D>::kBytes;
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kSmem = kWarps * kRing + kWarps * kRows * D * 4;
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -58,9 +61,52 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// rows {a0, a1} (k and k + 4 alike) times columns {b0, b1}, as tf32
+__device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%4,%5}, {%6,%7}, {%8,%8,%8,%8};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ uint32_t tf32_of(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return r;
+}
+// (a & kMask) | base in one instruction: the base in a register
+template <uint32_t kMask>
+__device__ __forceinline__ uint32_t field(uint32_t a, uint32_t base) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "n"(kMask), "r"(base));
+  return r;
+}
+// all as 64 + q
+__device__ __forceinline__ void spread_even(uint32_t w, uint32_t b64, uint32_t (&p)[4]) {
+  p[0] = field<0x00f000f0u>(w << 4, b64);
+  p[1] = field<0x00f000f0u>(w, b64);
+  p[2] = field<0x00f000f0u>(w >> 4, b64);
+  p[3] = field<0x00f000f0u>(w >> 8, b64);
+}
+// The four nibbles of either half of a word as f16 pairs: 1024 + q, 64 + q and, of the word moved down by 6, 256 + q and 16 + q.  What
+// they are above q - 8:
+__host__ __device__ constexpr float above_of(int p) { return p == 0 ? 1032.0f : p == 1 ? 72.0f : p == 2 ? 264.0f : 24.0f; }
+struct Bases {
+  uint32_t b1024, b64, b256, b16;
+};
+__device__ __forceinline__ void spread(uint32_t w, const Bases& b, uint32_t (&p)[4]) {
+  const uint32_t w6 = w >> 6;
+  p[0] = field<0x000f000fu>(w, b.b1024);
+  p[1] = field<0x00f000f0u>(w, b.b64);
+  p[2] = field<0x003c003cu>(w6, b.b256);
+  p[3] = field<0x03c003c0u>(w6, b.b16);
 }
 __device__ __forceinline__ uint32_t turn8x8(uint32_t v) {
   uint32_t r;
@@ -92,10 +138,28 @@ __device__ __forceinline__ float load_query(const AttendArgs& a, int64_t at) {
   if (a.type == EMELB_F16) return __half2float(static_cast<const __half*>(a.q)[at]);
   return __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[at]);
 }
-__device__ __forceinline__ void store_out(const AttendArgs& a, int64_t at, float v) {
-  if (a.type == EMELB_F32) static_cast<float*>(a.out)[at] = v;
-  else if (a.type == EMELB_F16) static_cast<__half*>(a.out)[at] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+// two neighbouring dims
+__device__ __forceinline__ void store_pair(const AttendArgs& a, int64_t at, float x, float y) {
+  if (a.type == EMELB_F32) {
+    float* p = static_cast<float*>(a.out) + at;
+    p[0] = x;
+    p[1] = y;
+    return;
+  }
+  uint32_t two;
+  if (a.type == EMELB_F16) {
+    two = half2_of(x, y);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    two = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  uint16_t* p = static_cast<uint16_t*>(a.out) + at;
+  if (a.out_pairs) {
+    *reinterpret_cast<uint32_t*>(p) = two;
+  } else {
+    p[0] = (uint16_t)two;
+    p[1] = (uint16_t)(two >> 16);
+  }
 }
 
 // one request's part of the line
@@ -103,7 +167,7 @@ struct Request {
   int rows;     // query rows
   int first;    // the first of them
   int length;   // tokens
-  int tiles;    // of one (head, row tile); at least one, so that rows that see nothing are written too
+  int steps;    // of one (head, row tile); at least one, so that rows that see nothing are written too
   int sides;    // (head, row tile) pairs
 };
 template <int ROWS>
@@ -119,7 +183,7 @@ __device__ __forceinline__ Request request_at(const AttendArgs& a, int b, bool* 
     r.rows = 0;
     r.length = 0;
   }
-  r.tiles = max(1, (r.length + 15) >> 4);
+  r.steps = max(1, (r.length + kStep - 1) / kStep);
   r.sides = a.kv_heads * ((r.rows * a.group + ROWS - 1) / ROWS);
   return r;
 }
@@ -131,195 +195,269 @@ __device__ __forceinline__ void team_barrier(int team, int threads) {
 
 // kExact: f32 queries and results; the queries and the weights then go in as two f16 operands each
 template <int D, int NT, bool kExact>
-__global__ void __launch_bounds__(kThreads, NT == 1 && !kExact ? 2 : 1) kv_attend_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_attend_kernel(const __grid_constant__ AttendArgs a) {
   using T = Tile<D>;
-  using S = Shape<D, NT>;
+  using S = Shape<D, NT, kExact>;
+  constexpr int kWarps = S::kWarps, kThreads = 32 * kWarps;
   constexpr int J = T::kGroups, kRows = S::kRows, kStages = S::kStages, kParts = kExact ? 2 : 1;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t bars[kWarps][kStages];
-  __shared__ int stage_ok[kWarps][kStages];
-  __shared__ i64 sums[2][kWarps];
-  __shared__ int start_b[kWarps];
-  __shared__ i64 start_at[kWarps];
-  __shared__ float join_m[kWarps][kRows], join_l[kWarps][kRows];
+  __shared__ i64 sums[3][kWarps];
+  __shared__ int2 scan[kWarps];
+  __shared__ int4 starts[kWarps];   // a team's request, where that begins, the team's steps
+  __shared__ __align__(16) float join_m[kWarps][kRows], join_l[kWarps][kRows];
   __shared__ int last_in[kWarps];
-  __shared__ volatile int gave_up;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * S::kRing;
-  float* joint = reinterpret_cast<float*>(smem + kWarps * S::kRing);
+  const uint32_t ring_at = tc::smem_u32(ring) + lane * 16;
+  float4* joint = reinterpret_cast<float4*>(smem + kWarps * S::kRing);
+  constexpr int kCells = kRows * D / 4;
   bool wrong = false;
 
-  if (tid < kWarps * kStages) tc::mbar_init(tc::smem_u32(&bars[tid / kStages][tid % kStages]), 1);
-  if (tid == 0) gave_up = 0;
-
   // ---- the line: its length, and where each team of this CTA starts
-  i64 mine = 0, sides = 0;
-  for (int b = tid; b < a.requests; b += kThreads) {
-    const Request r = request_at<kRows>(a, b, &wrong);
-    mine += (i64)r.sides * r.tiles;
-    sides += r.sides;
-  }
-  i64 line = mine;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    line += __shfl_xor_sync(kAll, line, o);
-    sides += __shfl_xor_sync(kAll, sides, o);
-  }
-  if (lane == 0) {
-    sums[0][warp] = line;
-    sums[1][warp] = sides;
-  }
-  __syncthreads();
-  line = sides = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    line += sums[0][w];
-    sides += sums[1][w];
-  }
-  if (wrong) *a.bad = 1;
-  if (line == 0) return;
-  // teams as small as their share still covers about one (request, head): joining warps costs less than joining units, and
-  // joining nothing least
   const int grid = gridDim.x;
-  int team_warps = 1;
-  while (team_warps < kWarps && sides * team_warps < (i64)grid * kWarps) team_warps *= 2;
-  const int teams = kWarps / team_warps;
-  i64 units = min((i64)grid * teams, (line + kMinShare * team_warps - 1) / (kMinShare * team_warps));
-  units = min(units, (i64)a.most_units);
-  auto start_of = [&](i64 u) { return u * line / units; };
-  auto unit_of = [&](i64 x) {
-    i64 u = x * units / line;
-    while (start_of(u + 1) <= x) ++u;
-    return u;
+  int team_warps, units, share, more;
+  bool split;
+  // From the sums over the requests (all: steps; sides: (head, row tile) pairs; most: steps of the longest): if a team each can
+  // take the pairs whole in about the time that even shares and joining the units' parts (worth about kJoinSteps steps) take,
+  // they do; else teams are as small as kMostParts parts a pair allow, since a team waits for its slowest warp at every pair.
+  auto plan = [&](i64 all, int sides, int most) {
+    const int warps = grid * kWarps, line = (int)all;
+    split = true;
+    for (team_warps = kWarps; team_warps >= 1; --team_warps)
+      if (kWarps % team_warps == 0 && (i64)sides * team_warps <= warps && (most + team_warps - 1) / team_warps <= line / warps + kJoinSteps) {
+        split = false;
+        break;
+      }
+    if (!split) {
+      units = sides;
+      return;
+    }
+    team_warps = 1;
+    while (team_warps < kWarps && (kWarps % team_warps != 0 || (i64)sides * team_warps * kMostParts < warps)) ++team_warps;
+    units = min(min(warps / team_warps, a.most_units), (line + kMinShare * team_warps - 1) / (kMinShare * team_warps));
+    share = line / units;
+    more = line - share * units;   // the first `more` units take one step more
   };
-  {
-    i64 carry = 0;
+  auto start_of = [&](int u) { return u * share + min(u, more); };
+  auto unit_of = [&](int x) {
+    const int edge = more * (share + 1);
+    return x < edge ? x / (share + 1) : more + (x - edge) / share;
+  };
+  constexpr i64 kMostSteps = 0x3fffffff;   // over a terabyte of cache
+  int team, member, unit, b_start, b_begin, lo, hi;
+  if (a.requests <= 32) {
+    // every warp for itself
+    Request r{};
+    if (lane < a.requests) r = request_at<kRows>(a, lane, &wrong);
+    i64 steps = (i64)r.sides * r.steps;
+    int pairs = r.sides, most = r.sides ? r.steps : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const i64 s = __shfl_up_sync(kAll, steps, o);
+      const int p = __shfl_up_sync(kAll, pairs, o);
+      if (lane >= o) {
+        steps += s;
+        pairs += p;
+      }
+    }
+    most = __reduce_max_sync(kAll, most);
+    const i64 all = __shfl_sync(kAll, steps, 31);
+    wrong |= all > kMostSteps;
+    if (wrong) *a.bad = 1;
+    if (all == 0 || all > kMostSteps) return;
+    plan(all, __shfl_sync(kAll, pairs, 31), most);
+    team = warp / team_warps;
+    unit = team * grid + blockIdx.x;
+    if (unit >= units) return;
+    const int upto = split ? (int)steps : pairs, from = split ? start_of(unit) : unit;
+    b_start = __ffs(__ballot_sync(kAll, upto > from)) - 1;
+    b_begin = __shfl_sync(kAll, (int)steps - r.sides * r.steps, b_start);
+    const int first_pair = __shfl_sync(kAll, pairs - r.sides, b_start), long_pair = __shfl_sync(kAll, r.steps, b_start);
+    lo = split ? from : b_begin + (unit - first_pair) * long_pair;
+    hi = split ? start_of(unit + 1) : lo + long_pair;
+  } else {
+    i64 all = 0;
+    int sides = 0, most = 0;
+    for (int b = tid; b < a.requests; b += kThreads) {
+      const Request r = request_at<kRows>(a, b, &wrong);
+      all += (i64)r.sides * r.steps;
+      sides += r.sides;
+      if (r.sides) most = max(most, r.steps);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      all += __shfl_xor_sync(kAll, all, o);
+      sides += __shfl_xor_sync(kAll, sides, o);
+    }
+    most = __reduce_max_sync(kAll, most);
+    if (lane == 0) {
+      sums[0][warp] = all;
+      sums[1][warp] = sides;
+      sums[2][warp] = most;
+    }
+    __syncthreads();
+    all = 0;
+    sides = most = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      all += sums[0][w];
+      sides += (int)sums[1][w];
+      most = max(most, (int)sums[2][w]);
+    }
+    wrong |= all > kMostSteps;
+    if (wrong) *a.bad = 1;
+    if (all == 0 || all > kMostSteps) return;
+    plan(all, sides, most);
+    const int teams = kWarps / team_warps;
+    int carry_s = 0, carry_p = 0;
     for (int b0 = 0; b0 < a.requests; b0 += kThreads) {
       const int b = b0 + tid;
       bool skip = false;
-      i64 v = 0;
-      if (b < a.requests) {
-        const Request r = request_at<kRows>(a, b, &skip);
-        v = (i64)r.sides * r.tiles;
-      }
-      i64 upto = v;
+      Request r{};
+      if (b < a.requests) r = request_at<kRows>(a, b, &skip);
+      const int v = r.sides * r.steps;
+      int steps = v, pairs = r.sides;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const i64 u = __shfl_up_sync(kAll, upto, o);
-        if (lane >= o) upto += u;
+        const int s = __shfl_up_sync(kAll, steps, o), p = __shfl_up_sync(kAll, pairs, o);
+        if (lane >= o) {
+          steps += s;
+          pairs += p;
+        }
       }
+      if (b0) __syncthreads();
+      if (lane == 31) scan[warp] = make_int2(steps, pairs);
       __syncthreads();
-      if (lane == 31) sums[0][warp] = upto;
-      __syncthreads();
-      i64 before = carry;
+      int before_s = carry_s, before_p = carry_p;
       for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += sums[0][w];
-        carry += sums[0][w];
+        const int2 c = scan[w];
+        if (w < warp) {
+          before_s += c.x;
+          before_p += c.y;
+        }
+        carry_s += c.x;
+        carry_p += c.y;
       }
-      upto += before;
+      steps += before_s;
+      pairs += before_p;
       for (int k = 0; k < teams; ++k) {
-        const i64 u = (i64)k * grid + blockIdx.x;
-        if (u < units) {
-          const i64 x = start_of(u);
-          if (x >= upto - v && x < upto) {
-            start_b[k] = b;
-            start_at[k] = x - (upto - v);
-          }
+        const int u = k * grid + blockIdx.x;
+        if (u >= units) break;
+        const int x = split ? start_of(u) : u;
+        if (split ? x >= steps - v && x < steps : x >= pairs - r.sides && x < pairs) {
+          const int from = split ? x : steps - v + (x - (pairs - r.sides)) * r.steps;
+          starts[k] = make_int4(b, steps - v, from, split ? start_of(u + 1) : from + r.steps);
         }
       }
     }
+    __syncthreads();
+    team = warp / team_warps;
+    unit = team * grid + blockIdx.x;
+    if (unit >= units) return;
+    const int4 s = starts[team];
+    b_start = s.x;
+    b_begin = s.y;
+    lo = s.z;
+    hi = s.w;
   }
-  __syncthreads();
-  const int team = warp / team_warps, member = warp % team_warps, team_threads = 32 * team_warps;
-  const i64 unit = (i64)team * grid + blockIdx.x;
-  if (unit >= units) return;
-  const i64 lo = start_of(unit), hi = start_of(unit + 1);
-  const int mine_tiles = (int)((hi - lo - member + team_warps - 1) / team_warps);   // this warp's: lo + member + k * team_warps
+  member = warp % team_warps;
+  const int team_threads = 32 * team_warps;
+  const int mine_steps = (hi - lo - member + team_warps - 1) / team_warps;   // this warp's: lo + member + k * team_warps
 
-  // ---- copies: lane l of a batch of 32 finds the l-th tile of the warp from there
-  int walk_b = start_b[team];
-  i64 walk_at = lo - start_at[team];    // where that request begins in the line
-  i64 tile_addr = 0;                    // of this lane's tile of the batch; 0: nothing to copy
+  // ---- copies: lane l of a batch of 32 finds the l-th step of the warp from there, one batch ahead, so that nobody waits for
+  // the table
+  constexpr uint32_t kNone = 0xffffffffu;
+  const int page_tiles = a.page_tokens >> 4;
+  int walk_b = b_start, walk_at = b_begin;    // a request at or before the batch's first step, where it begins
+  uint32_t ahead[2] = {kNone, kNone}, now[2] = {kNone, kNone};   // tiles of this lane's step, counted through the cache
   auto find_batch = [&](int k0) {
-    const i64 x = lo + member + (i64)(k0 + lane) * team_warps;
-    tile_addr = 0;
-    if (k0 + lane < mine_tiles) {
+    const int x = lo + member + (k0 + lane) * team_warps;
+    const bool mine_too = k0 + lane < mine_steps;
+    ahead[0] = ahead[1] = kNone;
+    if (mine_too) {
       bool skip = false;
-      int b = walk_b;
-      i64 begin = walk_at;
+      int b = walk_b, begin = walk_at;
       Request r = request_at<kRows>(a, b, &skip);
-      while (x >= begin + (i64)r.sides * r.tiles) {
-        begin += (i64)r.sides * r.tiles;
+      while (x >= begin + r.sides * r.steps) {
+        begin += r.sides * r.steps;
         ++b;
         r = request_at<kRows>(a, b, &skip);
       }
-      const i64 at = x - begin;
-      const int side = (int)(at / r.tiles), tile = (int)(at - (i64)side * r.tiles), head = side / (r.sides / a.kv_heads);
-      if (tile * 16 < r.length) {
-        const int page = a.table[b * a.table_stride + (tile * 16 >> a.page_shift)];
-        if (page < 0 || page >= a.pages) *a.bad = 1;
-        else
-          tile_addr = reinterpret_cast<i64>(a.data + page * a.page_bytes +
-                                            (int64_t)(head * (a.page_tokens >> 4) + (tile & ((a.page_tokens >> 4) - 1))) * T::kBytes);
+      const int at = x - begin, side = at / r.steps, step = at - side * r.steps, head = side / (r.sides / a.kv_heads);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int tile = 2 * step + h;
+        if (tile * 16 < r.length) {
+          const int page = a.table[b * a.table_stride + (tile * 16 >> a.page_shift)];
+          if (page < 0 || page >= a.pages) *a.bad = 1;
+          else ahead[h] = (uint32_t)(page * a.kv_heads + head) * page_tiles + (tile & (page_tiles - 1));
+        }
       }
       walk_b = b;
       walk_at = begin;
     }
     // the next batch starts from the last lane that found one
-    const unsigned found = __ballot_sync(kAll, k0 + lane < mine_tiles);
+    const unsigned found = __ballot_sync(kAll, mine_too);
     const int from = found ? 31 - __clz(found) : 0;
     walk_b = __shfl_sync(kAll, walk_b, from);
     walk_at = __shfl_sync(kAll, walk_at, from);
   };
-  auto issue = [&](int k) {
-    if ((k & 31) == 0) find_batch(k);
-    const i64 addr = __shfl_sync(kAll, tile_addr, k & 31);
-    if (lane == 0) {
-      const int s = k % kStages;
-      const uint32_t bar = tc::smem_u32(&bars[warp][s]);
-      stage_ok[warp][s] = addr != 0;
-      if (addr) {
-        tc::mbar_arrive_expect_tx(bar, T::kBytes);
-        tc::bulk_g2s(ring + s * T::kBytes, reinterpret_cast<const void*>(addr), T::kBytes, bar);
-      } else {
-        tc::mbar_arrive(bar);
+  // 16 bytes a lane; a tile that is not there is filled with zeros
+  auto issue = [&](int k, int s) {
+    if (k < mine_steps) {
+      if ((k & 31) == 0) {
+        now[0] = ahead[0];
+        now[1] = ahead[1];
+        if (k + 32 < mine_steps) find_batch(k + 32);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t tile = __shfl_sync(kAll, now[h], k & 31);
+        const uint32_t bytes = tile == kNone ? 0 : 16;
+        const uint8_t* from = a.data + (int64_t)(tile == kNone ? 0 : tile) * T::kBytes + lane * 16;
+        const uint32_t to = ring_at + s * S::kStage + h * T::kBytes;
+#pragma unroll
+        for (int c = 0; c < (T::kBytes + 511) / 512; ++c)
+          if (T::kBytes >= 512 * (c + 1) || lane * 16 < T::kBytes - 512 * c)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 512 * c), "l"(from + 512 * c), "r"(bytes) : "memory");
       }
     }
+    cp_async_commit();
   };
-  int issued = 0, taken = 0;
-  bool alive = true;
-  int stuck = 0;                        // the copy whose wait ran out
-  for (; issued < kStages && issued < mine_tiles; ++issued) issue(issued);
+  int taken = 0, stage = 0;             // steps done, the stage of the next
+  find_batch(0);
+  for (int k = 0; k < kStages; ++k) issue(k, k);
+  const Bases bases{tc::in_register(0x64006400u), tc::in_register(0x54005400u), tc::in_register(0x5c005c00u), tc::in_register(0x4c004c00u)};
+  constexpr uint32_t above[4] = {0xe408e408u, 0xd480d480u, 0xdc20dc20u, 0xce00ce00u};   // -1032, -72, -264, -24
 
   // ---- (request, head, row tile) after (request, head, row tile)
-  int b = start_b[team];
-  i64 begin = lo - start_at[team];
+  int b = b_start, begin = b_begin;
   bool skip = false;
   Request r = request_at<kRows>(a, b, &skip);
-  i64 x = lo;
+  int x = lo;
   while (x < hi) {
-    while (x >= begin + (i64)r.sides * r.tiles) {
-      begin += (i64)r.sides * r.tiles;
+    while (x >= begin + r.sides * r.steps) {
+      begin += r.sides * r.steps;
       ++b;
       r = request_at<kRows>(a, b, &skip);
     }
-    const i64 at = x - begin;
-    const int side = (int)(at / r.tiles), tile0 = (int)(at - (i64)side * r.tiles);
+    const int at = x - begin, side = at / r.steps, step0 = at - side * r.steps;
     const int row_tiles = r.sides / a.kv_heads, head = side / row_tiles, row0 = (side - head * row_tiles) * kRows;
     const int all_rows = r.rows * a.group;
-    const i64 piece_end = min(hi, x - tile0 + r.tiles);
+    const int piece_end = min(hi, x - step0 + r.steps);
 
     // queries: this lane's row g of each tile of 8, dims 8t .. 8t+7 of each group
     uint32_t qf[kParts][NT][J][4];
-    float offset[NT][J][2];
+    uint32_t off[NT][2];                                          // of group t and row g, as two tf32
     int see[NT][2];
-    float m[NT][2], l[NT][2], o[NT][D / 16][4];
+    float m[NT][2], cap[NT][2], l[NT][2], o[NT][D / 16][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = row0 + nt * 8 + g;
       const bool live = row < all_rows;
       const int i = live ? row / a.group : 0;
       const int64_t from = (int64_t)(r.first + i) * a.qs + (int64_t)(head * a.group + (live ? row - i * a.group : 0)) * a.qh;
+      off[nt][0] = off[nt][1] = 0;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         float v[8];
@@ -350,23 +488,26 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && !kExact ? 2 : 1) kv_atten
         for (int e = 0; e < 4; ++e) {
           const uint32_t hi2 = half2_of(v[2 * e], v[2 * e + 1]);
           qf[0][nt][j][e] = hi2;
-          sum += low_of(hi2) + high_of(hi2);
+          float two = low_of(hi2) + high_of(hi2);
           if constexpr (kExact) {
             const uint32_t lo2 = half2_of(v[2 * e] - low_of(hi2), v[2 * e + 1] - high_of(hi2));
             qf[1][nt][j][e] = lo2;
-            sum += low_of(lo2) + high_of(lo2);
+            two += low_of(lo2) + high_of(lo2);
           }
+          sum = fmaf(kExact ? -72.0f : -above_of(e), two, sum);
         }
         sum += __shfl_xor_sync(kAll, sum, 1);
         sum += __shfl_xor_sync(kAll, sum, 2);
-        offset[nt][j][0] = -72.0f * __shfl_sync(kAll, sum, 8 * t);
-        offset[nt][j][1] = -72.0f * __shfl_sync(kAll, sum, 8 * t + 4);
+        if (t == j) {
+          off[nt][0] = tf32_of(sum);
+          off[nt][1] = tf32_of(sum - __uint_as_float(off[nt][0]));
+        }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int rr = row0 + nt * 8 + 2 * t + h;
         see[nt][h] = r.length - r.rows + min(rr, all_rows - 1) / a.group + 1;
-        m[nt][h] = kLowest;
+        m[nt][h] = cap[nt][h] = kLowest;
         l[nt][h] = 0.0f;
       }
 #pragma unroll
@@ -375,114 +516,126 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && !kExact ? 2 : 1) kv_atten
         for (int e = 0; e < 4; ++e) o[nt][i16][e] = 0.0f;
     }
     const int all_see = r.length - r.rows + row0 / a.group + 1;   // the first row's
-    int scale_exp = -11;                                          // see below
+    // A weight times a value's scale is rounded to f16, whose range is small: weights are taken times 2^-scale_exp, the running
+    // exponent of the largest scale, as part of the running maximum m.  cap: the score that moves m; scale_cap: the scale that
+    // moves scale_exp.  Neither happens often.
+    int scale_exp = -11;
+    uint32_t scale_cap = 0x14001400u;                             // 2^-10
+    float neg_m[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) neg_m[nt][0] = neg_m[nt][1] = -kLowest;
 
-    for (; taken < mine_tiles; ++taken) {
-      const i64 pos = lo + member + (i64)taken * team_warps;
+    for (; taken < mine_steps; ++taken) {
+      const int pos = lo + member + taken * team_warps;
       if (pos >= piece_end) break;
-      const int s = taken % kStages;
-      if (alive && !tc::mbar_wait(tc::smem_u32(&bars[warp][s]), (taken / kStages) & 1, &gave_up)) {
-        alive = false;
-        stuck = taken;
-        *a.status = 1;
-      }
-      if (__any_sync(kAll, !alive)) {
-        if (alive) stuck = taken;
-        alive = false;
-        continue;
-      }
-      const int token0 = (tile0 + (int)(pos - x)) * 16;
-      const uint8_t* tile = ring + s * T::kBytes;
-      const bool here = stage_ok[warp][s];
-      const bool whole = here && token0 + 16 <= all_see;
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      const int token0 = (step0 + pos - x) * kStep;
+      const uint8_t* tiles = ring + stage * S::kStage;
+      const bool whole = token0 + kStep <= all_see;
 
-      // scores: rows are tokens token0 + g and + 8, columns the query rows
-      float score[NT][4];
+      // scores: rows are tokens token0 + 16 u + g and + 8, columns the query rows
+      float score[2][NT][4];
+      uint32_t word[2];                   // this lane's share of the values' scales
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int u = 0; u < 2; ++u) {
+        const uint8_t* tile = tiles + u * T::kBytes;
+        word[u] = lane < 8 * J ? *reinterpret_cast<const uint32_t*>(tile + T::kScaleV + lane * 4) & 0x7fff7fffu : 0u;
+        uint32_t kw[2][J];
+        float dk[2][J];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) score[nt][e] = 0.0f;
-      uint32_t kw[2][J];
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+          for (int jv = 0; jv < J / T::kVecK; ++jv) {
+            uint32_t w[T::kVecK];
+            lds(w, tile + ((h * (J / T::kVecK) + jv) * 32 + lane) * T::kVecK * 4);
 #pragma unroll
-        for (int jv = 0; jv < J / T::kVecK; ++jv) {
-          uint32_t w[T::kVecK];
-          lds(w, tile + ((h * (J / T::kVecK) + jv) * 32 + lane) * T::kVecK * 4);
-#pragma unroll
-          for (int e = 0; e < T::kVecK; ++e) kw[h][jv * T::kVecK + e] = w[e];
-        }
-      const uint32_t nibbles = tc::in_register(0x00f000f0u), base64 = tc::in_register(0x54005400u);
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const uint32_t w0 = kw[0][j], w1 = kw[1][j];
-        const uint32_t a0[4] = {tc::mask_or(w0 << 4, nibbles, base64), tc::mask_or(w1 << 4, nibbles, base64),
-                                tc::mask_or(w0, nibbles, base64), tc::mask_or(w1, nibbles, base64)};
-        const uint32_t a1[4] = {tc::mask_or(w0 >> 4, nibbles, base64), tc::mask_or(w1 >> 4, nibbles, base64),
-                                tc::mask_or(w0 >> 8, nibbles, base64), tc::mask_or(w1 >> 8, nibbles, base64)};
-        const float d0 = __half2float(*reinterpret_cast<const __half*>(tile + T::key_scale(0, j) + g * J * 2));
-        const float d1 = __half2float(*reinterpret_cast<const __half*>(tile + T::key_scale(8, j) + g * J * 2));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float c[4] = {offset[nt][j][0], offset[nt][j][1], offset[nt][j][0], offset[nt][j][1]};
-#pragma unroll
-          for (int part = 0; part < kParts; ++part) {
-            mma(c, a0, qf[part][nt][j][0], qf[part][nt][j][1]);
-            mma(c, a1, qf[part][nt][j][2], qf[part][nt][j][3]);
+            for (int e = 0; e < T::kVecK; ++e) kw[h][jv * T::kVecK + e] = w[e];
           }
-          score[nt][0] = fmaf(d0, c[0], score[nt][0]);
-          score[nt][1] = fmaf(d0, c[1], score[nt][1]);
-          score[nt][2] = fmaf(d1, c[2], score[nt][2]);
-          score[nt][3] = fmaf(d1, c[3], score[nt][3]);
+          const uint8_t* sc = tile + T::key_scale(8 * h, 0) + g * J * 2;
+          if constexpr (J % 2 == 0) {
+            uint32_t w[J / 2];
+            lds(w, sc);
+#pragma unroll
+            for (int e = 0; e < J / 2; ++e) {
+              dk[h][2 * e] = low_of(w[e]);
+              dk[h][2 * e + 1] = high_of(w[e]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < J; ++j) dk[h][j] = __half2float(*reinterpret_cast<const __half*>(sc + 2 * j));
+          }
+        }
+        // the scales times what the operands are above q - 8, of all groups at once (k is the groups, twice), then group by group
+        const uint8_t* own = tile + T::key_scale(0, 0) + (g * J + (t < J ? t : 0)) * 2;
+        const float d0 = t < J ? __half2float(*reinterpret_cast<const __half*>(own)) : 0.0f;
+        const float d1 = t < J ? __half2float(*reinterpret_cast<const __half*>(own + 8 * J * 2)) : 0.0f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_tf32(score[u][nt], __float_as_uint(d0), __float_as_uint(d1), off[nt][0], off[nt][1]);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          uint32_t p0[4], p1[4];
+          if constexpr (kExact) {   // 22 bits of a score's sum of 32 are left below 64 + q, 18 below 1024 + q
+            spread_even(kw[0][j], bases.b64, p0);
+            spread_even(kw[1][j], bases.b64, p1);
+          } else {
+            spread(kw[0][j], bases, p0);
+            spread(kw[1][j], bases, p1);
+          }
+          const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float c[4];
+            mma_first(c, a0, qf[0][nt][j][0], qf[0][nt][j][1]);
+            mma(c, a1, qf[0][nt][j][2], qf[0][nt][j][3]);
+            if constexpr (kExact) {
+              mma(c, a0, qf[kParts - 1][nt][j][0], qf[kParts - 1][nt][j][1]);
+              mma(c, a1, qf[kParts - 1][nt][j][2], qf[kParts - 1][nt][j][3]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) score[u][nt][e] = fmaf(dk[e >> 1][j], c[e], score[u][nt][e]);
+          }
         }
       }
-      // values' scales of this lane's four tokens
-      uint32_t dv[J][2];
-#pragma unroll
-      for (int j = 0; j < J; ++j) lds(dv[j], tile + T::kScaleV + (t * J + j) * 8);
       if (!whole) {
+        // behind the request's tokens a page holds anything: no weight, and no say in the exponent
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int u = 0; u < 2; ++u) {
+          const int t0 = token0 + 16 * u;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!here || token0 + g + (e >> 1) * 8 >= see[nt][e & 1]) score[nt][e] = -INFINITY;
-        // behind the request's tokens a page holds anything: no weight, and a scale that keeps the product one
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < J; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int tok = token0 + 2 * t + 8 * h;
-            if (!here || tok >= r.length) dv[j][h] = 0;
-            else if (tok + 1 >= r.length) dv[j][h] &= 0xffffu;
-          }
+            for (int e = 0; e < 4; ++e)
+              if (t0 + g + (e >> 1) * 8 >= see[nt][e & 1]) score[u][nt][e] = -INFINITY;
+          const int tok = t0 + lane / (2 * J) * 2 + (lane & 1) * 8;
+          if (tok >= r.length) word[u] = 0;
+          else if (tok + 1 >= r.length) word[u] &= 0xffffu;
+        }
       }
-      // A weight times a value's scale is rounded to f16, whose range is small: weights are taken times 2^-scale_exp, the
-      // running exponent of the largest scale, as part of the running maximum.  Neither changes often.
-      uint32_t big = 0;
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) big = tc::h2_bits(__hmax2(tc::bits_h2(big), __habs2(tc::bits_h2(dv[j][h]))));
-      const int big_exp = min(4, max((int)((big >> 10) & 31), (int)(big >> 26)) - 15);
-      bool moves = big_exp > scale_exp;
+      // a half of `word` that reaches scale_cap keeps the bit above it
+      bool moves = ((((word[0] | 0x80008000u) - scale_cap) | ((word[1] | 0x80008000u) - scale_cap)) & 0x80008000u) != 0;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          moves |= fmaxf(score[nt][h], score[nt][h + 2]) * a.scale_log2 > m[nt][h] + kSlack;
+          moves |= fmaxf(fmaxf(score[0][nt][h], score[0][nt][h + 2]), fmaxf(score[1][nt][h], score[1][nt][h + 2])) > cap[nt][h];
       if (__any_sync(kAll, moves)) {
-        const int e_new = max(scale_exp, __reduce_max_sync(kAll, big_exp));
+        int big = (int)max(max(word[0] & 0xffffu, word[0] >> 16), max(word[1] & 0xffffu, word[1] >> 16)) >> 10;
+        big = min(4, __reduce_max_sync(kAll, big) - 15);
+        const int e_new = max(scale_exp, big);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float top = fmaxf(score[nt][h], score[nt][h + 2]) * a.scale_log2;
+            float top = fmaxf(fmaxf(score[0][nt][h], score[0][nt][h + 2]), fmaxf(score[1][nt][h], score[1][nt][h + 2])) * a.scale_log2;
             top = fmaxf(top, __shfl_xor_sync(kAll, top, 4));
             top = fmaxf(top, __shfl_xor_sync(kAll, top, 8));
             top = fmaxf(top, __shfl_xor_sync(kAll, top, 16));
             top = fmaxf(top, m[nt][h]);
             const float f = exp2_fast((m[nt][h] - top) + (float)(scale_exp - e_new));
             m[nt][h] = top;
+            cap[nt][h] = (top + kSlack) / a.scale_log2;
+            neg_m[nt][h] = -(top + (float)e_new);
             l[nt][h] *= f;
 #pragma unroll
             for (int i16 = 0; i16 < D / 16; ++i16) {
@@ -491,71 +644,97 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && !kExact ? 2 : 1) kv_atten
             }
           }
         scale_exp = e_new;
+        scale_cap = e_new == 4 ? 0x7c007c00u : (uint32_t)(e_new + 16) * 0x04000400u;
       }
-      float weight[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float m0 = m[nt][0] + (float)scale_exp, m1 = m[nt][1] + (float)scale_exp;
-        weight[nt][0] = exp2_fast(fmaf(score[nt][0], a.scale_log2, -m0));
-        weight[nt][1] = exp2_fast(fmaf(score[nt][1], a.scale_log2, -m1));
-        weight[nt][2] = exp2_fast(fmaf(score[nt][2], a.scale_log2, -m0));
-        weight[nt][3] = exp2_fast(fmaf(score[nt][3], a.scale_log2, -m1));
-        l[nt][0] += weight[nt][0] + weight[nt][2];
-        l[nt][1] += weight[nt][1] + weight[nt][3];
-      }
-      uint32_t pf[NT][2];
-      if constexpr (!kExact) {
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          pf[nt][0] = turn8x8(half2_of(weight[nt][0], weight[nt][1]));
-          pf[nt][1] = turn8x8(half2_of(weight[nt][2], weight[nt][3]));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) score[u][nt][e] = exp2_fast(fmaf(score[u][nt][e], a.scale_log2, neg_m[nt][e & 1]));
+          l[nt][0] += score[u][nt][0] + score[u][nt][2];
+          l[nt][1] += score[u][nt][1] + score[u][nt][3];
         }
-      }
-      const uint32_t low4 = tc::in_register(0x000f000fu), base1024 = tc::in_register(0x64006400u);
-      const __half2 c72 = __float2half2_rn(-72.0f), c1032 = __float2half2_rn(-1032.0f);
       constexpr int kVV = T::kVecV;
-      uint32_t vw[kVV];
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        uint32_t bf[kParts][NT][2];
+      for (int u = 0; u < 2; ++u) {
+        const uint8_t* tile = tiles + u * T::kBytes;
+        const int t0 = token0 + 16 * u;
+        // scales of this lane's four tokens, and the weights as operands
+        uint32_t dv[J][2], pf[NT][2];
+        if constexpr (J % 2 == 0) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if constexpr (!kExact) {
-            bf[0][nt][0] = tc::h2_bits(__hmul2(tc::bits_h2(pf[nt][0]), tc::bits_h2(dv[j][0])));
-            bf[0][nt][1] = tc::h2_bits(__hmul2(tc::bits_h2(pf[nt][1]), tc::bits_h2(dv[j][1])));
-          } else {
-            // in f32, tokens g and g + 8 a lane, then as two f16
+          for (int j = 0; j < J; j += 2) {
+            uint32_t w[4];
+            lds(w, tile + T::kScaleV + (t * J + j) * 8);
+            dv[j][0] = w[0]; dv[j][1] = w[1]; dv[j + 1][0] = w[2]; dv[j + 1][1] = w[3];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < J; ++j) lds(dv[j], tile + T::kScaleV + (t * J + j) * 8);
+        }
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float d = __half2float(*reinterpret_cast<const __half*>(tile + T::kScaleV + ((g >> 1) * J + j) * 8 + (g & 1) * 2 + 4 * h));
-              if (!here || token0 + g + 8 * h >= r.length) d = 0.0f;
-              const float p0 = weight[nt][2 * h] * d, p1 = weight[nt][2 * h + 1] * d;
-              const uint32_t hi2 = half2_of(p0, p1);
-              bf[0][nt][h] = turn8x8(hi2);
-              bf[kParts - 1][nt][h] = turn8x8(half2_of(p0 - low_of(hi2), p1 - high_of(hi2)));
+              const int tok = t0 + 2 * t + 8 * h;
+              if (tok >= r.length) dv[j][h] = 0;
+              else if (tok + 1 >= r.length) dv[j][h] &= 0xffffu;
             }
+        }
+        if constexpr (!kExact) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            pf[nt][0] = turn8x8(half2_of(score[u][nt][0], score[u][nt][1]));
+            pf[nt][1] = turn8x8(half2_of(score[u][nt][2], score[u][nt][3]));
           }
         }
+        uint32_t vw[kVV];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int i16 = 2 * j + half;
-          if (i16 % kVV == 0) lds(vw, tile + T::kV + (i16 / kVV * 32 + lane) * kVV * 4);
-          const uint32_t w = vw[i16 % kVV], w8 = w >> 8;
-          const uint32_t av[4] = {tc::h2_bits(__hadd2(tc::bits_h2(tc::mask_or(w, low4, base1024)), c1032)),
-                                  tc::h2_bits(__hadd2(tc::bits_h2(tc::mask_or(w, nibbles, base64)), c72)),
-                                  tc::h2_bits(__hadd2(tc::bits_h2(tc::mask_or(w8, low4, base1024)), c1032)),
-                                  tc::h2_bits(__hadd2(tc::bits_h2(tc::mask_or(w8, nibbles, base64)), c72))};
+        for (int j = 0; j < J; ++j) {
+          uint32_t bf[kParts][NT][2];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
+            if constexpr (!kExact) {
+              bf[0][nt][0] = tc::h2_bits(__hmul2(tc::bits_h2(pf[nt][0]), tc::bits_h2(dv[j][0])));
+              bf[0][nt][1] = tc::h2_bits(__hmul2(tc::bits_h2(pf[nt][1]), tc::bits_h2(dv[j][1])));
+            } else {
+              // in f32, tokens g and g + 8 a lane, then as two f16
 #pragma unroll
-            for (int part = 0; part < kParts; ++part) mma(o[nt][i16], av, bf[part][nt][0], bf[part][nt][1]);
+              for (int h = 0; h < 2; ++h) {
+                float d = __half2float(*reinterpret_cast<const __half*>(tile + T::kScaleV + ((g >> 1) * J + j) * 8 + (g & 1) * 2 + 4 * h));
+                if (t0 + g + 8 * h >= r.length) d = 0.0f;
+                const float p0 = score[u][nt][2 * h] * d, p1 = score[u][nt][2 * h + 1] * d;
+                const uint32_t hi2 = half2_of(p0, p1);
+                bf[0][nt][h] = turn8x8(hi2);
+                bf[kParts - 1][nt][h] = turn8x8(half2_of(p0 - low_of(hi2), p1 - high_of(hi2)));
+              }
+            }
+          }
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int i16 = 2 * j + half;
+            if (i16 % kVV == 0) lds(vw, tile + T::kV + (i16 / kVV * 32 + lane) * kVV * 4);
+            uint32_t av[4];
+            spread(vw[i16 % kVV], bases, av);
+            // centred before the product, exactly: a sum over the tokens would not survive the difference
+#pragma unroll
+            for (int e = 0; e < 4; ++e) av[e] = tc::h2_bits(__hadd2(tc::bits_h2(av[e]), tc::bits_h2(above[e])));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int part = 0; part < kParts; ++part) mma(o[nt][i16], av, bf[part][nt][0], bf[part][nt][1]);
+          }
         }
       }
       __syncwarp();
-      if (issued < mine_tiles) issue(issued++);
+      issue(taken + kStages, stage);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
     }
 
-    // ---- the team's warps together
+    // ---- the piece's results.  A cell is what a lane holds of 16 dims: rows 2t and 2t + 1, dims 16 i + 2g and the next.  Cells stay in
+    // this order all the way: through shared memory, through scratch, until the last sum is made
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -563,113 +742,152 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && !kExact ? 2 : 1) kv_atten
         m[nt][h] += (float)scale_exp;
 #pragma unroll
         for (int s = 4; s < 32; s <<= 1) l[nt][h] += __shfl_xor_sync(kAll, l[nt][h], s);
-        if (g == 0) {
-          join_m[warp][nt * 8 + 2 * t + h] = m[nt][h];
-          join_l[warp][nt * 8 + 2 * t + h] = l[nt][h];
-        }
       }
-    team_barrier(team, team_threads);
-    const int w0 = team * team_warps;
-    float* mine_o = joint + warp * kRows * S::kJoinLd;
+    const int w0 = team * team_warps, ttid = tid - w0 * 32;
+    if (team_warps > 1) {
+      if (g == 0)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<float2*>(&join_m[warp][nt * 8 + 2 * t]) = make_float2(m[nt][0], m[nt][1]);
+      team_barrier(team, team_threads);
+      float f[NT][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = nt * 8 + 2 * t + h;
-        float top = kLowest;
-        for (int w = 0; w < team_warps; ++w) top = fmaxf(top, join_m[w0 + w][row]);
-        const float f = exp2_fast(m[nt][h] - top);
+      for (int nt = 0; nt < NT; ++nt) {
+        float2 top = make_float2(kLowest, kLowest);
+        for (int w = 0; w < team_warps; ++w) {
+          const float2 o_m = *reinterpret_cast<const float2*>(&join_m[w0 + w][nt * 8 + 2 * t]);
+          top.x = fmaxf(top.x, o_m.x);
+          top.y = fmaxf(top.y, o_m.y);
+        }
+        f[nt][0] = exp2_fast(m[nt][0] - top.x);
+        f[nt][1] = exp2_fast(m[nt][1] - top.y);
+        m[nt][0] = top.x;
+        m[nt][1] = top.y;
+        if (g == 0) *reinterpret_cast<float2*>(&join_l[warp][nt * 8 + 2 * t]) = make_float2(l[nt][0] * f[nt][0], l[nt][1] * f[nt][1]);
 #pragma unroll
         for (int i16 = 0; i16 < D / 16; ++i16)
-          *reinterpret_cast<float2*>(mine_o + row * S::kJoinLd + i16 * 16 + 2 * g) =
-              make_float2(o[nt][i16][h] * f, o[nt][i16][h + 2] * f);
+          joint[(warp * kCells) + (nt * (D / 16) + i16) * 32 + lane] =
+              make_float4(o[nt][i16][0] * f[nt][0], o[nt][i16][1] * f[nt][1], o[nt][i16][2] * f[nt][0], o[nt][i16][3] * f[nt][1]);
       }
-    team_barrier(team, team_threads);
-
-    const int ttid = tid - w0 * 32;
-    const bool all_of_it = tile0 == 0 && piece_end == x + r.tiles;
-    const i64 seg = x - tile0;
-    const i64 u0 = all_of_it ? unit : unit_of(seg), u1 = all_of_it ? unit : unit_of(seg + r.tiles - 1);
-    const i64 slot = 2 * unit + (unit == u0 ? 1 : 0);
-    for (int e = ttid; e < kRows * D / 2; e += team_threads) {
-      const int row = e / (D / 2), d = e % (D / 2) * 2;
-      float top = kLowest, sum = 0.0f;
-      for (int w = 0; w < team_warps; ++w) top = fmaxf(top, join_m[w0 + w][row]);
-      float2 v = make_float2(0.0f, 0.0f);
-      for (int w = 0; w < team_warps; ++w) {
-        const float2 p = *reinterpret_cast<const float2*>(joint + (w0 + w) * kRows * S::kJoinLd + row * S::kJoinLd + d);
-        v.x += p.x;
-        v.y += p.y;
-        sum += join_l[w0 + w][row] * exp2_fast(join_m[w0 + w][row] - top);
-      }
-      if (all_of_it) {
-        const int rr = row0 + row;
-        if (rr < all_rows) {
-          const int i = rr / a.group;
-          const int64_t to = (int64_t)(r.first + i) * a.os + (int64_t)(head * a.group + rr - i * a.group) * a.oh + d;
-          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-          store_out(a, to, v.x * inv);
-          store_out(a, to + 1, v.y * inv);
+      team_barrier(team, team_threads);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        l[nt][0] = l[nt][1] = 0.0f;
+        for (int w = 0; w < team_warps; ++w) {
+          const float2 o_l = *reinterpret_cast<const float2*>(&join_l[w0 + w][nt * 8 + 2 * t]);
+          l[nt][0] += o_l.x;
+          l[nt][1] += o_l.y;
         }
-      } else {
-        *reinterpret_cast<float2*>(a.acc + (slot * kRows + row) * D + d) = v;
-        if (d == 0) *reinterpret_cast<float2*>(a.stats + (slot * kRows + row) * 2) = make_float2(top, sum);
       }
     }
+    auto cell_of = [&](int c, int nt, int i16) {
+      if (team_warps == 1) return make_float4(o[nt][i16][0], o[nt][i16][1], o[nt][i16][2], o[nt][i16][3]);
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int w = 0; w < team_warps; ++w) {
+        const float4 u = joint[(w0 + w) * kCells + c];
+        v.x += u.x;
+        v.y += u.y;
+        v.z += u.z;
+        v.w += u.w;
+      }
+      return v;
+    };
+    // rows 2t and 2t + 1 of row tile nt, where they are any
+    auto put = [&](int nt, int i16, const float4& v, float s0, float s1) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int rr = row0 + nt * 8 + 2 * t + h;
+        if (rr >= all_rows) continue;
+        const int i = rr / a.group;
+        const float sum = h ? s1 : s0, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        store_pair(a, (int64_t)(r.first + i) * a.os + (int64_t)(head * a.group + rr - i * a.group) * a.oh + i16 * 16 + 2 * g, (h ? v.y : v.x) * inv,
+                   (h ? v.w : v.z) * inv);
+      }
+    };
+    const bool all_of_it = step0 == 0 && piece_end == x + r.steps;
+    const int seg = x - step0, u0 = all_of_it ? unit : unit_of(seg), u1 = all_of_it ? unit : unit_of(seg + r.steps - 1);
+    auto part_of = [&](int u) { return 2 * (i64)u + (u == u0 ? 1 : 0); };
+    float4* acc = reinterpret_cast<float4*>(a.acc);
+    float4* stats = reinterpret_cast<float4*>(a.stats);
+#pragma unroll
+    for (int k = 0, turn = 0; k < kCells / 32; ++k) {
+      const bool others = turn != member;
+      turn = turn + 1 == team_warps ? 0 : turn + 1;
+      if (others) continue;
+      const int nt = k / (D / 16), i16 = k % (D / 16), c = k * 32 + lane;
+      const float4 v = cell_of(c, nt, i16);
+      if (all_of_it) put(nt, i16, v, l[nt][0], l[nt][1]);
+      else __stcg(acc + part_of(unit) * kCells + c, v);
+    }
     if (!all_of_it) {
-      // the last unit of the (request, head) to arrive joins all parts, in order
-      __threadfence();
+      if (member == 0 && g == 0)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          __stcg(stats + part_of(unit) * (kRows / 2) + nt * 4 + t, make_float4(m[nt][0], l[nt][0], m[nt][1], l[nt][1]));
+      // the last unit of the (request, head) to arrive joins all parts, in their order
       team_barrier(team, team_threads);
       if (ttid == 0) {
-        const int before = atomicAdd(a.arrived + u0, 1);
-        last_in[team] = before == (int)(u1 - u0);
-        if (last_in[team]) a.arrived[u0] = 0;
+        __threadfence();
+        const int last = atomicAdd(a.arrived + u0, 1) == u1 - u0;
+        if (last) a.arrived[u0] = 0;
+        __threadfence();
+        last_in[team] = last;
       }
       team_barrier(team, team_threads);
       if (last_in[team]) {
-        __threadfence();
-        for (int e = ttid; e < kRows * D / 2; e += team_threads) {
-          const int row = e / (D / 2), d = e % (D / 2) * 2, rr = row0 + row;
-          if (rr >= all_rows) continue;
-          float top = kLowest, sum = 0.0f;
-          float2 v = make_float2(0.0f, 0.0f);
-          for (i64 u = u0; u <= u1; ++u) {
-            const i64 at2 = (2 * u + (u == u0 ? 1 : 0)) * kRows + row;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.stats + at2 * 2));
-            const float2 p = __ldcg(reinterpret_cast<const float2*>(a.acc + at2 * D + d));
-            const float t2 = fmaxf(top, ml.x), keep = exp2_fast(top - t2), f = exp2_fast(ml.x - t2);
-            v.x = v.x * keep + p.x * f;
-            v.y = v.y * keep + p.y * f;
-            sum = sum * keep + ml.y * f;
-            top = t2;
+        float2 top[NT], sum[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          top[nt] = make_float2(kLowest, kLowest);
+          sum[nt] = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+          for (int u = u0; u <= u1; ++u) {
+            const float4 ml = __ldcg(stats + part_of(u) * (kRows / 2) + nt * 4 + t);
+            const float2 next = make_float2(fmaxf(top[nt].x, ml.x), fmaxf(top[nt].y, ml.z));
+            sum[nt].x = sum[nt].x * exp2_fast(top[nt].x - next.x) + ml.y * exp2_fast(ml.x - next.x);
+            sum[nt].y = sum[nt].y * exp2_fast(top[nt].y - next.y) + ml.w * exp2_fast(ml.z - next.y);
+            top[nt] = next;
           }
-          const int i = rr / a.group;
-          const int64_t to = (int64_t)(r.first + i) * a.os + (int64_t)(head * a.group + rr - i * a.group) * a.oh + d;
-          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-          store_out(a, to, v.x * inv);
-          store_out(a, to + 1, v.y * inv);
         }
+        constexpr int kAtOnce = D / 16 < 4 ? D / 16 : 4;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          for (int first = member; first < D / 16; first += kAtOnce * team_warps) {
+            float4 v[kAtOnce];
+#pragma unroll
+            for (int q = 0; q < kAtOnce; ++q) v[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+            for (int u = u0; u <= u1; ++u) {
+              const float4 ml = __ldcg(stats + part_of(u) * (kRows / 2) + nt * 4 + t);
+              const float f0 = exp2_fast(ml.x - top[nt].x), f1 = exp2_fast(ml.z - top[nt].y);
+#pragma unroll
+              for (int q = 0; q < kAtOnce; ++q) {
+                const int i16 = first + q * team_warps;
+                if (i16 >= D / 16) continue;
+                const float4 p = __ldcg(acc + part_of(u) * kCells + (nt * (D / 16) + i16) * 32 + lane);
+                v[q].x = fmaf(p.x, f0, v[q].x);
+                v[q].y = fmaf(p.y, f1, v[q].y);
+                v[q].z = fmaf(p.z, f0, v[q].z);
+                v[q].w = fmaf(p.w, f1, v[q].w);
+              }
+            }
+#pragma unroll
+            for (int q = 0; q < kAtOnce; ++q)
+              if (first + q * team_warps < D / 16) put(nt, first + q * team_warps, v[q], sum[nt].x, sum[nt].y);
+          }
       }
     }
     team_barrier(team, team_threads);
     x = piece_end;
   }
-  // a wait that ran out leaves copies in flight: they end before the warp does
-  if (!alive) {
-    volatile int own = 0;
-    for (; stuck < issued; ++stuck) {
-      own = 0;
-      tc::mbar_wait(tc::smem_u32(&bars[warp][stuck % kStages]), (stuck / kStages) & 1, &own);
-    }
-  }
 }
 
 template <int D, int NT, bool kExact>
 cudaError_t launch_one(const AttendArgs& a, int sm_count, cudaStream_t st) {
-  const int smem = Shape<D, NT>::kSmem;
+  using S = Shape<D, NT, kExact>;
+  const int smem = S::kSmem;
   cudaError_t e = cudaFuncSetAttribute(kv_attend_kernel<D, NT, kExact>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kv_attend_kernel<D, NT, kExact><<<sm_count * (NT == 1 && !kExact ? 2 : 1), kThreads, smem, st>>>(a);
+  kv_attend_kernel<D, NT, kExact><<<sm_count, 32 * S::kWarps, smem, st>>>(a);
   return cudaGetLastError();
 }
 template <int D>
@@ -686,7 +904,7 @@ cudaError_t launch_dim(AttendArgs& a, const KvAttendScratch& s, int sm_count, cu
 
 }  // namespace
 
-cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScratch& s, int sm_count, int* bad, int* status, cudaStream_t st) {
+cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScratch& s, int sm_count, int* bad, cudaStream_t st) {
   AttendArgs a{};
   a.data = static_cast<const uint8_t*>(r.cache.data);
   a.q = r.q;
@@ -712,12 +930,12 @@ cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScr
   a.type = r.type;
   const int64_t size = r.type == EMELB_F32 ? 4 : 2;
   a.q_vec = reinterpret_cast<uintptr_t>(r.q) % 16 == 0 && a.qs * size % 16 == 0 && a.qh * size % 16 == 0;
+  a.out_pairs = reinterpret_cast<uintptr_t>(r.out) % 4 == 0 && a.os % 2 == 0 && a.oh % 2 == 0;
   a.scale_log2 = r.scale * 1.44269504088896340736f;
   a.acc = s.acc;
   a.stats = s.stats;
   a.arrived = s.arrived;
   a.bad = bad;
-  a.status = status;
   switch (r.cache.head_dim) {
     case 32: return launch_dim<32>(a, s, sm_count, st);
     case 64: return launch_dim<64>(a, s, sm_count, st);

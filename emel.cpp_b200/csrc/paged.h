@@ -22,10 +22,9 @@ struct KvAttendScratch {
   int* arrived;
   uint64_t arrived_ints;
 };
-// `status`: raised to 1 when a bounded wait ran out
-cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScratch& s, int sm_count, int* bad, int* status,
-                             cudaStream_t st);
+cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScratch& s, int sm_count, int* bad, cudaStream_t st);
 
+// `status`: raised to 1 when a bounded wait ran out
 cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int sm_count, int* bad, int* status, cudaStream_t st);
 
 }  // namespace emelb

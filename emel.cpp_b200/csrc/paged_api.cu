@@ -229,7 +229,7 @@ uint32_t emelb_kv_attend(emelb_ctx* c, const emelb_kv_attend_request* r) {
   if (const uint32_t why = emelb_kv_attend_can_run(r)) return refuse(c, why);
   const KvAttendScratch s{c->fa_part_acc, kFlashPartFloats, c->fa_part_ml, kFlashPartFloats / 32, c->grp_cnt, c->grp_cnt_ints};
   return dispatch(c, {r->cache.data, r->q, r->out, r->table, r->lengths, r->query_begin}, 1,
-                  [&] { return launch_kv_attend(*r, s, c->sm_count, c->bad_word(), c->status_word(), c->stream); });
+                  [&] { return launch_kv_attend(*r, s, c->sm_count, c->bad_word(), c->stream); });
 }
 
 // ------------------------------------------------------------------ packed prompts

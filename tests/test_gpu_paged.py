@@ -330,15 +330,18 @@ def filled(be, rng, g, lengths, page, heads, dim, gain=(1.0, 1.0), extra=1):
 
 def attend_bound(q, k, v, out, size, total, t, scale):
     """How far a result may be off, from the roundings that are made.  Weights times value scales: two roundings to f16 each (f32:
-    one of the 22 bits of two f16 operands); scores: an f32 sum of 32 products of up to 79 |q| that starts at 72 times their sum, times
-    a scale; f32 accumulation over the tokens; ex2 to 2^-22; products below f16's normal range; the result's own rounding."""
+    one of the 22 bits of two f16 operands); scores: an f32 sum of 32 products (base + q) |query| less (base + 8) times the queries, which
+    is kept to 22 bits, times a scale; bases 1024, 64, 256 and 16 in turn for pairs of dims, with f32 queries all 64; f32 accumulation over
+    the tokens; ex2 to 2^-22; products below f16's normal range; the result's own rounding."""
     length = k.shape[0]
     if length == 0 or q.shape[0] == 0:
         return torch.zeros_like(out)
     heads, kv = q.shape[1], k.shape[1]
     group = heads // kv
     top = k.abs().view(length, kv, -1, 32).amax((0, 3)).repeat_interleave(group, 0) / 7      # at least the scale
-    score = scale * (q.abs().view(*q.shape[:2], -1, 32).sum(-1) * top).sum(-1, keepdim=True) * (34 * 151 * 2.0 ** -23)
+    base = torch.tensor([64.0] * 8 if t == "f32" else [1024.0] * 2 + [64.0] * 2 + [256.0] * 2 + [16.0] * 2, dtype=torch.float64, device=q.device).repeat(4)
+    off = 34 * 2.0 ** -23 * (2 * base + 23) + 2.0 ** -22 * (base + 8)
+    score = scale * ((q.abs().view(*q.shape[:2], -1, 32) * off).sum(-1) * top).sum(-1, keepdim=True)
     rel = (2.0 ** -20 if t == "f32" else 2.0 ** -10) + 2 * score + (length / 16 + 20) * 2.0 ** -23 + 2.0 ** -21
     tiny = length * 2.0 ** -22 * v.abs().max() / total
     return rel * size + tiny + plain.HALF_STEP[t] * out.abs() + 1e-30
