@@ -14,6 +14,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "kv_tile.cuh"
 #include "paged.h"
 #include "tc_common.cuh"
@@ -29,6 +31,7 @@ constexpr float kSlack = 3.0f;        // a score may pass the running maximum by
 constexpr int kMinShare = 1;          // steps a warp, below which fewer units share the work
 constexpr int kJoinSteps = 5;         // what joining the parts of units costs, in steps of a warp
 constexpr int kMostParts = 6;             // parts of a (head, row tile) up to which a team may be smaller
+constexpr int kEach = 4;              // requests a lane in the search that a warp makes alone
 constexpr int kStep = 32;             // tokens a warp takes at a time: two tiles
 
 struct AttendArgs {
@@ -45,10 +48,10 @@ struct AttendArgs {
   int* bad;
 };
 
-template <int D, int NT, bool kExact>
+template <int D, bool kExact>
 struct Shape {
-  static constexpr int kWarps = NT == 1 && !kExact ? 12 : 8;   // one CTA an SM: 168 registers a thread, or 255
-  static constexpr int kRows = 8 * NT;
+  static constexpr int kWarps = kExact ? 8 : 12;   // one CTA an SM: 255 registers a thread, or 168
+  static constexpr int kRows = 8;
   static constexpr int kStages = D == 128 ? 2 : D == 32 ? 4 : 3;
   static constexpr int kStage = 2 * Tile<D>::kBytes;
   static constexpr int kRing = kStages * kStage;
@@ -121,16 +124,19 @@ __device__ __forceinline__ float low_of(uint32_t v) { return __low2float(tc::bit
 __device__ __forceinline__ float high_of(uint32_t v) { return __high2float(tc::bits_h2(v)); }
 
 template <int N>
-__device__ __forceinline__ void lds(uint32_t (&v)[N], const uint8_t* p) {
-  if constexpr (N == 4) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-  } else if constexpr (N == 2) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    v[0] = u.x; v[1] = u.y;
-  } else {
-    v[0] = *reinterpret_cast<const uint32_t*>(p);
-  }
+__device__ __forceinline__ void lds(uint32_t (&v)[N], uint32_t at) {
+  static_assert(N == 1 || N == 2 || N == 4, "words");
+  if constexpr (N == 4)
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at));
+  else if constexpr (N == 2)
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(at));
+  else
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[0]) : "r"(at));
+}
+__device__ __forceinline__ float lds_half(uint32_t at) {
+  uint16_t v;
+  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at));
+  return __half2float(__ushort_as_half(v));
 }
 
 __device__ __forceinline__ float load_query(const AttendArgs& a, int64_t at) {
@@ -159,6 +165,28 @@ __device__ __forceinline__ void store_pair(const AttendArgs& a, int64_t at, floa
   } else {
     p[0] = (uint16_t)two;
     p[1] = (uint16_t)(two >> 16);
+  }
+}
+
+__device__ __forceinline__ void cp_async16_fill(uint32_t to, const uint8_t* from, uint32_t size) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(size) : "memory");
+}
+// Two tiles behind one another in shared memory, 16 bytes a lane and row of 512; the row where they meet comes from both, the last
+// may be short.
+template <int kBytes, int kAt>
+__device__ __forceinline__ void copy_stage(uint32_t to, const uint8_t* from0, uint32_t size0, const uint8_t* from1, uint32_t size1, int lane) {
+  if constexpr (kAt < 2 * kBytes) {
+    constexpr bool kFirst = kAt + 512 <= kBytes, kSecond = kAt >= kBytes;
+    const bool first = kFirst || (!kSecond && lane * 16 < kBytes - kAt);
+    const uint8_t* from = first ? from0 : from1;
+    const uint32_t size = first ? size0 : size1;
+    if constexpr (kFirst)
+      asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %4], 16, %2;" ::"r"(to), "l"(from0), "r"(size0), "n"(kAt), "n"(kAt) : "memory");
+    else if constexpr (kSecond && kAt + 512 <= 2 * kBytes)
+      asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %4], 16, %2;" ::"r"(to), "l"(from1), "r"(size1), "n"(kAt), "n"(kAt - kBytes) : "memory");
+    else if (kAt + lane * 16 < 2 * kBytes)
+      cp_async16_fill(to + kAt, from + (first ? kAt : kAt - kBytes), size);
+    copy_stage<kBytes, kAt + 512>(to, from0, size0, from1, size1, lane);
   }
 }
 
@@ -194,10 +222,10 @@ __device__ __forceinline__ void team_barrier(int team, int threads) {
 }
 
 // kExact: f32 queries and results; the queries and the weights then go in as two f16 operands each
-template <int D, int NT, bool kExact>
-__global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_attend_kernel(const __grid_constant__ AttendArgs a) {
+template <int D, bool kExact>
+__global__ void __launch_bounds__(32 * Shape<D, kExact>::kWarps, 1) kv_attend_kernel(const __grid_constant__ AttendArgs a) {
   using T = Tile<D>;
-  using S = Shape<D, NT, kExact>;
+  using S = Shape<D, kExact>;
   constexpr int kWarps = S::kWarps, kThreads = 32 * kWarps;
   constexpr int J = T::kGroups, kRows = S::kRows, kStages = S::kStages, kParts = kExact ? 2 : 1;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -245,12 +273,25 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
   };
   constexpr i64 kMostSteps = 0x3fffffff;   // over a terabyte of cache
   int team, member, unit, b_start, b_begin, lo, hi;
-  if (a.requests <= 32) {
-    // every warp for itself
-    Request r{};
-    if (lane < a.requests) r = request_at<kRows>(a, lane, &wrong);
-    i64 steps = (i64)r.sides * r.steps;
-    int pairs = r.sides, most = r.sides ? r.steps : 0;
+  if (a.requests <= 32 * kEach) {
+    // every warp for itself, a few requests a lane
+    Request each[kEach];
+    i64 steps = 0;
+    int pairs = 0, most = 0;
+    const int per = (a.requests + 31) >> 5;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      each[i] = Request{};
+      if (i < per && lane * per + i < a.requests) each[i] = request_at<kRows>(a, lane * per + i, &wrong);
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      steps += (i64)each[i].sides * each[i].steps;
+      pairs += each[i].sides;
+      if (each[i].sides) most = max(most, each[i].steps);
+    }
+    const int my_pairs = pairs;
+    const i64 my_steps = steps;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const i64 s = __shfl_up_sync(kAll, steps, o);
@@ -269,10 +310,27 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
     team = warp / team_warps;
     unit = team * grid + blockIdx.x;
     if (unit >= units) return;
-    const int upto = split ? (int)steps : pairs, from = split ? start_of(unit) : unit;
-    b_start = __ffs(__ballot_sync(kAll, upto > from)) - 1;
-    b_begin = __shfl_sync(kAll, (int)steps - r.sides * r.steps, b_start);
-    const int first_pair = __shfl_sync(kAll, pairs - r.sides, b_start), long_pair = __shfl_sync(kAll, r.steps, b_start);
+    const int from = split ? start_of(unit) : unit;
+    const int owner = __ffs(__ballot_sync(kAll, (split ? (int)steps : pairs) > from)) - 1;
+    // in the owner's few
+    int at = (int)(steps - my_steps), first_pair = pairs - my_pairs, long_pair = 0, i = 0;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int n = each[k].sides * each[k].steps;
+      if (i == k) {
+        if (split ? at + n <= from : first_pair + each[k].sides <= from) {
+          at += n;
+          first_pair += each[k].sides;
+          ++i;
+        } else {
+          long_pair = each[k].steps;
+        }
+      }
+    }
+    b_start = __shfl_sync(kAll, lane * per + i, owner);
+    b_begin = __shfl_sync(kAll, at, owner);
+    first_pair = __shfl_sync(kAll, first_pair, owner);
+    long_pair = __shfl_sync(kAll, long_pair, owner);
     lo = split ? from : b_begin + (unit - first_pair) * long_pair;
     hi = split ? start_of(unit + 1) : lo + long_pair;
   } else {
@@ -366,14 +424,13 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
 
   // ---- copies: lane l of a batch of 32 finds the l-th step of the warp from there, one batch ahead, so that nobody waits for
   // the table
-  constexpr uint32_t kNone = 0xffffffffu;
   const int page_tiles = a.page_tokens >> 4;
   int walk_b = b_start, walk_at = b_begin;    // a request at or before the batch's first step, where it begins
-  uint32_t ahead[2] = {kNone, kNone}, now[2] = {kNone, kNone};   // tiles of this lane's step, counted through the cache
+  uint32_t ahead[2] = {0, 0}, now[2] = {0, 0};   // tiles of this lane's step, counted through the cache, twice and 1; 0: none
   auto find_batch = [&](int k0) {
     const int x = lo + member + (k0 + lane) * team_warps;
     const bool mine_too = k0 + lane < mine_steps;
-    ahead[0] = ahead[1] = kNone;
+    ahead[0] = ahead[1] = 0;
     if (mine_too) {
       bool skip = false;
       int b = walk_b, begin = walk_at;
@@ -390,7 +447,7 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
         if (tile * 16 < r.length) {
           const int page = a.table[b * a.table_stride + (tile * 16 >> a.page_shift)];
           if (page < 0 || page >= a.pages) *a.bad = 1;
-          else ahead[h] = (uint32_t)(page * a.kv_heads + head) * page_tiles + (tile & (page_tiles - 1));
+          else ahead[h] = ((uint32_t)(page * a.kv_heads + head) * page_tiles + (tile & (page_tiles - 1))) << 1 | 1;
         }
       }
       walk_b = b;
@@ -403,30 +460,26 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
     walk_at = __shfl_sync(kAll, walk_at, from);
   };
   // 16 bytes a lane; a tile that is not there is filled with zeros
+  const uint8_t* from_lane = a.data + lane * 16;
   auto issue = [&](int k, int s) {
     if (k < mine_steps) {
       if ((k & 31) == 0) {
         now[0] = ahead[0];
         now[1] = ahead[1];
-        if (k + 32 < mine_steps) find_batch(k + 32);
       }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t tile = __shfl_sync(kAll, now[h], k & 31);
-        const uint32_t bytes = tile == kNone ? 0 : 16;
-        const uint8_t* from = a.data + (int64_t)(tile == kNone ? 0 : tile) * T::kBytes + lane * 16;
-        const uint32_t to = ring_at + s * S::kStage + h * T::kBytes;
-#pragma unroll
-        for (int c = 0; c < (T::kBytes + 511) / 512; ++c)
-          if (T::kBytes >= 512 * (c + 1) || lane * 16 < T::kBytes - 512 * c)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 512 * c), "l"(from + 512 * c), "r"(bytes) : "memory");
-      }
+      const uint32_t t0 = __shfl_sync(kAll, now[0], k & 31), t1 = __shfl_sync(kAll, now[1], k & 31);
+      const uint32_t to = ring_at + s * S::kStage;
+      copy_stage<T::kBytes, 0>(to, from_lane + (uint64_t)(t0 >> 1) * T::kBytes, (t0 & 1) << 4, from_lane + (uint64_t)(t1 >> 1) * T::kBytes, (t1 & 1) << 4, lane);
+      // the next batch's places, while there is time
+      if ((k & 31) == kStages && k + 32 - kStages < mine_steps) find_batch(k + 32 - kStages);
     }
     cp_async_commit();
   };
   int taken = 0, stage = 0;             // steps done, the stage of the next
   find_batch(0);
   for (int k = 0; k < kStages; ++k) issue(k, k);
+  // lanes past the last group, or past the values' scales, look at another's (times 0, or once more)
+  const int lane_v = lane % (8 * J), own_scale = (g * J + t % J) * 2;
   const Bases bases{tc::in_register(0x64006400u), tc::in_register(0x54005400u), tc::in_register(0x5c005c00u), tc::in_register(0x4c004c00u)};
   constexpr uint32_t above[4] = {0xe408e408u, 0xd480d480u, 0xdc20dc20u, 0xce00ce00u};   // -1032, -72, -264, -24
 
@@ -447,83 +500,78 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
     const int piece_end = min(hi, x - step0 + r.steps);
 
     // queries: this lane's row g of each tile of 8, dims 8t .. 8t+7 of each group
-    uint32_t qf[kParts][NT][J][4];
-    uint32_t off[NT][2];                                          // of group t and row g, as two tf32
-    int see[NT][2];
-    float m[NT][2], cap[NT][2], l[NT][2], o[NT][D / 16][4];
+    uint32_t qf[kParts][J][4];
+    uint32_t off[2];                                          // of group t and row g, as two tf32
+    int see[2];
+    float m[2], cap[2], l[2], o[D / 16][4];
+    const int row = row0 + g;
+    const bool live = row < all_rows;
+    const int i = live ? row / a.group : 0;
+    const int64_t from = (int64_t)(r.first + i) * a.qs + (int64_t)(head * a.group + (live ? row - i * a.group : 0)) * a.qh;
+    off[0] = off[1] = 0;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int row = row0 + nt * 8 + g;
-      const bool live = row < all_rows;
-      const int i = live ? row / a.group : 0;
-      const int64_t from = (int64_t)(r.first + i) * a.qs + (int64_t)(head * a.group + (live ? row - i * a.group : 0)) * a.qh;
-      off[nt][0] = off[nt][1] = 0;
+    for (int j = 0; j < J; ++j) {
+      float v[8];
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        float v[8];
+      for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+      if (live) {
+        const int64_t at8 = from + 32 * j + 8 * t;
+        if (a.q_vec && !kExact) {
+          const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at8);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-        if (live) {
-          const int64_t at8 = from + 32 * j + 8 * t;
-          if (a.q_vec && !kExact) {
-            const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at8);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (a.type == EMELB_F16) {
-                v[2 * e] = low_of(w[e]);
-                v[2 * e + 1] = high_of(w[e]);
-              } else {
-                v[2 * e] = __uint_as_float(w[e] << 16);
-                v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-              }
+          for (int e = 0; e < 4; ++e) {
+            if (a.type == EMELB_F16) {
+              v[2 * e] = low_of(w[e]);
+              v[2 * e + 1] = high_of(w[e]);
+            } else {
+              v[2 * e] = __uint_as_float(w[e] << 16);
+              v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
             }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = load_query(a, at8 + e);
           }
-        }
-        float sum = 0.0f;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t hi2 = half2_of(v[2 * e], v[2 * e + 1]);
-          qf[0][nt][j][e] = hi2;
-          float two = low_of(hi2) + high_of(hi2);
-          if constexpr (kExact) {
-            const uint32_t lo2 = half2_of(v[2 * e] - low_of(hi2), v[2 * e + 1] - high_of(hi2));
-            qf[1][nt][j][e] = lo2;
-            two += low_of(lo2) + high_of(lo2);
-          }
-          sum = fmaf(kExact ? -72.0f : -above_of(e), two, sum);
-        }
-        sum += __shfl_xor_sync(kAll, sum, 1);
-        sum += __shfl_xor_sync(kAll, sum, 2);
-        if (t == j) {
-          off[nt][0] = tf32_of(sum);
-          off[nt][1] = tf32_of(sum - __uint_as_float(off[nt][0]));
+          for (int e = 0; e < 8; ++e) v[e] = load_query(a, at8 + e);
         }
       }
+      float sum = 0.0f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int rr = row0 + nt * 8 + 2 * t + h;
-        see[nt][h] = r.length - r.rows + min(rr, all_rows - 1) / a.group + 1;
-        m[nt][h] = cap[nt][h] = kLowest;
-        l[nt][h] = 0.0f;
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t hi2 = half2_of(v[2 * e], v[2 * e + 1]);
+        qf[0][j][e] = hi2;
+        float two = low_of(hi2) + high_of(hi2);
+        if constexpr (kExact) {
+          const uint32_t lo2 = half2_of(v[2 * e] - low_of(hi2), v[2 * e + 1] - high_of(hi2));
+          qf[1][j][e] = lo2;
+          two += low_of(lo2) + high_of(lo2);
+        }
+        sum = fmaf(kExact ? -72.0f : -above_of(e), two, sum);
       }
-#pragma unroll
-      for (int i16 = 0; i16 < D / 16; ++i16)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[nt][i16][e] = 0.0f;
+      sum += __shfl_xor_sync(kAll, sum, 1);
+      sum += __shfl_xor_sync(kAll, sum, 2);
+      if (t == j) {
+        off[0] = tf32_of(sum);
+        off[1] = tf32_of(sum - __uint_as_float(off[0]));
+      }
     }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int rr = min(row0 + 2 * t + h, all_rows - 1);
+      see[h] = r.length - r.rows + rr / a.group + 1;
+      m[h] = cap[h] = kLowest;
+      l[h] = 0.0f;
+    }
+#pragma unroll
+    for (int i16 = 0; i16 < D / 16; ++i16)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i16][e] = 0.0f;
     const int all_see = r.length - r.rows + row0 / a.group + 1;   // the first row's
     // A weight times a value's scale is rounded to f16, whose range is small: weights are taken times 2^-scale_exp, the running
     // exponent of the largest scale, as part of the running maximum m.  cap: the score that moves m; scale_cap: the scale that
     // moves scale_exp.  Neither happens often.
     int scale_exp = -11;
     uint32_t scale_cap = 0x14001400u;                             // 2^-10
-    float neg_m[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) neg_m[nt][0] = neg_m[nt][1] = -kLowest;
+    float neg_m[2] = {-kLowest, -kLowest};
 
     for (; taken < mine_steps; ++taken) {
       const int pos = lo + member + taken * team_warps;
@@ -531,16 +579,20 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
       cp_async_wait<kStages - 1>();
       __syncwarp();
       const int token0 = (step0 + pos - x) * kStep;
-      const uint8_t* tiles = ring + stage * S::kStage;
+      const uint32_t tiles = tc::smem_u32(ring) + stage * S::kStage;
+      const uint32_t at_k = tiles + lane * T::kVecK * 4, at_v = tiles + lane * T::kVecV * 4, at_scale = tiles + g * J * 2, at_own = tiles + own_scale,
+                     at_word = tiles + lane_v * 4, at_dv = tiles + t * J * 8;
       const bool whole = token0 + kStep <= all_see;
 
       // scores: rows are tokens token0 + 16 u + g and + 8, columns the query rows
-      float score[2][NT][4];
+      float score[2][4];
       uint32_t word[2];                   // this lane's share of the values' scales
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const uint8_t* tile = tiles + u * T::kBytes;
-        word[u] = lane < 8 * J ? *reinterpret_cast<const uint32_t*>(tile + T::kScaleV + lane * 4) & 0x7fff7fffu : 0u;
+        const int tile = u * T::kBytes;
+        uint32_t one[1];
+        lds(one, at_word + tile + T::kScaleV);
+        word[u] = one[0] & 0x7fff7fffu;
         uint32_t kw[2][J];
         float dk[2][J];
 #pragma unroll
@@ -548,11 +600,11 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
 #pragma unroll
           for (int jv = 0; jv < J / T::kVecK; ++jv) {
             uint32_t w[T::kVecK];
-            lds(w, tile + ((h * (J / T::kVecK) + jv) * 32 + lane) * T::kVecK * 4);
+            lds(w, at_k + tile + (h * (J / T::kVecK) + jv) * 32 * T::kVecK * 4);
 #pragma unroll
             for (int e = 0; e < T::kVecK; ++e) kw[h][jv * T::kVecK + e] = w[e];
           }
-          const uint8_t* sc = tile + T::key_scale(8 * h, 0) + g * J * 2;
+          const uint32_t sc = at_scale + tile + T::key_scale(8 * h, 0);
           if constexpr (J % 2 == 0) {
             uint32_t w[J / 2];
             lds(w, sc);
@@ -563,15 +615,12 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
             }
           } else {
 #pragma unroll
-            for (int j = 0; j < J; ++j) dk[h][j] = __half2float(*reinterpret_cast<const __half*>(sc + 2 * j));
+            for (int j = 0; j < J; ++j) dk[h][j] = lds_half(sc + 2 * j);
           }
         }
         // the scales times what the operands are above q - 8, of all groups at once (k is the groups, twice), then group by group
-        const uint8_t* own = tile + T::key_scale(0, 0) + (g * J + (t < J ? t : 0)) * 2;
-        const float d0 = t < J ? __half2float(*reinterpret_cast<const __half*>(own)) : 0.0f;
-        const float d1 = t < J ? __half2float(*reinterpret_cast<const __half*>(own + 8 * J * 2)) : 0.0f;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_tf32(score[u][nt], __float_as_uint(d0), __float_as_uint(d1), off[nt][0], off[nt][1]);
+        const float d0 = lds_half(at_own + tile + T::key_scale(0, 0)), d1 = lds_half(at_own + tile + T::key_scale(8, 0));
+        mma_tf32(score[u], __float_as_uint(d0), __float_as_uint(d1), off[0], off[1]);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           uint32_t p0[4], p1[4];
@@ -583,18 +632,15 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
             spread(kw[1][j], bases, p1);
           }
           const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float c[4];
-            mma_first(c, a0, qf[0][nt][j][0], qf[0][nt][j][1]);
-            mma(c, a1, qf[0][nt][j][2], qf[0][nt][j][3]);
-            if constexpr (kExact) {
-              mma(c, a0, qf[kParts - 1][nt][j][0], qf[kParts - 1][nt][j][1]);
-              mma(c, a1, qf[kParts - 1][nt][j][2], qf[kParts - 1][nt][j][3]);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) score[u][nt][e] = fmaf(dk[e >> 1][j], c[e], score[u][nt][e]);
+          float c[4];
+          mma_first(c, a0, qf[0][j][0], qf[0][j][1]);
+          mma(c, a1, qf[0][j][2], qf[0][j][3]);
+          if constexpr (kExact) {
+            mma(c, a0, qf[kParts - 1][j][0], qf[kParts - 1][j][1]);
+            mma(c, a1, qf[kParts - 1][j][2], qf[kParts - 1][j][3]);
           }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) score[u][e] = fmaf(dk[e >> 1][j], c[e], score[u][e]);
         }
       }
       if (!whole) {
@@ -603,11 +649,9 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
         for (int u = 0; u < 2; ++u) {
           const int t0 = token0 + 16 * u;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (t0 + g + (e >> 1) * 8 >= see[nt][e & 1]) score[u][nt][e] = -INFINITY;
-          const int tok = t0 + lane / (2 * J) * 2 + (lane & 1) * 8;
+          for (int e = 0; e < 4; ++e)
+            if (t0 + g + (e >> 1) * 8 >= see[e & 1]) score[u][e] = -INFINITY;
+          const int tok = t0 + lane_v / (2 * J) * 2 + (lane_v & 1) * 8;
           if (tok >= r.length) word[u] = 0;
           else if (tok + 1 >= r.length) word[u] &= 0xffffu;
         }
@@ -615,63 +659,56 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
       // a half of `word` that reaches scale_cap keeps the bit above it
       bool moves = ((((word[0] | 0x80008000u) - scale_cap) | ((word[1] | 0x80008000u) - scale_cap)) & 0x80008000u) != 0;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          moves |= fmaxf(fmaxf(score[0][nt][h], score[0][nt][h + 2]), fmaxf(score[1][nt][h], score[1][nt][h + 2])) > cap[nt][h];
+      for (int h = 0; h < 2; ++h)
+        moves |= fmaxf(fmaxf(score[0][h], score[0][h + 2]), fmaxf(score[1][h], score[1][h + 2])) > cap[h];
       if (__any_sync(kAll, moves)) {
         int big = (int)max(max(word[0] & 0xffffu, word[0] >> 16), max(word[1] & 0xffffu, word[1] >> 16)) >> 10;
         big = min(4, __reduce_max_sync(kAll, big) - 15);
         const int e_new = max(scale_exp, big);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int h = 0; h < 2; ++h) {
+          float top = fmaxf(fmaxf(score[0][h], score[0][h + 2]), fmaxf(score[1][h], score[1][h + 2])) * a.scale_log2;
+          top = fmaxf(top, __shfl_xor_sync(kAll, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(kAll, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(kAll, top, 16));
+          top = fmaxf(top, m[h]);
+          const float f = exp2_fast((m[h] - top) + (float)(scale_exp - e_new));
+          m[h] = top;
+          cap[h] = (top + kSlack) / a.scale_log2;
+          neg_m[h] = -(top + (float)e_new);
+          l[h] *= f;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float top = fmaxf(fmaxf(score[0][nt][h], score[0][nt][h + 2]), fmaxf(score[1][nt][h], score[1][nt][h + 2])) * a.scale_log2;
-            top = fmaxf(top, __shfl_xor_sync(kAll, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(kAll, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(kAll, top, 16));
-            top = fmaxf(top, m[nt][h]);
-            const float f = exp2_fast((m[nt][h] - top) + (float)(scale_exp - e_new));
-            m[nt][h] = top;
-            cap[nt][h] = (top + kSlack) / a.scale_log2;
-            neg_m[nt][h] = -(top + (float)e_new);
-            l[nt][h] *= f;
-#pragma unroll
-            for (int i16 = 0; i16 < D / 16; ++i16) {
-              o[nt][i16][h] *= f;
-              o[nt][i16][h + 2] *= f;
-            }
+          for (int i16 = 0; i16 < D / 16; ++i16) {
+            o[i16][h] *= f;
+            o[i16][h + 2] *= f;
           }
+        }
         scale_exp = e_new;
         scale_cap = e_new == 4 ? 0x7c007c00u : (uint32_t)(e_new + 16) * 0x04000400u;
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) score[u][nt][e] = exp2_fast(fmaf(score[u][nt][e], a.scale_log2, neg_m[nt][e & 1]));
-          l[nt][0] += score[u][nt][0] + score[u][nt][2];
-          l[nt][1] += score[u][nt][1] + score[u][nt][3];
-        }
+        for (int e = 0; e < 4; ++e) score[u][e] = exp2_fast(fmaf(score[u][e], a.scale_log2, neg_m[e & 1]));
+        l[0] += score[u][0] + score[u][2];
+        l[1] += score[u][1] + score[u][3];
+      }
       constexpr int kVV = T::kVecV;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const uint8_t* tile = tiles + u * T::kBytes;
-        const int t0 = token0 + 16 * u;
+        const int tile = u * T::kBytes, t0 = token0 + 16 * u;
         // scales of this lane's four tokens, and the weights as operands
-        uint32_t dv[J][2], pf[NT][2];
+        uint32_t dv[J][2], pf[2];
         if constexpr (J % 2 == 0) {
 #pragma unroll
           for (int j = 0; j < J; j += 2) {
             uint32_t w[4];
-            lds(w, tile + T::kScaleV + (t * J + j) * 8);
+            lds(w, at_dv + tile + T::kScaleV + j * 8);
             dv[j][0] = w[0]; dv[j][1] = w[1]; dv[j + 1][0] = w[2]; dv[j + 1][1] = w[3];
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < J; ++j) lds(dv[j], tile + T::kScaleV + (t * J + j) * 8);
+          for (int j = 0; j < J; ++j) lds(dv[j], at_dv + tile + T::kScaleV + j * 8);
         }
         if (!whole) {
 #pragma unroll
@@ -684,47 +721,39 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
             }
         }
         if constexpr (!kExact) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            pf[nt][0] = turn8x8(half2_of(score[u][nt][0], score[u][nt][1]));
-            pf[nt][1] = turn8x8(half2_of(score[u][nt][2], score[u][nt][3]));
-          }
+          pf[0] = turn8x8(half2_of(score[u][0], score[u][1]));
+          pf[1] = turn8x8(half2_of(score[u][2], score[u][3]));
         }
         uint32_t vw[kVV];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-          uint32_t bf[kParts][NT][2];
+          uint32_t bf[kParts][2];
+          if constexpr (!kExact) {
+            bf[0][0] = tc::h2_bits(__hmul2(tc::bits_h2(pf[0]), tc::bits_h2(dv[j][0])));
+            bf[0][1] = tc::h2_bits(__hmul2(tc::bits_h2(pf[1]), tc::bits_h2(dv[j][1])));
+          } else {
+            // in f32, tokens g and g + 8 a lane, then as two f16
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if constexpr (!kExact) {
-              bf[0][nt][0] = tc::h2_bits(__hmul2(tc::bits_h2(pf[nt][0]), tc::bits_h2(dv[j][0])));
-              bf[0][nt][1] = tc::h2_bits(__hmul2(tc::bits_h2(pf[nt][1]), tc::bits_h2(dv[j][1])));
-            } else {
-              // in f32, tokens g and g + 8 a lane, then as two f16
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float d = __half2float(*reinterpret_cast<const __half*>(tile + T::kScaleV + ((g >> 1) * J + j) * 8 + (g & 1) * 2 + 4 * h));
-                if (t0 + g + 8 * h >= r.length) d = 0.0f;
-                const float p0 = score[u][nt][2 * h] * d, p1 = score[u][nt][2 * h + 1] * d;
-                const uint32_t hi2 = half2_of(p0, p1);
-                bf[0][nt][h] = turn8x8(hi2);
-                bf[kParts - 1][nt][h] = turn8x8(half2_of(p0 - low_of(hi2), p1 - high_of(hi2)));
-              }
+            for (int h = 0; h < 2; ++h) {
+              float d = lds_half(tiles + tile + T::kScaleV + ((g >> 1) * J + j) * 8 + (g & 1) * 2 + 4 * h);
+              if (t0 + g + 8 * h >= r.length) d = 0.0f;
+              const float p0 = score[u][2 * h] * d, p1 = score[u][2 * h + 1] * d;
+              const uint32_t hi2 = half2_of(p0, p1);
+              bf[0][h] = turn8x8(hi2);
+              bf[kParts - 1][h] = turn8x8(half2_of(p0 - low_of(hi2), p1 - high_of(hi2)));
             }
           }
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int i16 = 2 * j + half;
-            if (i16 % kVV == 0) lds(vw, tile + T::kV + (i16 / kVV * 32 + lane) * kVV * 4);
+            if (i16 % kVV == 0) lds(vw, at_v + tile + T::kV + i16 / kVV * 32 * kVV * 4);
             uint32_t av[4];
             spread(vw[i16 % kVV], bases, av);
             // centred before the product, exactly: a sum over the tokens would not survive the difference
 #pragma unroll
             for (int e = 0; e < 4; ++e) av[e] = tc::h2_bits(__hadd2(tc::bits_h2(av[e]), tc::bits_h2(above[e])));
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int part = 0; part < kParts; ++part) mma(o[nt][i16], av, bf[part][nt][0], bf[part][nt][1]);
+            for (int part = 0; part < kParts; ++part) mma(o[i16], av, bf[part][0], bf[part][1]);
           }
         }
       }
@@ -736,52 +765,45 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
     // ---- the piece's results.  A cell is what a lane holds of 16 dims: rows 2t and 2t + 1, dims 16 i + 2g and the next.  Cells stay in
     // this order all the way: through shared memory, through scratch, until the last sum is made
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int h = 0; h < 2; ++h) {
+      m[h] += (float)scale_exp;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        m[nt][h] += (float)scale_exp;
-#pragma unroll
-        for (int s = 4; s < 32; s <<= 1) l[nt][h] += __shfl_xor_sync(kAll, l[nt][h], s);
-      }
+      for (int s = 4; s < 32; s <<= 1) l[h] += __shfl_xor_sync(kAll, l[h], s);
+    }
     const int w0 = team * team_warps, ttid = tid - w0 * 32;
     if (team_warps > 1) {
-      if (g == 0)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<float2*>(&join_m[warp][nt * 8 + 2 * t]) = make_float2(m[nt][0], m[nt][1]);
+      if (g == 0) *reinterpret_cast<float2*>(&join_m[warp][2 * t]) = make_float2(m[0], m[1]);
       team_barrier(team, team_threads);
-      float f[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float2 top = make_float2(kLowest, kLowest);
-        for (int w = 0; w < team_warps; ++w) {
-          const float2 o_m = *reinterpret_cast<const float2*>(&join_m[w0 + w][nt * 8 + 2 * t]);
-          top.x = fmaxf(top.x, o_m.x);
-          top.y = fmaxf(top.y, o_m.y);
-        }
-        f[nt][0] = exp2_fast(m[nt][0] - top.x);
-        f[nt][1] = exp2_fast(m[nt][1] - top.y);
-        m[nt][0] = top.x;
-        m[nt][1] = top.y;
-        if (g == 0) *reinterpret_cast<float2*>(&join_l[warp][nt * 8 + 2 * t]) = make_float2(l[nt][0] * f[nt][0], l[nt][1] * f[nt][1]);
-#pragma unroll
-        for (int i16 = 0; i16 < D / 16; ++i16)
-          joint[(warp * kCells) + (nt * (D / 16) + i16) * 32 + lane] =
-              make_float4(o[nt][i16][0] * f[nt][0], o[nt][i16][1] * f[nt][1], o[nt][i16][2] * f[nt][0], o[nt][i16][3] * f[nt][1]);
+      float f[2];
+      float2 top = make_float2(kLowest, kLowest);
+#pragma unroll 4
+      for (int w = 0; w < team_warps; ++w) {
+        const float2 o_m = *reinterpret_cast<const float2*>(&join_m[w0 + w][2 * t]);
+        top.x = fmaxf(top.x, o_m.x);
+        top.y = fmaxf(top.y, o_m.y);
       }
-      team_barrier(team, team_threads);
+      f[0] = exp2_fast(m[0] - top.x);
+      f[1] = exp2_fast(m[1] - top.y);
+      m[0] = top.x;
+      m[1] = top.y;
+      if (g == 0) *reinterpret_cast<float2*>(&join_l[warp][2 * t]) = make_float2(l[0] * f[0], l[1] * f[1]);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        l[nt][0] = l[nt][1] = 0.0f;
-        for (int w = 0; w < team_warps; ++w) {
-          const float2 o_l = *reinterpret_cast<const float2*>(&join_l[w0 + w][nt * 8 + 2 * t]);
-          l[nt][0] += o_l.x;
-          l[nt][1] += o_l.y;
-        }
+      for (int i16 = 0; i16 < D / 16; ++i16)
+        joint[warp * kCells + i16 * 32 + lane] =
+            make_float4(o[i16][0] * f[0], o[i16][1] * f[1], o[i16][2] * f[0], o[i16][3] * f[1]);
+      team_barrier(team, team_threads);
+      l[0] = l[1] = 0.0f;
+#pragma unroll 4
+      for (int w = 0; w < team_warps; ++w) {
+        const float2 o_l = *reinterpret_cast<const float2*>(&join_l[w0 + w][2 * t]);
+        l[0] += o_l.x;
+        l[1] += o_l.y;
       }
     }
-    auto cell_of = [&](int c, int nt, int i16) {
-      if (team_warps == 1) return make_float4(o[nt][i16][0], o[nt][i16][1], o[nt][i16][2], o[nt][i16][3]);
+    auto cell_of = [&](int c, int i16) {
+      if (team_warps == 1) return make_float4(o[i16][0], o[i16][1], o[i16][2], o[i16][3]);
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
       for (int w = 0; w < team_warps; ++w) {
         const float4 u = joint[(w0 + w) * kCells + c];
         v.x += u.x;
@@ -791,18 +813,18 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
       }
       return v;
     };
-    // rows 2t and 2t + 1 of row tile nt, where they are any
-    auto put = [&](int nt, int i16, const float4& v, float s0, float s1) {
+    // rows 2t and 2t + 1 where they are any
+    int64_t to[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int rr = row0 + nt * 8 + 2 * t + h;
-        if (rr >= all_rows) continue;
-        const int i = rr / a.group;
-        const float sum = h ? s1 : s0, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        store_pair(a, (int64_t)(r.first + i) * a.os + (int64_t)(head * a.group + rr - i * a.group) * a.oh + i16 * 16 + 2 * g, (h ? v.y : v.x) * inv,
-                   (h ? v.w : v.z) * inv);
-      }
+    for (int h = 0; h < 2; ++h) {
+      const int rr = row0 + 2 * t + h, i = see[h] - 1 - (r.length - r.rows);
+      to[h] = rr < all_rows ? (int64_t)(r.first + i) * a.os + (int64_t)(head * a.group + rr - i * a.group) * a.oh + 2 * g : -1;
+    }
+    auto put = [&](int i16, const float4& v, float inv0, float inv1) {
+      if (to[0] >= 0) store_pair(a, to[0] + i16 * 16, v.x * inv0, v.z * inv0);
+      if (to[1] >= 0) store_pair(a, to[1] + i16 * 16, v.y * inv1, v.w * inv1);
     };
+    auto inverse = [](float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; };
     const bool all_of_it = step0 == 0 && piece_end == x + r.steps;
     const int seg = x - step0, u0 = all_of_it ? unit : unit_of(seg), u1 = all_of_it ? unit : unit_of(seg + r.steps - 1);
     auto part_of = [&](int u) { return 2 * (i64)u + (u == u0 ? 1 : 0); };
@@ -813,16 +835,13 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
       const bool others = turn != member;
       turn = turn + 1 == team_warps ? 0 : turn + 1;
       if (others) continue;
-      const int nt = k / (D / 16), i16 = k % (D / 16), c = k * 32 + lane;
-      const float4 v = cell_of(c, nt, i16);
-      if (all_of_it) put(nt, i16, v, l[nt][0], l[nt][1]);
+      const int c = k * 32 + lane;
+      const float4 v = cell_of(c, k);
+      if (all_of_it) put(k, v, inverse(l[0]), inverse(l[1]));
       else __stcg(acc + part_of(unit) * kCells + c, v);
     }
     if (!all_of_it) {
-      if (member == 0 && g == 0)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          __stcg(stats + part_of(unit) * (kRows / 2) + nt * 4 + t, make_float4(m[nt][0], l[nt][0], m[nt][1], l[nt][1]));
+      if (member == 0 && g == 0) __stcg(stats + part_of(unit) * (kRows / 2) + t, make_float4(m[0], l[0], m[1], l[1]));
       // the last unit of the (request, head) to arrive joins all parts, in their order
       team_barrier(team, team_threads);
       if (ttid == 0) {
@@ -834,46 +853,41 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
       }
       team_barrier(team, team_threads);
       if (last_in[team]) {
-        float2 top[NT], sum[NT];
+        // this warp's cells, so many at once and of so many parts that about 16 loads are on their way
+        auto join = [&](auto cells, auto parts) {
+          constexpr int kAtOnce = decltype(cells)::value, kUnroll = decltype(parts)::value;
+          float2 top = make_float2(kLowest, kLowest), sum = make_float2(0.0f, 0.0f);
+          float4 v[kAtOnce];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          top[nt] = make_float2(kLowest, kLowest);
-          sum[nt] = make_float2(0.0f, 0.0f);
-#pragma unroll 4
+          for (int q = 0; q < kAtOnce; ++q) v[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll kUnroll
           for (int u = u0; u <= u1; ++u) {
-            const float4 ml = __ldcg(stats + part_of(u) * (kRows / 2) + nt * 4 + t);
-            const float2 next = make_float2(fmaxf(top[nt].x, ml.x), fmaxf(top[nt].y, ml.z));
-            sum[nt].x = sum[nt].x * exp2_fast(top[nt].x - next.x) + ml.y * exp2_fast(ml.x - next.x);
-            sum[nt].y = sum[nt].y * exp2_fast(top[nt].y - next.y) + ml.w * exp2_fast(ml.z - next.y);
-            top[nt] = next;
-          }
-        }
-        constexpr int kAtOnce = D / 16 < 4 ? D / 16 : 4;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          for (int first = member; first < D / 16; first += kAtOnce * team_warps) {
-            float4 v[kAtOnce];
-#pragma unroll
-            for (int q = 0; q < kAtOnce; ++q) v[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 2
-            for (int u = u0; u <= u1; ++u) {
-              const float4 ml = __ldcg(stats + part_of(u) * (kRows / 2) + nt * 4 + t);
-              const float f0 = exp2_fast(ml.x - top[nt].x), f1 = exp2_fast(ml.z - top[nt].y);
-#pragma unroll
-              for (int q = 0; q < kAtOnce; ++q) {
-                const int i16 = first + q * team_warps;
-                if (i16 >= D / 16) continue;
-                const float4 p = __ldcg(acc + part_of(u) * kCells + (nt * (D / 16) + i16) * 32 + lane);
-                v[q].x = fmaf(p.x, f0, v[q].x);
-                v[q].y = fmaf(p.y, f1, v[q].y);
-                v[q].z = fmaf(p.z, f0, v[q].z);
-                v[q].w = fmaf(p.w, f1, v[q].w);
-              }
-            }
+            const float4 ml = __ldcg(stats + part_of(u) * (kRows / 2) + t);
+            float4 p[kAtOnce];
 #pragma unroll
             for (int q = 0; q < kAtOnce; ++q)
-              if (first + q * team_warps < D / 16) put(nt, first + q * team_warps, v[q], sum[nt].x, sum[nt].y);
+              if (member + q * team_warps < D / 16) p[q] = __ldcg(acc + part_of(u) * kCells + (member + q * team_warps) * 32 + lane);
+            const float2 next = make_float2(fmaxf(top.x, ml.x), fmaxf(top.y, ml.z));
+            const float k0 = exp2_fast(top.x - next.x), k1 = exp2_fast(top.y - next.y), f0 = exp2_fast(ml.x - next.x), f1 = exp2_fast(ml.z - next.y);
+            sum.x = sum.x * k0 + ml.y * f0;
+            sum.y = sum.y * k1 + ml.w * f1;
+            top = next;
+#pragma unroll
+            for (int q = 0; q < kAtOnce; ++q)
+              if (member + q * team_warps < D / 16) {
+                v[q].x = fmaf(v[q].x, k0, p[q].x * f0);
+                v[q].y = fmaf(v[q].y, k1, p[q].y * f1);
+                v[q].z = fmaf(v[q].z, k0, p[q].z * f0);
+                v[q].w = fmaf(v[q].w, k1, p[q].w * f1);
+              }
           }
+          sum = make_float2(inverse(sum.x), inverse(sum.y));
+#pragma unroll
+          for (int q = 0; q < kAtOnce; ++q)
+            if (member + q * team_warps < D / 16) put(member + q * team_warps, v[q], sum.x, sum.y);
+        };
+        if (team_warps * 2 < D / 16) join(std::integral_constant<int, D / 16>{}, std::integral_constant<int, 2>{});
+        else if (member < D / 16) join(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{});
       }
     }
     team_barrier(team, team_threads);
@@ -881,25 +895,24 @@ __global__ void __launch_bounds__(32 * Shape<D, NT, kExact>::kWarps, 1) kv_atten
   }
 }
 
-template <int D, int NT, bool kExact>
+template <int D, bool kExact>
 cudaError_t launch_one(const AttendArgs& a, int sm_count, cudaStream_t st) {
-  using S = Shape<D, NT, kExact>;
+  using S = Shape<D, kExact>;
   const int smem = S::kSmem;
-  cudaError_t e = cudaFuncSetAttribute(kv_attend_kernel<D, NT, kExact>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(kv_attend_kernel<D, kExact>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kv_attend_kernel<D, NT, kExact><<<sm_count, 32 * S::kWarps, smem, st>>>(a);
+  kv_attend_kernel<D, kExact><<<sm_count, 32 * S::kWarps, smem, st>>>(a);
   return cudaGetLastError();
 }
 template <int D>
 cudaError_t launch_dim(AttendArgs& a, const KvAttendScratch& s, int sm_count, cudaStream_t st) {
-  const int nt = (int64_t)a.max_queries * a.group > 8 ? 2 : 1;
-  const uint64_t rows = 8 * nt;
+  constexpr uint64_t rows = 8;
   uint64_t units = s.acc_floats / (2 * rows * D);
   units = units < s.stats_floats / (4 * rows) ? units : s.stats_floats / (4 * rows);
   units = units < s.arrived_ints ? units : s.arrived_ints;
   a.most_units = (int)units;
-  if (a.type == EMELB_F32) return nt == 1 ? launch_one<D, 1, true>(a, sm_count, st) : launch_one<D, 2, true>(a, sm_count, st);
-  return nt == 1 ? launch_one<D, 1, false>(a, sm_count, st) : launch_one<D, 2, false>(a, sm_count, st);
+  if (a.type == EMELB_F32) return launch_one<D, true>(a, sm_count, st);
+  return launch_one<D, false>(a, sm_count, st);
 }
 
 }  // namespace
