@@ -205,7 +205,6 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ P
 }
 
 // ------------------------------------------------------------------ elements
-__device__ __forceinline__ float finite_or_zero(float x) { return x == x ? x : 0.0f; }
 template <class E>
 struct Elem;
 template <>
@@ -226,36 +225,32 @@ struct Elem<__nv_bfloat16> {
 
 // 8 values of a row, by 16-byte loads where the rows allow them
 template <class E>
-__device__ __forceinline__ void load8(const E* p, bool vec, float (&x)[8]) {
+struct Eight {
   __align__(16) E e[8];
-  if (vec) {
+  __device__ __forceinline__ void load(const E* p, bool vec) {
+    if (vec) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(e) / 16; ++i) reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p)[i];
-  } else {
+      for (int i = 0; i < (int)sizeof(e) / 16; ++i) reinterpret_cast<uint4*>(e)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = p[i];
+      for (int i = 0; i < 8; ++i) e[i] = p[i];
+    }
   }
+  __device__ __forceinline__ void store(E* p, bool vec) const {
+    if (vec) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = Elem<E>::in(e[i]);
-}
-template <class E>
-__device__ __forceinline__ void store8(E* p, bool vec, const float (&x)[8]) {
-  __align__(16) E e[8];
+      for (int i = 0; i < (int)sizeof(e) / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e)[i];
+    } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = Elem<E>::out(x[i]);
-  if (vec) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(e) / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e)[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = e[i];
+      for (int i = 0; i < 8; ++i) p[i] = e[i];
+    }
   }
-}
+};
 
 // ------------------------------------------------------------------ store
 // A CTA takes 16 packed rows of one head.  Four lanes share a group of 32 values, 8 each, which is a word of keys; the scale
 // comes from the group's largest value by two shuffles.  Values go by bytes, each with its own address: they wait in shared memory
-// until a warp can store one pair of dims of 16 rows at a time, which are 16 neighbouring bytes where the rows fill a tile.
+// until a warp can store one pair of dims of 16 rows at a time, which are neighbours where the rows fill a tile.
 struct StoreArgs {
   uint8_t* data;
   const void *k, *v;
@@ -265,44 +260,73 @@ struct StoreArgs {
   int* bad;
 };
 
-// the 4-bit form of 8 of a group's 32 values; d: the group's scale
-__device__ __forceinline__ void quantize8(const float (&x)[8], float& d, int (&q)[8]) {
-  float m = 0.0f, best = -1.0f;
+constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23: a sum with it has the rounded addend in its low bits
+
+// The scale of the group and the quants of this lane's 8 values, in the low bits of `bits`.
+//
+// q = floor(x / d + 8.5) within 0 .. 15 is the rounded x / d + 8, ties upwards.  With x and d of 11 bits or fewer a quotient that is
+// no tie is at least 2^-12 from one: x * (1 / d) + 8 + 2^-16, off by 2^-19, rounds to the right side of it.  Clamping is left to
+// the multiply-add's saturation, of the sum over 15.25.  f32 values may be closer: the borders (c - 8.5) d and (c - 7.5) d, exact in
+// f32, are looked at.
+template <class E>
+__device__ __forceinline__ void quantize8(const Eight<E>& in, __half& scale, uint32_t (&bits)[8]) {
+  float x[8], top = 0.0f, low = 0.0f;
+  bool nan = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float s = fabsf(x[i]);
-    if (s > best) {
-      best = s;
-      m = x[i];
-    }
+    x[i] = Elem<E>::in(in.e[i]);
+    top = fmaxf(top, x[i]);
+    low = fminf(low, x[i]);
+    nan |= x[i] != x[i];
   }
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
-    const float ob = __shfl_xor_sync(kAll, best, o), om = __shfl_xor_sync(kAll, m, o);
-    // of equal ones the lower lane's, which stands first in the row
-    if (ob > best || (ob == best && (threadIdx.x & o))) {
-      best = ob;
-      m = om;
-    }
+    top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
+    low = fminf(low, __shfl_xor_sync(kAll, low, o));
   }
-  d = __half2float(__float2half_rn(fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f)));
+  float m = top > -low ? top : low;
+  if (__any_sync(kAll, top == -low && top > 0.0f)) {
+    // both signs at the largest magnitude: the first of them
+    int at = 32;
+#pragma unroll
+    for (int i = 7; i >= 0; --i)
+      if (fabsf(x[i]) == top) at = i * 2 + (x[i] < 0.0f);
+    if (at < 32) at += 16 * (threadIdx.x & 3);
+    else at = 64;
+    at = min(at, __shfl_xor_sync(kAll, at, 1));
+    at = min(at, __shfl_xor_sync(kAll, at, 2));
+    if (top == -low) m = at & 1 ? low : top;
+  }
+  scale = __float2half_rn(fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f));
+  const float d = __half2float(scale);
+  float inv = 0.0f;
+  if (d != 0.0f) inv = sizeof(E) == 4 ? __frcp_rn(d) : __fdividef(1.0f, d);
+  const float a = inv * (1.0f / 15.25f), b = (8.0f + 0x1p-16f) * (1.0f / 15.25f);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    // x / d rounded never passes a border j - 8.5 that the quotient itself does not reach (the quotient's distance from it is
-    // at least half a step there), but the sum with 8.5 may: taken back by an exact comparison
-    const float t = __fdiv_rn(x[i], d);
-    float c = floorf(t + 8.5f);
-    if (t < c - 8.5f) c -= 1.0f;
-    q[i] = d == 0.0f ? 8 : (int)fminf(fmaxf(c, 0.0f), 15.0f);
+    const float c = fmaf(__saturatef(fmaf(x[i], a, b)), 15.25f, kMagic);
+    bits[i] = __float_as_uint(c);
+    if constexpr (sizeof(E) == 4) {
+      const float q = c - kMagic, xs = d < 0.0f ? -x[i] : x[i], ds = fabsf(d);
+      if (xs < (q - 8.5f) * ds && q > 0.0f) bits[i] -= 1;
+      else if (xs >= (q - 7.5f) * ds && q < 15.0f && d != 0.0f) bits[i] += 1;
+    }
+    if (d == 0.0f) bits[i] = __float_as_uint(kMagic + 8.0f);
+  }
+  if (__any_sync(kAll, nan)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (x[i] != x[i]) bits[i] = __float_as_uint(kMagic + 8.0f);
   }
 }
 
 template <int D, class E>
 __global__ void __launch_bounds__(128) kv_store_kernel(const StoreArgs a) {
   using T = Tile<D>;
+  constexpr int kOcts = D / 8, kTurns = (kTile * kOcts + 127) / 128;   // 8-value pieces of a row, turns of a thread
   __shared__ uint8_t* base[kTile];              // the row's tile of this head; null: skipped
   __shared__ int place[kTile];
-  __shared__ uint8_t bytes[D / 2][kTile + 4];   // values, a pair of dims by 16 rows
+  __shared__ __align__(16) uint8_t bytes[kTile][D / 2 + 4];   // values, a pair of dims a byte
   const int tid = threadIdx.x, head = blockIdx.y, row0 = blockIdx.x * kTile;
   if (tid < kTile) {
     uint8_t* p = nullptr;
@@ -320,41 +344,48 @@ __global__ void __launch_bounds__(128) kv_store_kernel(const StoreArgs a) {
     base[tid] = p;
     place[tid] = tau;
   }
-  __syncthreads();
-  constexpr int kOcts = D / 8;   // 8-value pieces of a row
-  for (int w = tid; w < kTile * kOcts; w += 128) {
-    const int row = w / kOcts, o = w % kOcts, j = o >> 2, t = o & 3;
-    uint8_t* p = base[row];
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0}, y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (p) {
-      load8(static_cast<const E*>(a.k) + (int64_t)(row0 + row) * a.ks + head * a.kh + 8 * o, a.vec, x);
-      load8(static_cast<const E*>(a.v) + (int64_t)(row0 + row) * a.vs + head * a.vh + 8 * o, a.vec, y);
-    }
+  // the loads do not wait for the slots: rows that are skipped are rows all the same
+  Eight<E> x[kTurns], y[kTurns];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = finite_or_zero(x[i]);
-      y[i] = finite_or_zero(y[i]);
-    }
-    float dk, dv;
-    int q[8];
-    quantize8(x, dk, q);
-    if (p) {
-      uint32_t word = 0;
+  for (int k = 0; k < kTurns; ++k) {
+    const int w = tid + 128 * k, row = w / kOcts, o = w % kOcts;
+    if (row < kTile && row0 + row < a.tokens) {
+      x[k].load(static_cast<const E*>(a.k) + (int64_t)(row0 + row) * a.ks + head * a.kh + 8 * o, a.vec);
+      y[k].load(static_cast<const E*>(a.v) + (int64_t)(row0 + row) * a.vs + head * a.vh + 8 * o, a.vec);
+    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) word |= (uint32_t)q[2 * i] << (4 * i) | (uint32_t)q[2 * i + 1] << (4 * i + 16);
-      *reinterpret_cast<uint32_t*>(p + T::key_word(place[row], j, t)) = word;
-      if (t == 0) *reinterpret_cast<__half*>(p + T::key_scale(place[row], j)) = __float2half_rn(dk);
+      for (int i = 0; i < 8; ++i) x[k].e[i] = y[k].e[i] = Elem<E>::out(0.0f);
     }
-    quantize8(y, dv, q);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bytes[4 * o + i][row] = (uint8_t)(q[2 * i] | q[2 * i + 1] << 4);
-    if (p && t == 0) *reinterpret_cast<__half*>(p + T::value_scale(place[row], j)) = __float2half_rn(dv);
   }
   __syncthreads();
-  for (int w = tid; w < kTile * D / 2; w += 128) {
-    const int row = w & 15, pair = w >> 4;
+#pragma unroll
+  for (int k = 0; k < kTurns; ++k) {
+    const int w = tid + 128 * k, row = w / kOcts, o = w % kOcts, j = o >> 2, t = o & 3;
+    if (row >= kTile) break;   // whole warps
     uint8_t* p = base[row];
-    if (p) p[T::value_byte(place[row], 2 * pair)] = bytes[pair][row];
+    __half dk, dv;
+    uint32_t q[8];
+    quantize8(x[k], dk, q);
+    // only the low bits of a sum with the magic number's bits are kept, where those are 0
+    const uint32_t even = ((q[6] * 16 + q[4]) * 16 + q[2]) * 16 + q[0], odd = ((q[7] * 16 + q[5]) * 16 + q[3]) * 16 + q[1];
+    if (p) {
+      const int tau = place[row];
+      *reinterpret_cast<uint32_t*>(p + T::key_word(tau, j, t)) = __byte_perm(even, odd, 0x5410);
+      if (t == 0) *reinterpret_cast<__half*>(p + T::key_scale(tau, j)) = dk;
+    }
+    quantize8(y[k], dv, q);
+    const uint32_t b01 = __byte_perm(q[1] * 16 + q[0], q[3] * 16 + q[2], 0x0040), b23 = __byte_perm(q[5] * 16 + q[4], q[7] * 16 + q[6], 0x0040);
+    *reinterpret_cast<uint32_t*>(&bytes[row][4 * o]) = __byte_perm(b01, b23, 0x5410);
+    if (p && t == 0) *reinterpret_cast<__half*>(p + T::value_scale(place[row], j)) = dv;
+  }
+  __syncthreads();
+  // thread: a row and a row pair g of every 16 dims
+  const int row = tid & 15, g = tid >> 4;
+  uint8_t* p = base[row];
+  if (p) {
+    p += T::value_byte(place[row], 2 * g);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) p[T::value_byte(0, 16 * i) - T::value_byte(0, 0)] = bytes[row][8 * i + g];
   }
 }
 
@@ -368,30 +399,44 @@ struct LoadArgs {
   int* bad;
 };
 
-// last request b in [lo, hi] with begin[b] <= row
-__device__ __forceinline__ int request_of(const int32_t* begin, int lo, int hi, int row) {
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (begin[mid] <= row) lo = mid;
-    else hi = mid - 1;
+// 8 quants as values: nibble i of `word` (low 16 bits) times d, nibble i + 4 the next (kPairs), or nibbles in order
+template <bool kPairs, class E>
+__device__ __forceinline__ void dequantize8(uint32_t word, __half scale, Eight<E>& out) {
+  const float d = __half2float(scale);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t two = (word >> (4 * i) & 0x000f000fu) | 0x64006400u;   // 1024 + nibbles i and i + 4
+    const __half2 q = __hsub2(*reinterpret_cast<const __half2*>(&two), __float2half2_rn(1032.0f));
+    out.e[kPairs ? 2 * i : i] = Elem<E>::out(__low2float(q) * d);
+    out.e[kPairs ? 2 * i + 1 : i + 4] = Elem<E>::out(__high2float(q) * d);
   }
-  return lo;
 }
+
+constexpr int kWindow = 127;   // requests behind the first row's whose beginnings are looked at together
 
 template <int D, class E>
 __global__ void __launch_bounds__(128) kv_load_kernel(const LoadArgs a) {
   using T = Tile<D>;
   __shared__ const uint8_t* base[kTile];
   __shared__ int place[kTile];
-  __shared__ uint8_t bytes[D / 2][kTile + 4];
+  __shared__ int begins[kWindow + 1];
+  __shared__ __align__(16) uint8_t bytes[kTile][D / 2 + 4];
   const int tid = threadIdx.x, head = blockIdx.y, row0 = blockIdx.x * kTile;
+  // the request of the first row: how many begin at or before it
+  int before = 0;
+  for (int b0 = 0; b0 < a.requests; b0 += 128) before += __syncthreads_count(b0 + tid < a.requests && a.row_begin[b0 + tid] <= row0);
+  const int b0 = max(before - 1, 0);
+  begins[tid] = a.row_begin[min(b0 + tid, a.requests)];
+  __syncthreads();
   if (tid < kTile) {
     const uint8_t* p = nullptr;
     int tau = 0;
     const int row = row0 + tid;
-    if (row < a.rows && row >= a.row_begin[0] && row < a.row_begin[a.requests]) {
-      const int b = request_of(a.row_begin, 0, a.requests - 1, row);
-      const int64_t from = a.first ? a.first[b] : 0, pos = from + row - a.row_begin[b];
+    int b = b0;
+    while (b < a.requests && (b + 1 - b0 <= kWindow ? begins[b + 1 - b0] : a.row_begin[b + 1]) <= row) ++b;
+    if (row < a.rows && b < a.requests && row >= begins[0]) {
+      const int begin = b - b0 <= kWindow ? begins[b - b0] : a.row_begin[b];
+      const int64_t from = a.first ? a.first[b] : 0, pos = from + row - begin;
       if (from < 0 || pos < from) *a.bad = 1;
       else if (pos < a.lengths[b]) {
         const int64_t col = pos >> a.page_shift;
@@ -408,31 +453,35 @@ __global__ void __launch_bounds__(128) kv_load_kernel(const LoadArgs a) {
     place[tid] = tau;
   }
   __syncthreads();
-  for (int w = tid; w < kTile * D / 2; w += 128) {
-    const int row = w & 15, pair = w >> 4;
+  {
+    const int row = tid & 15, g = tid >> 4;
     const uint8_t* p = base[row];
-    if (p) bytes[pair][row] = p[T::value_byte(place[row], 2 * pair)];
+    if (p) {
+      p += T::value_byte(place[row], 2 * g);
+      uint8_t v[D / 16];
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) v[i] = p[T::value_byte(0, 16 * i) - T::value_byte(0, 0)];
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) bytes[row][8 * i + g] = v[i];
+    }
   }
-  __syncthreads();
   constexpr int kOcts = D / 8;
   for (int w = tid; w < kTile * kOcts; w += 128) {
     const int row = w / kOcts, o = w % kOcts, j = o >> 2, t = o & 3;
     const uint8_t* p = base[row];
     if (!p) continue;
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(p + T::key_word(place[row], j, t));
-    const float dk = __half2float(*reinterpret_cast<const __half*>(p + T::key_scale(place[row], j)));
-    const float dv = __half2float(*reinterpret_cast<const __half*>(p + T::value_scale(place[row], j)));
-    float x[8], y[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = (float)((int)(word >> (4 * i) & 15) - 8) * dk;
-      x[2 * i + 1] = (float)((int)(word >> (4 * i + 16) & 15) - 8) * dk;
-      const int two = bytes[4 * o + i][row];
-      y[2 * i] = (float)((two & 15) - 8) * dv;
-      y[2 * i + 1] = (float)((two >> 4) - 8) * dv;
-    }
-    store8(static_cast<E*>(a.k) + (int64_t)(row0 + row) * a.ks + head * a.kh + 8 * o, a.vec, x);
-    store8(static_cast<E*>(a.v) + (int64_t)(row0 + row) * a.vs + head * a.vh + 8 * o, a.vec, y);
+    Eight<E> x;
+    dequantize8<true>(*reinterpret_cast<const uint32_t*>(p + T::key_word(place[row], j, t)), *reinterpret_cast<const __half*>(p + T::key_scale(place[row], j)), x);
+    x.store(static_cast<E*>(a.k) + (int64_t)(row0 + row) * a.ks + head * a.kh + 8 * o, a.vec);
+  }
+  __syncthreads();
+  for (int w = tid; w < kTile * kOcts; w += 128) {
+    const int row = w / kOcts, o = w % kOcts, j = o >> 2;
+    const uint8_t* p = base[row];
+    if (!p) continue;
+    Eight<E> y;
+    dequantize8<false>(*reinterpret_cast<const uint32_t*>(&bytes[row][4 * o]), *reinterpret_cast<const __half*>(p + T::value_scale(place[row], j)), y);
+    y.store(static_cast<E*>(a.v) + (int64_t)(row0 + row) * a.vs + head * a.vh + 8 * o, a.vec);
   }
 }
 
