@@ -2,6 +2,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "kv_tile.cuh"
 #include "paged.h"
@@ -16,39 +18,46 @@ typedef long long i64;
 
 // ------------------------------------------------------------------ plan
 // Three running sums over the requests (tokens, pages lacking, pages given back) decide everything else: new page j is
-// entry top - 1 - j of the stack that the ended requests' pages lie on, and row i's request is found by bisection.  One cluster
-// makes the step: every CTA takes the sums for itself, since that is cheaper than handing them over, then the cluster shares
-// the pages and, behind a barrier (which also separates the last read of an array from the first write of one that may be
-// the same), the rows.
+// entry top - 1 - j of the stack that the ended requests' pages lie on, and row i's request is found by bisection.  Every CTA
+// takes the sums for itself, since that is cheaper than handing them over, and then its share of the pages and of the rows, which
+// look a new page up where it comes from and not in the table, so that no CTA waits for another.  What is read and what is written
+// do not meet, but for `lengths` and free_left where they are `cached` and free_count: with more than one CTA those wait in scratch
+// for a second launch.
+// 1000 requests, 121,984 rows: 21 us by a cluster of 8 CTAs with a barrier between pages and rows, whose rows took half of it.
 constexpr int kPlanMost = EMELB_KV_MAX_REQUESTS;
 constexpr unsigned kAll = 0xffffffffu;
 
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-// inclusive sum over the block; `carry` comes in and goes out as the sum of all blocks of requests so far
-__device__ __forceinline__ i64 block_sum(i64 v, i64& carry, i64* warp_sums) {
+// inclusive sums over the block; `carry` comes in and goes out as the sums of all blocks of requests so far
+template <int N>
+__device__ __forceinline__ void block_sums(i64 (&v)[N], i64 (&carry)[N], i64 (*warp_sums)[32]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const i64 u = __shfl_up_sync(kAll, v, o);
-    if (lane >= o) v += u;
-  }
-  if (lane == 31) warp_sums[warp] = v;
-  __syncthreads();
-  i64 w = lane < warps ? warp_sums[lane] : 0;
+  for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const i64 u = __shfl_up_sync(kAll, w, o);
-    if (lane >= o) w += u;
-  }
-  const i64 before = warp ? __shfl_sync(kAll, w, warp - 1) : 0;
-  const i64 all = __shfl_sync(kAll, w, 31);
+    for (int k = 0; k < N; ++k) {
+      const i64 u = __shfl_up_sync(kAll, v[k], o);
+      if (lane >= o) v[k] += u;
+    }
+  if (lane == 31)
+#pragma unroll
+    for (int k = 0; k < N; ++k) warp_sums[k][warp] = v[k];
   __syncthreads();
-  const i64 out = carry + before + v;
-  carry += all;
-  return out;
+  i64 w[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) w[k] = lane < warps ? warp_sums[k][lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const i64 u = __shfl_up_sync(kAll, w[k], o);
+      if (lane >= o) w[k] += u;
+    }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    v[k] += carry[k] + (warp ? __shfl_sync(kAll, w[k], max(warp - 1, 0)) : 0);
+    carry[k] += __shfl_sync(kAll, w[k], 31);
+  }
+  __syncthreads();
 }
 
 // first request whose running sum is above x
@@ -66,17 +75,18 @@ __device__ __forceinline__ int clip(i64 v) { return (int)(v < 0 ? 0 : v > 0x7fff
 
 struct PlanArgs {
   emelb_kv_plan_request r;
+  int *lengths, *free_left;   // the request's own, or scratch
   int page_shift;
   int* bad;
 };
 
-__global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ PlanArgs a) {
+__global__ void __launch_bounds__(512) kv_plan_kernel(const __grid_constant__ PlanArgs a) {
   extern __shared__ int plan_smem[];
-  __shared__ i64 warp_sums[32];
-  __shared__ i64 most_taken;
+  __shared__ i64 warp_sums[3][32];
+  __shared__ int most_taken;
   const emelb_kv_plan_request& r = a.r;
   const int n = r.requests, P = r.page_tokens, shift = a.page_shift, tid = threadIdx.x, T = blockDim.x;
-  const unsigned ranks = gridDim.x, rank = blockIdx.x;   // the grid is one cluster
+  const int ranks = gridDim.x, rank = blockIdx.x;
   int* tok = plan_smem;         // running sums, each request's own included
   int* need = tok + n;
   int* back = need + n;
@@ -85,43 +95,48 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ P
   bool wrong = false;
   if (tid == 0) most_taken = 0;
 
-  i64 tok_sum = 0, need_sum = 0, back_sum = 0;
-  i64 count = *r.free_count;
+  i64 all[3] = {0, 0, 0};   // tokens, pages lacking, pages given back
+  const int free_count = *r.free_count;
+  // a thread has `per` neighbouring requests: their sums from its first on, then what stands before that
+  const int per = (n + T - 1) / T, b_first = min(n, tid * per), b_last = min(n, b_first + per);
+  i64 mine[3] = {0, 0, 0};
+#pragma unroll 4
+  for (int b = b_first; b < b_last; ++b) {
+    i64 cached = r.cached[b];
+    const i64 fresh = r.fresh[b];
+    const bool ok = cached >= 0 && fresh >= -1 && cached + (fresh > 0 ? fresh : 0) <= room, ended = fresh < 0;
+    wrong |= !ok;
+    cached = cached < 0 ? 0 : cached > room ? room : cached;
+    const int have = (int)((cached + P - 1) >> shift);
+    mine[0] += ended ? 0 : fresh;
+    mine[1] += ok && !ended ? ((cached + fresh + P - 1) >> shift) - have : 0;
+    mine[2] += ok && ended ? have : 0;
+    tok[b] = clip(mine[0]);
+    need[b] = clip(mine[1]);
+    back[b] = clip(mine[2]);
+    had[b] = ok ? (int)cached : ~(int)cached;
+  }
+  i64 upto[3] = {mine[0], mine[1], mine[2]};
+  block_sums(upto, all, warp_sums);
+  for (int b = b_first; b < b_last; ++b) {
+    const i64 rows_upto = upto[0] - mine[0] + tok[b];
+    tok[b] = clip(rows_upto);
+    need[b] = clip(upto[1] - mine[1] + need[b]);
+    back[b] = clip(upto[2] - mine[2] + back[b]);
+    if (rows_upto > r.token_capacity && had[b] >= 0 && r.fresh[b] >= 0) {   // no rows for them, nor for any behind
+      had[b] = ~had[b];
+      wrong = true;
+    }
+  }
+  const i64 tok_sum = all[0], need_sum = all[1], back_sum = all[2];
+  __syncthreads();
+  i64 count = free_count;
   if (count < 0 || count > r.pages) {
     wrong = true;
     count = count < 0 ? 0 : r.pages;
   }
-  for (int b0 = 0; b0 < n; b0 += T) {
-    const int b = b0 + tid;
-    i64 cached = 0, fresh = 0;
-    bool ok = b < n;
-    if (b < n) {
-      cached = r.cached[b];
-      fresh = r.fresh[b];
-      ok = cached >= 0 && fresh >= -1 && cached + (fresh > 0 ? fresh : 0) <= room;
-      wrong |= !ok;
-      cached = cached < 0 ? 0 : cached > room ? room : cached;
-    }
-    const bool ended = fresh < 0;
-    const i64 upto = block_sum(ended ? 0 : fresh, tok_sum, warp_sums);
-    if (b < n && !ended && upto > r.token_capacity) {
-      ok = false;
-      wrong = true;
-    }
-    const int have = (int)((cached + P - 1) >> shift);
-    const i64 lacks = ok && !ended ? ((cached + fresh + P - 1) >> shift) - have : 0;
-    const i64 n_upto = block_sum(lacks, need_sum, warp_sums);
-    const i64 r_upto = block_sum(ok && ended ? have : 0, back_sum, warp_sums);
-    if (b < n) {
-      tok[b] = clip(upto);
-      need[b] = clip(n_upto);
-      back[b] = clip(r_upto);
-      had[b] = ok ? (int)cached : ~(int)cached;
-    }
-  }
-  __syncthreads();
   const i64 top = count + back_sum;
-  i64 taken = 0;
+  int taken = 0;
   for (int b = tid; b < n; b += T) {
     const int lacks = need[b] - (b ? need[b - 1] : 0);
     if (had[b] >= 0 && lacks > 0) {
@@ -129,22 +144,21 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ P
       else had[b] = ~had[b];
     }
   }
-  if (taken) atomicMax(&most_taken, taken);
+  taken = __reduce_max_sync(kAll, taken);
+  if ((tid & 31) == 0 && taken) atomicMax(&most_taken, taken);
   __syncthreads();
   taken = most_taken;
 
-  // new pages into the tables
-  const int step = (int)ranks * T, me = (int)rank * T + tid;
-  for (int j = me; j < taken; j += step) {
-    const int b = owner_of(need, n, j);
+  // new page j: from the top of the stack, or of what the ended requests lay on it
+  auto new_page = [&](int j) {
     const i64 at = top - 1 - j;
-    int page;
-    if (at < count) {
-      page = r.free_pages[at];
-    } else {
-      const int x = (int)(at - count), e = owner_of(back, n, x);
-      page = r.table[e * r.table_stride + (x - (e ? back[e - 1] : 0))];
-    }
+    if (at < count) return r.free_pages[at];
+    const int x = (int)(at - count), e = owner_of(back, n, x);
+    return r.table[e * r.table_stride + (x - (e ? back[e - 1] : 0))];
+  };
+  const int step = ranks * T, me = rank * T + tid;
+  for (int j = me; j < taken; j += step) {
+    const int b = owner_of(need, n, j), page = new_page(j);
     if (page < 0 || page >= r.pages) wrong = true;
     r.table[b * r.table_stride + ((had[b] + P - 1) >> shift) + (j - (b ? need[b - 1] : 0))] = page;
   }
@@ -154,54 +168,84 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(const __grid_constant__ P
     if (count + x < r.pages) r.free_pages[count + x] = r.table[e * r.table_stride + (x - (e ? back[e - 1] : 0))];
     else wrong = true;
   }
-  if (ranks > 1) cluster_barrier();
-  else __syncthreads();
-
-  // slots and positions
+  // slots and positions: four neighbouring rows a thread, of which the first is searched for
   const int total = clip(tok_sum < r.token_capacity ? tok_sum : r.token_capacity);
-  for (int i = me; i < r.token_capacity; i += step) {
-    i64 slot = -1;
-    int p = 0;
-    if (i < total) {
-      const int b = owner_of(tok, n, i), at = i - (b ? tok[b - 1] : 0);
-      const int h = had[b];
-      p = (h < 0 ? ~h : h) + at;
-      if (h >= 0) {
-        const int page = r.table[b * r.table_stride + (p >> shift)];
-        if (page >= 0 && page < r.pages) slot = ((i64)page << shift) + (p & (P - 1));
-        else wrong = true;
+  const bool wide = reinterpret_cast<uintptr_t>(r.slots) % 16 == 0 && reinterpret_cast<uintptr_t>(r.positions) % 16 == 0;
+  for (int i0 = 4 * me; i0 < r.token_capacity; i0 = i0 > 0x7fffffff - 4 * step ? 0x7fffffff : i0 + 4 * step) {
+    i64 slot[4];
+    int p[4], page[4], b = i0 < total ? owner_of(tok, n, i0) : 0;
+    constexpr i64 kNew = (i64)1 << 62;
+    i64 entry[4];                     // in the table, or the number of a new page
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      entry[e] = -1;
+      p[e] = 0;
+      if (i0 + e < total) {
+        while (tok[b] <= i0 + e) ++b;
+        const int h = had[b];
+        p[e] = (h < 0 ? ~h : h) + i0 + e - (b ? tok[b - 1] : 0);
+        const int col = p[e] >> shift, have = (h + P - 1) >> shift;
+        if (h >= 0) entry[e] = col < have ? b * r.table_stride + col : kNew | ((b ? need[b - 1] : 0) + col - have);
       }
     }
-    r.slots[i] = slot;
-    r.positions[i] = p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e && entry[e] == entry[e - 1]) page[e] = page[e - 1];   // rows of one page: looked up once
+      else page[e] = entry[e] < 0 ? 0 : entry[e] < kNew ? r.table[entry[e]] : new_page((int)(entry[e] & ~kNew));
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool sound = page[e] >= 0 && page[e] < r.pages;
+      if (!sound) wrong = true;
+      slot[e] = entry[e] >= 0 && sound ? ((i64)page[e] << shift) + (p[e] & (P - 1)) : -1;
+    }
+    if (wide && i0 + 3 < r.token_capacity) {
+      *reinterpret_cast<longlong2*>(r.slots + i0) = make_longlong2(slot[0], slot[1]);
+      *reinterpret_cast<longlong2*>(r.slots + i0 + 2) = make_longlong2(slot[2], slot[3]);
+      *reinterpret_cast<int4*>(r.positions + i0) = make_int4(p[0], p[1], p[2], p[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i0 + e < r.token_capacity) {
+          r.slots[i0 + e] = slot[e];
+          r.positions[i0 + e] = p[e];
+        }
+    }
   }
-  // each request's share, by the first CTA (fresh may not be read from an array that was written: it never is one)
-  if (rank == 0) {
-    i64 key_sum = 0;
-    for (int b0 = 0; b0 < n; b0 += T) {
-      const int b = b0 + tid;
-      i64 len = 0;
-      if (b < n) {
-        const int h = had[b];
-        const bool ended = r.fresh[b] < 0;
-        len = ended ? 0 : h >= 0 ? (i64)h + (tok[b] - (b ? tok[b - 1] : 0)) : (i64)~h;
-      }
-      const i64 upto = block_sum(len, key_sum, warp_sums);
-      if (b < n) {
-        r.lengths[b] = (int)len;
-        r.query_begin[b + 1] = tok[b] < r.token_capacity ? tok[b] : r.token_capacity;
-        r.key_begin[b + 1] = clip(upto);
-        if (upto > 0x7fffffff) wrong = true;
-      }
+  // each request's share, by the last CTA, which has the fewest rows; the barriers of the sums stand between reads and writes of one CTA
+  if (rank == ranks - 1) {
+    auto length_of = [&](int b) {
+      const int h = had[b];
+      return r.fresh[b] < 0 ? 0 : h >= 0 ? h + (tok[b] - (b ? tok[b - 1] : 0)) : ~h;
+    };
+    i64 key_sum[1] = {0}, keys[1] = {0};
+#pragma unroll 4
+    for (int b = b_first; b < b_last; ++b) keys[0] += length_of(b);
+    i64 at = -keys[0];
+    block_sums(keys, key_sum, warp_sums);
+    at += keys[0];
+    for (int b = b_first; b < b_last; ++b) {
+      const int len = length_of(b);
+      at += len;
+      a.lengths[b] = len;
+      r.query_begin[b + 1] = tok[b] < r.token_capacity ? tok[b] : r.token_capacity;
+      r.key_begin[b + 1] = clip(at);
+      if (at > 0x7fffffff) wrong = true;
     }
     if (tid == 0) {
       r.query_begin[0] = 0;
       r.key_begin[0] = 0;
-      *r.free_left = clip(top - taken);
+      *a.free_left = clip(top - taken);
       *r.shortage = clip(need_sum > top ? need_sum - top : 0);
     }
   }
   if (wrong) *a.bad = 1;
+}
+
+__global__ void __launch_bounds__(256) kv_plan_in_place_kernel(const int* lengths, const int* free_left, int n, int* to_lengths, int* to_free_left) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) to_lengths[i] = lengths[i];
+  if (i == 0) *to_free_left = *free_left;
 }
 
 // ------------------------------------------------------------------ elements
@@ -432,13 +476,22 @@ __global__ void __launch_bounds__(128) kv_load_kernel(const LoadArgs a) {
     const uint8_t* p = nullptr;
     int tau = 0;
     const int row = row0 + tid;
-    int b = b0;
-    while (b < a.requests && (b + 1 - b0 <= kWindow ? begins[b + 1 - b0] : a.row_begin[b + 1]) <= row) ++b;
+    // the last request that begins at or before the row: in the window, or past it one by one
+    int lo = 0, hi = min(kWindow, a.requests - b0);
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (begins[mid] <= row) lo = mid;
+      else hi = mid - 1;
+    }
+    int b = b0 + lo;
+    if (lo == kWindow)
+      while (b < a.requests && a.row_begin[b + 1] <= row) ++b;
     if (row < a.rows && b < a.requests && row >= begins[0]) {
       const int begin = b - b0 <= kWindow ? begins[b - b0] : a.row_begin[b];
+      const int length = a.lengths[b];
       const int64_t from = a.first ? a.first[b] : 0, pos = from + row - begin;
       if (from < 0 || pos < from) *a.bad = 1;
-      else if (pos < a.lengths[b]) {
+      else if (pos < length) {
         const int64_t col = pos >> a.page_shift;
         const int page = col < a.table_width ? a.table[b * a.table_stride + col] : -1;
         if (page < 0 || page >= a.pages) *a.bad = 1;
@@ -518,24 +571,21 @@ cudaError_t load_typed(int D, dim3 grid, const LoadArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-cudaError_t launch_kv_plan(const emelb_kv_plan_request& r, int* bad, cudaStream_t st) {
-  PlanArgs a{r, log2_of(r.page_tokens), bad};
-  const bool small = r.requests <= 256 && r.token_capacity <= 1024;
-  const int smem = 16 * r.requests;
-  cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 16 * kPlanMost);
+cudaError_t launch_kv_plan(const emelb_kv_plan_request& r, int* scratch, int sm_count, int* launches, int* bad, cudaStream_t st) {
+  const cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 16 * kPlanMost);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(small ? 1 : 8);
-  cfg.blockDim = dim3(small ? 256 : 1024);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cfg.gridDim.x;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = small ? 0 : 1;
-  return cudaLaunchKernelEx(&cfg, kv_plan_kernel, a);
+  // a CTA's sums cost what 2000 rows do: few rows and requests are one CTA's
+  const int threads = r.requests <= 256 && r.token_capacity <= 2048 ? 256 : 512;
+  const int ctas = threads == 256 ? 1 : std::min(sm_count, (r.token_capacity - 1) / 2048 + 1);
+  const bool aside = ctas > 1 && (r.lengths == r.cached || r.free_left == r.free_count);
+  const PlanArgs a{r, aside ? scratch + 1 : r.lengths, aside ? scratch : r.free_left, log2_of(r.page_tokens), bad};
+  kv_plan_kernel<<<ctas, threads, 16 * r.requests, st>>>(a);
+  *launches = 1;
+  if (aside) {
+    kv_plan_in_place_kernel<<<(r.requests + 255) / 256, 256, 0, st>>>(scratch + 1, scratch, r.requests, r.lengths, r.free_left);
+    *launches = 2;
+  }
+  return cudaGetLastError();
 }
 
 cudaError_t launch_kv_store(const emelb_kv_store_request& r, int* bad, cudaStream_t st) {

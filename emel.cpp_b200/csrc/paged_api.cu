@@ -132,8 +132,12 @@ uint32_t emelb_kv_plan_can_run(const emelb_kv_plan_request* r) {
 uint32_t emelb_kv_plan(emelb_ctx* c, const emelb_kv_plan_request* r) {
   if (!c || !r) return EMELB_INVALID_REQUEST;
   if (const uint32_t why = emelb_kv_plan_can_run(r)) return refuse(c, why);
-  return dispatch(c, {r->cached, r->fresh, r->table, r->free_pages, r->free_count, r->free_left, r->lengths, r->query_begin, r->key_begin, r->slots,
-                      r->positions, r->shortage}, 1, [&] { return launch_kv_plan(*r, c->bad_word(), c->stream); });
+  int launches = 0;
+  const uint32_t err = dispatch(c, {r->cached, r->fresh, r->table, r->free_pages, r->free_count, r->free_left, r->lengths, r->query_begin, r->key_begin,
+                                    r->slots, r->positions, r->shortage}, 0,
+                                [&] { return launch_kv_plan(*r, reinterpret_cast<int*>(c->fa_part_ml), c->sm_count, &launches, c->bad_word(), c->stream); });
+  c->diag.kernel_launches += launches;
+  return err;
 }
 
 // ------------------------------------------------------------------ store, load

@@ -133,6 +133,32 @@ def test_plan_in_place_replayed(be):
     be.graph_destroy(graph)
 
 
+def test_plan_in_place_of_many_rows(be):
+    """Steps in place that several CTAs make: lengths and the stack's size wait for the last read of the ones before."""
+    n, page, width, pages, cap = 700, 16, 30, 12000, 20000
+    rng = np.random.default_rng(8)
+    for lengths_too in (True, False):
+        s = Step(n, width, pages, page, cap, in_place=True)
+        if not lengths_too:
+            s.lengths = torch.zeros(n, dtype=torch.int32, device="cuda")
+        cached, count = np.zeros(n, np.int64), pages
+        table, stack = np.full((n, width), -1, np.int32), rng.permutation(pages).astype(np.int32)
+        s.cached.zero_()
+        s.table.fill_(-1)
+        s.stack.copy_(torch.from_numpy(stack))
+        s.count.fill_(count)
+        for step in range(6):
+            fresh = np.where((step > 1) & (rng.random(n) < 0.2), -1, np.minimum(rng.integers(0, 56, n), width * page - cached))
+            s.fresh.copy_(dev(fresh.tolist()))
+            if not lengths_too:
+                s.cached.copy_(dev(cached.tolist()))
+            torch.cuda.synchronize()
+            done(be, be.kv_plan(s.request()))
+            want = plain.plan(cached, fresh, table, stack, count, page, cap)
+            s.check(want)
+            cached, count, table, stack = np.asarray(want["lengths"]), want["free_left"], want["table"], want["free_pages"]
+
+
 @pytest.mark.parametrize("what", ["negative", "fresh", "long", "capacity", "count", "page"])
 def test_plan_reports_values_out_of_range(be, what):
     s = Step(4, 4, 30, 16, 20)
