@@ -24,6 +24,9 @@ namespace {
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kTileRows = 128, kTileKeys = 128, kTiles = 2;   // tiles of a CTA
 constexpr int kLoadWarp = 8, kMmaWarp = 9, kThreads = 384;
+// registers a thread behind the start, of the 168 that 384 threads launch with: 8 warps x 208 + 4 x 88 = 12 x 168
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(8 * kSoftmaxRegs + 4 * kOtherRegs <= 12 * 168, "registers");
 constexpr float kLowest = -3.0e38f;
 constexpr float kSlack = 8.0f;
 constexpr int kTmemCols = 512;
@@ -114,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using S = Smem<DP>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t bars[2 * kStages + 4 * kTiles + 2];
+  __shared__ uint64_t bars[2 * kStages + 5 * kTiles + 2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int gave_up;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -124,9 +127,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto empty = [&](int s) { return bar0 + 8 * (kStages + s); };
   auto q_ready = [&](int t) { return bar0 + 8 * (2 * kStages + t); };
   auto s_ready = [&](int t) { return bar0 + 8 * (2 * kStages + kTiles + t); };
-  auto p_ready = [&](int t) { return bar0 + 8 * (2 * kStages + 2 * kTiles + t); };
-  auto o_ready = [&](int t) { return bar0 + 8 * (2 * kStages + 3 * kTiles + t); };
-  const uint32_t raw_bar = bar0 + 8 * (2 * kStages + 4 * kTiles), drain_bar = raw_bar + 8;
+  auto o_ready = [&](int t) { return bar0 + 8 * (2 * kStages + 2 * kTiles + t); };
+  auto p_ready = [&](int t, int half) { return bar0 + 8 * (2 * kStages + (3 + half) * kTiles + t); };   // 64 keys each
+  const uint32_t raw_bar = bar0 + 8 * (2 * kStages + 5 * kTiles), drain_bar = raw_bar + 8;
 
   // ---- which rows
   const int head = blockIdx.x % a.kv_heads;
@@ -163,9 +166,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::mbar_init(empty(s), 1);
     }
     for (int t = 0; t < kTiles; ++t) {
-      tc::mbar_init(q_ready(t), kTileRows);
+      tc::mbar_init(q_ready(t), kTileRows / 32);
       tc::mbar_init(s_ready(t), 1);
-      tc::mbar_init(p_ready(t), kTileRows);
+      tc::mbar_init(p_ready(t, 0), kTileRows / 32);
+      tc::mbar_init(p_ready(t, 1), kTileRows / 32);
       tc::mbar_init(o_ready(t), 1);
     }
     tc::mbar_init(raw_bar, 1);
@@ -185,6 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int used = 0;            // MMA warp: tiles waited for
 
   if (warp == kLoadWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     // K tile, V tile, K tile, ... of the walk
     bool alive = true;
     for (; alive && loaded < 2 * n; ++loaded) {
@@ -212,6 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (tc::elect_one()) {
       constexpr uint32_t type = kBf16 ? 1u : 0u;
       constexpr uint32_t common = 1u << 4 | type << 7 | type << 10 | (uint32_t)(kTileRows >> 4) << 24;
@@ -236,12 +242,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = -1; alive && j < n; ++j) {
         for (int t = 0; t < kTiles && alive; ++t) {
           if (j >= 0 && j < n_of[t]) {
-            alive = wait_tile(2 * j + 1) && tc::mbar_wait(p_ready(t), j & 1, &gave_up);
-            if (!alive) break;
-            tc::fence_after();
+            alive = wait_tile(2 * j + 1);
 #pragma unroll
-            for (int kk = 0; kk < kTileKeys / 16; ++kk)
-              tc::mma_f16(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, value_desc(stage(2 * j + 1) + kk * 2048), idesc_o, j > 0 || kk > 0);
+            for (int half = 0; half < 2; ++half) {
+              alive = alive && tc::mbar_wait(p_ready(t, half), j & 1, &gave_up);
+              if (!alive) break;
+              tc::fence_after();
+#pragma unroll
+              for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                tc::mma_f16(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, value_desc(stage(2 * j + 1) + kk * 2048), idesc_o, j > 0 || kk > 0);
+            }
+            if (!alive) break;
             if (j + 1 == n_of[t]) tc::mma_commit(o_ready(t));
           }
           if (j + 1 < n_of[t]) {
@@ -263,7 +274,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp < kLoadWarp) {
+  } else if (warp > kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int t = warp >> 2, r = tid & 127, n_mine = t ? n1 : n0;
     const int64_t row = row0 + t * kTileRows + r;
     const bool live = row < rows;
@@ -284,7 +298,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      tc::mbar_arrive(q_ready(t));
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(q_ready(t));
     }
     const int see = sees(live ? row : rows - 1), see_all = n_mine > 0 ? sees(first) : 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -346,10 +361,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           p[i] = pack16<kBf16>(e0, e1);
         }
         tc::tmem_st32(s_col + 32 * c, p);
+        tc::tmem_wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(p_ready(t, c));
       }
-      tc::tmem_wait_st();
-      tc::fence_before();
-      tc::mbar_arrive(p_ready(t));
     }
     if (alive && n_mine > 0) alive = tc::mbar_wait(o_ready(t), 0, &gave_up);
     alive = __all_sync(kAll, alive);
