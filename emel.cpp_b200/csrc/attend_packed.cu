@@ -40,7 +40,7 @@ struct PackedArgs {
   void* out;
   const int32_t *query_begin, *key_begin;
   int64_t qs, qh, os, oh;
-  int requests, kv_heads, group, head_dim, queries, keys, max_queries, causal;
+  int requests, kv_heads, group, group_inv, head_dim, queries, keys, max_queries, causal;
   float scale_log2;
   int *bad, *status;
 };
@@ -151,12 +151,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t rows = (int64_t)nq * a.group;
   const int64_t tiles = (rows + kTiles * kTileRows - 1) / (kTiles * kTileRows), local = slot - first_slot(a, b);
   if (local < 0 || local >= tiles) return;
-  const int64_t row0 = (tiles - 1 - local) * (kTiles * kTileRows);   // long walks first
-  // keys that a row of the request sees; row tiles of this CTA walk turns(t) key tiles
-  auto sees = [&](int64_t row) { return a.causal ? max(0, min(nk, nk - nq + (int)(row / a.group) + 1)) : nk; };
+  // rows of this CTA, counted from its first, which is head `part0` of token tok0; long walks first
+  const int64_t row0 = (tiles - 1 - local) * (kTiles * kTileRows);
+  const int n_rows = (int)min(rows - row0, (int64_t)(kTiles * kTileRows)), tok0 = (int)(row0 / a.group), part0 = (int)(row0 - (int64_t)tok0 * a.group);
+  // (part0 + row) / group by a product: exact, since (part0 + row) * group < 2^16
+  auto token_of = [&](int row) { return (int)((uint32_t)(part0 + row) * a.group_inv >> 16); };
+  // keys that a row sees; row tiles of this CTA walk turns(t) key tiles
+  auto sees = [&](int row) { return a.causal ? max(0, min(nk, nk - nq + tok0 + token_of(row) + 1)) : nk; };
   auto turns = [&](int t) {
-    const int64_t r = row0 + t * kTileRows;
-    return r >= rows ? 0 : (sees(min(rows, r + kTileRows) - 1) + kTileKeys - 1) / kTileKeys;
+    const int r = t * kTileRows;
+    return r >= n_rows ? 0 : (sees(min(n_rows, r + kTileRows) - 1) + kTileKeys - 1) / kTileKeys;
   };
   const int n0 = turns(0), n1 = turns(1), n = max(n0, n1);
 
@@ -279,29 +283,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int t = warp >> 2, r = tid & 127, n_mine = t ? n1 : n0;
-    const int64_t row = row0 + t * kTileRows + r;
-    const bool live = row < rows;
-    const int64_t first = row0 + t * kTileRows;
+    const int row = t * kTileRows + r;
+    const bool live = row < n_rows;
     if (n_mine > 0) {
-      // queries: 16-byte pieces of rows into the swizzled K-major layout, zeros behind the last row and the last dim
-      constexpr int kPieces = DP / 8;
-#pragma unroll 4
-      for (int i = r; i < kTileRows * kPieces; i += kTileRows) {
-        const int rr = i / kPieces, c = i % kPieces;
-        const int64_t g_row = first + rr;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (g_row < rows && c * 8 < a.head_dim) {
-          const int tok = (int)(g_row / a.group), h = (int)(g_row - (int64_t)tok * a.group);
-          v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (q0 + tok) * a.qs + (int64_t)(head * a.group + h) * a.qh + c * 8);
-        }
+      // queries: 16-byte pieces of rows into the swizzled K-major layout, zeros behind the last row and the last dim; a thread has
+      // the same piece of every eighth (or sixteenth) row, all of them on their way at once
+      constexpr int kPieces = DP / 8, kRowStep = kTileRows / kPieces;
+      const int c = r % kPieces;
+      const uint16_t* from = static_cast<const uint16_t*>(a.q) + (int64_t)(q0 + tok0) * a.qs + (int64_t)head * a.group * a.qh + c * 8;
+#pragma unroll
+      for (int k = 0; k < kPieces; ++k) {
+        const int rr = r / kPieces + kRowStep * k, in_cta = t * kTileRows + rr, tok = token_of(in_cta), h = part0 + in_cta - tok * a.group;
+        const bool there = in_cta < n_rows && c * 8 < a.head_dim;
         const uint32_t dst = smem + t * S::kTile + c / 8 * S::kHalf + rr * 128 + ((c % 8) ^ (rr & 7)) * 16;
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(there ? from + tok * a.qs + h * a.qh : static_cast<const uint16_t*>(a.q)),
+                     "r"(there ? 16 : 0)
+                     : "memory");
       }
+      cp_async_commit();
+      cp_async_wait<0>();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(q_ready(t));
     }
-    const int see = sees(live ? row : rows - 1), see_all = n_mine > 0 ? sees(first) : 0;
+    const int see = sees(live ? row : n_rows - 1), see_all = n_mine > 0 ? sees(t * kTileRows) : 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + t * 128 + lanes, o_col = tmem + 256 + t * 128 + lanes;
     const tc::f2 scale2 = tc::pack2(a.scale_log2, a.scale_log2);
@@ -373,8 +378,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_after();
       const float2 two = tc::unpack2(sum2);
       const float sum = two.x + two.y, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const int tok = (int)((live ? row : 0) / a.group), h = (int)((live ? row : 0) - (int64_t)tok * a.group);
-      uint16_t* out = static_cast<uint16_t*>(a.out) + (q0 + tok) * a.os + (int64_t)(head * a.group + h) * a.oh;
+      const int tok = token_of(live ? row : 0), h = part0 + (live ? row : 0) - tok * a.group;
+      uint16_t* out = static_cast<uint16_t*>(a.out) + (int64_t)(q0 + tok0 + tok) * a.os + (int64_t)(head * a.group + h) * a.oh;
 #pragma unroll 1
       for (int c = 0; c < DP; c += 32) {
         uint32_t o[32];
@@ -462,6 +467,7 @@ cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int sm_co
   a.requests = r.requests;
   a.kv_heads = r.kv_heads;
   a.group = r.heads / r.kv_heads;
+  a.group_inv = (65536 + a.group - 1) / a.group;
   a.head_dim = r.head_dim;
   a.queries = r.queries;
   a.keys = r.keys;
