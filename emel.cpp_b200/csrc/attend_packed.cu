@@ -9,7 +9,14 @@
 // taken against follows the true one only when that has passed it by 2^8: only then does O, in TMEM, have to be rescaled.
 //
 // Two matrix products of 128 x 128 x head_dim and 128 x 128 exponentials a tile: at head_dim 128 both take the same time (4096
-// products, 16 exponentials a cycle and SM), at 64 the exponentials bound it.
+// products, 16 exponentials a cycle and SM: 2048 cycles for two row tiles and 128 keys), at 64 the exponentials bound it.  What a
+// row tile waits for, between its last weight and its next score, is the other's time; together they take about 2,900 cycles.
+//
+// us, two prompts of 4100 and 8190 tokens, 32 heads of 128: 756 with weights handed over at once and an arrival a thread, 659 by
+// halves and with registers split, 578 (1,189 TFLOP/s) since queries come by asynchronous copies.  Measured and left out: an issuer of
+// products for each row tile 613 (they fall into step and wait for the same pipes); scores of 64 keys in two buffers a row tile, so
+// that none waits for a mix, 588 (products with 64 columns take longer); weights against a stale maximum, looked at afterwards, 604;
+// an eighth, a quarter of the exponentials by polynomials on the multiply-adds 578, 586.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -59,6 +66,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 template <bool kBf16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   uint32_t r;
@@ -90,19 +102,29 @@ __device__ __forceinline__ void wait_ld(uint32_t (&v)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
 }
 
-// both operands in shared memory, or A in TMEM
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Operands in shared memory go by the low words of their descriptors, the address / 16 and, of values, the step to the next 64 dims;
+// the high words are alike: 8 rows of 128 bytes an atom, 128-byte swizzle
+constexpr uint32_t kDescHigh = (1024 >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t row_desc(uint32_t saddr) { return saddr >> 4 | 1u << 16; }
+// V {keys, dims} as the B operand: 16 keys further 2048 bytes, the next 64 dims kTileKeys * 128
+__device__ __forceinline__ uint32_t value_desc(uint32_t saddr) { return saddr >> 4 | (uint32_t)(kTileKeys * 128 >> 4) << 16; }
+// d (+)= a * b, both operands in shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
       : "memory");
 }
-
-// V {keys, dims} as the B operand: 8 keys of 64 dims an atom, 16 keys further 2048 bytes, the next 64 dims kTileKeys * 128
-__device__ __forceinline__ uint64_t value_desc(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3fffu) | (uint64_t)(kTileKeys * 128 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
-         (uint64_t)2 << 61;
+// the same with A in TMEM
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
+      : "memory");
 }
 
 // Row tiles of request b stand in slots first_slot(b) .. first_slot(b + 1) - 1, of which it may leave one empty: rows before it / 256
@@ -162,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = t * kTileRows;
     return r >= n_rows ? 0 : (sees(min(n_rows, r + kTileRows) - 1) + kTileKeys - 1) / kTileKeys;
   };
-  const int n0 = turns(0), n1 = turns(1), n = max(n0, n1);
+  const int n0 = turns(0), n1 = turns(1), key_tiles = max(n0, n1);
 
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -190,13 +212,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after();
   const uint32_t tmem = tmem_slot;
   int loaded = 0;          // loader: tiles asked for
-  int used = 0;            // MMA warp: tiles waited for
 
   if (warp == kLoadWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     // K tile, V tile, K tile, ... of the walk
     bool alive = true;
-    for (; alive && loaded < 2 * n; ++loaded) {
+    for (; alive && loaded < 2 * key_tiles; ++loaded) {
       const int s = loaded % kStages, j = loaded >> 1;
       if (loaded >= kStages) alive = tc::mbar_wait(empty(s), (loaded / kStages - 1) & 1, &gave_up);
       if (!__all_sync(kAll, alive)) break;
@@ -227,26 +248,43 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t common = 1u << 4 | type << 7 | type << 10 | (uint32_t)(kTileRows >> 4) << 24;
       constexpr uint32_t idesc_s = common | (uint32_t)(kTileKeys >> 3) << 17;
       constexpr uint32_t idesc_o = common | 1u << 16 | (uint32_t)(DP >> 3) << 17;
-      auto stage = [&](int e) { return smem + S::kQ + e % kStages * S::kTile; };
-      auto scores = [&](int t, int e) {
+      // the stages that keys and values are in now, and the parity of their use
+      int k_stage = 0, v_stage = 1;
+      uint32_t k_parity = 0, v_parity = 0;
+      auto next = [&](int& stage, uint32_t& parity) {
+        stage += 2;
+        if (stage >= kStages) {
+          stage -= kStages;
+          parity ^= 1;
+        }
+      };
+      auto scores = [&](int t) {
+        const uint32_t keys = row_desc(smem + S::kQ + k_stage * S::kTile), queries = row_desc(smem + t * S::kTile);
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint32_t off = kk / 4 * S::kHalf + kk % 4 * 32;
-          mma_ss(tmem + t * 128, tc::operand_desc(smem + t * S::kTile + off, 1024), tc::operand_desc(stage(e) + off, 1024), idesc_s, kk > 0);
+          const uint32_t off = (kk / 4 * S::kHalf + kk % 4 * 32) >> 4;
+          mma_ss(tmem + t * 128, queries + off, keys + off, idesc_s, kk > 0);
         }
         tc::mma_commit(s_ready(t));
       };
-      auto wait_tile = [&](int e) {
-        if (e < used) return true;
-        used = e + 1;
-        return tc::mbar_wait(full(e % kStages), e / kStages & 1, &gave_up);
-      };
-      bool alive = true;
-      const int n_of[2] = {n0, n1};
-      for (int j = -1; alive && j < n; ++j) {
-        for (int t = 0; t < kTiles && alive; ++t) {
-          if (j >= 0 && j < n_of[t]) {
-            alive = wait_tile(2 * j + 1);
+      // One issuer for both row tiles, in turns: the products of one run while the other's exponentials are taken.  (An issuer each
+      // let the tiles fall into step and wait for the same pipes: 613 us instead of 578 for 4100 and 8190 tokens.)
+      bool alive = key_tiles == 0 || tc::mbar_wait(full(0), 0, &gave_up);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+        if (alive && (t ? n1 : n0) > 0) {
+          alive = tc::mbar_wait(q_ready(t), 0, &gave_up);
+          if (alive) scores(t);
+        }
+      for (int j = 0; alive && j < key_tiles; ++j) {
+        tc::mma_commit(empty(k_stage));
+        next(k_stage, k_parity);
+        alive = tc::mbar_wait(full(v_stage), v_parity, &gave_up);
+        const uint32_t values = value_desc(smem + S::kQ + v_stage * S::kTile);
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          const int n_mine = t ? n1 : n0;
+          if (j < n_mine) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               alive = alive && tc::mbar_wait(p_ready(t, half), j & 1, &gave_up);
@@ -254,21 +292,16 @@ __global__ void __launch_bounds__(kThreads, 1)
               tc::fence_after();
 #pragma unroll
               for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                tc::mma_f16(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, value_desc(stage(2 * j + 1) + kk * 2048), idesc_o, j > 0 || kk > 0);
+                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, values + (kk * 2048 >> 4), idesc_o, kk > 0 ? 1 : j > 0);
             }
-            if (!alive) break;
-            if (j + 1 == n_of[t]) tc::mma_commit(o_ready(t));
+            if (alive && j + 1 == n_mine) tc::mma_commit(o_ready(t));
           }
-          if (j + 1 < n_of[t]) {
-            alive = wait_tile(2 * j + 2) && (j >= 0 || tc::mbar_wait(q_ready(t), 0, &gave_up));
-            if (!alive) break;
-            tc::fence_after();
-            scores(t, 2 * j + 2);
-          }
+          if (t == 0 && j + 1 < key_tiles) alive = alive && tc::mbar_wait(full(k_stage), k_parity, &gave_up);
+          if (!alive) break;
+          if (j + 1 < n_mine) scores(t);
         }
-        // the tiles of this turn are free once everything issued so far is done
-        if (alive && j >= 0) tc::mma_commit(empty((2 * j + 1) % kStages));
-        if (alive && j + 1 < n) tc::mma_commit(empty((2 * j + 2) % kStages));
+        if (alive) tc::mma_commit(empty(v_stage));
+        next(v_stage, v_parity);
       }
       if (!alive) {
         // let what was issued end
@@ -334,10 +367,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < 128; i += 8)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(__uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1])));
-      const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
-      if (__any_sync(kAll, now > m + kSlack)) {
-        const float next = fmaxf(m, now), f = exp2_fast(m - next);
+        for (int e = 0; e < 4; ++e) top[e] = max_nan(top[e], max_nan(__uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1])));
+      // a NaN stays the maximum: the row's weights are all NaN then
+      const float now = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * a.scale_log2;
+      if (__any_sync(kAll, !(now <= m + kSlack))) {
+        const float next = max_nan(m, now), f = exp2_fast(m - next);
         m = next;
         sum2 = tc::mul2(sum2, tc::pack2(f, f));
         // the mix so far: its last product was issued before these scores, so it is done
@@ -355,21 +389,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const tc::f2 minus_m = tc::pack2(-m, -m);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int half = 0; half < 2; ++half) {
         uint32_t p[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          const tc::f2 x = tc::fma2(tc::pack2u(s[64 * c + 2 * i], s[64 * c + 2 * i + 1]), scale2, minus_m);
-          const float2 xy = tc::unpack2(x);
-          const float e0 = exp2_fast(xy.x), e1 = exp2_fast(xy.y);
+          const float2 x = tc::unpack2(tc::fma2(tc::pack2u(s[64 * half + 2 * i], s[64 * half + 2 * i + 1]), scale2, minus_m));
+          const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
           sum2 = tc::add2(sum2, tc::pack2(e0, e1));
           p[i] = pack16<kBf16>(e0, e1);
         }
-        tc::tmem_st32(s_col + 32 * c, p);
+        tc::tmem_st32(s_col + 32 * half, p);
         tc::tmem_wait_st();
         tc::fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(p_ready(t, c));
+        if (lane == 0) tc::mbar_arrive(p_ready(t, half));
       }
     }
     if (alive && n_mine > 0) alive = tc::mbar_wait(o_ready(t), 0, &gave_up);
@@ -380,23 +413,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float sum = two.x + two.y, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       const int tok = token_of(live ? row : 0), h = part0 + (live ? row : 0) - tok * a.group;
       uint16_t* out = static_cast<uint16_t*>(a.out) + (int64_t)(q0 + tok0 + tok) * a.os + (int64_t)(head * a.group + h) * a.oh;
-#pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32];
-        if (n_mine > 0) {
-          tmem_ld32(o_col + c, o);
-          wait_ld(o);
-        }
+      uint32_t o[DP];
+      if (n_mine > 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t w[4];
+        for (int c = 0; c < DP; c += 32) tmem_ld32(o_col + c, o + c);
+        wait_ld(o);
+      }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = __uint_as_float(o[8 * i + 2 * e]) * inv, y = __uint_as_float(o[8 * i + 2 * e + 1]) * inv;
-            w[e] = inv == 0.0f ? 0u : pack16<kBf16>(x, y);
-          }
-          if (live && c + 8 * i < a.head_dim) *reinterpret_cast<uint4*>(out + c + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+      for (int c = 0; c < DP; c += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = inv == 0.0f ? 0u : pack16<kBf16>(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv);
+        if (live && c < a.head_dim) *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
   }
