@@ -1,26 +1,35 @@
 // Attention of packed prompts of different lengths, on the Blackwell tensor cores.
 //
 // Per request and key / value head, the query rows of the head's group stand behind one another, token after token, so that a
-// short prompt fills tiles of rows too.  A CTA takes 256 of them as two tiles of 128 and walks the keys in tiles of 128:
-//   S = Q K^T       tcgen05.mma, operands in shared memory, K by TMA; S {128 rows, 128 keys} in TMEM, a row a lane
+// short prompt fills tiles of rows too.  A pair of tiles of 128 rows walks the keys in tiles of 128:
+//   S = Q K^T       tcgen05.mma, operands in shared memory, by TMA; S {128 rows, 128 keys} in TMEM, a row a lane
 //   P = exp2(S - m) a thread a row: 128 scores out of TMEM, running maximum and sum, P as 16-bit values back over S
 //   O += P V        tcgen05.mma, P as the A operand out of TMEM, V by TMA as it lies in memory (its dims are contiguous: MN-major)
 // While the warps of one tile take the exponentials, the tensor cores work for the other.  The running maximum a row's weights are
-// taken against follows the true one only when that has passed it by 2^8: only then does O, in TMEM, have to be rescaled.
+// taken against follows the true one only when that has passed it by 2^8: only then does O, in TMEM, have to be rescaled.  Weights
+// are rounded to the operands' 16 bits, as the tensor cores take them; the sum is of the f32 ones.
+//
+// A CTA stays and takes pairs of tiles from a common counter (their walks differ by far): a warp finds the next one and asks for its
+// queries as soon as the last scores against the ones before are done, another asks for keys and values ahead across pairs, another
+// looks at values that not every row may see.  Nothing but the rows' own warps waits while they store results.
 //
 // Two matrix products of 128 x 128 x head_dim and 128 x 128 exponentials a tile: at head_dim 128 both take the same time (4096
 // products, 16 exponentials a cycle and SM: 2048 cycles for two row tiles and 128 keys), at 64 the exponentials bound it.  What a
-// row tile waits for, between its last weight and its next score, is the other's time; together they take about 2,900 cycles.
+// row tile waits for, between its last weight and its next score, is the other's time; together they take about 2,900 cycles, and
+// a pair of tiles about 5,000 besides (first scores, last mix, results).
 //
-// us, two prompts of 4100 and 8190 tokens, 32 heads of 128: 756 with weights handed over at once and an arrival a thread, 659 by
-// halves and with registers split, 578 (1,189 TFLOP/s) since queries come by asynchronous copies.  Measured and left out: an issuer of
-// products for each row tile 613 (they fall into step and wait for the same pipes); scores of 64 keys in two buffers a row tile, so
-// that none waits for a mix, 588 (products with 64 columns take longer); weights against a stale maximum, looked at afterwards, 604;
-// an eighth, a quarter of the exponentials by polynomials on the multiply-adds 578, 586.
+// us, two prompts of 4100 and 8190 tokens / 13 of 17 to 600, 32 heads of 128: 756 with weights handed over at once and an arrival a
+// thread; 659 / 95 by halves and with registers split; 578 / 61 with queries by asynchronous copies; 544 (1,263 TFLOP/s) / 52 since
+// CTAs stay.  One prompt of 8192 and heads of 64: 411 (667 TFLOP/s; its exponentials alone take 252).  Measured and left out: an
+// issuer of products for each row tile 613 / - (they fall into step and wait for the same pipes); scores of 64 keys in two buffers a
+// row tile, so that none waits for a mix, 588 (products with 64 columns take longer); weights against a stale maximum, looked at
+// afterwards, 604; an eighth, a quarter of the exponentials by polynomials on the multiply-adds, no gain, +8.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 #include "paged.h"
 #include "tc_common.cuh"
@@ -30,7 +39,7 @@ namespace {
 
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kTileRows = 128, kTileKeys = 128, kTiles = 2;   // tiles of a CTA
-constexpr int kLoadWarp = 8, kMmaWarp = 9, kThreads = 384;
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kCheckWarp = 10, kPlanWarp = 11, kThreads = 384;   // behind the softmax warps
 // registers a thread behind the start, of the 168 that 384 threads launch with: 8 warps x 208 + 4 x 88 = 12 x 168
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(8 * kSoftmaxRegs + 4 * kOtherRegs <= 12 * 168, "registers");
@@ -43,12 +52,14 @@ struct __align__(64) Map {
 };
 
 struct PackedArgs {
-  const void* q;
+  const void *q, *v;
   void* out;
   const int32_t *query_begin, *key_begin;
-  int64_t qs, qh, os, oh;
-  int requests, kv_heads, group, group_inv, head_dim, queries, keys, max_queries, causal;
+  int64_t qs, qh, vs, vh, os, oh;
+  int requests, kv_heads, group, group_inv, tile_tokens, head_dim, queries, keys, max_queries, causal;
   float scale_log2;
+  int64_t items;
+  int* next;           // the next item, CTAs that are done: zero between launches
   int *bad, *status;
 };
 
@@ -56,9 +67,10 @@ template <int DP>
 struct Smem {
   static constexpr int kHalf = kTileKeys * 128;          // 64 dims of 128 rows
   static constexpr int kTile = DP / 64 * kHalf;
-  static constexpr int kStages = DP == 128 ? 5 : 10;     // of K and V tiles in turn
+  static constexpr int kStages = DP == 128 ? 4 : 8;      // of K and V tiles in turn
   static constexpr int kQ = kTiles * kTile;
-  static constexpr int kBytes = kQ + kStages * kTile + 1024;
+  static constexpr int kTurn = 32 * 128;                 // where a softmax warp's results turn into rows
+  static constexpr int kBytes = kQ + kStages * kTile + 8 * kTurn + 1024;
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -70,6 +82,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+__device__ __forceinline__ uint4 load_shared(uint32_t saddr) {
+  uint4 w;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(saddr) : "memory");
+  return w;
 }
 template <bool kBf16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -127,78 +144,81 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       : "memory");
 }
 
-// Row tiles of request b stand in slots first_slot(b) .. first_slot(b + 1) - 1, of which it may leave one empty: rows before it / 256
-// + b is known from query_begin alone, without a sum over the requests in front.
-__device__ __forceinline__ int64_t first_slot(const PackedArgs& a, int b) {
-  return (int64_t)(a.query_begin[b] - a.query_begin[0]) * a.group / (kTiles * kTileRows) + b;
+// Pairs of row tiles of request b stand in slots first_slot(b) .. first_slot(b + 1) - 1, of which it may leave one empty: tokens
+// before it / (two tiles') + b is known from query_begin alone, without a sum over the requests in front.
+__device__ __forceinline__ int first_slot(const PackedArgs& a, int b) {
+  return (int)((uint32_t)(a.query_begin[b] - a.query_begin[0]) / (uint32_t)(kTiles * a.tile_tokens)) + b;
+}
+
+// two row tiles of a request and key / value head
+struct Item {
+  int valid;                 // 0: no more
+  int token, tokens;         // the first query row and how many
+  int head;
+  int first_key, keys;       // of the request
+  int see;                   // keys that the first token sees, were there no end to them (or keys, if no row is hidden anything)
+  int n0, n1;                // key tiles that either row tile walks
+  int odd;                   // values that are not finite, of keys that only some of the rows see are not in the products
+};
+
+// 16 bits as a float; whether they are an infinity or NaN; z + 0 * w for both halves of w
+template <bool kBf16>
+__device__ __forceinline__ float as_float(uint32_t half) {
+  return kBf16 ? __uint_as_float(half << 16) : __half2float(__ushort_as_half((unsigned short)half));
+}
+template <bool kBf16>
+__device__ __forceinline__ bool odd_half(uint32_t half) {
+  constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
+  return (half & kExp) == kExp;
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t fma_zero(uint32_t z, uint32_t w) {
+  uint32_t r;
+  if (kBf16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0), "r"(z));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0), "r"(z));
+  return r;
 }
 
 template <int DP, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1)
-    attend_packed_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ Map k_map, const __grid_constant__ Map v_map) {
+    attend_packed_kernel(const __grid_constant__ PackedArgs a, const __grid_constant__ Map q_map, const __grid_constant__ Map k_map,
+                         const __grid_constant__ Map v_map) {
   using S = Smem<DP>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t bars[2 * kStages + 5 * kTiles + 2];
+  __shared__ uint64_t bars[3 * kStages + 4 * kTiles + 7];
+  __shared__ Item items[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int gave_up;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t smem = (tc::smem_u32(raw) + 1023u) & ~1023u;
-  const uint32_t bar0 = tc::smem_u32(bars);
+  const uint32_t bar0 = tc::smem_u32(bars), bar1 = bar0 + 24 * kStages, bar2 = bar1 + 32 * kTiles;
   auto full = [&](int s) { return bar0 + 8 * s; };
   auto empty = [&](int s) { return bar0 + 8 * (kStages + s); };
-  auto q_ready = [&](int t) { return bar0 + 8 * (2 * kStages + t); };
-  auto s_ready = [&](int t) { return bar0 + 8 * (2 * kStages + kTiles + t); };
-  auto o_ready = [&](int t) { return bar0 + 8 * (2 * kStages + 2 * kTiles + t); };
-  auto p_ready = [&](int t, int half) { return bar0 + 8 * (2 * kStages + (3 + half) * kTiles + t); };   // 64 keys each
-  const uint32_t raw_bar = bar0 + 8 * (2 * kStages + 5 * kTiles), drain_bar = raw_bar + 8;
-
-  // ---- which rows
-  const int head = blockIdx.x % a.kv_heads;
-  const int64_t slot = blockIdx.x / a.kv_heads;
-  int lo = 0, hi = a.requests;          // first_slot(lo) <= slot, first_slot(hi) > slot (or hi = requests)
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32, b = lo + lane * step;
-    const unsigned before = __ballot_sync(kAll, b < hi && first_slot(a, b) <= slot);
-    const int last = before ? 31 - __clz(before) : 0;
-    hi = min(hi, lo + (last + 1) * step);
-    lo = lo + last * step;
-  }
-  const int b = lo;
-  const int q0 = a.query_begin[b], nq = a.query_begin[b + 1] - q0, k0 = a.key_begin[b], nk = a.key_begin[b + 1] - k0;
-  if (a.query_begin[0] < 0 || q0 < 0 || nq < 0 || nq > a.max_queries || q0 > a.queries - nq || k0 < 0 || nk < 0 || k0 > a.keys - nk) {
-    if (tid == 0) *a.bad = 1;
-    return;
-  }
-  const int64_t rows = (int64_t)nq * a.group;
-  const int64_t tiles = (rows + kTiles * kTileRows - 1) / (kTiles * kTileRows), local = slot - first_slot(a, b);
-  if (local < 0 || local >= tiles) return;
-  // rows of this CTA, counted from its first, which is head `part0` of token tok0; long walks first
-  const int64_t row0 = (tiles - 1 - local) * (kTiles * kTileRows);
-  const int n_rows = (int)min(rows - row0, (int64_t)(kTiles * kTileRows)), tok0 = (int)(row0 / a.group), part0 = (int)(row0 - (int64_t)tok0 * a.group);
-  // (part0 + row) / group by a product: exact, since (part0 + row) * group < 2^16
-  auto token_of = [&](int row) { return (int)((uint32_t)(part0 + row) * a.group_inv >> 16); };
-  // keys that a row sees; row tiles of this CTA walk turns(t) key tiles
-  auto sees = [&](int row) { return a.causal ? max(0, min(nk, nk - nq + tok0 + token_of(row) + 1)) : nk; };
-  auto turns = [&](int t) {
-    const int r = t * kTileRows;
-    return r >= n_rows ? 0 : (sees(min(n_rows, r + kTileRows) - 1) + kTileKeys - 1) / kTileKeys;
-  };
-  const int n0 = turns(0), n1 = turns(1), key_tiles = max(n0, n1);
+  auto landed = [&](int s) { return bar0 + 8 * (2 * kStages + s); };   // values that the check warp hands on as full
+  auto s_ready = [&](int t) { return bar1 + 8 * t; };
+  auto o_ready = [&](int t) { return bar1 + 8 * (kTiles + t); };
+  auto p_ready = [&](int t, int half) { return bar1 + 8 * ((2 + half) * kTiles + t); };   // 64 keys each
+  auto item_full = [&](int n) { return bar2 + 8 * (n & 1); };
+  auto item_empty = [&](int n) { return bar2 + 8 * (2 + (n & 1)); };
+  const uint32_t q_ready = bar2 + 32, q_empty = bar2 + 40, drain_bar = bar2 + 48;
 
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
       tc::mbar_init(full(s), 1);
       tc::mbar_init(empty(s), 1);
+      tc::mbar_init(landed(s), 1);
     }
     for (int t = 0; t < kTiles; ++t) {
-      tc::mbar_init(q_ready(t), kTileRows / 32);
       tc::mbar_init(s_ready(t), 1);
       tc::mbar_init(p_ready(t, 0), kTileRows / 32);
       tc::mbar_init(p_ready(t, 1), kTileRows / 32);
       tc::mbar_init(o_ready(t), 1);
+      tc::mbar_init(item_full(t), 1);
+      tc::mbar_init(item_empty(t), 11);   // all warps but the one that fills it
     }
-    tc::mbar_init(raw_bar, 1);
+    tc::mbar_init(q_ready, 1);
+    tc::mbar_init(q_empty, 1);
     tc::mbar_init(drain_bar, 1);
     gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -207,38 +227,184 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&tmem_slot)), "r"(kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // row / group by a product: exact, since row < 128 and group <= 128
+  auto token_of = [&](int row) { return (int)((uint32_t)row * a.group_inv >> 16); };
+  auto sees = [&](const Item& it, int token) { return max(0, min(it.keys, a.causal ? it.see + token : it.see)); };
+  auto sound = [&](int b) {
+    const int q0 = a.query_begin[b], nq = a.query_begin[b + 1] - q0, k0 = a.key_begin[b], nk = a.key_begin[b + 1] - k0, first = a.query_begin[0];
+    return first >= 0 && q0 >= first && nq >= 0 && nq <= a.max_queries && q0 <= a.queries - nq && k0 >= 0 && nk >= 0 && k0 <= a.keys - nk;
+  };
+  // the w-th item, by a warp; nothing valid where the slot is empty or the request's numbers are out of range
+  auto item_of = [&](int w) {
+    Item it{};
+    const int head = w % a.kv_heads;
+    const int slot = w / a.kv_heads;
+    int lo = 0, hi = a.requests;          // first_slot(lo) <= slot, first_slot(hi) > slot (or hi = requests)
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, b = lo + lane * step;
+      const unsigned before = __ballot_sync(kAll, b < hi && first_slot(a, b) <= slot);
+      const int last = before ? 31 - __clz(before) : 0;
+      hi = min(hi, lo + (last + 1) * step);
+      lo = lo + last * step;
+    }
+    const int b = lo, q0 = a.query_begin[b], nq = a.query_begin[b + 1] - q0, k0 = a.key_begin[b], nk = a.key_begin[b + 1] - k0;
+    const int most = kTiles * a.tile_tokens;
+    const int pairs = (int)(((uint32_t)nq + most - 1) / (uint32_t)most), local = slot - first_slot(a, b);
+    if (sound(b) && local >= 0 && local < pairs) {
+      const int from = (pairs - 1 - local) * most;   // long walks first
+      it.valid = 1;
+      it.token = q0 + from;
+      it.tokens = min(nq - from, most);
+      it.head = head;
+      it.first_key = k0;
+      it.keys = nk;
+      it.see = a.causal ? nk - nq + from + 1 : nk;
+      it.n0 = (sees(it, min(it.tokens, a.tile_tokens) - 1) + kTileKeys - 1) / kTileKeys;
+      it.n1 = it.tokens > a.tile_tokens ? (sees(it, it.tokens - 1) + kTileKeys - 1) / kTileKeys : 0;
+    }
+    return it;
+  };
+  Item it{};
+  if (warp == kPlanWarp) {
+    if (lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &q_map : lane == 1 ? &k_map : &v_map) : "memory");
+    it = item_of(blockIdx.x);
+  }
+  // rows of a tile that no token fills (128 is no multiple of the group): zero for good
+  for (int i = a.tile_tokens * a.group * 8 + tid; i < kTileRows * 8; i += kThreads)
+    for (int h = 0; h < kTiles * DP / 64; ++h) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem + h * S::kHalf + i * 16), "r"(0) : "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = tmem_slot;
-  int loaded = 0;          // loader: tiles asked for
+  int loaded = 0, asked = 0;                       // loader: tiles asked for; plan: items whose queries were
+  uint32_t on_landed = 0, landed_parity = 0;       // bits of stages: the last tile goes by `landed`; which phase comes next
 
-  if (warp == kLoadWarp) {
+  // the CTA's n-th item; `one`: a thread alone takes it for its warp
+  auto take = [&](int n, Item& it, bool one) {
+    bool ok = tc::mbar_wait(item_full(n), n >> 1 & 1, &gave_up);
+    if (!one) ok = __all_sync(kAll, ok);
+    if (!ok) return false;
+    it = items[n & 1];
+    if (!one) __syncwarp();
+    if (one || lane == 0) tc::mbar_arrive(item_empty(n));
+    return it.valid != 0;
+  };
+  // V tiles that are looked at before the products.  Behind the last key stand other rows, of which P = 0 would make NaN where they
+  // hold one: zeroed.  So would a value that is not finite, of a key that only some of the rows see: the product goes without it,
+  // and the rows that do see it add it in the end.
+  auto ragged = [&](const Item& it, int j) { return it.keys - j * kTileKeys < kTileKeys; };
+  auto parted = [&](const Item& it, int j) { return a.causal && (j + 1) * kTileKeys > sees(it, 0); };
+
+  if (warp == kPlanWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    // K tile, V tile, K tile, ... of the walk
+    // items while the others work on the one before: the first by the CTA's number, then from the common counter
     bool alive = true;
-    for (; alive && loaded < 2 * key_tiles; ++loaded) {
-      const int s = loaded % kStages, j = loaded >> 1;
-      if (loaded >= kStages) alive = tc::mbar_wait(empty(s), (loaded / kStages - 1) & 1, &gave_up);
-      if (!__all_sync(kAll, alive)) break;
-      const bool values = loaded & 1;
-      const int left = nk - j * kTileKeys;
-      // behind the last key stand other rows, of which P = 0 would make NaN where they hold one: zeroed before anyone reads them
-      const bool ragged = values && left < kTileKeys;
-      const uint32_t dst = smem + S::kQ + s * S::kTile, bar = ragged ? raw_bar : full(s);
-      if (lane == 0) {
-        tc::mbar_arrive_expect_tx(bar, S::kTile);
-        for (int h = 0; h < DP / 64; ++h) tma_load_3d(dst + h * S::kHalf, values ? &v_map : &k_map, 64 * h, head, k0 + j * kTileKeys, bar);
+    for (int n = 0, w = blockIdx.x;;) {
+      const bool more = alive && w < a.items;
+      if (w != (int)blockIdx.x) it = more ? item_of(w) : Item{};
+      if (it.valid || !more) {
+        if (n >= 2) alive = __all_sync(kAll, tc::mbar_wait(item_empty(n), (n >> 1) - 1 & 1, &gave_up)) && alive;
+        if (alive && lane == 0) {
+          items[n & 1] = it;
+          tc::mbar_arrive(item_full(n));
+        }
       }
-      if (ragged) {
-        __syncwarp();
-        alive = tc::mbar_wait(raw_bar, 0, &gave_up);
-        for (int i = left * 8 + lane; i < kTileKeys * 8; i += 32)
+      if (!more || !alive) break;
+      if (it.valid) {
+        // its queries, once the scores of the item before are done with theirs
+        if (n > 0) alive = __all_sync(kAll, tc::mbar_wait(q_empty, n - 1 & 1, &gave_up));
+        if (alive && lane == 0) {
+          const int tiles = it.tokens > a.tile_tokens ? 2 : 1;
+          tc::mbar_arrive_expect_tx(q_ready, tiles * (DP / 64) * a.tile_tokens * a.group * 128);
+          for (int t = 0; t < tiles; ++t)
+            for (int h = 0; h < DP / 64; ++h)
+              tma_load_3d(smem + t * S::kTile + h * S::kHalf, &q_map, 64 * h, it.head * a.group, it.token + t * a.tile_tokens, q_ready);
+        }
+        asked += alive;
+        ++n;
+      }
+      if (lane == 0) w = atomicAdd(a.next, 1) + gridDim.x;
+      w = __shfl_sync(kAll, w, 0);
+    }
+    if (lane == 0 && atomicAdd(a.next + 1, 1) == (int)gridDim.x - 1) {
+      a.next[0] = 0;
+      a.next[1] = 0;
+    }
+  } else if (warp == kCheckWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    for (int b = blockIdx.x * 32 + lane; b < a.requests; b += gridDim.x * 32)
+      if (!sound(b)) *a.bad = 1;
+    bool alive = true;
+    Item it;
+    for (int n = 0, first = 0; alive && take(n, it, false); ++n) {
+      const int tiles = max(it.n0, it.n1);
+      for (int j = 0; alive && j < tiles; ++j) {
+        const bool some = ragged(it, j), part = parted(it, j);
+        if (!some && !part) continue;
+        const int s = (first + 2 * j + 1) % kStages;
+        alive = __all_sync(kAll, tc::mbar_wait(landed(s), landed_parity >> s & 1, &gave_up));
+        landed_parity ^= 1u << s;
+        if (!alive) break;
+        const uint32_t tile = smem + S::kQ + s * S::kTile;
+        if (some) {
+          for (int i = (it.keys - j * kTileKeys) * 8 + lane; i < kTileKeys * 8; i += 32)
+            for (int h = 0; h < DP / 64; ++h)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + h * S::kHalf + i * 16), "r"(0) : "memory");
+          __syncwarp();
+        }
+        if (part) {
+          const int from = max(0, sees(it, 0) - j * kTileKeys) * 8, to = min(it.keys - j * kTileKeys, kTileKeys) * 8;
+          uint32_t zero = 0;   // sums of 0 * x
           for (int h = 0; h < DP / 64; ++h)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + h * S::kHalf + i * 16), "r"(0) : "memory");
+#pragma unroll 8
+            for (int i = from + lane; i < to; i += 32) {
+              const uint4 w = load_shared(tile + h * S::kHalf + i * 16);
+              zero = fma_zero<kBf16>(fma_zero<kBf16>(fma_zero<kBf16>(fma_zero<kBf16>(zero, w.x), w.y), w.z), w.w);
+            }
+          if (__any_sync(kAll, zero & 0x7fff7fffu)) {
+            for (int h = 0; h < DP / 64; ++h)
+              for (int i = 4 * from + lane; i < 4 * to; i += 32) {
+                const uint32_t at = tile + h * S::kHalf + i * 4;
+                uint32_t w;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at));
+                if (odd_half<kBf16>(w & 0xffffu)) w &= 0xffff0000u;
+                if (odd_half<kBf16>(w >> 16)) w &= 0xffffu;
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(w) : "memory");
+              }
+            if (lane == 0) *const_cast<volatile int*>(&items[n & 1].odd) = 1;
+            __threadfence_block();
+          }
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(full(s));
+      }
+      first = (first + 2 * tiles) % kStages;
+    }
+  } else if (warp == kLoadWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    // K tile, V tile, K tile, ... of the walks
+    bool alive = true;
+    Item it;
+    for (int n = 0; alive && take(n, it, false); ++n) {
+      const int count = 2 * max(it.n0, it.n1);
+      for (int e = 0; e < count; ++e, ++loaded) {
+        const int s = loaded % kStages, j = e >> 1;
+        if (loaded >= kStages) alive = __all_sync(kAll, tc::mbar_wait(empty(s), (loaded / kStages - 1) & 1, &gave_up));
+        if (!alive) break;
+        const bool values = e & 1, check = values && (ragged(it, j) || parted(it, j));
+        if (check) {
+          landed_parity ^= 1u << s;
+          on_landed |= 1u << s;
+        } else {
+          on_landed &= ~(1u << s);
+        }
+        if (lane == 0) {
+          const uint32_t dst = smem + S::kQ + s * S::kTile, bar = check ? landed(s) : full(s);
+          tc::mbar_arrive_expect_tx(bar, S::kTile);
+          for (int h = 0; h < DP / 64; ++h) tma_load_3d(dst + h * S::kHalf, values ? &v_map : &k_map, 64 * h, it.head, it.first_key + j * kTileKeys, bar);
+        }
       }
     }
   } else if (warp == kMmaWarp) {
@@ -248,9 +414,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t common = 1u << 4 | type << 7 | type << 10 | (uint32_t)(kTileRows >> 4) << 24;
       constexpr uint32_t idesc_s = common | (uint32_t)(kTileKeys >> 3) << 17;
       constexpr uint32_t idesc_o = common | 1u << 16 | (uint32_t)(DP >> 3) << 17;
-      // the stages that keys and values are in now, and the parity of their use
+      // the stages that keys and values are in now, and the parity of their use; of a row tile's weights
       int k_stage = 0, v_stage = 1;
-      uint32_t k_parity = 0, v_parity = 0;
+      uint32_t k_parity = 0, v_parity = 0, p_parity[kTiles] = {0, 0};
       auto next = [&](int& stage, uint32_t& parity) {
         stage += 2;
         if (stage >= kStages) {
@@ -267,41 +433,47 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc::mma_commit(s_ready(t));
       };
-      // One issuer for both row tiles, in turns: the products of one run while the other's exponentials are taken.  (An issuer each
-      // let the tiles fall into step and wait for the same pipes: 613 us instead of 578 for 4100 and 8190 tokens.)
-      bool alive = key_tiles == 0 || tc::mbar_wait(full(0), 0, &gave_up);
+      // One issuer for both row tiles, in turns: the products of one run while the other's exponentials are taken
+      bool alive = true;
+      Item it;
+      for (int n = 0; alive && take(n, it, true); ++n) {
+        const int key_tiles = max(it.n0, it.n1);
+        alive = tc::mbar_wait(q_ready, n & 1, &gave_up) && (key_tiles == 0 || tc::mbar_wait(full(k_stage), k_parity, &gave_up));
+        if (!alive) break;
+        tc::fence_after();
+        // an item's first scores go where the last weights of the item before stood, behind the mix that reads those
+        if (it.n0 > 0) scores(0);
+        if (it.n1 > 0) scores(1);
+        if (key_tiles <= 1) tc::mma_commit(q_empty);
+        for (int j = 0; alive && j < key_tiles; ++j) {
+          tc::mma_commit(empty(k_stage));
+          next(k_stage, k_parity);
+          alive = tc::mbar_wait(full(v_stage), v_parity, &gave_up);
+          const uint32_t values = value_desc(smem + S::kQ + v_stage * S::kTile);
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-        if (alive && (t ? n1 : n0) > 0) {
-          alive = tc::mbar_wait(q_ready(t), 0, &gave_up);
-          if (alive) scores(t);
-        }
-      for (int j = 0; alive && j < key_tiles; ++j) {
-        tc::mma_commit(empty(k_stage));
-        next(k_stage, k_parity);
-        alive = tc::mbar_wait(full(v_stage), v_parity, &gave_up);
-        const uint32_t values = value_desc(smem + S::kQ + v_stage * S::kTile);
+          for (int t = 0; t < kTiles; ++t) {
+            const int n_mine = t ? it.n1 : it.n0;
+            if (j < n_mine) {
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          const int n_mine = t ? n1 : n0;
-          if (j < n_mine) {
+              for (int half = 0; half < 2; ++half) {
+                alive = alive && tc::mbar_wait(p_ready(t, half), p_parity[t], &gave_up);
+                if (!alive) break;
+                tc::fence_after();
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              alive = alive && tc::mbar_wait(p_ready(t, half), j & 1, &gave_up);
-              if (!alive) break;
-              tc::fence_after();
-#pragma unroll
-              for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, values + (kk * 2048 >> 4), idesc_o, kk > 0 ? 1 : j > 0);
+                for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                  mma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, values + (kk * 2048 >> 4), idesc_o, kk > 0 ? 1 : j > 0);
+              }
+              p_parity[t] ^= 1;
+              if (alive && j + 1 == n_mine) tc::mma_commit(o_ready(t));
             }
-            if (alive && j + 1 == n_mine) tc::mma_commit(o_ready(t));
+            if (t == 0 && j + 1 < key_tiles) alive = alive && tc::mbar_wait(full(k_stage), k_parity, &gave_up);
+            if (!alive) break;
+            if (j + 1 < n_mine) scores(t);
           }
-          if (t == 0 && j + 1 < key_tiles) alive = alive && tc::mbar_wait(full(k_stage), k_parity, &gave_up);
-          if (!alive) break;
-          if (j + 1 < n_mine) scores(t);
+          if (alive && j + 2 == key_tiles) tc::mma_commit(q_empty);   // the last scores have been issued
+          if (alive) tc::mma_commit(empty(v_stage));
+          next(v_stage, v_parity);
         }
-        if (alive) tc::mma_commit(empty(v_stage));
-        next(v_stage, v_parity);
       }
       if (!alive) {
         // let what was issued end
@@ -311,122 +483,145 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp > kMmaWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    const int t = warp >> 2, r = tid & 127, n_mine = t ? n1 : n0;
-    const int row = t * kTileRows + r;
-    const bool live = row < n_rows;
-    if (n_mine > 0) {
-      // queries: 16-byte pieces of rows into the swizzled K-major layout, zeros behind the last row and the last dim; a thread has
-      // the same piece of every eighth (or sixteenth) row, all of them on their way at once
-      constexpr int kPieces = DP / 8, kRowStep = kTileRows / kPieces;
-      const int c = r % kPieces;
-      const uint16_t* from = static_cast<const uint16_t*>(a.q) + (int64_t)(q0 + tok0) * a.qs + (int64_t)head * a.group * a.qh + c * 8;
-#pragma unroll
-      for (int k = 0; k < kPieces; ++k) {
-        const int rr = r / kPieces + kRowStep * k, in_cta = t * kTileRows + rr, tok = token_of(in_cta), h = part0 + in_cta - tok * a.group;
-        const bool there = in_cta < n_rows && c * 8 < a.head_dim;
-        const uint32_t dst = smem + t * S::kTile + c / 8 * S::kHalf + rr * 128 + ((c % 8) ^ (rr & 7)) * 16;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(there ? from + tok * a.qs + h * a.qh : static_cast<const uint16_t*>(a.q)),
-                     "r"(there ? 16 : 0)
-                     : "memory");
-      }
-      cp_async_commit();
-      cp_async_wait<0>();
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(q_ready(t));
-    }
-    const int see = sees(live ? row : n_rows - 1), see_all = n_mine > 0 ? sees(t * kTileRows) : 0;
+    const int t = warp >> 2, row = tid & 127, token = t * a.tile_tokens + min(token_of(row), a.tile_tokens - 1);   // of the item
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + t * 128 + lanes, o_col = tmem + 256 + t * 128 + lanes;
+    const uint32_t turn = smem + S::kQ + kStages * S::kTile + warp * S::kTurn;
     const tc::f2 scale2 = tc::pack2(a.scale_log2, a.scale_log2);
-    float m = kLowest;
-    tc::f2 sum2 = tc::pack2(0.0f, 0.0f);
+    uint32_t s_parity = 0, o_parity = 0;
     bool alive = true;
-    for (int j = 0; j < n_mine; ++j) {
-      alive = tc::mbar_wait(s_ready(t), j & 1, &gave_up);
-      if (!__all_sync(kAll, alive)) {
-        alive = false;
-        break;
-      }
-      tc::fence_after();
-      uint32_t s[128];
+    // the item stays in shared memory until it is done: this warp's registers hold scores
+    for (int n = 0;; ++n) {
+      alive = __all_sync(kAll, tc::mbar_wait(item_full(n), n >> 1 & 1, &gave_up));
+      const Item& it = items[n & 1];
+      if (!alive || !it.valid) break;
+      const int n_mine = t ? it.n1 : it.n0;
+      const int see = sees(it, min(token, it.tokens - 1)), see_all = sees(it, t * a.tile_tokens);   // of the row, of every row
+      float m = kLowest;
+      tc::f2 sum2 = tc::pack2(0.0f, 0.0f);
+      for (int j = 0; j < n_mine; ++j) {
+        alive = __all_sync(kAll, tc::mbar_wait(s_ready(t), s_parity, &gave_up));
+        if (!alive) break;
+        s_parity ^= 1;
+        tc::fence_after();
+        uint32_t s[128];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_col + 32 * c, s + 32 * c);
-      wait_ld(s);
-      if ((j + 1) * kTileKeys > see_all) {
-        const int in_tile = see - j * kTileKeys;
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_col + 32 * c, s + 32 * c);
+        wait_ld(s);
+        if ((j + 1) * kTileKeys > see_all) {
+          const int in_tile = see - j * kTileKeys;
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (i >= in_tile) s[i] = __float_as_uint(-INFINITY);
-      }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int i = 0; i < 128; ++i)
+            if (i >= in_tile) s[i] = __float_as_uint(-INFINITY);
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 128; i += 8)
+        for (int i = 0; i < 128; i += 8)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top[e] = max_nan(top[e], max_nan(__uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1])));
-      // a NaN stays the maximum: the row's weights are all NaN then
-      const float now = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * a.scale_log2;
-      if (__any_sync(kAll, !(now <= m + kSlack))) {
-        const float next = max_nan(m, now), f = exp2_fast(m - next);
-        m = next;
-        sum2 = tc::mul2(sum2, tc::pack2(f, f));
-        // the mix so far: its last product was issued before these scores, so it is done
-        if (j > 0) {
+          for (int e = 0; e < 4; ++e) top[e] = max_nan(top[e], max_nan(__uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1])));
+        // a NaN stays the maximum: the row's weights are all NaN then
+        const float now = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * a.scale_log2;
+        if (__any_sync(kAll, !(now <= m + kSlack))) {
+          const float next = max_nan(m, now), f = exp2_fast(m - next);
+          m = next;
+          sum2 = tc::mul2(sum2, tc::pack2(f, f));
+          // the mix so far: its last product was issued before these scores, so it is done
+          if (j > 0) {
 #pragma unroll 1
-          for (int c = 0; c < DP; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(o_col + c, o);
-            wait_ld(o);
+            for (int c = 0; c < DP; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_col + c, o);
+              wait_ld(o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tc::tmem_st32(o_col + c, o);
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tc::tmem_st32(o_col + c, o);
+            }
           }
         }
-      }
-      const tc::f2 minus_m = tc::pack2(-m, -m);
+        const tc::f2 minus_m = tc::pack2(-m, -m);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t p[32];
+        for (int half = 0; half < 2; ++half) {
+          uint32_t p[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float2 x = tc::unpack2(tc::fma2(tc::pack2u(s[64 * half + 2 * i], s[64 * half + 2 * i + 1]), scale2, minus_m));
-          const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
-          sum2 = tc::add2(sum2, tc::pack2(e0, e1));
-          p[i] = pack16<kBf16>(e0, e1);
+          for (int i = 0; i < 32; ++i) {
+            const float2 x = tc::unpack2(tc::fma2(tc::pack2u(s[64 * half + 2 * i], s[64 * half + 2 * i + 1]), scale2, minus_m));
+            const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
+            sum2 = tc::add2(sum2, tc::pack2(e0, e1));
+            p[i] = pack16<kBf16>(e0, e1);
+          }
+          tc::tmem_st32(s_col + 32 * half, p);
+          tc::tmem_wait_st();
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(p_ready(t, half));
         }
-        tc::tmem_st32(s_col + 32 * half, p);
-        tc::tmem_wait_st();
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(p_ready(t, half));
       }
-    }
-    if (alive && n_mine > 0) alive = tc::mbar_wait(o_ready(t), 0, &gave_up);
-    alive = __all_sync(kAll, alive);
-    if (alive) {
+      if (alive && n_mine > 0) {
+        alive = __all_sync(kAll, tc::mbar_wait(o_ready(t), o_parity, &gave_up));
+        o_parity ^= 1;
+      }
+      if (!alive) break;
       tc::fence_after();
       const float2 two = tc::unpack2(sum2);
       const float sum = two.x + two.y, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const int tok = token_of(live ? row : 0), h = part0 + (live ? row : 0) - tok * a.group;
-      uint16_t* out = static_cast<uint16_t*>(a.out) + (int64_t)(q0 + tok0 + tok) * a.os + (int64_t)(head * a.group + h) * a.oh;
-      uint32_t o[DP];
-      if (n_mine > 0) {
-#pragma unroll
-        for (int c = 0; c < DP; c += 32) tmem_ld32(o_col + c, o + c);
+      // 64 dims at a time through shared memory, so that a warp stores 128 bytes of a row at once; addresses are made here, not kept
+      // in registers from item to item
+      int l = lane;
+      asm volatile("" : "+r"(l));
+      const int tokens = it.tokens;
+      uint16_t* out = static_cast<uint16_t*>(a.out) + it.token * a.os + (int64_t)it.head * a.group * a.oh;
+#pragma unroll 1
+      for (int half = 0; half < DP / 64; ++half) {
+        if (t * a.tile_tokens >= tokens) break;
+        uint32_t o[64];
+        tmem_ld32(o_col + 64 * half, o);   // of rows that saw nothing (inv = 0): whatever stands there
+        tmem_ld32(o_col + 64 * half + 32, o + 32);
         wait_ld(o);
-      }
+        if (*const_cast<const volatile int*>(&it.odd)) {
+#pragma unroll 1
+          for (int key = sees(it, 0); key < see; ++key)
 #pragma unroll
-      for (int c = 0; c < DP; c += 8) {
-        uint32_t w[4];
+            for (int c = 0; c < 8; ++c) {
+              if (64 * half + 8 * c >= a.head_dim) break;
+              const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.v) + (int64_t)(it.first_key + key) * a.vs +
+                                                              (int64_t)it.head * a.vh + 64 * half + 8 * c);
+              const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          w[e] = inv == 0.0f ? 0u : pack16<kBf16>(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv);
-        if (live && c < a.head_dim) *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t x = word[e / 2] >> 16 * (e & 1) & 0xffffu;
+                if (odd_half<kBf16>(x)) o[8 * c + e] = __float_as_uint(__uint_as_float(o[8 * c + e]) + as_float<kBf16>(x));
+              }
+            }
+        }
+        if (__any_sync(kAll, inv == 0.0f)) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) o[i] = inv == 0.0f ? 0u : o[i];
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = pack16<kBf16>(__uint_as_float(o[8 * c + 2 * e]) * inv, __uint_as_float(o[8 * c + 2 * e + 1]) * inv);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(turn + l * 128 + (c ^ (l & 7)) * 16), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                       : "memory");
+        }
+        __syncwarp();
+        const int c = l & 7;
+        uint4 w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = load_shared(turn + (4 * k + (l >> 3)) * 128 + (c ^ ((4 * k + (l >> 3)) & 7)) * 16);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int to_row = (row & ~31) + 4 * k + (l >> 3), in_tile = token_of(to_row), to = t * a.tile_tokens + in_tile, h = to_row - in_tile * a.group;
+          if (in_tile < a.tile_tokens && to < tokens && 64 * half + 8 * c < a.head_dim)
+            *reinterpret_cast<uint4*>(out + (int64_t)to * a.os + (int64_t)h * a.oh + 64 * half + 8 * c) = w[k];
+        }
+        __syncwarp();
       }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(item_empty(n));
     }
   }
   // a wait that ran out: copies in flight end before the CTA does
@@ -436,9 +631,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kLoadWarp) {
       volatile int own = 0;
       for (int e = max(0, loaded - kStages); e < loaded; ++e) {
+        const int s = e % kStages;
         own = 0;
-        tc::mbar_wait(full(e % kStages), e / kStages & 1, &own);
+        if (on_landed >> s & 1) tc::mbar_wait(landed(s), ~landed_parity >> s & 1, &own);
+        else tc::mbar_wait(full(s), e / kStages & 1, &own);
       }
+    }
+    if (warp == kPlanWarp && asked > 0) {
+      volatile int own = 0;
+      tc::mbar_wait(q_ready, asked - 1 & 1, &own);
     }
   }
   tc::fence_before();
@@ -446,8 +647,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-// rows {keys, kv_heads, head_dim} for boxes of 128 keys of one head, 64 dims wide
-bool encode_rows(Map* map, const void* base, bool bf16, int head_dim, int heads, int keys, int64_t token_stride, int64_t head_stride) {
+// rows {tokens, heads, head_dim} for boxes 64 dims wide
+bool encode_rows(Map* map, const void* base, bool bf16, int head_dim, int heads, int tokens, int64_t token_stride, int64_t head_stride, int box_heads,
+                 int box_tokens) {
   static_assert(sizeof(CUtensorMap) == sizeof(Map), "tensor map size");
   static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
     void* fn = nullptr;
@@ -461,34 +663,35 @@ bool encode_rows(Map* map, const void* base, bool bf16, int head_dim, int heads,
   if (!encode) return false;
   // a stride that no second row or head uses may be anything in the request
   if (heads == 1) head_stride = head_dim;
-  if (keys <= 1) token_stride = (int64_t)head_dim * heads;
-  const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)(keys > 0 ? keys : 1)};
+  if (tokens <= 1) token_stride = (int64_t)head_dim * heads;
+  const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)(tokens > 0 ? tokens : 1)};
   const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
-  const cuuint32_t box[3] = {64, 1, kTileKeys}, steps[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens}, steps[3] = {1, 1, 1};
   return encode(reinterpret_cast<CUtensorMap*>(map), bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
                 dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int DP, bool kBf16>
-cudaError_t launch_one(const PackedArgs& a, const Map& k, const Map& v, cudaStream_t st) {
+cudaError_t launch_one(const PackedArgs& a, const Map& q, const Map& k, const Map& v, int sm_count, cudaStream_t st) {
   const int smem = Smem<DP>::kBytes;
   cudaError_t e = cudaFuncSetAttribute(attend_packed_kernel<DP, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const int64_t slots = (int64_t)a.queries * a.group / (kTiles * kTileRows) + a.requests;
-  if (slots * a.kv_heads > 0x7fffffff) return cudaErrorInvalidValue;
-  attend_packed_kernel<DP, kBf16><<<(unsigned)(slots * a.kv_heads), kThreads, smem, st>>>(a, k, v);
+  attend_packed_kernel<DP, kBf16><<<(unsigned)std::min<int64_t>(a.items, sm_count), kThreads, smem, st>>>(a, q, k, v);
   return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int sm_count, int* bad, int* status, cudaStream_t st) {
+cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int* next, int sm_count, int* bad, int* status, cudaStream_t st) {
   PackedArgs a{};
   a.q = r.q;
   a.out = r.out;
   a.query_begin = r.query_begin;
   a.key_begin = r.key_begin;
+  a.v = r.v;
+  a.vs = r.v_token_stride;
+  a.vh = r.v_head_stride;
   a.qs = r.q_token_stride;
   a.qh = r.q_head_stride;
   a.os = r.out_token_stride;
@@ -497,21 +700,26 @@ cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int sm_co
   a.kv_heads = r.kv_heads;
   a.group = r.heads / r.kv_heads;
   a.group_inv = (65536 + a.group - 1) / a.group;
+  a.tile_tokens = kTileRows / a.group;
   a.head_dim = r.head_dim;
   a.queries = r.queries;
   a.keys = r.keys;
   a.max_queries = r.max_queries;
   a.causal = r.causal != 0;
   a.scale_log2 = r.scale * 1.44269504088896340736f;
+  a.items = ((int64_t)a.queries / (kTiles * a.tile_tokens) + a.requests) * a.kv_heads;
+  if (a.items > 0x3fffffff) return cudaErrorInvalidValue;
+  a.next = next;
   a.bad = bad;
   a.status = status;
   const bool bf16 = r.type == EMELB_BF16;
-  Map k, v;
-  if (!encode_rows(&k, r.k, bf16, r.head_dim, r.kv_heads, r.keys, r.k_token_stride, r.k_head_stride) ||
-      !encode_rows(&v, r.v, bf16, r.head_dim, r.kv_heads, r.keys, r.v_token_stride, r.v_head_stride))
+  Map q, k, v;
+  if (!encode_rows(&q, r.q, bf16, r.head_dim, r.heads, r.queries, r.q_token_stride, r.q_head_stride, a.group, a.tile_tokens) ||
+      !encode_rows(&k, r.k, bf16, r.head_dim, r.kv_heads, r.keys, r.k_token_stride, r.k_head_stride, 1, kTileKeys) ||
+      !encode_rows(&v, r.v, bf16, r.head_dim, r.kv_heads, r.keys, r.v_token_stride, r.v_head_stride, 1, kTileKeys))
     return cudaErrorInvalidValue;
-  if (r.head_dim <= 64) return bf16 ? launch_one<64, true>(a, k, v, st) : launch_one<64, false>(a, k, v, st);
-  return bf16 ? launch_one<128, true>(a, k, v, st) : launch_one<128, false>(a, k, v, st);
+  if (r.head_dim <= 64) return bf16 ? launch_one<64, true>(a, q, k, v, sm_count, st) : launch_one<64, false>(a, q, k, v, sm_count, st);
+  return bf16 ? launch_one<128, true>(a, q, k, v, sm_count, st) : launch_one<128, false>(a, q, k, v, sm_count, st);
 }
 
 }  // namespace emelb

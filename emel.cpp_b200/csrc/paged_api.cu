@@ -259,7 +259,12 @@ uint32_t emelb_attend_packed_can_run(const emelb_attend_packed_request* r) {
                      rows_span(r->v, r->v_token_stride, r->v_head_stride, D, keys, r->kv_heads, size), {r->query_begin, n * 4 + 4}, {r->key_begin, n * 4 + 4}};
   for (const Span& s : in)
     if (!apart(s, out)) return EMELB_INVALID_REQUEST;
-  if (D % 8 != 0 || D > 128 || r->heads / r->kv_heads > 128 || r->kv_heads > 65535) return EMELB_UNSUPPORTED_OP;
+  const int group = r->heads / r->kv_heads;
+  if (D % 8 != 0 || D > 128 || group > 128 || r->kv_heads > 65535) return EMELB_UNSUPPORTED_OP;
+  // pairs of row tiles that the CTAs count, and strides that a tensor map holds
+  if (((int64_t)r->queries / (256 / group) + r->requests) * r->kv_heads > 0x3fffffff) return EMELB_UNSUPPORTED_OP;
+  for (int64_t s : {r->q_token_stride, r->q_head_stride, r->k_token_stride, r->k_head_stride, r->v_token_stride, r->v_head_stride})
+    if (s >= (int64_t)1 << 39) return EMELB_UNSUPPORTED_OP;
   for (const void* p : {r->q, r->k, r->v, (const void*)r->out})
     if (!aligned(p, 16)) return EMELB_UNSUPPORTED_OP;
   for (int64_t s : {r->q_token_stride, r->q_head_stride, r->k_token_stride, r->k_head_stride, r->v_token_stride, r->v_head_stride, r->out_token_stride,
@@ -272,7 +277,7 @@ uint32_t emelb_attend_packed(emelb_ctx* c, const emelb_attend_packed_request* r)
   if (!c || !r) return EMELB_INVALID_REQUEST;
   if (const uint32_t why = emelb_attend_packed_can_run(r)) return refuse(c, why);
   return dispatch(c, {r->q, r->k, r->v, r->out, r->query_begin, r->key_begin}, 1,
-                  [&] { return launch_attend_packed(*r, c->sm_count, c->bad_word(), c->status_word(), c->stream); });
+                  [&] { return launch_attend_packed(*r, c->next_sched(), c->sm_count, c->bad_word(), c->status_word(), c->stream); });
 }
 
 }  // extern "C"

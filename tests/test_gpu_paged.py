@@ -579,6 +579,37 @@ def test_packed_many_requests(be):
     check_packed(be, lengths, lengths, 4, 2, 64, "bf16", 9)
 
 
+@pytest.mark.parametrize("heads,kv,dim,t", [(8, 2, 128, "bf16"), (3, 3, 64, "f16"), (16, 1, 40, "f16")])
+def test_packed_hidden_values_have_no_influence(be, heads, kv, dim, t):
+    """Keys and values that are not finite reach the rows that see them, in their heads and dims, and no other."""
+    lengths, g = [400, 70, 1], gen(heads)
+    n, dt = sum(lengths), plain.TORCH[t]
+    q = torch.randn(n, heads, dim, generator=g, device="cuda").to(dt)
+    k, v = (torch.randn(n, kv, dim, generator=g, device="cuda").to(dt) for _ in range(2))
+    begin = dev([0, 400, 470, 471])
+
+    def run():
+        out = torch.full_like(q, 7.0)
+        torch.cuda.synchronize()
+        assert be.attend_packed(paged.packed_request(q, k, v, out, t, begin, begin, 3, heads, kv, dim, n, n, max_queries=400))
+        assert be.sync()
+        return out
+
+    clean, inf, group, last = run(), float("inf"), heads // kv, kv - 1
+    v[150, last, 5], v[320, 0, dim - 1] = float("nan"), -inf
+    v[440, 0, 33], v[460, 0, 33], v[469, last, 0] = inf, -inf, float("nan")
+    k[468, 0, 2] = float("nan")
+    want = clean.clone()
+    want[150:400, last * group:, 5] = float("nan")
+    want[320:400, :group, dim - 1] = -inf
+    want[440:470, :group, 33] = inf
+    want[460:470, :group, 33] = float("nan")
+    want[469, last * group:, 0] = float("nan")
+    want[468:470, :group] = float("nan")
+    got = run()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(nan=3.0), want.nan_to_num(nan=3.0))
+
+
 def test_packed_reports_values_out_of_range(be):
     g = gen(7)
     q, k, v = (torch.randn(60, 4, 64, generator=g, device="cuda").half() for _ in range(3))
