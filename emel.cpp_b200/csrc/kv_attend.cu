@@ -509,9 +509,10 @@ __global__ void __launch_bounds__(32 * Shape<D, kExact>::kWarps, 1) kv_attend_ke
     const int i = live ? row / a.group : 0;
     const int64_t from = (int64_t)(r.first + i) * a.qs + (int64_t)(head * a.group + (live ? row - i * a.group : 0)) * a.qh;
     off[0] = off[1] = 0;
+    float all_v[J][8];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      float v[8];
+      float (&v)[8] = all_v[j];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = 0.0f;
       if (live) {
@@ -534,7 +535,24 @@ __global__ void __launch_bounds__(32 * Shape<D, kExact>::kWarps, 1) kv_attend_ke
           for (int e = 0; e < 8; ++e) v[e] = load_query(a, at8 + e);
         }
       }
+    }
+    // f16 reaches less far than bf16 and f32: the eight rows go in times the power of two (at most 2^60) that takes their largest value
+    // to 2^13 .. 2^14, and the scores come out times the inverse.  Values 2^27 below it are still normal f16 numbers.
+    float largest = 0.0f;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(all_v[j][e]) < INFINITY ? fabsf(all_v[j][e]) : 0.0f);
+    const uint32_t expo = __reduce_max_sync(kAll, __float_as_uint(largest)) >> 23;
+    const int power = expo ? min(60, 140 - (int)expo) : 0;
+    const float raise = __uint_as_float((uint32_t)(127 + power) << 23);
+    const float unit_score = fminf(fmaxf(a.scale_log2 * __uint_as_float((uint32_t)(127 - power) << 23), 1.2e-38f), 3.0e38f);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      float (&v)[8] = all_v[j];
       float sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= raise;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t hi2 = half2_of(v[2 * e], v[2 * e + 1]);
@@ -667,14 +685,14 @@ __global__ void __launch_bounds__(32 * Shape<D, kExact>::kWarps, 1) kv_attend_ke
         const int e_new = max(scale_exp, big);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float top = fmaxf(fmaxf(score[0][h], score[0][h + 2]), fmaxf(score[1][h], score[1][h + 2])) * a.scale_log2;
+          float top = fmaxf(fmaxf(score[0][h], score[0][h + 2]), fmaxf(score[1][h], score[1][h + 2])) * unit_score;
           top = fmaxf(top, __shfl_xor_sync(kAll, top, 4));
           top = fmaxf(top, __shfl_xor_sync(kAll, top, 8));
           top = fmaxf(top, __shfl_xor_sync(kAll, top, 16));
           top = fmaxf(top, m[h]);
           const float f = exp2_fast((m[h] - top) + (float)(scale_exp - e_new));
           m[h] = top;
-          cap[h] = (top + kSlack) / a.scale_log2;
+          cap[h] = (top + kSlack) / unit_score;
           neg_m[h] = -(top + (float)e_new);
           l[h] *= f;
 #pragma unroll
@@ -689,7 +707,7 @@ __global__ void __launch_bounds__(32 * Shape<D, kExact>::kWarps, 1) kv_attend_ke
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) score[u][e] = exp2_fast(fmaf(score[u][e], a.scale_log2, neg_m[e & 1]));
+        for (int e = 0; e < 4; ++e) score[u][e] = exp2_fast(fmaf(score[u][e], unit_score, neg_m[e & 1]));
         l[0] += score[u][0] + score[u][2];
         l[1] += score[u][1] + score[u][3];
       }

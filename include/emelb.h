@@ -139,7 +139,8 @@ typedef struct emelb_ctx emelb_ctx;
  * allocation happens in any dispatch call afterwards. ---- */
 EMELB_API uint32_t emelb_create(int device, emelb_ctx** out);
 EMELB_API uint32_t emelb_destroy(emelb_ctx* ctx);
-/* waits for the context's stream; EMELB_INTERNAL_ERROR on a CUDA error */
+/* waits for the context's stream; EMELB_INTERNAL_ERROR on a CUDA error,
+ * EMELB_INVALID_REQUEST when a call of emelb_paged.h met values out of range */
 EMELB_API uint32_t emelb_sync(emelb_ctx* ctx);
 /* the cudaStream_t all work of this context is enqueued on */
 EMELB_API uint32_t emelb_get_stream(emelb_ctx* ctx, void** stream_out);

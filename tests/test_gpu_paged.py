@@ -373,12 +373,13 @@ def attend_bound(q, k, v, out, size, total, t, scale):
     return rel * size + tiny + plain.HALF_STEP[t] * out.abs() + 1e-30
 
 
-def check_attend(be, lengths, rows, heads, kv, dim, page, t, seed, gain=(1.0, 1.0), layout="dense", begin=True, before=0, after=0):
-    """Requests with `rows` query rows each."""
+def check_attend(be, lengths, rows, heads, kv, dim, page, t, seed, gain=(1.0, 1.0), layout="dense", begin=True, before=0, after=0, q_gain=1.0):
+    """Requests with `rows` query rows each; q_gain: a number, or one for each head."""
     rng, g = np.random.default_rng(seed), gen(seed)
     c, table, k, v = filled(be, rng, g, lengths, page, kv, dim, gain)
     total = before + sum(rows) + after
-    q = placed(torch.randn((max(total, 1), heads, dim), generator=g, device="cuda") * 1.5, layout, plain.TORCH[t])
+    q_gain = torch.as_tensor(q_gain, device="cuda").reshape(1, -1, 1)
+    q = placed(torch.randn((max(total, 1), heads, dim), generator=g, device="cuda") * 1.5 * q_gain, layout, plain.TORCH[t])
     out = placed(torch.full((max(total, 1), heads, dim), 7.0, device="cuda"), layout, plain.TORCH[t])
     qb = np.concatenate([[before], before + np.cumsum(rows)])
     keep = [dev(lengths), dev(qb.tolist())]
@@ -391,7 +392,7 @@ def check_attend(be, lengths, rows, heads, kv, dim, page, t, seed, gain=(1.0, 1.
     first = out.clone()
     at = 0
     for b, (length, n) in enumerate(zip(lengths, rows)):
-        qr = q[qb[b]:qb[b + 1]].double().half().double() if t != "f32" else q[qb[b]:qb[b + 1]].double()
+        qr = q[qb[b]:qb[b + 1]].double()
         want, size, tot = plain.attention(qr, k[at:at + length], v[at:at + length], scale)
         bound = attend_bound(qr, k[at:at + length], v[at:at + length], want, size, tot, t, scale)
         err = (got[qb[b]:qb[b + 1]] - want).abs()
@@ -438,6 +439,15 @@ def test_attend_many_requests(be, n, lo, hi, heads, kv, dim):
 @pytest.mark.parametrize("t", ["bf16", "f32"])
 def test_attend_magnitudes(be, gain, t):
     check_attend(be, [700, 31], [1, 1], 8, 2, 128, 16, t, 5, gain=gain)
+
+
+@pytest.mark.parametrize("t,q_gain,k_gain", [
+    ("bf16", 1e6, 2e-6), ("f32", 1e6, 2e-6), ("bf16", 1e-6, 1e5), ("f32", 1e-6, 1e5), ("f16", 5e3, 2e-4), ("f16", 1e-4, 1e4),
+    ("bf16", [1e5, 1e3, 1e4, 1e2, 1e3, 1e3, 1e5, 1e2], 1e-3), ("f32", [1e-5, 1e-3, 1e-4, 1e-2, 1e-3, 1e-3, 1e-5, 1e-2], 1.0),
+])
+def test_attend_query_magnitudes(be, t, q_gain, k_gain):
+    """Queries far outside of f16's range."""
+    check_attend(be, [700, 31, 64], [1, 3, 1], 8, 2, 64, 16, t, 6, gain=(k_gain, 1.0), q_gain=q_gain)
 
 
 @pytest.mark.parametrize("layout", ["heads", "part", "odd"])
