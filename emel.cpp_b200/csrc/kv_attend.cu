@@ -1,16 +1,24 @@
 // Attention of a few query rows a request over the pages of the 4-bit key / value cache.
 //
 // The cache is read once: 18 bytes for 32 values, so HBM bounds it, with about 25 instructions of a warp to each token of a head
-// at that rate.  What keeps it under them: the cache is the A operand of mma.sync.m16n8k16 (16 tokens, or 16 dims, a side), the query
+// at that rate.  What keeps it near them: the cache is the A operand of mma.sync.m16n8k16 (16 tokens, or 16 dims, a side), the query
 // rows of a group of heads the other (8 of them, none of a tile wasted on a group of 8), so tokens and not heads fill the
 // tiles; quants become f16 by one lop3 a pair, as a power of two + q, and what that is above q - 8 leaves the scores through the
-// tensor cores too (one tf32 product a tile), the values by an addition, since sums over tokens would not survive it; a key's scale multiplies its sum of 32 products in f32, a value's scale joins the softmax weight;
-// weights turn from accumulators into operands by movmatrix.
+// tensor cores too (one tf32 product a tile), the values by an addition, since sums over tokens would not survive it; a key's scale
+// multiplies its sum of 32 products in f32, a value's scale joins the softmax weight; weights turn from accumulators into operands
+// by movmatrix.
 //
 // All steps of 32 tokens of all (request, key / value head, 8 rows) stand in one line, which the units share evenly, whatever the
 // requests' lengths.  A unit is a team of 1 to 12 warps, each with a ring of tiles of its own that asynchronous copies fill; the team
 // takes every tile in turn and joins its warps' results in shared memory.  What a unit has of a (request, head) that others
 // share goes to scratch, and the last to arrive joins the parts in the units' order, so results do not depend on timing.
+//
+// 64 requests of 1000 to 8000 tokens, 64 heads on 8 of 128: 139 us with steps of 16 tokens, 131 with 32 (one maximum, one exchange
+// for both), 116 with asynchronous copies in place of bulk ones (no barrier to wait at), 94 since a team takes whole pairs where
+// that costs no more, 90 (3.7 TB/s) with joins in the order of the fragments.  What bounds it is issue: about 300 instructions to 16
+// tokens of a head, two of the four that an SM could issue a cycle.  One document of 100,001 tokens and 16 rows reads as two tiles of
+// rows, each unpacked for itself: 68 us, 78 with both in one warp (registers).  12 warps with 168 registers do better than 16 with
+// 128 (105 us).  Small calls are a chain: the line from the lengths, the first tiles from memory, the joins.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -48,9 +56,12 @@ struct AttendArgs {
   int* bad;
 };
 
-template <int D, bool kExact>
+// what results are of: how far a softmax weight times a value's scale is rounded goes by it
+enum Kind { kBf16, kF16, kF32 };
+
+template <int D, Kind kind>
 struct Shape {
-  static constexpr int kWarps = kExact ? 8 : 12;   // one CTA an SM: 255 registers a thread, or 168
+  static constexpr int kWarps = kind == kF32 ? 8 : 12;   // one CTA an SM: 255 registers a thread, or 168
   static constexpr int kRows = 8;
   static constexpr int kStages = D == 128 ? 2 : D == 32 ? 4 : 3;
   static constexpr int kStage = 2 * Tile<D>::kBytes;
@@ -221,12 +232,15 @@ __device__ __forceinline__ void team_barrier(int team, int threads) {
   else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(threads) : "memory");
 }
 
-// kExact: f32 queries and results; the queries and the weights then go in as two f16 operands each
-template <int D, bool kExact>
-__global__ void __launch_bounds__(32 * Shape<D, kExact>::kWarps, 1) kv_attend_kernel(const __grid_constant__ AttendArgs a) {
+// kF32: the queries and the weights go in as two f16 operands each.  kF16: a weight's low part goes into its product with the scale,
+// so that there is one rounding to f16 and not two (one document of 100,001 tokens: 71 us for 68, its error against exact results 1.3
+// and not 1.6 times what the results' own rounding makes)
+template <int D, Kind kind>
+__global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kernel(const __grid_constant__ AttendArgs a) {
   using T = Tile<D>;
-  using S = Shape<D, kExact>;
+  using S = Shape<D, kind>;
   constexpr int kWarps = S::kWarps, kThreads = 32 * kWarps;
+  constexpr bool kExact = kind == kF32, kFine = kind == kF16;
   constexpr int J = T::kGroups, kRows = S::kRows, kStages = S::kStages, kParts = kExact ? 2 : 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ i64 sums[3][kWarps];
@@ -716,7 +730,7 @@ __global__ void __launch_bounds__(32 * Shape<D, kExact>::kWarps, 1) kv_attend_ke
       for (int u = 0; u < 2; ++u) {
         const int tile = u * T::kBytes, t0 = token0 + 16 * u;
         // scales of this lane's four tokens, and the weights as operands
-        uint32_t dv[J][2], pf[2];
+        uint32_t dv[J][2], pf[2], low[2];
         if constexpr (J % 2 == 0) {
 #pragma unroll
           for (int j = 0; j < J; j += 2) {
@@ -739,16 +753,24 @@ __global__ void __launch_bounds__(32 * Shape<D, kExact>::kWarps, 1) kv_attend_ke
             }
         }
         if constexpr (!kExact) {
-          pf[0] = turn8x8(half2_of(score[u][0], score[u][1]));
-          pf[1] = turn8x8(half2_of(score[u][2], score[u][3]));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t two = half2_of(score[u][2 * h], score[u][2 * h + 1]);
+            pf[h] = turn8x8(two);
+            if constexpr (kFine) low[h] = turn8x8(half2_of(score[u][2 * h] - low_of(two), score[u][2 * h + 1] - high_of(two)));
+          }
         }
         uint32_t vw[kVV];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           uint32_t bf[kParts][2];
           if constexpr (!kExact) {
-            bf[0][0] = tc::h2_bits(__hmul2(tc::bits_h2(pf[0]), tc::bits_h2(dv[j][0])));
-            bf[0][1] = tc::h2_bits(__hmul2(tc::bits_h2(pf[1]), tc::bits_h2(dv[j][1])));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const __half2 d = tc::bits_h2(dv[j][h]);
+              const __half2 p = kFine ? __hfma2(tc::bits_h2(pf[h]), d, __hmul2(tc::bits_h2(low[h]), d)) : __hmul2(tc::bits_h2(pf[h]), d);
+              bf[0][h] = tc::h2_bits(p);
+            }
           } else {
             // in f32, tokens g and g + 8 a lane, then as two f16
 #pragma unroll
@@ -913,13 +935,13 @@ __global__ void __launch_bounds__(32 * Shape<D, kExact>::kWarps, 1) kv_attend_ke
   }
 }
 
-template <int D, bool kExact>
+template <int D, Kind kind>
 cudaError_t launch_one(const AttendArgs& a, int sm_count, cudaStream_t st) {
-  using S = Shape<D, kExact>;
+  using S = Shape<D, kind>;
   const int smem = S::kSmem;
-  cudaError_t e = cudaFuncSetAttribute(kv_attend_kernel<D, kExact>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(kv_attend_kernel<D, kind>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kv_attend_kernel<D, kExact><<<sm_count, 32 * S::kWarps, smem, st>>>(a);
+  kv_attend_kernel<D, kind><<<sm_count, 32 * S::kWarps, smem, st>>>(a);
   return cudaGetLastError();
 }
 template <int D>
@@ -929,8 +951,8 @@ cudaError_t launch_dim(AttendArgs& a, const KvAttendScratch& s, int sm_count, cu
   units = units < s.stats_floats / (4 * rows) ? units : s.stats_floats / (4 * rows);
   units = units < s.arrived_ints ? units : s.arrived_ints;
   a.most_units = (int)units;
-  if (a.type == EMELB_F32) return launch_one<D, true>(a, sm_count, st);
-  return launch_one<D, false>(a, sm_count, st);
+  if (a.type == EMELB_F32) return launch_one<D, kF32>(a, sm_count, st);
+  return a.type == EMELB_F16 ? launch_one<D, kF16>(a, sm_count, st) : launch_one<D, kBf16>(a, sm_count, st);
 }
 
 }  // namespace
