@@ -3,6 +3,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kv_tile.cuh"
@@ -23,7 +24,8 @@ typedef long long i64;
 // look a new page up where it comes from and not in the table, so that no CTA waits for another.  What is read and what is written
 // do not meet, but for `lengths` and free_left where they are `cached` and free_count: with more than one CTA those wait in scratch
 // for a second launch.
-// 1000 requests, 121,984 rows: 21 us by a cluster of 8 CTAs with a barrier between pages and rows, whose rows took half of it.
+// 1000 requests, 121,984 rows: 12.8 us, 21 by a cluster of 8 CTAs with a barrier between pages and rows, whose rows took half of it.
+// Its 1.6 MB take 0.3 us of bandwidth: what is left is the chain of sums, bisection and stores behind a launch.
 constexpr int kPlanMost = EMELB_KV_MAX_REQUESTS;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -295,14 +297,32 @@ struct Eight {
 // A CTA takes 16 packed rows of one head.  Four lanes share a group of 32 values, 8 each, which is a word of keys; the scale
 // comes from the group's largest value by two shuffles.  Values go by bytes, each with its own address: they wait in shared memory
 // until a warp can store one pair of dims of 16 rows at a time, which are neighbours where the rows fill a tile.
+// 32,760 rows of 8 heads of 128 f16: 47 us (3.6 TB/s), 90 with divisions, 50 with the largest value looked for one by one.  Issue
+// bounds it (0.8 of the cycles), some 150 instructions to 8 values of a warp; memory alone would take 26.
 struct StoreArgs {
   uint8_t* data;
   const void *k, *v;
   const int64_t* slots;
   int64_t ks, kh, vs, vh, limit, page_bytes;
-  int tokens, page_shift, vec;
+  int tokens, heads, page_shift, vec;
   int* bad;
 };
+
+// the larger, the smaller of either half's values; NaN if one is
+template <class E>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (std::is_same<E, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <class E>
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (std::is_same<E, __half>::value) asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 
 constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23: a sum with it has the rounded addend in its low bits
 
@@ -315,18 +335,36 @@ constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23: a sum with it has the rou
 template <class E>
 __device__ __forceinline__ void quantize8(const Eight<E>& in, __half& scale, uint32_t (&bits)[8]) {
   float x[8], top = 0.0f, low = 0.0f;
-  bool nan = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = Elem<E>::in(in.e[i]);
-    top = fmaxf(top, x[i]);
-    low = fminf(low, x[i]);
-    nan |= x[i] != x[i];
+  for (int i = 0; i < 8; ++i) x[i] = Elem<E>::in(in.e[i]);
+  bool nan = false, look = true;
+  if constexpr (sizeof(E) == 2) {
+    // two values an instruction; in the end the largest stands beside the least, negated, and a NaN in either's place
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(in.e);
+    const uint32_t hi = max2<E>(max2<E>(w[0], w[1]), max2<E>(w[2], w[3])), lo = min2<E>(min2<E>(w[0], w[1]), min2<E>(w[2], w[3])) ^ 0x80008000u;
+    uint32_t both = max2<E>(__byte_perm(hi, lo, 0x5410), __byte_perm(hi, lo, 0x7632));
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) both = max2<E>(both, __shfl_xor_sync(kAll, both, o));
+    Eight<E> ends;
+    *reinterpret_cast<uint32_t*>(ends.e) = both;
+    const float most = Elem<E>::in(ends.e[0]), least = -Elem<E>::in(ends.e[1]);
+    look = __any_sync(kAll, most != most || least != least);
+    top = fmaxf(most, 0.0f);
+    low = fminf(least, 0.0f);
   }
+  if (look) {
+    top = low = 0.0f;
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
-    low = fminf(low, __shfl_xor_sync(kAll, low, o));
+    for (int i = 0; i < 8; ++i) {
+      top = fmaxf(top, x[i]);
+      low = fminf(low, x[i]);
+      nan |= x[i] != x[i];
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
+      low = fminf(low, __shfl_xor_sync(kAll, low, o));
+    }
   }
   float m = top > -low ? top : low;
   if (__any_sync(kAll, top == -low && top > 0.0f)) {
@@ -355,9 +393,9 @@ __device__ __forceinline__ void quantize8(const Eight<E>& in, __half& scale, uin
       if (xs < (q - 8.5f) * ds && q > 0.0f) bits[i] -= 1;
       else if (xs >= (q - 7.5f) * ds && q < 15.0f && d != 0.0f) bits[i] += 1;
     }
-    if (d == 0.0f) bits[i] = __float_as_uint(kMagic + 8.0f);
+    if (sizeof(E) == 4 && d == 0.0f) bits[i] = __float_as_uint(kMagic + 8.0f);   // 16 bits: 0 * x + b has rounded to it
   }
-  if (__any_sync(kAll, nan)) {
+  if (look && __any_sync(kAll, nan)) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (x[i] != x[i]) bits[i] = __float_as_uint(kMagic + 8.0f);
@@ -371,7 +409,7 @@ __global__ void __launch_bounds__(128) kv_store_kernel(const StoreArgs a) {
   __shared__ uint8_t* base[kTile];              // the row's tile of this head; null: skipped
   __shared__ int place[kTile];
   __shared__ __align__(16) uint8_t bytes[kTile][D / 2 + 4];   // values, a pair of dims a byte
-  const int tid = threadIdx.x, head = blockIdx.y, row0 = blockIdx.x * kTile;
+  const int tid = threadIdx.x, head = blockIdx.x % a.heads, row0 = blockIdx.x / a.heads * kTile;
   if (tid < kTile) {
     uint8_t* p = nullptr;
     int tau = 0;
@@ -439,7 +477,7 @@ struct LoadArgs {
   void *k, *v;
   const int32_t *table, *first, *lengths, *row_begin;
   int64_t table_stride, ks, kh, vs, vh, page_bytes;
-  int requests, table_width, rows, pages, page_shift, vec;
+  int requests, heads, table_width, rows, pages, page_shift, vec;
   int* bad;
 };
 
@@ -456,85 +494,61 @@ __device__ __forceinline__ void dequantize8(uint32_t word, __half scale, Eight<E
   }
 }
 
-constexpr int kWindow = 127;   // requests behind the first row's whose beginnings are looked at together
-
+// A CTA takes a tile of a request and head: its 18 * D bytes by 16-byte loads, then rows of 8 values a thread.  Request b's tiles stand
+// in slots row_begin[b] / 16 + b * spare and further (two spare ones where its first position may lie inside a tile, else one), so a
+// slot finds its request by bisection, without a sum over the requests in front; heads are neighbours, whose rows are.
+// 32,760 rows of 8 heads of 128 f16: 37 us (4.6 TB/s); 44 when a CTA took 16 packed rows, each with a place of its own in the pages.
+// Memory bounds it, and the three reads in a row before its first byte.
 template <int D, class E>
 __global__ void __launch_bounds__(128) kv_load_kernel(const LoadArgs a) {
   using T = Tile<D>;
-  __shared__ const uint8_t* base[kTile];
-  __shared__ int place[kTile];
-  __shared__ int begins[kWindow + 1];
-  __shared__ __align__(16) uint8_t bytes[kTile][D / 2 + 4];
-  const int tid = threadIdx.x, head = blockIdx.y, row0 = blockIdx.x * kTile;
-  // the request of the first row: how many begin at or before it
-  int before = 0;
-  for (int b0 = 0; b0 < a.requests; b0 += 128) before += __syncthreads_count(b0 + tid < a.requests && a.row_begin[b0 + tid] <= row0);
-  const int b0 = max(before - 1, 0);
-  begins[tid] = a.row_begin[min(b0 + tid, a.requests)];
-  __syncthreads();
-  if (tid < kTile) {
-    const uint8_t* p = nullptr;
-    int tau = 0;
-    const int row = row0 + tid;
-    // the last request that begins at or before the row: in the window, or past it one by one
-    int lo = 0, hi = min(kWindow, a.requests - b0);
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (begins[mid] <= row) lo = mid;
-      else hi = mid - 1;
-    }
-    int b = b0 + lo;
-    if (lo == kWindow)
-      while (b < a.requests && a.row_begin[b + 1] <= row) ++b;
-    if (row < a.rows && b < a.requests && row >= begins[0]) {
-      const int begin = b - b0 <= kWindow ? begins[b - b0] : a.row_begin[b];
-      const int length = a.lengths[b];
-      const int64_t from = a.first ? a.first[b] : 0, pos = from + row - begin;
-      if (from < 0 || pos < from) *a.bad = 1;
-      else if (pos < length) {
-        const int64_t col = pos >> a.page_shift;
-        const int page = col < a.table_width ? a.table[b * a.table_stride + col] : -1;
-        if (page < 0 || page >= a.pages) *a.bad = 1;
-        else {
-          const int in_page = (int)(pos & ((1 << a.page_shift) - 1)), tiles = 1 << (a.page_shift - 4);
-          p = a.data + page * a.page_bytes + (int64_t)(head * tiles + (in_page >> 4)) * T::kBytes;
-          tau = in_page & 15;
-        }
-      }
-    }
-    base[tid] = p;
-    place[tid] = tau;
+  __shared__ __align__(16) uint8_t tile[T::kBytes];
+  const int tid = threadIdx.x, lane = tid & 31, slot = blockIdx.x / a.heads, head = blockIdx.x % a.heads, spare = a.first ? 2 : 1;
+  if (head == 0 && tid == 127 && slot < a.requests && (a.row_begin[slot] < 0 || a.row_begin[slot + 1] < a.row_begin[slot])) *a.bad = 1;
+  int lo = 0, hi = a.requests;          // the last request whose slots begin at or before this one
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, b = lo + lane * step;
+    const unsigned before = __ballot_sync(kAll, b < hi && (a.row_begin[b] >> 4) + b * spare <= slot);
+    const int last = before ? 31 - __clz(before) : 0;
+    hi = min(hi, lo + (last + 1) * step);
+    lo += last * step;
   }
-  __syncthreads();
-  {
-    const int row = tid & 15, g = tid >> 4;
-    const uint8_t* p = base[row];
-    if (p) {
-      p += T::value_byte(place[row], 2 * g);
-      uint8_t v[D / 16];
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) v[i] = p[T::value_byte(0, 16 * i) - T::value_byte(0, 0)];
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) bytes[row][8 * i + g] = v[i];
-    }
+  const int b = lo, begin = a.row_begin[b], end = min(a.row_begin[b + 1], a.rows);
+  const int64_t length = a.lengths[b], first = a.first ? a.first[b] : 0;
+  if (begin < 0 || end <= begin) return;
+  if (first < 0) {
+    if (tid == 0) *a.bad = 1;
+    return;
   }
+  // positions first .. until - 1 go to rows begin and further
+  const int64_t until = min(first + (end - begin), length), at = ((first >> 4) + slot - ((begin >> 4) + b * spare)) * kTile;
+  const int from = (int)max(first - at, (int64_t)0), to = (int)min(until - at, (int64_t)kTile);
+  if (at < 0 || from >= to) return;
+  const int64_t col = at >> a.page_shift;
+  const int page = col < a.table_width ? a.table[b * a.table_stride + col] : -1;
+  if (page < 0 || page >= a.pages) {
+    if (tid == 0) *a.bad = 1;
+    return;
+  }
+  const uint8_t* p = a.data + page * a.page_bytes + (int64_t)((head << (a.page_shift - 4)) + (int)(at >> 4 & ((1 << (a.page_shift - 4)) - 1))) * T::kBytes;
+#pragma unroll
+  for (int i = 0; i < T::kBytes / 16; i += 128)
+    if (i + tid < T::kBytes / 16) reinterpret_cast<uint4*>(tile)[i + tid] = reinterpret_cast<const uint4*>(p)[i + tid];
+  __syncthreads();
   constexpr int kOcts = D / 8;
-  for (int w = tid; w < kTile * kOcts; w += 128) {
-    const int row = w / kOcts, o = w % kOcts, j = o >> 2, t = o & 3;
-    const uint8_t* p = base[row];
-    if (!p) continue;
+  const int64_t row0 = begin + (at - first);
+#pragma unroll
+  for (int k = 0; k < kTile * kOcts; k += 128) {
+    const int w = tid + k, tau = w / kOcts, o = w % kOcts, j = o >> 2, t = o & 3;
+    if (tau < from || tau >= to) continue;
     Eight<E> x;
-    dequantize8<true>(*reinterpret_cast<const uint32_t*>(p + T::key_word(place[row], j, t)), *reinterpret_cast<const __half*>(p + T::key_scale(place[row], j)), x);
-    x.store(static_cast<E*>(a.k) + (int64_t)(row0 + row) * a.ks + head * a.kh + 8 * o, a.vec);
-  }
-  __syncthreads();
-  for (int w = tid; w < kTile * kOcts; w += 128) {
-    const int row = w / kOcts, o = w % kOcts, j = o >> 2;
-    const uint8_t* p = base[row];
-    if (!p) continue;
-    Eight<E> y;
-    dequantize8<false>(*reinterpret_cast<const uint32_t*>(&bytes[row][4 * o]), *reinterpret_cast<const __half*>(p + T::value_scale(place[row], j)), y);
-    y.store(static_cast<E*>(a.v) + (int64_t)(row0 + row) * a.vs + head * a.vh + 8 * o, a.vec);
+    dequantize8<true>(*reinterpret_cast<const uint32_t*>(tile + T::key_word(tau, j, t)), *reinterpret_cast<const __half*>(tile + T::key_scale(tau, j)), x);
+    x.store(static_cast<E*>(a.k) + (row0 + tau) * a.ks + head * a.kh + 8 * o, a.vec);
+    uint32_t two[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) two[e] = tile[T::value_byte(tau, 8 * o + 2 * e)];
+    dequantize8<false>(two[0] | two[1] << 8 | two[2] << 16 | two[3] << 24, *reinterpret_cast<const __half*>(tile + T::value_scale(tau, j)), x);
+    x.store(static_cast<E*>(a.v) + (row0 + tau) * a.vs + head * a.vh + 8 * o, a.vec);
   }
 }
 
@@ -549,7 +563,7 @@ bool rows_aligned(const void* p, int64_t token, int64_t head, size_t size) {
 size_t size_of(int type) { return type == EMELB_F32 ? 4 : 2; }
 
 template <class E>
-cudaError_t store_typed(int D, dim3 grid, const StoreArgs& a, cudaStream_t st) {
+cudaError_t store_typed(int D, unsigned grid, const StoreArgs& a, cudaStream_t st) {
   switch (D) {
     case 32: kv_store_kernel<32, E><<<grid, 128, 0, st>>>(a); break;
     case 64: kv_store_kernel<64, E><<<grid, 128, 0, st>>>(a); break;
@@ -559,7 +573,7 @@ cudaError_t store_typed(int D, dim3 grid, const StoreArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 template <class E>
-cudaError_t load_typed(int D, dim3 grid, const LoadArgs& a, cudaStream_t st) {
+cudaError_t load_typed(int D, unsigned grid, const LoadArgs& a, cudaStream_t st) {
   switch (D) {
     case 32: kv_load_kernel<32, E><<<grid, 128, 0, st>>>(a); break;
     case 64: kv_load_kernel<64, E><<<grid, 128, 0, st>>>(a); break;
@@ -602,10 +616,11 @@ cudaError_t launch_kv_store(const emelb_kv_store_request& r, int* bad, cudaStrea
   a.limit = (int64_t)r.cache.pages * r.cache.page_tokens;
   a.page_bytes = (int64_t)emelb_kv_page_bytes(r.cache.head_dim, r.cache.kv_heads, r.cache.page_tokens);
   a.tokens = r.tokens;
+  a.heads = r.cache.kv_heads;
   a.page_shift = log2_of(r.cache.page_tokens);
   a.vec = rows_aligned(r.k, a.ks, a.kh, size) && rows_aligned(r.v, a.vs, a.vh, size);
   a.bad = bad;
-  const dim3 grid((r.tokens + kTile - 1) / kTile, r.cache.kv_heads);
+  const unsigned grid = (unsigned)((r.tokens + kTile - 1) / kTile) * r.cache.kv_heads;   // heads are neighbours, as their rows
   if (r.type == EMELB_F32) return store_typed<float>(r.cache.head_dim, grid, a, st);
   if (r.type == EMELB_F16) return store_typed<__half>(r.cache.head_dim, grid, a, st);
   return store_typed<__nv_bfloat16>(r.cache.head_dim, grid, a, st);
@@ -628,13 +643,14 @@ cudaError_t launch_kv_load(const emelb_kv_load_request& r, int* bad, cudaStream_
   a.vh = r.v_head_stride;
   a.page_bytes = (int64_t)emelb_kv_page_bytes(r.cache.head_dim, r.cache.kv_heads, r.cache.page_tokens);
   a.requests = r.requests;
+  a.heads = r.cache.kv_heads;
   a.table_width = r.table_width;
   a.rows = r.rows;
   a.pages = r.cache.pages;
   a.page_shift = log2_of(r.cache.page_tokens);
   a.vec = rows_aligned(r.k, a.ks, a.kh, size) && rows_aligned(r.v, a.vs, a.vh, size);
   a.bad = bad;
-  const dim3 grid((r.rows + kTile - 1) / kTile, r.cache.kv_heads);
+  const unsigned grid = (unsigned)(r.rows / kTile + r.requests * (r.first ? 2 : 1)) * r.cache.kv_heads;
   if (r.type == EMELB_F32) return load_typed<float>(r.cache.head_dim, grid, a, st);
   if (r.type == EMELB_F16) return load_typed<__half>(r.cache.head_dim, grid, a, st);
   return load_typed<__nv_bfloat16>(r.cache.head_dim, grid, a, st);

@@ -155,6 +155,7 @@ uint32_t emelb_kv_store_can_run(const emelb_kv_store_request* r) {
       !apart(cache, rows_span(r->v, r->v_token_stride, r->v_head_stride, D, r->tokens, H, size)) ||
       !apart(cache, Span{r->slots, (uint64_t)r->tokens * 8}))
     return EMELB_INVALID_REQUEST;
+  if (((int64_t)r->tokens + 15) / 16 * H > 0x3fffffff) return EMELB_UNSUPPORTED_OP;   // CTAs
   return EMELB_OK;
 }
 
@@ -190,6 +191,7 @@ uint32_t emelb_kv_load_can_run(const emelb_kv_load_request* r) {
     const int64_t step = r->k_token_stride, row = (H - 1) * r->k_head_stride + D, from = off < 0 ? off + step : off;
     if (r->rows == 1 || r->v_token_stride != step || r->v_head_stride != r->k_head_stride || from < row || from > step - row) return EMELB_INVALID_REQUEST;
   }
+  if (((int64_t)r->rows / 16 + (int64_t)r->requests * 2) * H > 0x3fffffff) return EMELB_UNSUPPORTED_OP;   // CTAs
   return EMELB_OK;
 }
 
