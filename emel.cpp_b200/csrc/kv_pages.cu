@@ -297,8 +297,8 @@ struct Eight {
 // A CTA takes 16 packed rows of one head.  Four lanes share a group of 32 values, 8 each, which is a word of keys; the scale
 // comes from the group's largest value by two shuffles.  Values go by bytes, each with its own address: they wait in shared memory
 // until a warp can store one pair of dims of 16 rows at a time, which are neighbours where the rows fill a tile.
-// 32,760 rows of 8 heads of 128 f16: 47 us (3.6 TB/s), 90 with divisions, 50 with the largest value looked for one by one.  Issue
-// bounds it (0.8 of the cycles), some 150 instructions to 8 values of a warp; memory alone would take 26.
+// 32,760 rows of 8 heads of 128 f16: 47 us (3.6 TB/s), 50 with the largest value looked for one by one; with its reader 154 when
+// quotients were divisions, 97 by reciprocals.  Issue bounds it (0.8 of the cycles), some 150 instructions to 8 values of a warp; memory alone would take 26.
 struct StoreArgs {
   uint8_t* data;
   const void *k, *v;

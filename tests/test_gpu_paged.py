@@ -273,6 +273,39 @@ def test_store_and_load(be, dim, heads, page, t, layout):
     assert torch.equal(got[0][3], plain.kept(k)[0].float()) and (got[0][:3] == 7.0).all() and (got[0][4:] == 7.0).all()
 
 
+@pytest.mark.parametrize("n,with_first,short", [(1500, True, 0), (1500, False, 0), (40, True, 100), (33, False, 7), (1, True, 0)])
+def test_load_many_requests(be, n, with_first, short):
+    """Requests of every length from none up, behind rows of no request, into fewer rows than they have (`short`)."""
+    rng, g = np.random.default_rng(n + short), gen(n)
+    lengths = rng.integers(0, 50, n)
+    lengths[0] = 21
+    first = np.minimum(rng.integers(0, 40, n), lengths) if with_first else np.zeros(n, np.int64)
+    c, table, k, v = filled(be, rng, g, lengths.tolist(), 16, 2, 64)
+    begin = 5 + np.concatenate([[0], np.cumsum(lengths - first)])
+    rows = int(begin[-1]) - short
+    got = [torch.full((int(begin[-1]) + 2, 2, 64), 7.0, device="cuda") for _ in range(2)]
+    keep = [dev(lengths.tolist()), dev(begin.tolist()), dev(first.tolist()) if with_first else None]
+    torch.cuda.synchronize()
+    done(be, be.kv_load(paged.load_request(c.pages, *got, "f32", table, table.shape[1], keep[0], keep[1], n, rows, first=keep[2])))
+    at = np.concatenate([[0], np.cumsum(lengths)])
+    pick = dev(np.concatenate([np.arange(at[b] + first[b], at[b + 1]) for b in range(n)]).tolist(), torch.int64)
+    for y, z in zip((k, v), got):
+        want = y[pick].reshape(-1, 2, 64).float()
+        assert torch.equal(z[5:rows], want[:rows - 5]) and (z[:5] == 7.0).all() and (z[rows:] == 7.0).all()
+
+
+def test_load_reports_beginnings_out_of_order(be):
+    c = Cache(8, 16, 2, 64)
+    table, lengths = dev([[0], [1], [2]]), dev([10, 10, 10])
+    for begin in ([0, 20, 10, 30], [-5, 5, 10, 20], [0, 10, 20, 15]):
+        out = [torch.full((40, 2, 64), 7.0, device="cuda") for _ in range(2)]
+        begins = dev(begin)
+        torch.cuda.synchronize()
+        assert be.kv_load(paged.load_request(c.pages, *out, "f32", table, 1, lengths, begins, 3, 30))
+        assert not be.sync() and be.last_error == eb.INVALID_REQUEST
+        assert be.sync() and (out[0][30:] == 7.0).all() and (out[1][30:] == 7.0).all()
+
+
 def test_store_of_special_values(be):
     """Ties, borders, both signs at the largest magnitude, zeros, tiny and huge values, infinities, NaN."""
     g = gen(3)
