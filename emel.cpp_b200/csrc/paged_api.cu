@@ -17,14 +17,16 @@ struct Span {
 bool aligned(const void* p, uint64_t a) { return p && reinterpret_cast<uintptr_t>(p) % a == 0; }
 bool apart(const Span& a, const Span& b) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
-  return x + a.bytes <= y || y + b.bytes <= x;
+  return x <= y ? a.bytes <= y - x : b.bytes <= x - y;
 }
 uint64_t elem_bytes(int type) { return type == EMELB_F32 ? 4 : type == EMELB_F16 || type == EMELB_BF16 ? 2 : 0; }
 
 // strides between rows, or heads, that keep the address arithmetic inside 64 bits and rows apart from themselves
 constexpr int64_t kMostStride = (int64_t)1 << 40;
+constexpr int64_t kMostElems = (int64_t)1 << 58;
 bool strides_ok(int64_t token, int64_t head, int64_t row, int tokens, int heads) {
   if (token < 0 || head < 0 || token > kMostStride || head > kMostStride) return false;
+  if (tokens > 1 && token > kMostElems / (tokens - 1)) return false;   // heads, at most 2^16 of them, stay below 2^56
   return (tokens == 1 || token >= row) && (heads == 1 || head >= row);
 }
 // results may not fall on one another: one of the two strides steps over all of the other's
@@ -35,6 +37,7 @@ bool distinct_rows(int64_t token, int64_t head, int64_t row, int64_t tokens, int
 Span rows_span(const void* p, int64_t token, int64_t head, int64_t row, int64_t tokens, int64_t heads, uint64_t size) {
   return Span{p, (uint64_t)((tokens - 1) * token + (heads - 1) * head + row) * size};
 }
+bool table_ok(int64_t stride, int64_t rows, int64_t width) { return stride >= width && stride <= kMostStride && stride <= kMostElems / rows; }
 Span table_span(const int32_t* p, int64_t stride, int64_t rows, int64_t width) { return Span{p, (uint64_t)((rows - 1) * stride + width) * 4}; }
 
 // a page's sizes: invalid, known but not taken, or fine
@@ -99,7 +102,7 @@ uint64_t emelb_kv_page_bytes(int32_t head_dim, int32_t kv_heads, int32_t page_to
 uint32_t emelb_kv_plan_can_run(const emelb_kv_plan_request* r) {
   if (!r) return EMELB_INVALID_REQUEST;
   if (r->requests <= 0 || r->table_width <= 0 || r->pages <= 0 || r->page_tokens <= 0 || r->token_capacity <= 0) return EMELB_INVALID_REQUEST;
-  if (r->table_stride < r->table_width || r->table_stride > kMostStride) return EMELB_INVALID_REQUEST;
+  if (!table_ok(r->table_stride, r->requests, r->table_width)) return EMELB_INVALID_REQUEST;
   for (const void* p : {(const void*)r->cached, (const void*)r->fresh, (const void*)r->table, (const void*)r->free_pages, (const void*)r->free_count,
                         (const void*)r->free_left, (const void*)r->lengths, (const void*)r->query_begin, (const void*)r->key_begin,
                         (const void*)r->positions, (const void*)r->shortage})
@@ -166,7 +169,7 @@ uint32_t emelb_kv_store(emelb_ctx* c, const emelb_kv_store_request* r) {
 }
 
 uint32_t emelb_kv_load_can_run(const emelb_kv_load_request* r) {
-  if (!r || r->requests <= 0 || r->table_width <= 0 || r->rows <= 0 || r->table_stride < r->table_width || r->table_stride > kMostStride)
+  if (!r || r->requests <= 0 || r->table_width <= 0 || r->rows <= 0 || !table_ok(r->table_stride, r->requests, r->table_width))
     return EMELB_INVALID_REQUEST;
   if (const uint32_t why = cache_ok(r->cache)) return why;
   const uint64_t size = elem_bytes(r->type);
@@ -204,8 +207,8 @@ uint32_t emelb_kv_load(emelb_ctx* c, const emelb_kv_load_request* r) {
 
 // ------------------------------------------------------------------ attend
 uint32_t emelb_kv_attend_can_run(const emelb_kv_attend_request* r) {
-  if (!r || r->requests <= 0 || r->table_width <= 0 || r->heads <= 0 || r->queries <= 0 || r->max_queries <= 0 || r->table_stride < r->table_width ||
-      r->table_stride > kMostStride)
+  if (!r || r->requests <= 0 || r->table_width <= 0 || r->heads <= 0 || r->queries <= 0 || r->max_queries <= 0 ||
+      !table_ok(r->table_stride, r->requests, r->table_width))
     return EMELB_INVALID_REQUEST;
   if (const uint32_t why = cache_ok(r->cache)) return why;
   const uint64_t size = elem_bytes(r->type);

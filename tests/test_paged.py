@@ -67,6 +67,8 @@ def test_plan_requests(change, why):
     ({}, dict(k_strides=(63, 64)), eb.INVALID_REQUEST), ({}, dict(k_strides=(128, 63)), eb.INVALID_REQUEST),
     ({}, dict(v_strides=(-128, 64)), eb.INVALID_REQUEST), ({}, dict(v_strides=(64, 64 * 9)), eb.OK), ({}, dict(k=at(0) + 1024), eb.INVALID_REQUEST),
     ({}, dict(slots=at(0)), eb.INVALID_REQUEST), ({}, dict(k_strides=(1 << 41, 64)), eb.INVALID_REQUEST),
+    ({}, dict(tokens=1 << 30, k_strides=(1 << 40, 64)), eb.INVALID_REQUEST), (dict(data=at(100), kv_heads=60000), dict(k=at(101), v=at(200), slots=at(300)), eb.INVALID_REQUEST),
+    (dict(data=at(60000000), kv_heads=8000), dict(k=at(0), v=at(20000000), slots=at(40000000), tokens=1 << 30), eb.UNSUPPORTED_OP),
 ])
 def test_store_requests(kw, change, why):
     a = dict(k=at(1), v=at(2), type="f16", slots=at(3), tokens=9)
@@ -82,6 +84,8 @@ def test_store_requests(kw, change, why):
     ({}, dict(v=at(1) + 256, k_strides=(256, 64), v_strides=(256, 64)), eb.OK),   # keys and values side by side in a row
     ({}, dict(v=at(1) + 128, k_strides=(256, 128), v_strides=(256, 128)), eb.INVALID_REQUEST),
     ({}, dict(k=at(0)), eb.INVALID_REQUEST), ({}, dict(v=at(3)), eb.INVALID_REQUEST), ({}, dict(k=at(4) - 8), eb.INVALID_REQUEST),
+    (dict(data=at(1000)), dict(requests=1 << 30, table_stride=1 << 30, lengths=at(5000), row_begin=at(6000)), eb.INVALID_REQUEST),
+    ({}, dict(requests=300000000, table=at(100), table_width=1, lengths=at(1000), row_begin=at(2000)), eb.UNSUPPORTED_OP),
 ])
 def test_load_requests(kw, change, why):
     a = dict(k=at(1), v=at(2), type="bf16", table=at(3), table_width=4, lengths=at(4), row_begin=at(5), requests=3, rows=10)
