@@ -31,6 +31,7 @@
 
 #include <algorithm>
 
+#include "kernels.h"
 #include "paged.h"
 #include "tc_common.cuh"
 
@@ -190,6 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Item items[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int gave_up;
+  pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t smem = (tc::smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t bar0 = tc::smem_u32(bars), bar1 = bar0 + 24 * kStages, bar2 = bar1 + 32 * kTiles;
@@ -267,6 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Item it{};
   if (warp == kPlanWarp) {
     if (lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &q_map : lane == 1 ? &k_map : &v_map) : "memory");
+    pdl_wait();
     it = item_of(blockIdx.x);
   }
   // rows of a tile that no token fills (128 is no multiple of the group): zero for good
@@ -276,6 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
+  pdl_wait();
   const uint32_t tmem = tmem_slot;
   int loaded = 0, asked = 0;                       // loader: tiles asked for; plan: items whose queries were
   uint32_t on_landed = 0, landed_parity = 0;       // bits of stages: the last tile goes by `landed`; which phase comes next
@@ -673,17 +677,16 @@ bool encode_rows(Map* map, const void* base, bool bf16, int head_dim, int heads,
 }
 
 template <int DP, bool kBf16>
-cudaError_t launch_one(const PackedArgs& a, const Map& q, const Map& k, const Map& v, int sm_count, cudaStream_t st) {
+cudaError_t launch_one(const PackedArgs& a, const Map& q, const Map& k, const Map& v, int sm_count, bool pdl, cudaStream_t st) {
   const int smem = Smem<DP>::kBytes;
   cudaError_t e = cudaFuncSetAttribute(attend_packed_kernel<DP, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  attend_packed_kernel<DP, kBf16><<<(unsigned)std::min<int64_t>(a.items, sm_count), kThreads, smem, st>>>(a, q, k, v);
-  return cudaGetLastError();
+  return launch_kernel(attend_packed_kernel<DP, kBf16>, dim3((unsigned)std::min<int64_t>(a.items, sm_count)), dim3(kThreads), smem, st, pdl, a, q, k, v);
 }
 
 }  // namespace
 
-cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int* next, int sm_count, int* bad, int* status, cudaStream_t st) {
+cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int* next, int sm_count, int* bad, int* status, bool pdl, cudaStream_t st) {
   PackedArgs a{};
   a.q = r.q;
   a.out = r.out;
@@ -718,8 +721,8 @@ cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int* next
       !encode_rows(&k, r.k, bf16, r.head_dim, r.kv_heads, r.keys, r.k_token_stride, r.k_head_stride, 1, kTileKeys) ||
       !encode_rows(&v, r.v, bf16, r.head_dim, r.kv_heads, r.keys, r.v_token_stride, r.v_head_stride, 1, kTileKeys))
     return cudaErrorInvalidValue;
-  if (r.head_dim <= 64) return bf16 ? launch_one<64, true>(a, q, k, v, sm_count, st) : launch_one<64, false>(a, q, k, v, sm_count, st);
-  return bf16 ? launch_one<128, true>(a, q, k, v, sm_count, st) : launch_one<128, false>(a, q, k, v, sm_count, st);
+  if (r.head_dim <= 64) return bf16 ? launch_one<64, true>(a, q, k, v, sm_count, pdl, st) : launch_one<64, false>(a, q, k, v, sm_count, pdl, st);
+  return bf16 ? launch_one<128, true>(a, q, k, v, sm_count, pdl, st) : launch_one<128, false>(a, q, k, v, sm_count, pdl, st);
 }
 
 }  // namespace emelb

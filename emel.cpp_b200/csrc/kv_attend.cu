@@ -24,6 +24,7 @@
 
 #include <type_traits>
 
+#include "kernels.h"
 #include "kv_tile.cuh"
 #include "paged.h"
 #include "tc_common.cuh"
@@ -237,6 +238,8 @@ __device__ __forceinline__ void team_barrier(int team, int threads) {
 // and not 1.6 times what the results' own rounding makes)
 template <int D, Kind kind>
 __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kernel(const __grid_constant__ AttendArgs a) {
+  pdl_trigger();
+  pdl_wait();
   using T = Tile<D>;
   using S = Shape<D, kind>;
   constexpr int kWarps = S::kWarps, kThreads = 32 * kWarps;
@@ -936,28 +939,27 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
 }
 
 template <int D, Kind kind>
-cudaError_t launch_one(const AttendArgs& a, int sm_count, cudaStream_t st) {
+cudaError_t launch_one(const AttendArgs& a, int sm_count, bool pdl, cudaStream_t st) {
   using S = Shape<D, kind>;
   const int smem = S::kSmem;
   cudaError_t e = cudaFuncSetAttribute(kv_attend_kernel<D, kind>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kv_attend_kernel<D, kind><<<sm_count, 32 * S::kWarps, smem, st>>>(a);
-  return cudaGetLastError();
+  return launch_kernel(kv_attend_kernel<D, kind>, dim3(sm_count), dim3(32 * S::kWarps), smem, st, pdl, a);
 }
 template <int D>
-cudaError_t launch_dim(AttendArgs& a, const KvAttendScratch& s, int sm_count, cudaStream_t st) {
+cudaError_t launch_dim(AttendArgs& a, const KvAttendScratch& s, int sm_count, bool pdl, cudaStream_t st) {
   constexpr uint64_t rows = 8;
   uint64_t units = s.acc_floats / (2 * rows * D);
   units = units < s.stats_floats / (4 * rows) ? units : s.stats_floats / (4 * rows);
   units = units < s.arrived_ints ? units : s.arrived_ints;
   a.most_units = (int)units;
-  if (a.type == EMELB_F32) return launch_one<D, kF32>(a, sm_count, st);
-  return a.type == EMELB_F16 ? launch_one<D, kF16>(a, sm_count, st) : launch_one<D, kBf16>(a, sm_count, st);
+  if (a.type == EMELB_F32) return launch_one<D, kF32>(a, sm_count, pdl, st);
+  return a.type == EMELB_F16 ? launch_one<D, kF16>(a, sm_count, pdl, st) : launch_one<D, kBf16>(a, sm_count, pdl, st);
 }
 
 }  // namespace
 
-cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScratch& s, int sm_count, int* bad, cudaStream_t st) {
+cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScratch& s, int sm_count, int* bad, bool pdl, cudaStream_t st) {
   AttendArgs a{};
   a.data = static_cast<const uint8_t*>(r.cache.data);
   a.q = r.q;
@@ -990,10 +992,10 @@ cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScr
   a.arrived = s.arrived;
   a.bad = bad;
   switch (r.cache.head_dim) {
-    case 32: return launch_dim<32>(a, s, sm_count, st);
-    case 64: return launch_dim<64>(a, s, sm_count, st);
-    case 96: return launch_dim<96>(a, s, sm_count, st);
-    default: return launch_dim<128>(a, s, sm_count, st);
+    case 32: return launch_dim<32>(a, s, sm_count, pdl, st);
+    case 64: return launch_dim<64>(a, s, sm_count, pdl, st);
+    case 96: return launch_dim<96>(a, s, sm_count, pdl, st);
+    default: return launch_dim<128>(a, s, sm_count, pdl, st);
   }
 }
 

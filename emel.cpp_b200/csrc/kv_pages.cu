@@ -6,6 +6,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "kernels.h"
 #include "kv_tile.cuh"
 #include "paged.h"
 
@@ -83,6 +84,8 @@ struct PlanArgs {
 };
 
 __global__ void __launch_bounds__(512) kv_plan_kernel(const __grid_constant__ PlanArgs a) {
+  pdl_trigger();
+  pdl_wait();
   extern __shared__ int plan_smem[];
   __shared__ i64 warp_sums[3][32];
   __shared__ int most_taken;
@@ -245,6 +248,8 @@ __global__ void __launch_bounds__(512) kv_plan_kernel(const __grid_constant__ Pl
 }
 
 __global__ void __launch_bounds__(256) kv_plan_in_place_kernel(const int* lengths, const int* free_left, int n, int* to_lengths, int* to_free_left) {
+  pdl_trigger();
+  pdl_wait();
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i < n) to_lengths[i] = lengths[i];
   if (i == 0) *to_free_left = *free_left;
@@ -404,6 +409,8 @@ __device__ __forceinline__ void quantize8(const Eight<E>& in, __half& scale, uin
 
 template <int D, class E>
 __global__ void __launch_bounds__(128) kv_store_kernel(const StoreArgs a) {
+  pdl_trigger();
+  pdl_wait();
   using T = Tile<D>;
   constexpr int kOcts = D / 8, kTurns = (kTile * kOcts + 127) / 128;   // 8-value pieces of a row, turns of a thread
   __shared__ uint8_t* base[kTile];              // the row's tile of this head; null: skipped
@@ -501,6 +508,8 @@ __device__ __forceinline__ void dequantize8(uint32_t word, __half scale, Eight<E
 // Memory bounds it, and the three reads in a row before its first byte.
 template <int D, class E>
 __global__ void __launch_bounds__(128) kv_load_kernel(const LoadArgs a) {
+  pdl_trigger();
+  pdl_wait();
   using T = Tile<D>;
   __shared__ __align__(16) uint8_t tile[T::kBytes];
   const int tid = threadIdx.x, lane = tid & 31, slot = blockIdx.x / a.heads, head = blockIdx.x % a.heads, spare = a.first ? 2 : 1;
@@ -563,46 +572,44 @@ bool rows_aligned(const void* p, int64_t token, int64_t head, size_t size) {
 size_t size_of(int type) { return type == EMELB_F32 ? 4 : 2; }
 
 template <class E>
-cudaError_t store_typed(int D, unsigned grid, const StoreArgs& a, cudaStream_t st) {
+cudaError_t store_typed(int D, unsigned grid, const StoreArgs& a, bool pdl, cudaStream_t st) {
   switch (D) {
-    case 32: kv_store_kernel<32, E><<<grid, 128, 0, st>>>(a); break;
-    case 64: kv_store_kernel<64, E><<<grid, 128, 0, st>>>(a); break;
-    case 96: kv_store_kernel<96, E><<<grid, 128, 0, st>>>(a); break;
-    default: kv_store_kernel<128, E><<<grid, 128, 0, st>>>(a); break;
+    case 32: return launch_kernel(kv_store_kernel<32, E>, dim3(grid), dim3(128), 0, st, pdl, a);
+    case 64: return launch_kernel(kv_store_kernel<64, E>, dim3(grid), dim3(128), 0, st, pdl, a);
+    case 96: return launch_kernel(kv_store_kernel<96, E>, dim3(grid), dim3(128), 0, st, pdl, a);
+    default: return launch_kernel(kv_store_kernel<128, E>, dim3(grid), dim3(128), 0, st, pdl, a);
   }
-  return cudaGetLastError();
 }
 template <class E>
-cudaError_t load_typed(int D, unsigned grid, const LoadArgs& a, cudaStream_t st) {
+cudaError_t load_typed(int D, unsigned grid, const LoadArgs& a, bool pdl, cudaStream_t st) {
   switch (D) {
-    case 32: kv_load_kernel<32, E><<<grid, 128, 0, st>>>(a); break;
-    case 64: kv_load_kernel<64, E><<<grid, 128, 0, st>>>(a); break;
-    case 96: kv_load_kernel<96, E><<<grid, 128, 0, st>>>(a); break;
-    default: kv_load_kernel<128, E><<<grid, 128, 0, st>>>(a); break;
+    case 32: return launch_kernel(kv_load_kernel<32, E>, dim3(grid), dim3(128), 0, st, pdl, a);
+    case 64: return launch_kernel(kv_load_kernel<64, E>, dim3(grid), dim3(128), 0, st, pdl, a);
+    case 96: return launch_kernel(kv_load_kernel<96, E>, dim3(grid), dim3(128), 0, st, pdl, a);
+    default: return launch_kernel(kv_load_kernel<128, E>, dim3(grid), dim3(128), 0, st, pdl, a);
   }
-  return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t launch_kv_plan(const emelb_kv_plan_request& r, int* scratch, int sm_count, int* launches, int* bad, cudaStream_t st) {
-  const cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 16 * kPlanMost);
+cudaError_t launch_kv_plan(const emelb_kv_plan_request& r, int* scratch, int sm_count, int* launches, int* bad, bool pdl, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 16 * kPlanMost);
   if (e != cudaSuccess) return e;
   // a CTA's sums cost what 2000 rows do: few rows and requests are one CTA's
   const int threads = r.requests <= 256 && r.token_capacity <= 2048 ? 256 : 512;
   const int ctas = threads == 256 ? 1 : std::min(sm_count, (r.token_capacity - 1) / 2048 + 1);
   const bool aside = ctas > 1 && (r.lengths == r.cached || r.free_left == r.free_count);
   const PlanArgs a{r, aside ? scratch + 1 : r.lengths, aside ? scratch : r.free_left, log2_of(r.page_tokens), bad};
-  kv_plan_kernel<<<ctas, threads, 16 * r.requests, st>>>(a);
+  e = launch_kernel(kv_plan_kernel, dim3(ctas), dim3(threads), 16 * r.requests, st, pdl, a);
+  if (e != cudaSuccess) return e;
   *launches = 1;
-  if (aside) {
-    kv_plan_in_place_kernel<<<(r.requests + 255) / 256, 256, 0, st>>>(scratch + 1, scratch, r.requests, r.lengths, r.free_left);
-    *launches = 2;
-  }
-  return cudaGetLastError();
+  if (!aside) return e;
+  e = launch_kernel(kv_plan_in_place_kernel, dim3((r.requests + 255) / 256), dim3(256), 0, st, pdl, scratch + 1, scratch, r.requests, r.lengths, r.free_left);
+  if (e == cudaSuccess) *launches = 2;
+  return e;
 }
 
-cudaError_t launch_kv_store(const emelb_kv_store_request& r, int* bad, cudaStream_t st) {
+cudaError_t launch_kv_store(const emelb_kv_store_request& r, int* bad, bool pdl, cudaStream_t st) {
   const size_t size = size_of(r.type);
   StoreArgs a{};
   a.data = static_cast<uint8_t*>(r.cache.data);
@@ -621,12 +628,12 @@ cudaError_t launch_kv_store(const emelb_kv_store_request& r, int* bad, cudaStrea
   a.vec = rows_aligned(r.k, a.ks, a.kh, size) && rows_aligned(r.v, a.vs, a.vh, size);
   a.bad = bad;
   const unsigned grid = (unsigned)((r.tokens + kTile - 1) / kTile) * r.cache.kv_heads;   // heads are neighbours, as their rows
-  if (r.type == EMELB_F32) return store_typed<float>(r.cache.head_dim, grid, a, st);
-  if (r.type == EMELB_F16) return store_typed<__half>(r.cache.head_dim, grid, a, st);
-  return store_typed<__nv_bfloat16>(r.cache.head_dim, grid, a, st);
+  if (r.type == EMELB_F32) return store_typed<float>(r.cache.head_dim, grid, a, pdl, st);
+  if (r.type == EMELB_F16) return store_typed<__half>(r.cache.head_dim, grid, a, pdl, st);
+  return store_typed<__nv_bfloat16>(r.cache.head_dim, grid, a, pdl, st);
 }
 
-cudaError_t launch_kv_load(const emelb_kv_load_request& r, int* bad, cudaStream_t st) {
+cudaError_t launch_kv_load(const emelb_kv_load_request& r, int* bad, bool pdl, cudaStream_t st) {
   const size_t size = size_of(r.type);
   LoadArgs a{};
   a.data = static_cast<const uint8_t*>(r.cache.data);
@@ -651,9 +658,9 @@ cudaError_t launch_kv_load(const emelb_kv_load_request& r, int* bad, cudaStream_
   a.vec = rows_aligned(r.k, a.ks, a.kh, size) && rows_aligned(r.v, a.vs, a.vh, size);
   a.bad = bad;
   const unsigned grid = (unsigned)(r.rows / kTile + r.requests * (r.first ? 2 : 1)) * r.cache.kv_heads;
-  if (r.type == EMELB_F32) return load_typed<float>(r.cache.head_dim, grid, a, st);
-  if (r.type == EMELB_F16) return load_typed<__half>(r.cache.head_dim, grid, a, st);
-  return load_typed<__nv_bfloat16>(r.cache.head_dim, grid, a, st);
+  if (r.type == EMELB_F32) return load_typed<float>(r.cache.head_dim, grid, a, pdl, st);
+  if (r.type == EMELB_F16) return load_typed<__half>(r.cache.head_dim, grid, a, pdl, st);
+  return load_typed<__nv_bfloat16>(r.cache.head_dim, grid, a, pdl, st);
 }
 
 }  // namespace emelb

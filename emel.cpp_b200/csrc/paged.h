@@ -10,9 +10,9 @@ namespace emelb {
 
 // `bad`: raised to 1 by a kernel that met a length, page or slot out of range and left it alone
 // `scratch`: requests + 1 ints
-cudaError_t launch_kv_plan(const emelb_kv_plan_request& r, int* scratch, int sm_count, int* launches, int* bad, cudaStream_t st);
-cudaError_t launch_kv_store(const emelb_kv_store_request& r, int* bad, cudaStream_t st);
-cudaError_t launch_kv_load(const emelb_kv_load_request& r, int* bad, cudaStream_t st);
+cudaError_t launch_kv_plan(const emelb_kv_plan_request& r, int* scratch, int sm_count, int* launches, int* bad, bool pdl, cudaStream_t st);
+cudaError_t launch_kv_store(const emelb_kv_store_request& r, int* bad, bool pdl, cudaStream_t st);
+cudaError_t launch_kv_load(const emelb_kv_load_request& r, int* bad, bool pdl, cudaStream_t st);
 
 // scratch of emelb_kv_attend: two partial results a unit, its arrival counter (zero between launches)
 struct KvAttendScratch {
@@ -23,9 +23,9 @@ struct KvAttendScratch {
   int* arrived;
   uint64_t arrived_ints;
 };
-cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScratch& s, int sm_count, int* bad, cudaStream_t st);
+cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScratch& s, int sm_count, int* bad, bool pdl, cudaStream_t st);
 
 // `next`: two ints, zero between launches; `status`: raised to 1 when a bounded wait ran out
-cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int* next, int sm_count, int* bad, int* status, cudaStream_t st);
+cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int* next, int sm_count, int* bad, int* status, bool pdl, cudaStream_t st);
 
 }  // namespace emelb

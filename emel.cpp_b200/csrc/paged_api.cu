@@ -138,7 +138,7 @@ uint32_t emelb_kv_plan(emelb_ctx* c, const emelb_kv_plan_request* r) {
   int launches = 0;
   const uint32_t err = dispatch(c, {r->cached, r->fresh, r->table, r->free_pages, r->free_count, r->free_left, r->lengths, r->query_begin, r->key_begin,
                                     r->slots, r->positions, r->shortage}, 0,
-                                [&] { return launch_kv_plan(*r, reinterpret_cast<int*>(c->fa_part_ml), c->sm_count, &launches, c->bad_word(), c->stream); });
+                                [&] { return launch_kv_plan(*r, reinterpret_cast<int*>(c->fa_part_ml), c->sm_count, &launches, c->bad_word(), c->pdl & 1, c->stream); });
   c->diag.kernel_launches += launches;
   return err;
 }
@@ -165,7 +165,7 @@ uint32_t emelb_kv_store_can_run(const emelb_kv_store_request* r) {
 uint32_t emelb_kv_store(emelb_ctx* c, const emelb_kv_store_request* r) {
   if (!c || !r) return EMELB_INVALID_REQUEST;
   if (const uint32_t why = emelb_kv_store_can_run(r)) return refuse(c, why);
-  return dispatch(c, {r->cache.data, r->k, r->v, r->slots}, 1, [&] { return launch_kv_store(*r, c->bad_word(), c->stream); });
+  return dispatch(c, {r->cache.data, r->k, r->v, r->slots}, 1, [&] { return launch_kv_store(*r, c->bad_word(), c->pdl & 1, c->stream); });
 }
 
 uint32_t emelb_kv_load_can_run(const emelb_kv_load_request* r) {
@@ -202,7 +202,7 @@ uint32_t emelb_kv_load(emelb_ctx* c, const emelb_kv_load_request* r) {
   if (!c || !r) return EMELB_INVALID_REQUEST;
   if (const uint32_t why = emelb_kv_load_can_run(r)) return refuse(c, why);
   return dispatch(c, {r->cache.data, r->k, r->v, r->table, r->first, r->lengths, r->row_begin}, 1,
-                  [&] { return launch_kv_load(*r, c->bad_word(), c->stream); });
+                  [&] { return launch_kv_load(*r, c->bad_word(), c->pdl & 1, c->stream); });
 }
 
 // ------------------------------------------------------------------ attend
@@ -238,7 +238,7 @@ uint32_t emelb_kv_attend(emelb_ctx* c, const emelb_kv_attend_request* r) {
   if (const uint32_t why = emelb_kv_attend_can_run(r)) return refuse(c, why);
   const KvAttendScratch s{c->fa_part_acc, kFlashPartFloats, c->fa_part_ml, kFlashPartFloats / 32, c->grp_cnt, c->grp_cnt_ints};
   return dispatch(c, {r->cache.data, r->q, r->out, r->table, r->lengths, r->query_begin}, 1,
-                  [&] { return launch_kv_attend(*r, s, c->sm_count, c->bad_word(), c->stream); });
+                  [&] { return launch_kv_attend(*r, s, c->sm_count, c->bad_word(), c->pdl & 1, c->stream); });
 }
 
 // ------------------------------------------------------------------ packed prompts
@@ -282,7 +282,7 @@ uint32_t emelb_attend_packed(emelb_ctx* c, const emelb_attend_packed_request* r)
   if (!c || !r) return EMELB_INVALID_REQUEST;
   if (const uint32_t why = emelb_attend_packed_can_run(r)) return refuse(c, why);
   return dispatch(c, {r->q, r->k, r->v, r->out, r->query_begin, r->key_begin}, 1,
-                  [&] { return launch_attend_packed(*r, c->next_sched(), c->sm_count, c->bad_word(), c->status_word(), c->stream); });
+                  [&] { return launch_attend_packed(*r, c->next_sched(), c->sm_count, c->bad_word(), c->status_word(), c->pdl & 1, c->stream); });
 }
 
 }  // extern "C"
