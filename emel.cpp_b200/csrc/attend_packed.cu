@@ -145,7 +145,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       : "memory");
 }
 
-// Pairs of row tiles of request b stand in slots first_slot(b) .. first_slot(b + 1) - 1, of which it may leave one empty: tokens
+// With many requests, pairs of row tiles of request b stand in slots first_slot(b) .. first_slot(b + 1) - 1, of which it may leave one empty: tokens
 // before it / (two tiles') + b is known from query_begin alone, without a sum over the requests in front.
 __device__ __forceinline__ int first_slot(const PackedArgs& a, int b) {
   return (int)((uint32_t)(a.query_begin[b] - a.query_begin[0]) / (uint32_t)(kTiles * a.tile_tokens)) + b;
@@ -190,6 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint64_t bars[3 * kStages + 4 * kTiles + 7];
   __shared__ Item items[2];
   __shared__ uint32_t tmem_slot;
+  __shared__ int order[32];
   __shared__ volatile int gave_up;
   pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -236,11 +237,61 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int q0 = a.query_begin[b], nq = a.query_begin[b + 1] - q0, k0 = a.key_begin[b], nk = a.key_begin[b + 1] - k0, first = a.query_begin[0];
     return first >= 0 && q0 >= first && nq >= 0 && nq <= a.max_queries && q0 <= a.queries - nq && k0 >= 0 && nk >= 0 && k0 <= a.keys - nk;
   };
+  const int most = kTiles * a.tile_tokens;
+  auto pairs_of = [&](int nq) { return (int)(((uint32_t)nq + most - 1) / (uint32_t)most); };
+  // pair `local` of a request, from its end on: long walks first
+  auto make_item = [&](int head, int q0, int nq, int k0, int nk, int local) {
+    Item it{};
+    const int from = (pairs_of(nq) - 1 - local) * most;
+    it.valid = 1;
+    it.token = q0 + from;
+    it.tokens = min(nq - from, most);
+    it.head = head;
+    it.first_key = k0;
+    it.keys = nk;
+    it.see = a.causal ? nk - nq + from + 1 : nk;
+    it.n0 = (sees(it, min(it.tokens, a.tile_tokens) - 1) + kTileKeys - 1) / kTileKeys;
+    it.n1 = it.tokens > a.tile_tokens ? (sees(it, it.tokens - 1) + kTileKeys - 1) / kTileKeys : 0;
+    return it;
+  };
+  // 2 to 32 requests: the plan warp has one a lane, those with the most keys first, so that the last items are short ones; `upto`
+  // are the running sums of their pairs in that order, `who` the lane of the place.
+  const bool few = a.requests > 1 && a.requests <= 32;
+  int q0 = 0, nq = 0, k0 = 0, nk = 0, who = lane, pairs = 0, upto = 0, items_all = (int)a.items;
+  auto rank_requests = [&] {
+    if (lane < a.requests && sound(lane)) {
+      q0 = a.query_begin[lane];
+      nq = a.query_begin[lane + 1] - q0;
+      k0 = a.key_begin[lane];
+      nk = a.key_begin[lane + 1] - k0;
+    }
+    pairs = pairs_of(nq);
+    int rank = 0;
+#pragma unroll 8
+    for (int b = 0; b < a.requests; ++b) {   // lanes behind the last stand behind it
+      const int keys = __shfl_sync(kAll, nk, b);
+      rank += keys > nk || (keys == nk && b < lane);
+    }
+    order[lane < a.requests ? rank : lane] = lane;
+    __syncwarp();
+    who = order[lane];
+    pairs = __shfl_sync(kAll, pairs, who);
+    upto = pairs;
+    for (int o = 1; o < a.requests; o <<= 1) {
+      const int u = __shfl_up_sync(kAll, upto, o);
+      if (lane >= o) upto += u;
+    }
+    items_all = (int)min((int64_t)__shfl_sync(kAll, upto, a.requests - 1) * a.kv_heads, a.items);
+  };
   // the w-th item, by a warp; nothing valid where the slot is empty or the request's numbers are out of range
   auto item_of = [&](int w) {
-    Item it{};
-    const int head = w % a.kv_heads;
-    const int slot = w / a.kv_heads;
+    const int head = w % a.kv_heads, slot = w / a.kv_heads;
+    if (few) {
+      const unsigned behind = __ballot_sync(kAll, upto > slot);
+      if (!behind) return Item{};
+      const int place = __ffs(behind) - 1, from = __shfl_sync(kAll, who, place), local = slot - __shfl_sync(kAll, upto - pairs, place);
+      return make_item(head, __shfl_sync(kAll, q0, from), __shfl_sync(kAll, nq, from), __shfl_sync(kAll, k0, from), __shfl_sync(kAll, nk, from), local);
+    }
     int lo = 0, hi = a.requests;          // first_slot(lo) <= slot, first_slot(hi) > slot (or hi = requests)
     while (hi - lo > 1) {
       const int step = (hi - lo + 31) / 32, b = lo + lane * step;
@@ -249,27 +300,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       hi = min(hi, lo + (last + 1) * step);
       lo = lo + last * step;
     }
-    const int b = lo, q0 = a.query_begin[b], nq = a.query_begin[b + 1] - q0, k0 = a.key_begin[b], nk = a.key_begin[b + 1] - k0;
-    const int most = kTiles * a.tile_tokens;
-    const int pairs = (int)(((uint32_t)nq + most - 1) / (uint32_t)most), local = slot - first_slot(a, b);
-    if (sound(b) && local >= 0 && local < pairs) {
-      const int from = (pairs - 1 - local) * most;   // long walks first
-      it.valid = 1;
-      it.token = q0 + from;
-      it.tokens = min(nq - from, most);
-      it.head = head;
-      it.first_key = k0;
-      it.keys = nk;
-      it.see = a.causal ? nk - nq + from + 1 : nk;
-      it.n0 = (sees(it, min(it.tokens, a.tile_tokens) - 1) + kTileKeys - 1) / kTileKeys;
-      it.n1 = it.tokens > a.tile_tokens ? (sees(it, it.tokens - 1) + kTileKeys - 1) / kTileKeys : 0;
-    }
-    return it;
+    const int begin = a.query_begin[lo], n = a.query_begin[lo + 1] - begin, first = a.key_begin[lo], keys = a.key_begin[lo + 1] - first, local = slot - first_slot(a, lo);
+    return sound(lo) && local >= 0 && local < pairs_of(n) ? make_item(head, begin, n, first, keys, local) : Item{};
   };
   Item it{};
   if (warp == kPlanWarp) {
     if (lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &q_map : lane == 1 ? &k_map : &v_map) : "memory");
     pdl_wait();
+    if (few) rank_requests();
     it = item_of(blockIdx.x);
   }
   // rows of a tile that no token fills (128 is no multiple of the group): zero for good
@@ -305,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // items while the others work on the one before: the first by the CTA's number, then from the common counter
     bool alive = true;
     for (int n = 0, w = blockIdx.x;;) {
-      const bool more = alive && w < a.items;
+      const bool more = alive && w < items_all;
       if (w != (int)blockIdx.x) it = more ? item_of(w) : Item{};
       if (it.valid || !more) {
         if (n >= 2) alive = __all_sync(kAll, tc::mbar_wait(item_empty(n), (n >> 1) - 1 & 1, &gave_up)) && alive;

@@ -266,7 +266,8 @@ uint32_t emelb_attend_packed_can_run(const emelb_attend_packed_request* r) {
     if (!apart(s, out)) return EMELB_INVALID_REQUEST;
   const int group = r->heads / r->kv_heads;
   if (D % 8 != 0 || D > 128 || group > 128 || r->kv_heads > 65535) return EMELB_UNSUPPORTED_OP;
-  // pairs of row tiles that the CTAs count, and strides that a tensor map holds
+  // a walk that its waits would take for one that hangs, pairs of row tiles that the CTAs count, and strides that a tensor map holds
+  if (r->keys > 1 << 25) return EMELB_UNSUPPORTED_OP;
   if (((int64_t)r->queries / (256 / group) + r->requests) * r->kv_heads > 0x3fffffff) return EMELB_UNSUPPORTED_OP;
   for (int64_t s : {r->q_token_stride, r->q_head_stride, r->k_token_stride, r->k_head_stride, r->v_token_stride, r->v_head_stride})
     if (s >= (int64_t)1 << 39) return EMELB_UNSUPPORTED_OP;

@@ -114,6 +114,7 @@ def test_attend_requests(kw, change, why):
     (dict(q=at(0) + 2), eb.UNSUPPORTED_OP), (dict(q=at(0) + 1), eb.INVALID_REQUEST), (dict(k_strides=(132, 64)), eb.UNSUPPORTED_OP),
     (dict(k_strides=(136, 64)), eb.OK), (dict(v_strides=(64, 1280)), eb.OK), (dict(out=at(0)), eb.INVALID_REQUEST), (dict(out=at(2) + 16), eb.INVALID_REQUEST),
     (dict(out_strides=(64, 64)), eb.INVALID_REQUEST), (dict(query_begin=at(4) + 2), eb.INVALID_REQUEST), (dict(max_queries=0), eb.INVALID_REQUEST),
+    (dict(keys=1 << 25, k=at(1000), v=at(2000), out=at(3000)), eb.OK), (dict(keys=(1 << 25) + 1, k=at(1000), v=at(2000), out=at(3000)), eb.UNSUPPORTED_OP),
     (dict(heads=60000, kv_heads=60000, requests=20000, q=at(10), k=at(20), v=at(30), out=at(40)), eb.UNSUPPORTED_OP),
     (dict(k=at(50), k_strides=(1 << 39, 64)), eb.UNSUPPORTED_OP), (dict(v=at(50), v_strides=(64, (1 << 39) - 8)), eb.OK),
 ])
