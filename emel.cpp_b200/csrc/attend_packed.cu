@@ -23,7 +23,9 @@
 // CTAs stay.  One prompt of 8192 and heads of 64: 411 (667 TFLOP/s; its exponentials alone take 252).  Measured and left out: an
 // issuer of products for each row tile 613 / - (they fall into step and wait for the same pipes); scores of 64 keys in two buffers a
 // row tile, so that none waits for a mix, 588 (products with 64 columns take longer); weights against a stale maximum, looked at
-// afterwards, 604; an eighth, a quarter of the exponentials by polynomials on the multiply-adds, no gain, +8.
+// afterwards, 604; an eighth, a quarter of the exponentials by polynomials on the multiply-adds, no gain, +8; at head_dim 64, where
+// TMEM has room, weights beside the scores so that the next scores need not wait for the mix, 421 for 394, and turns at the exponentials
+// for the two warps of a scheduler, 394 (558 for 538 at 128).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
