@@ -278,8 +278,9 @@ struct Elem<__nv_bfloat16> {
 template <class E>
 struct Eight {
   __align__(16) E e[8];
-  __device__ __forceinline__ void load(const E* p, bool vec) {
-    if (vec) {
+  template <bool kVec>
+  __device__ __forceinline__ void load(const E* p) {
+    if constexpr (kVec) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(e) / 16; ++i) reinterpret_cast<uint4*>(e)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
     } else {
@@ -287,8 +288,9 @@ struct Eight {
       for (int i = 0; i < 8; ++i) e[i] = p[i];
     }
   }
-  __device__ __forceinline__ void store(E* p, bool vec) const {
-    if (vec) {
+  template <bool kVec>
+  __device__ __forceinline__ void store(E* p) const {
+    if constexpr (kVec) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(e) / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e)[i];
     } else {
@@ -299,17 +301,19 @@ struct Eight {
 };
 
 // ------------------------------------------------------------------ store
-// A CTA takes 16 packed rows of one head.  Four lanes share a group of 32 values, 8 each, which is a word of keys; the scale
-// comes from the group's largest value by two shuffles.  Values go by bytes, each with its own address: they wait in shared memory
-// until a warp can store one pair of dims of 16 rows at a time, which are neighbours where the rows fill a tile.
-// 32,760 rows of 8 heads of 128 f16: 47 us (3.6 TB/s), 50 with the largest value looked for one by one; with its reader 154 when
-// quotients were divisions, 97 by reciprocals.  Issue bounds it (0.8 of the cycles), some 150 instructions to 8 values of a warp; memory alone would take 26.
+// A CTA takes 16 packed rows of a head, or of several in turn where there are CTAs enough.  Four lanes share a group of 32 values, 8
+// each, which is a word of keys; the scale comes from the group's largest value by two shuffles.  Values go by bytes, each with its
+// own address: they wait in shared memory until a warp can store one pair of dims of 16 rows at a time, which are neighbours where
+// the rows fill a tile.
+// 32,760 rows of 8 heads of 128 f16: 43 us (4.0 TB/s), 47 with a CTA for each head and rows of either alignment in one kernel, 50
+// with the largest value looked for one by one; with its reader 154 when quotients were divisions, 97 by reciprocals.  Issue bounds
+// it, 130 instructions to 8 values of a warp; memory alone would take 26.
 struct StoreArgs {
   uint8_t* data;
   const void *k, *v;
   const int64_t* slots;
   int64_t ks, kh, vs, vh, limit, page_bytes;
-  int tokens, heads, page_shift, vec;
+  int tokens, heads, per, page_shift;   // per: heads of a CTA
   int* bad;
 };
 
@@ -353,9 +357,9 @@ __device__ __forceinline__ void quantize8(const Eight<E>& in, __half& scale, uin
     Eight<E> ends;
     *reinterpret_cast<uint32_t*>(ends.e) = both;
     const float most = Elem<E>::in(ends.e[0]), least = -Elem<E>::in(ends.e[1]);
-    look = __any_sync(kAll, most != most || least != least);
     top = fmaxf(most, 0.0f);
     low = fminf(least, 0.0f);
+    look = __any_sync(kAll, most != most || least != least || (top == -low && top > 0.0f));
   }
   if (look) {
     top = low = 0.0f;
@@ -372,7 +376,7 @@ __device__ __forceinline__ void quantize8(const Eight<E>& in, __half& scale, uin
     }
   }
   float m = top > -low ? top : low;
-  if (__any_sync(kAll, top == -low && top > 0.0f)) {
+  if (look && __any_sync(kAll, top == -low && top > 0.0f)) {
     // both signs at the largest magnitude: the first of them
     int at = 32;
 #pragma unroll
@@ -386,8 +390,7 @@ __device__ __forceinline__ void quantize8(const Eight<E>& in, __half& scale, uin
   }
   scale = __float2half_rn(fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f));
   const float d = __half2float(scale);
-  float inv = 0.0f;
-  if (d != 0.0f) inv = sizeof(E) == 4 ? __frcp_rn(d) : __fdividef(1.0f, d);
+  const float r = sizeof(E) == 4 ? __frcp_rn(d) : __fdividef(1.0f, d), inv = d != 0.0f ? r : 0.0f;
   const float a = inv * (1.0f / 15.25f), b = (8.0f + 0x1p-16f) * (1.0f / 15.25f);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -407,26 +410,26 @@ __device__ __forceinline__ void quantize8(const Eight<E>& in, __half& scale, uin
   }
 }
 
-template <int D, class E>
-__global__ void __launch_bounds__(128) kv_store_kernel(const StoreArgs a) {
+template <int D, class E, bool kVec>
+__global__ void __launch_bounds__(128, 8) kv_store_kernel(const StoreArgs a) {
   pdl_trigger();
   pdl_wait();
   using T = Tile<D>;
   constexpr int kOcts = D / 8, kTurns = (kTile * kOcts + 127) / 128;   // 8-value pieces of a row, turns of a thread
-  __shared__ uint8_t* base[kTile];              // the row's tile of this head; null: skipped
+  __shared__ int64_t base[kTile];               // the row's tile of the first head in the cache; -1: skipped
   __shared__ int place[kTile];
   __shared__ __align__(16) uint8_t bytes[kTile][D / 2 + 4];   // values, a pair of dims a byte
-  const int tid = threadIdx.x, head = blockIdx.x % a.heads, row0 = blockIdx.x / a.heads * kTile;
+  const int tid = threadIdx.x, groups = (a.heads + a.per - 1) / a.per, row0 = blockIdx.x / groups * kTile;
+  const int head0 = blockIdx.x % groups * a.per, head1 = min(head0 + a.per, a.heads), head_bytes = T::kBytes << (a.page_shift - 4);
   if (tid < kTile) {
-    uint8_t* p = nullptr;
+    int64_t p = -1;
     int tau = 0;
     if (row0 + tid < a.tokens) {
       const int64_t s = a.slots[row0 + tid];
       if (s >= a.limit) *a.bad = 1;
       else if (s >= 0) {
         const int in_page = (int)(s & ((1 << a.page_shift) - 1));
-        const int tiles = 1 << (a.page_shift - 4);
-        p = a.data + (s >> a.page_shift) * a.page_bytes + (int64_t)(head * tiles + (in_page >> 4)) * T::kBytes;
+        p = (s >> a.page_shift) * a.page_bytes + (int64_t)head0 * head_bytes + (in_page >> 4) * T::kBytes;
         tau = in_page & 15;
       }
     }
@@ -435,46 +438,54 @@ __global__ void __launch_bounds__(128) kv_store_kernel(const StoreArgs a) {
   }
   // the loads do not wait for the slots: rows that are skipped are rows all the same
   Eight<E> x[kTurns], y[kTurns];
+  auto load = [&](int head) {
 #pragma unroll
-  for (int k = 0; k < kTurns; ++k) {
-    const int w = tid + 128 * k, row = w / kOcts, o = w % kOcts;
-    if (row < kTile && row0 + row < a.tokens) {
-      x[k].load(static_cast<const E*>(a.k) + (int64_t)(row0 + row) * a.ks + head * a.kh + 8 * o, a.vec);
-      y[k].load(static_cast<const E*>(a.v) + (int64_t)(row0 + row) * a.vs + head * a.vh + 8 * o, a.vec);
-    } else {
+    for (int k = 0; k < kTurns; ++k) {
+      const int w = tid + 128 * k, row = w / kOcts, o = w % kOcts;
+      if (row < kTile && row0 + row < a.tokens) {
+        x[k].template load<kVec>(static_cast<const E*>(a.k) + (int64_t)(row0 + row) * a.ks + head * a.kh + 8 * o);
+        y[k].template load<kVec>(static_cast<const E*>(a.v) + (int64_t)(row0 + row) * a.vs + head * a.vh + 8 * o);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[k].e[i] = y[k].e[i] = Elem<E>::out(0.0f);
+        for (int i = 0; i < 8; ++i) x[k].e[i] = y[k].e[i] = Elem<E>::out(0.0f);
+      }
     }
-  }
+  };
+  load(head0);
   __syncthreads();
+  const int byte_row = tid & 15, byte_g = tid >> 4;   // in the second half: a row and a row pair g of every 16 dims
+  const bool byte_live = base[byte_row] >= 0;
+  uint8_t* byte_to = a.data + base[byte_row] + T::value_byte(place[byte_row], 2 * byte_g);
+  for (int head = head0; head < head1; ++head) {
+    const int64_t at = (int64_t)(head - head0) * head_bytes;
 #pragma unroll
-  for (int k = 0; k < kTurns; ++k) {
-    const int w = tid + 128 * k, row = w / kOcts, o = w % kOcts, j = o >> 2, t = o & 3;
-    if (row >= kTile) break;   // whole warps
-    uint8_t* p = base[row];
-    __half dk, dv;
-    uint32_t q[8];
-    quantize8(x[k], dk, q);
-    // only the low bits of a sum with the magic number's bits are kept, where those are 0
-    const uint32_t even = ((q[6] * 16 + q[4]) * 16 + q[2]) * 16 + q[0], odd = ((q[7] * 16 + q[5]) * 16 + q[3]) * 16 + q[1];
-    if (p) {
-      const int tau = place[row];
-      *reinterpret_cast<uint32_t*>(p + T::key_word(tau, j, t)) = __byte_perm(even, odd, 0x5410);
-      if (t == 0) *reinterpret_cast<__half*>(p + T::key_scale(tau, j)) = dk;
+    for (int k = 0; k < kTurns; ++k) {
+      const int w = tid + 128 * k, row = w / kOcts, o = w % kOcts, j = o >> 2, t = o & 3;
+      if (row >= kTile) break;   // whole warps
+      const bool live = base[row] >= 0;
+      uint8_t* p = a.data + base[row] + at;
+      __half dk, dv;
+      uint32_t q[8];
+      quantize8(x[k], dk, q);
+      // only the low bits of a sum with the magic number's bits are kept, where those are 0
+      const uint32_t even = ((q[6] * 16 + q[4]) * 16 + q[2]) * 16 + q[0], odd = ((q[7] * 16 + q[5]) * 16 + q[3]) * 16 + q[1];
+      if (live) {
+        const int tau = place[row];
+        *reinterpret_cast<uint32_t*>(p + T::key_word(tau, j, t)) = __byte_perm(even, odd, 0x5410);
+        if (t == 0) *reinterpret_cast<__half*>(p + T::key_scale(tau, j)) = dk;
+      }
+      quantize8(y[k], dv, q);
+      const uint32_t b01 = __byte_perm(q[1] * 16 + q[0], q[3] * 16 + q[2], 0x0040), b23 = __byte_perm(q[5] * 16 + q[4], q[7] * 16 + q[6], 0x0040);
+      *reinterpret_cast<uint32_t*>(&bytes[row][4 * o]) = __byte_perm(b01, b23, 0x5410);
+      if (live && t == 0) *reinterpret_cast<__half*>(p + T::value_scale(place[row], j)) = dv;
     }
-    quantize8(y[k], dv, q);
-    const uint32_t b01 = __byte_perm(q[1] * 16 + q[0], q[3] * 16 + q[2], 0x0040), b23 = __byte_perm(q[5] * 16 + q[4], q[7] * 16 + q[6], 0x0040);
-    *reinterpret_cast<uint32_t*>(&bytes[row][4 * o]) = __byte_perm(b01, b23, 0x5410);
-    if (p && t == 0) *reinterpret_cast<__half*>(p + T::value_scale(place[row], j)) = dv;
-  }
-  __syncthreads();
-  // thread: a row and a row pair g of every 16 dims
-  const int row = tid & 15, g = tid >> 4;
-  uint8_t* p = base[row];
-  if (p) {
-    p += T::value_byte(place[row], 2 * g);
+    if (head + 1 < head1) load(head + 1);
+    __syncthreads();
+    if (byte_live) {
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) p[T::value_byte(0, 16 * i) - T::value_byte(0, 0)] = bytes[row][8 * i + g];
+      for (int i = 0; i < D / 16; ++i) byte_to[at + T::value_byte(0, 16 * i) - T::value_byte(0, 0)] = bytes[byte_row][8 * i + byte_g];
+    }
+    if (head + 1 < head1) __syncthreads();
   }
 }
 
@@ -484,36 +495,43 @@ struct LoadArgs {
   void *k, *v;
   const int32_t *table, *first, *lengths, *row_begin;
   int64_t table_stride, ks, kh, vs, vh, page_bytes;
-  int requests, heads, table_width, rows, pages, page_shift, vec;
+  int requests, heads, per, table_width, rows, pages, page_shift;   // per: heads of a CTA
   int* bad;
 };
 
-// 8 quants as values: nibble i of `word` (low 16 bits) times d, nibble i + 4 the next (kPairs), or nibbles in order
-template <bool kPairs, class E>
-__device__ __forceinline__ void dequantize8(uint32_t word, __half scale, Eight<E>& out) {
-  const float d = __half2float(scale);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t two = (word >> (4 * i) & 0x000f000fu) | 0x64006400u;   // 1024 + nibbles i and i + 4
-    const __half2 q = __hsub2(*reinterpret_cast<const __half2*>(&two), __float2half2_rn(1032.0f));
-    out.e[kPairs ? 2 * i : i] = Elem<E>::out(__low2float(q) * d);
-    out.e[kPairs ? 2 * i + 1 : i + 4] = Elem<E>::out(__high2float(q) * d);
+// Two quants, in bits 0 and 16 of `two`, as values.  (q - 8) * d has 15 bits at most: f32 holds it, and f16's product rounds it once.
+template <class E>
+__device__ __forceinline__ void dequantize2(uint32_t two, __half2 d, float df, E* out) {
+  two = (two & 0x000f000fu) | 0x64006400u;   // 1024 + q
+  const __half2 q = __hsub2(*reinterpret_cast<const __half2*>(&two), __float2half2_rn(1032.0f));
+  if constexpr (std::is_same<E, __half>::value) {
+    *reinterpret_cast<__half2*>(out) = __hmul2(q, d);
+  } else if constexpr (std::is_same<E, __nv_bfloat16>::value) {
+    *reinterpret_cast<__nv_bfloat162*>(out) = __floats2bfloat162_rn(__low2float(q) * df, __high2float(q) * df);
+  } else {
+    out[0] = __low2float(q) * df;
+    out[1] = __high2float(q) * df;
   }
 }
 
-// A CTA takes a tile of a request and head: its 18 * D bytes by 16-byte loads, then rows of 8 values a thread.  Request b's tiles stand
-// in slots row_begin[b] / 16 + b * spare and further (two spare ones where its first position may lie inside a tile, else one), so a
-// slot finds its request by bisection, without a sum over the requests in front; heads are neighbours, whose rows are.
-// 32,760 rows of 8 heads of 128 f16: 37 us (4.6 TB/s); 44 when a CTA took 16 packed rows, each with a place of its own in the pages.
-// Memory bounds it, and the three reads in a row before its first byte.
-template <int D, class E>
-__global__ void __launch_bounds__(128) kv_load_kernel(const LoadArgs a) {
+// heads of a CTA at most: 1, 2 and 8 of them took 40, 36 and 35 us in the example below, and 50, 45 and 47 in the one above
+constexpr int kLoadHeads = 4, kStoreHeads = 4;
+
+// A CTA takes a tile of a request and head, or of up to kLoadHeads: its 18 * D bytes by 16-byte loads, then rows of 8 values a
+// thread.  Request b's tiles stand in slots row_begin[b] / 16 + b * spare and further (two spare ones where its first position may
+// lie inside a tile, else one), so a slot finds its request by bisection, without a sum over the requests in front; heads are
+// neighbours, whose rows are.
+// 32,760 rows of 8 heads of 128 f16: 31 us (5.5 TB/s); 44 when a CTA took 16 packed rows, each with a place of its own in the pages,
+// 37 with a tile and a head.  Memory bounds it, and the three reads in a row before a CTA's first byte.
+template <int D, class E, bool kVec>
+__global__ void __launch_bounds__(128, 10) kv_load_kernel(const LoadArgs a) {
   pdl_trigger();
   pdl_wait();
   using T = Tile<D>;
-  __shared__ __align__(16) uint8_t tile[T::kBytes];
-  const int tid = threadIdx.x, lane = tid & 31, slot = blockIdx.x / a.heads, head = blockIdx.x % a.heads, spare = a.first ? 2 : 1;
-  if (head == 0 && tid == 127 && slot < a.requests && (a.row_begin[slot] < 0 || a.row_begin[slot + 1] < a.row_begin[slot])) *a.bad = 1;
+  __shared__ __align__(16) uint8_t tiles[kLoadHeads][T::kBytes];
+  const int tid = threadIdx.x, lane = tid & 31, groups = (a.heads + a.per - 1) / a.per, slot = blockIdx.x / groups, spare = a.first ? 2 : 1;
+  const int head0 = blockIdx.x % groups * a.per, heads = min(a.per, a.heads - head0);
+  if (head0 == 0 && tid == 127 && slot < a.requests && (a.row_begin[slot] < 0 || a.row_begin[slot + 1] < a.row_begin[slot])) *a.bad = 1;
   int lo = 0, hi = a.requests;          // the last request whose slots begin at or before this one
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32, b = lo + lane * step;
@@ -539,10 +557,12 @@ __global__ void __launch_bounds__(128) kv_load_kernel(const LoadArgs a) {
     if (tid == 0) *a.bad = 1;
     return;
   }
-  const uint8_t* p = a.data + page * a.page_bytes + (int64_t)((head << (a.page_shift - 4)) + (int)(at >> 4 & ((1 << (a.page_shift - 4)) - 1))) * T::kBytes;
+  const int shift = a.page_shift - 4;
+  const uint8_t* p = a.data + page * a.page_bytes + (int64_t)((head0 << shift) + (int)(at >> 4 & ((1 << shift) - 1))) * T::kBytes;
+  for (int h = 0; h < heads; ++h, p += T::kBytes << shift)
 #pragma unroll
-  for (int i = 0; i < T::kBytes / 16; i += 128)
-    if (i + tid < T::kBytes / 16) reinterpret_cast<uint4*>(tile)[i + tid] = reinterpret_cast<const uint4*>(p)[i + tid];
+    for (int i = 0; i < T::kBytes / 16; i += 128)
+      if (i + tid < T::kBytes / 16) reinterpret_cast<uint4*>(tiles[h])[i + tid] = reinterpret_cast<const uint4*>(p)[i + tid];
   __syncthreads();
   constexpr int kOcts = D / 8;
   const int64_t row0 = begin + (at - first);
@@ -550,15 +570,29 @@ __global__ void __launch_bounds__(128) kv_load_kernel(const LoadArgs a) {
   for (int k = 0; k < kTile * kOcts; k += 128) {
     const int w = tid + k, tau = w / kOcts, o = w % kOcts, j = o >> 2, t = o & 3;
     if (tau < from || tau >= to) continue;
-    Eight<E> x;
-    dequantize8<true>(*reinterpret_cast<const uint32_t*>(tile + T::key_word(tau, j, t)), *reinterpret_cast<const __half*>(tile + T::key_scale(tau, j)), x);
-    x.store(static_cast<E*>(a.k) + (row0 + tau) * a.ks + head * a.kh + 8 * o, a.vec);
-    uint32_t two[4];
+    E* to_k = static_cast<E*>(a.k) + (row0 + tau) * a.ks + head0 * a.kh + 8 * o;
+    E* to_v = static_cast<E*>(a.v) + (row0 + tau) * a.vs + head0 * a.vh + 8 * o;
+    const uint8_t* tile = tiles[0];
+    for (int h = 0; h < heads; ++h, tile += T::kBytes, to_k += a.kh, to_v += a.vh) {
+      Eight<E> x;
+      const uint32_t word = *reinterpret_cast<const uint32_t*>(tile + T::key_word(tau, j, t));
+      const __half dk = *reinterpret_cast<const __half*>(tile + T::key_scale(tau, j)), dv = *reinterpret_cast<const __half*>(tile + T::value_scale(tau, j));
+      const __half2 dk2 = __half2half2(dk), dv2 = __half2half2(dv);
+      const float dkf = __half2float(dk), dvf = __half2float(dv);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) two[e] = tile[T::value_byte(tau, 8 * o + 2 * e)];
-    dequantize8<false>(two[0] | two[1] << 8 | two[2] << 16 | two[3] << 24, *reinterpret_cast<const __half*>(tile + T::value_scale(tau, j)), x);
-    x.store(static_cast<E*>(a.v) + (row0 + tau) * a.vs + head * a.vh + 8 * o, a.vec);
+      for (int e = 0; e < 4; ++e) dequantize2(word >> (4 * e), dk2, dkf, x.e + 2 * e);
+      x.template store<kVec>(to_k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dequantize2(tile[T::value_byte(tau, 8 * o + 2 * e)] * 0x1001u, dv2, dvf, x.e + 2 * e);
+      x.template store<kVec>(to_v);
+    }
   }
+}
+
+// heads of a CTA: as many as leave 16 CTAs to an SM
+int heads_each(int64_t tiles, int heads, int sm_count, int most) {
+  const int64_t spare = tiles * heads / ((int64_t)sm_count * 16);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({spare, (int64_t)most, (int64_t)heads}));
 }
 
 int log2_of(int v) {
@@ -571,23 +605,31 @@ bool rows_aligned(const void* p, int64_t token, int64_t head, size_t size) {
 }
 size_t size_of(int type) { return type == EMELB_F32 ? 4 : 2; }
 
-template <class E>
+template <class E, bool kVec>
 cudaError_t store_typed(int D, unsigned grid, const StoreArgs& a, bool pdl, cudaStream_t st) {
   switch (D) {
-    case 32: return launch_kernel(kv_store_kernel<32, E>, dim3(grid), dim3(128), 0, st, pdl, a);
-    case 64: return launch_kernel(kv_store_kernel<64, E>, dim3(grid), dim3(128), 0, st, pdl, a);
-    case 96: return launch_kernel(kv_store_kernel<96, E>, dim3(grid), dim3(128), 0, st, pdl, a);
-    default: return launch_kernel(kv_store_kernel<128, E>, dim3(grid), dim3(128), 0, st, pdl, a);
+    case 32: return launch_kernel(kv_store_kernel<32, E, kVec>, dim3(grid), dim3(128), 0, st, pdl, a);
+    case 64: return launch_kernel(kv_store_kernel<64, E, kVec>, dim3(grid), dim3(128), 0, st, pdl, a);
+    case 96: return launch_kernel(kv_store_kernel<96, E, kVec>, dim3(grid), dim3(128), 0, st, pdl, a);
+    default: return launch_kernel(kv_store_kernel<128, E, kVec>, dim3(grid), dim3(128), 0, st, pdl, a);
   }
 }
 template <class E>
+cudaError_t store_typed(bool vec, int D, unsigned grid, const StoreArgs& a, bool pdl, cudaStream_t st) {
+  return vec ? store_typed<E, true>(D, grid, a, pdl, st) : store_typed<E, false>(D, grid, a, pdl, st);
+}
+template <class E, bool kVec>
 cudaError_t load_typed(int D, unsigned grid, const LoadArgs& a, bool pdl, cudaStream_t st) {
   switch (D) {
-    case 32: return launch_kernel(kv_load_kernel<32, E>, dim3(grid), dim3(128), 0, st, pdl, a);
-    case 64: return launch_kernel(kv_load_kernel<64, E>, dim3(grid), dim3(128), 0, st, pdl, a);
-    case 96: return launch_kernel(kv_load_kernel<96, E>, dim3(grid), dim3(128), 0, st, pdl, a);
-    default: return launch_kernel(kv_load_kernel<128, E>, dim3(grid), dim3(128), 0, st, pdl, a);
+    case 32: return launch_kernel(kv_load_kernel<32, E, kVec>, dim3(grid), dim3(128), 0, st, pdl, a);
+    case 64: return launch_kernel(kv_load_kernel<64, E, kVec>, dim3(grid), dim3(128), 0, st, pdl, a);
+    case 96: return launch_kernel(kv_load_kernel<96, E, kVec>, dim3(grid), dim3(128), 0, st, pdl, a);
+    default: return launch_kernel(kv_load_kernel<128, E, kVec>, dim3(grid), dim3(128), 0, st, pdl, a);
   }
+}
+template <class E>
+cudaError_t load_typed(bool vec, int D, unsigned grid, const LoadArgs& a, bool pdl, cudaStream_t st) {
+  return vec ? load_typed<E, true>(D, grid, a, pdl, st) : load_typed<E, false>(D, grid, a, pdl, st);
 }
 
 }  // namespace
@@ -609,7 +651,7 @@ cudaError_t launch_kv_plan(const emelb_kv_plan_request& r, int* scratch, int sm_
   return e;
 }
 
-cudaError_t launch_kv_store(const emelb_kv_store_request& r, int* bad, bool pdl, cudaStream_t st) {
+cudaError_t launch_kv_store(const emelb_kv_store_request& r, int sm_count, int* bad, bool pdl, cudaStream_t st) {
   const size_t size = size_of(r.type);
   StoreArgs a{};
   a.data = static_cast<uint8_t*>(r.cache.data);
@@ -625,15 +667,17 @@ cudaError_t launch_kv_store(const emelb_kv_store_request& r, int* bad, bool pdl,
   a.tokens = r.tokens;
   a.heads = r.cache.kv_heads;
   a.page_shift = log2_of(r.cache.page_tokens);
-  a.vec = rows_aligned(r.k, a.ks, a.kh, size) && rows_aligned(r.v, a.vs, a.vh, size);
+  const bool vec = rows_aligned(r.k, a.ks, a.kh, size) && rows_aligned(r.v, a.vs, a.vh, size);
   a.bad = bad;
-  const unsigned grid = (unsigned)((r.tokens + kTile - 1) / kTile) * r.cache.kv_heads;   // heads are neighbours, as their rows
-  if (r.type == EMELB_F32) return store_typed<float>(r.cache.head_dim, grid, a, pdl, st);
-  if (r.type == EMELB_F16) return store_typed<__half>(r.cache.head_dim, grid, a, pdl, st);
-  return store_typed<__nv_bfloat16>(r.cache.head_dim, grid, a, pdl, st);
+  const int tiles = (r.tokens + kTile - 1) / kTile;
+  a.per = heads_each(tiles, a.heads, sm_count, kStoreHeads);
+  const unsigned grid = (unsigned)tiles * ((a.heads + a.per - 1) / a.per);   // heads are neighbours, as their rows
+  if (r.type == EMELB_F32) return store_typed<float>(vec, r.cache.head_dim, grid, a, pdl, st);
+  if (r.type == EMELB_F16) return store_typed<__half>(vec, r.cache.head_dim, grid, a, pdl, st);
+  return store_typed<__nv_bfloat16>(vec, r.cache.head_dim, grid, a, pdl, st);
 }
 
-cudaError_t launch_kv_load(const emelb_kv_load_request& r, int* bad, bool pdl, cudaStream_t st) {
+cudaError_t launch_kv_load(const emelb_kv_load_request& r, int sm_count, int* bad, bool pdl, cudaStream_t st) {
   const size_t size = size_of(r.type);
   LoadArgs a{};
   a.data = static_cast<const uint8_t*>(r.cache.data);
@@ -655,12 +699,14 @@ cudaError_t launch_kv_load(const emelb_kv_load_request& r, int* bad, bool pdl, c
   a.rows = r.rows;
   a.pages = r.cache.pages;
   a.page_shift = log2_of(r.cache.page_tokens);
-  a.vec = rows_aligned(r.k, a.ks, a.kh, size) && rows_aligned(r.v, a.vs, a.vh, size);
+  const bool vec = rows_aligned(r.k, a.ks, a.kh, size) && rows_aligned(r.v, a.vs, a.vh, size);
   a.bad = bad;
-  const unsigned grid = (unsigned)(r.rows / kTile + r.requests * (r.first ? 2 : 1)) * r.cache.kv_heads;
-  if (r.type == EMELB_F32) return load_typed<float>(r.cache.head_dim, grid, a, pdl, st);
-  if (r.type == EMELB_F16) return load_typed<__half>(r.cache.head_dim, grid, a, pdl, st);
-  return load_typed<__nv_bfloat16>(r.cache.head_dim, grid, a, pdl, st);
+  const int tiles = r.rows / kTile + r.requests * (r.first ? 2 : 1);
+  a.per = heads_each(r.rows / kTile, a.heads, sm_count, kLoadHeads);
+  const unsigned grid = (unsigned)tiles * ((a.heads + a.per - 1) / a.per);
+  if (r.type == EMELB_F32) return load_typed<float>(vec, r.cache.head_dim, grid, a, pdl, st);
+  if (r.type == EMELB_F16) return load_typed<__half>(vec, r.cache.head_dim, grid, a, pdl, st);
+  return load_typed<__nv_bfloat16>(vec, r.cache.head_dim, grid, a, pdl, st);
 }
 
 }  // namespace emelb

@@ -11,8 +11,8 @@ namespace emelb {
 // `bad`: raised to 1 by a kernel that met a length, page or slot out of range and left it alone
 // `scratch`: requests + 1 ints
 cudaError_t launch_kv_plan(const emelb_kv_plan_request& r, int* scratch, int sm_count, int* launches, int* bad, bool pdl, cudaStream_t st);
-cudaError_t launch_kv_store(const emelb_kv_store_request& r, int* bad, bool pdl, cudaStream_t st);
-cudaError_t launch_kv_load(const emelb_kv_load_request& r, int* bad, bool pdl, cudaStream_t st);
+cudaError_t launch_kv_store(const emelb_kv_store_request& r, int sm_count, int* bad, bool pdl, cudaStream_t st);
+cudaError_t launch_kv_load(const emelb_kv_load_request& r, int sm_count, int* bad, bool pdl, cudaStream_t st);
 
 // scratch of emelb_kv_attend: two partial results a unit, its arrival counter (zero between launches)
 struct KvAttendScratch {

@@ -165,7 +165,7 @@ uint32_t emelb_kv_store_can_run(const emelb_kv_store_request* r) {
 uint32_t emelb_kv_store(emelb_ctx* c, const emelb_kv_store_request* r) {
   if (!c || !r) return EMELB_INVALID_REQUEST;
   if (const uint32_t why = emelb_kv_store_can_run(r)) return refuse(c, why);
-  return dispatch(c, {r->cache.data, r->k, r->v, r->slots}, 1, [&] { return launch_kv_store(*r, c->bad_word(), c->pdl & 1, c->stream); });
+  return dispatch(c, {r->cache.data, r->k, r->v, r->slots}, 1, [&] { return launch_kv_store(*r, c->sm_count, c->bad_word(), c->pdl & 1, c->stream); });
 }
 
 uint32_t emelb_kv_load_can_run(const emelb_kv_load_request* r) {
@@ -202,7 +202,7 @@ uint32_t emelb_kv_load(emelb_ctx* c, const emelb_kv_load_request* r) {
   if (!c || !r) return EMELB_INVALID_REQUEST;
   if (const uint32_t why = emelb_kv_load_can_run(r)) return refuse(c, why);
   return dispatch(c, {r->cache.data, r->k, r->v, r->table, r->first, r->lengths, r->row_begin}, 1,
-                  [&] { return launch_kv_load(*r, c->bad_word(), c->pdl & 1, c->stream); });
+                  [&] { return launch_kv_load(*r, c->sm_count, c->bad_word(), c->pdl & 1, c->stream); });
 }
 
 // ------------------------------------------------------------------ attend

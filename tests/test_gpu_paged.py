@@ -294,6 +294,26 @@ def test_load_many_requests(be, n, with_first, short):
         assert torch.equal(z[5:rows], want[:rows - 5]) and (z[:5] == 7.0).all() and (z[rows:] == 7.0).all()
 
 
+@pytest.mark.parametrize("heads,dim,lengths,layout", [(8, 32, [9000, 3001, 7], "dense"), (7, 64, [6000, 5, 8000], "part"), (3, 96, [26000], "heads")])
+def test_store_and_load_many_rows(be, heads, dim, lengths, layout):
+    """So many rows that a CTA takes several heads, and not all CTAs the same number."""
+    rng, g = np.random.default_rng(heads), gen(heads)
+    table, pages = tables(rng, lengths, 32)
+    slots = slots_of(table, [0] * len(lengths), lengths, 32)
+    n = len(slots)
+    slots[5], slots[n - 3] = -1, -4
+    k, v = (placed(torch.randn((n, heads, dim), generator=g, device="cuda"), layout, torch.bfloat16) for _ in range(2))
+    c = Cache(pages, 32, heads, dim)
+    got = [torch.full((n, heads, dim), 7.0, dtype=torch.float16, device="cuda") for _ in range(2)]
+    keep = [dev(slots.tolist(), torch.int64), torch.from_numpy(table).cuda(), dev(lengths), dev(np.concatenate([[0], np.cumsum(lengths)]).tolist())]
+    torch.cuda.synchronize()
+    done(be, be.kv_store(paged.store_request(c.pages, k, v, "bf16", keep[0], n)))
+    done(be, be.kv_load(paged.load_request(c.pages, *got, "f16", keep[1], table.shape[1], keep[2], keep[3], len(lengths), n)))
+    live = keep[0] >= 0
+    for y, z in zip((k, v), got):
+        assert torch.equal(z[live], plain.kept(y)[live].half())
+
+
 def test_load_reports_beginnings_out_of_order(be):
     c = Cache(8, 16, 2, 64)
     table, lengths = dev([[0], [1], [2]]), dev([10, 10, 10])
