@@ -20,12 +20,14 @@
 //
 // us, two prompts of 4100 and 8190 tokens / 13 of 17 to 600, 32 heads of 128: 756 with weights handed over at once and an arrival a
 // thread; 659 / 95 by halves and with registers split; 578 / 61 with queries by asynchronous copies; 544 (1,263 TFLOP/s) / 52 since
-// CTAs stay.  One prompt of 8192 and heads of 64: 411 (667 TFLOP/s; its exponentials alone take 252).  Measured and left out: an
-// issuer of products for each row tile 613 / - (they fall into step and wait for the same pipes); scores of 64 keys in two buffers a
-// row tile, so that none waits for a mix, 588 (products with 64 columns take longer); weights against a stale maximum, looked at
-// afterwards, 604; an eighth, a quarter of the exponentials by polynomials on the multiply-adds, no gain, +8; at head_dim 64, where
-// TMEM has room, weights beside the scores so that the next scores need not wait for the mix, 421 for 394, and turns at the exponentials
-// for the two warps of a scheduler, 394 (558 for 538 at 128).
+// CTAs stay (640 when repeated for seconds: the chip is at 990 W then, at 1.58 GHz).  One prompt of 8192 and heads of 64: 394 (698
+// TFLOP/s; its exponentials alone take 252).
+//
+// Measured and left out: an issuer of products for each row tile 613 / - (they fall into step and wait for the same pipes); scores
+// of 64 keys in two buffers a row tile, so that none waits for a mix, 588 (products with 64 columns take longer); weights against a
+// stale maximum, looked at afterwards, 604; an eighth, a quarter of the exponentials by polynomials on the multiply-adds, no gain,
+// +8; at head_dim 64, where TMEM has room, weights beside the scores so that the next scores need not wait for the mix, 421 for 394,
+// and turns at the exponentials for the two warps of a scheduler, 394 (558 for 538 at 128).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
