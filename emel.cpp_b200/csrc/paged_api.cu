@@ -1,6 +1,4 @@
 // C entry points of include/emelb_paged.h: what a request may be, where its memory lies, the launch.
-#include <cmath>
-
 #include "ctx.h"
 #include "paged.h"
 
@@ -214,7 +212,7 @@ uint32_t emelb_kv_attend_can_run(const emelb_kv_attend_request* r) {
   const uint64_t size = elem_bytes(r->type);
   if (size == 0) return EMELB_UNSUPPORTED_OP;
   const int D = r->cache.head_dim;
-  if (r->heads % r->cache.kv_heads != 0 || !std::isfinite(r->scale) || !(r->scale > 0.0f)) return EMELB_INVALID_REQUEST;
+  if (r->heads % r->cache.kv_heads != 0 || !(r->scale > 0.0f && r->scale < 0x1p127f)) return EMELB_INVALID_REQUEST;
   if (!r->query_begin && r->queries < r->requests) return EMELB_INVALID_REQUEST;
   if (!aligned(r->q, size) || !aligned(r->out, size) || !aligned(r->table, 4) || !aligned(r->lengths, 4) || (r->query_begin && !aligned(r->query_begin, 4)))
     return EMELB_INVALID_REQUEST;
@@ -245,7 +243,7 @@ uint32_t emelb_kv_attend(emelb_ctx* c, const emelb_kv_attend_request* r) {
 uint32_t emelb_attend_packed_can_run(const emelb_attend_packed_request* r) {
   if (!r || r->requests <= 0 || r->heads <= 0 || r->kv_heads <= 0 || r->head_dim <= 0 || r->queries <= 0 || r->keys < 0 || r->max_queries <= 0)
     return EMELB_INVALID_REQUEST;
-  if (r->heads % r->kv_heads != 0 || !std::isfinite(r->scale) || !(r->scale > 0.0f)) return EMELB_INVALID_REQUEST;
+  if (r->heads % r->kv_heads != 0 || !(r->scale > 0.0f && r->scale < 0x1p127f)) return EMELB_INVALID_REQUEST;
   const uint64_t size = elem_bytes(r->type);
   if (size != 2) return EMELB_UNSUPPORTED_OP;
   const int D = r->head_dim, keys = r->keys > 0 ? r->keys : 1;

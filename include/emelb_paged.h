@@ -19,6 +19,7 @@
  *  - Lengths, tables and slots are read by the kernels.  Values that are out of range are skipped, never followed, and
  *    make the next emelb_sync return EMELB_INVALID_REQUEST.
  *  - Strides count elements.  The head_dim values of a row are contiguous.
+ *  - No result overlaps an input, but for emelb_kv_plan's in-place step; a request where one does is refused.
  */
 #ifndef EMELB_PAGED_H
 #define EMELB_PAGED_H
@@ -54,6 +55,7 @@ EMELB_API uint64_t emelb_kv_page_bytes(int32_t head_dim, int32_t kv_heads, int32
  * top of the stack free_pages (free_count entries before) in request and table order; then each request in order takes
  * the pages it lacks from the top and appends them to its row of `table`.  The first request for which they do not suffice
  * gets nothing in this step, nor does any after it that lacks a page: its slots are -1 and its length stays cached[b].
+ * A page belongs to one request: one that stands in two rows of the table is given back twice.
  *
  *   lengths[b]      tokens of the request behind the step (0 when ended)
  *   query_begin[b]  first packed row of the request's fresh tokens; [requests] = all of them (waiting requests included)
@@ -132,7 +134,7 @@ typedef struct emelb_kv_attend_request {
   const int32_t* query_begin; /* [requests + 1] or null */
   int64_t table_stride, q_token_stride, q_head_stride, out_token_stride, out_head_stride;
   int32_t requests, table_width, heads, queries, max_queries;
-  float scale;            /* positive */
+  float scale;            /* positive, below 2^127 */
   uint8_t type;
 } emelb_kv_attend_request;
 EMELB_API uint32_t emelb_kv_attend_can_run(const emelb_kv_attend_request* request);
@@ -158,7 +160,7 @@ typedef struct emelb_attend_packed_request {
       out_head_stride;
   int32_t requests, heads, kv_heads, head_dim, queries, keys, max_queries;
   int32_t causal;
-  float scale;            /* positive */
+  float scale;            /* positive, below 2^127 */
   uint8_t type;
 } emelb_attend_packed_request;
 EMELB_API uint32_t emelb_attend_packed_can_run(const emelb_attend_packed_request* request);

@@ -96,7 +96,7 @@ def test_load_requests(kw, change, why):
     ({}, {}, eb.OK), ({}, dict(query_begin=at(5), queries=20, max_queries=8), eb.OK), ({}, dict(type="f32"), eb.OK), ({}, dict(type=3), eb.UNSUPPORTED_OP),
     ({}, dict(heads=5), eb.INVALID_REQUEST), ({}, dict(heads=128), eb.OK), ({}, dict(heads=130), eb.UNSUPPORTED_OP), ({}, dict(heads=0), eb.INVALID_REQUEST),
     ({}, dict(scale=0.0), eb.INVALID_REQUEST), ({}, dict(scale=-1.0), eb.INVALID_REQUEST), ({}, dict(scale=float("nan")), eb.INVALID_REQUEST),
-    ({}, dict(scale=float("inf")), eb.INVALID_REQUEST), ({}, dict(queries=2), eb.INVALID_REQUEST), ({}, dict(max_queries=0), eb.INVALID_REQUEST),
+    ({}, dict(scale=float("inf")), eb.INVALID_REQUEST), ({}, dict(scale=3e38), eb.INVALID_REQUEST), ({}, dict(scale=float("nan")), eb.INVALID_REQUEST), ({}, dict(queries=2), eb.INVALID_REQUEST), ({}, dict(max_queries=0), eb.INVALID_REQUEST),
     ({}, dict(requests=8193, queries=8193), eb.UNSUPPORTED_OP), ({}, dict(out=at(1)), eb.INVALID_REQUEST), ({}, dict(out=at(0)), eb.INVALID_REQUEST),
     ({}, dict(out_strides=(64, 64)), eb.INVALID_REQUEST), ({}, dict(q_strides=(512, 64)), eb.OK), ({}, dict(table_stride=1), eb.INVALID_REQUEST),
     (dict(head_dim=160), {}, eb.UNSUPPORTED_OP), (dict(page_tokens=17), {}, eb.UNSUPPORTED_OP), ({}, dict(lengths=at(4) + 2), eb.INVALID_REQUEST),
@@ -111,6 +111,7 @@ def test_attend_requests(kw, change, why):
     (dict(type="f32"), eb.UNSUPPORTED_OP), (dict(head_dim=68), eb.UNSUPPORTED_OP), (dict(head_dim=136), eb.UNSUPPORTED_OP),
     (dict(head_dim=0), eb.INVALID_REQUEST), (dict(heads=3), eb.INVALID_REQUEST), (dict(heads=256), eb.OK), (dict(heads=258), eb.UNSUPPORTED_OP),
     (dict(queries=0), eb.INVALID_REQUEST), (dict(keys=-1), eb.INVALID_REQUEST), (dict(requests=0), eb.INVALID_REQUEST), (dict(scale=0.0), eb.INVALID_REQUEST),
+    (dict(scale=2.0 ** 127), eb.INVALID_REQUEST), (dict(scale=2.0 ** 126), eb.OK), (dict(scale=float("nan")), eb.INVALID_REQUEST),
     (dict(q=at(0) + 2), eb.UNSUPPORTED_OP), (dict(q=at(0) + 1), eb.INVALID_REQUEST), (dict(k_strides=(132, 64)), eb.UNSUPPORTED_OP),
     (dict(k_strides=(136, 64)), eb.OK), (dict(v_strides=(64, 1280)), eb.OK), (dict(out=at(0)), eb.INVALID_REQUEST), (dict(out=at(2) + 16), eb.INVALID_REQUEST),
     (dict(out_strides=(64, 64)), eb.INVALID_REQUEST), (dict(query_begin=at(4) + 2), eb.INVALID_REQUEST), (dict(max_queries=0), eb.INVALID_REQUEST),
