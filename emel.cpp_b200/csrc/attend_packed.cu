@@ -196,7 +196,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ int order[32];
   __shared__ volatile int gave_up;
-  pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t smem = (tc::smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t bar0 = tc::smem_u32(bars), bar1 = bar0 + 24 * kStages, bar2 = bar1 + 32 * kTiles;
@@ -230,7 +229,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  // no kernel holds TMEM while it waits for one that may still ask for some: allocation behind the wait, the next one's start behind it
   if (warp == kMmaWarp) {
+    pdl_wait();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&tmem_slot)), "r"(kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -322,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc::fence_after();
   pdl_wait();
+  pdl_trigger();
   const uint32_t tmem = tmem_slot;
   int loaded = 0, asked = 0;                       // loader: tiles asked for; plan: items whose queries were
   uint32_t on_landed = 0, landed_parity = 0;       // bits of stages: the last tile goes by `landed`; which phase comes next
