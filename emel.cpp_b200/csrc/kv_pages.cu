@@ -21,12 +21,14 @@ typedef long long i64;
 // ------------------------------------------------------------------ plan
 // Three running sums over the requests (tokens, pages lacking, pages given back) decide everything else: new page j is
 // entry top - 1 - j of the stack that the ended requests' pages lie on, and row i's request is found by bisection.  Every CTA
-// takes the sums for itself, since that is cheaper than handing them over, and then its share of the pages and of the rows, which
-// look a new page up where it comes from and not in the table, so that no CTA waits for another.  What is read and what is written
-// do not meet, but for `lengths` and free_left where they are `cached` and free_count: with more than one CTA those wait in scratch
-// for a second launch.
-// 1000 requests, 121,984 rows: 12.8 us, 21 by a cluster of 8 CTAs with a barrier between pages and rows, whose rows took half of it.
-// Its 1.6 MB take 0.3 us of bandwidth: what is left is the chain of sums, bisection and stores behind a launch.
+// takes the sums for itself, since that is cheaper than handing them over, and then its share of the pages, of the rows, which
+// look a new page up where it comes from and not in the table, or of what is left, so that no CTA waits for another.  What is read
+// and what is written do not meet, but for `lengths` and free_left where they are `cached` and free_count: with more than one CTA
+// those wait in scratch for a second launch.
+//
+// 1000 requests, 121,984 rows: 10.3 us one behind the other, 12.4 with pages, rows and the requests' numbers in the same CTAs, 21 by a
+// cluster of 8 CTAs with a barrier between pages and rows.  Its 1.6 MB take 0.3 us of bandwidth: what is left is a chain, in cycles
+// first reads 2,200, sums 3,500, a row's bisection, page and stores 5,400, and the launch.
 constexpr int kPlanMost = EMELB_KV_MAX_REQUESTS;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -91,7 +93,9 @@ __global__ void __launch_bounds__(512) kv_plan_kernel(const __grid_constant__ Pl
   __shared__ int most_taken;
   const emelb_kv_plan_request& r = a.r;
   const int n = r.requests, P = r.page_tokens, shift = a.page_shift, tid = threadIdx.x, T = blockDim.x;
-  const int ranks = gridDim.x, rank = blockIdx.x;
+  // one CTA for all, or some for the rows, as many for the pages and one for the requests' numbers
+  const int ranks = max(((int)gridDim.x - 1) / 2, 1), rank = blockIdx.x % ranks;
+  const bool alone = gridDim.x == 1, has_rows = blockIdx.x < ranks, has_pages = alone || (blockIdx.x >= ranks && blockIdx.x < 2 * ranks);
   int* tok = plan_smem;         // running sums, each request's own included
   int* need = tok + n;
   int* back = need + n;
@@ -161,14 +165,15 @@ __global__ void __launch_bounds__(512) kv_plan_kernel(const __grid_constant__ Pl
     const int x = (int)(at - count), e = owner_of(back, n, x);
     return r.table[e * r.table_stride + (x - (e ? back[e - 1] : 0))];
   };
-  const int step = ranks * T, me = rank * T + tid;
-  for (int j = me; j < taken; j += step) {
+  // shares by warps in turn, so that every CTA has some of the rows that cost most
+  const int step = ranks * T, me = ((tid >> 5) * ranks + rank) * 32 + (tid & 31);
+  for (int j = has_pages ? me : taken; j < taken; j += step) {
     const int b = owner_of(need, n, j), page = new_page(j);
     if (page < 0 || page >= r.pages) wrong = true;
     r.table[b * r.table_stride + ((had[b] + P - 1) >> shift) + (j - (b ? need[b - 1] : 0))] = page;
   }
   // what the ended requests gave back and nobody took
-  for (i64 x = me; x < top - taken - count; x += step) {
+  for (i64 x = has_pages ? me : top; x < top - taken - count; x += step) {
     const int e = owner_of(back, n, (int)x);
     if (count + x < r.pages) r.free_pages[count + x] = r.table[e * r.table_stride + (x - (e ? back[e - 1] : 0))];
     else wrong = true;
@@ -176,7 +181,7 @@ __global__ void __launch_bounds__(512) kv_plan_kernel(const __grid_constant__ Pl
   // slots and positions: four neighbouring rows a thread, of which the first is searched for
   const int total = clip(tok_sum < r.token_capacity ? tok_sum : r.token_capacity);
   const bool wide = reinterpret_cast<uintptr_t>(r.slots) % 16 == 0 && reinterpret_cast<uintptr_t>(r.positions) % 16 == 0;
-  for (int i0 = 4 * me; i0 < r.token_capacity; i0 = i0 > 0x7fffffff - 4 * step ? 0x7fffffff : i0 + 4 * step) {
+  for (int i0 = has_rows ? 4 * me : 0x7fffffff; i0 < r.token_capacity; i0 = i0 > 0x7fffffff - 4 * step ? 0x7fffffff : i0 + 4 * step) {
     i64 slot[4];
     int p[4], page[4], b = i0 < total ? owner_of(tok, n, i0) : 0;
     constexpr i64 kNew = (i64)1 << 62;
@@ -193,10 +198,16 @@ __global__ void __launch_bounds__(512) kv_plan_kernel(const __grid_constant__ Pl
         if (h >= 0) entry[e] = col < have ? b * r.table_stride + col : kNew | ((b ? need[b - 1] : 0) + col - have);
       }
     }
+    // a page once for its rows: mostly one or two of them, which the warp's lanes look up together
+    for (unsigned left = 15; left;) {
+      const i64 at = left & 1 ? entry[0] : left & 2 ? entry[1] : left & 4 ? entry[2] : entry[3];
+      const int found = at < 0 ? 0 : at < kNew ? r.table[at] : new_page((int)(at & ~kNew));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (e && entry[e] == entry[e - 1]) page[e] = page[e - 1];   // rows of one page: looked up once
-      else page[e] = entry[e] < 0 ? 0 : entry[e] < kNew ? r.table[entry[e]] : new_page((int)(entry[e] & ~kNew));
+      for (int e = 0; e < 4; ++e)
+        if (entry[e] == at) {
+          page[e] = found;
+          left &= ~(1u << e);
+        }
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -217,8 +228,8 @@ __global__ void __launch_bounds__(512) kv_plan_kernel(const __grid_constant__ Pl
         }
     }
   }
-  // each request's share, by the last CTA, which has the fewest rows; the barriers of the sums stand between reads and writes of one CTA
-  if (rank == ranks - 1) {
+  // each request's numbers; the barriers of the sums stand between reads and writes of one CTA
+  if (blockIdx.x == gridDim.x - 1) {
     auto length_of = [&](int b) {
       const int h = had[b];
       return r.fresh[b] < 0 ? 0 : h >= 0 ? h + (tok[b] - (b ? tok[b - 1] : 0)) : ~h;
@@ -639,7 +650,7 @@ cudaError_t launch_kv_plan(const emelb_kv_plan_request& r, int* scratch, int sm_
   if (e != cudaSuccess) return e;
   // a CTA's sums cost what 2000 rows do: few rows and requests are one CTA's
   const int threads = r.requests <= 256 && r.token_capacity <= 2048 ? 256 : 512;
-  const int ctas = threads == 256 ? 1 : std::min(sm_count, (r.token_capacity - 1) / 2048 + 1);
+  const int ctas = threads == 256 ? 1 : 2 * std::min(sm_count, (r.token_capacity - 1) / 2048 + 1) + 1;
   const bool aside = ctas > 1 && (r.lengths == r.cached || r.free_left == r.free_count);
   const PlanArgs a{r, aside ? scratch + 1 : r.lengths, aside ? scratch : r.free_left, log2_of(r.page_tokens), bad};
   // one behind the other: one CTA 5.6 us for 7.2 when it may start early, 60 of them 15.3 for 12.4
