@@ -648,10 +648,13 @@ cudaError_t load_typed(bool vec, int D, unsigned grid, const LoadArgs& a, bool p
 cudaError_t launch_kv_plan(const emelb_kv_plan_request& r, int* scratch, int sm_count, int* launches, int* bad, bool pdl, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 16 * kPlanMost);
   if (e != cudaSuccess) return e;
-  // a CTA's sums cost what 2000 rows do: few rows and requests are one CTA's
+  // a CTA's sums cost what 2000 rows do: few rows and requests are one CTA's.  2048 rows at most of 300 / 1000 / 2000 requests by
+  // one CTA 7.1 / 8.3 / 11.2 us, by three 8.4 / 8.4 / 10.5; in place, which three do by two launches, 7.3 / 8.6 / 11.5 and 8.6 / 10.5 / 11.3
   const int threads = r.requests <= 256 && r.token_capacity <= 2048 ? 256 : 512;
-  const int ctas = threads == 256 ? 1 : 2 * std::min(sm_count, (r.token_capacity - 1) / 2048 + 1) + 1;
-  const bool aside = ctas > 1 && (r.lengths == r.cached || r.free_left == r.free_count);
+  const int teams = std::min(sm_count, (r.token_capacity - 1) / 2048 + 1);
+  const bool in_place = r.lengths == r.cached || r.free_left == r.free_count;
+  const int ctas = teams == 1 && r.requests <= 1024 ? 1 : 2 * teams + 1;
+  const bool aside = ctas > 1 && in_place;
   const PlanArgs a{r, aside ? scratch + 1 : r.lengths, aside ? scratch : r.free_left, log2_of(r.page_tokens), bad};
   // one behind the other: one CTA 5.6 us for 7.2 when it may start early, 60 of them 15.3 for 12.4
   e = launch_kernel(kv_plan_kernel, dim3(ctas), dim3(threads), 16 * r.requests, st, pdl && ctas == 1, a);
