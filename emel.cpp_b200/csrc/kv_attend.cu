@@ -15,9 +15,9 @@
 //
 // 64 requests of 1000 to 8000 tokens, 64 heads on 8 of 128: 139 us with steps of 16 tokens, 131 with 32 (one maximum, one exchange
 // for both), 116 with asynchronous copies in place of bulk ones (no barrier to wait at), 94 since a team takes whole pairs where
-// that costs no more, 90 (3.7 TB/s) with joins in the order of the fragments.  What bounds it is issue: about 300 instructions to 16
-// tokens of a head, two of the four that an SM could issue a cycle.  One document of 100,001 tokens and 16 rows reads as two tiles of
-// rows, each unpacked for itself: 68 us, 78 with both in one warp (registers).  12 warps with 168 registers do better than 16 with
+// that costs no more, 90 with joins in the order of the fragments, 85 (3.9 TB/s) with a kernel for each type.  What bounds it is issue:
+// about 300 instructions to 16 tokens of a head, two of the four that an SM could issue a cycle.  One document of 100,001 tokens and 16
+// rows reads as two tiles of rows, each unpacked for itself: 68 us, 78 with both in one warp (registers).  12 warps with 168 registers do better than 16 with
 // 128 (105 us).  Small calls are a chain: the line from the lengths, the first tiles from memory, the joins.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -151,21 +151,23 @@ __device__ __forceinline__ float lds_half(uint32_t at) {
   return __half2float(__ushort_as_half(v));
 }
 
+template <Kind kind>
 __device__ __forceinline__ float load_query(const AttendArgs& a, int64_t at) {
-  if (a.type == EMELB_F32) return static_cast<const float*>(a.q)[at];
-  if (a.type == EMELB_F16) return __half2float(static_cast<const __half*>(a.q)[at]);
+  if (kind == kF32) return static_cast<const float*>(a.q)[at];
+  if (kind == kF16) return __half2float(static_cast<const __half*>(a.q)[at]);
   return __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[at]);
 }
 // two neighbouring dims
+template <Kind kind>
 __device__ __forceinline__ void store_pair(const AttendArgs& a, int64_t at, float x, float y) {
-  if (a.type == EMELB_F32) {
+  if (kind == kF32) {
     float* p = static_cast<float*>(a.out) + at;
     p[0] = x;
     p[1] = y;
     return;
   }
   uint32_t two;
-  if (a.type == EMELB_F16) {
+  if (kind == kF16) {
     two = half2_of(x, y);
   } else {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
@@ -234,7 +236,7 @@ __device__ __forceinline__ void team_barrier(int team, int threads) {
 }
 
 // kF32: the queries and the weights go in as two f16 operands each.  kF16: a weight's low part goes into its product with the scale,
-// so that there is one rounding to f16 and not two (one document of 100,001 tokens: 71 us for 68, its error against exact results 1.3
+// so that there is one rounding to f16 and not two (one document of 100,001 tokens: 3 us of 70, its error against exact results 1.3
 // and not 1.6 times what the results' own rounding makes)
 template <int D, Kind kind>
 __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kernel(const __grid_constant__ AttendArgs a) {
@@ -493,8 +495,6 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
     cp_async_commit();
   };
   int taken = 0, stage = 0;             // steps done, the stage of the next
-  find_batch(0);
-  for (int k = 0; k < kStages; ++k) issue(k, k);
   // lanes past the last group, or past the values' scales, look at another's (times 0, or once more)
   const int lane_v = lane % (8 * J), own_scale = (g * J + t % J) * 2;
   const Bases bases{tc::in_register(0x64006400u), tc::in_register(0x54005400u), tc::in_register(0x5c005c00u), tc::in_register(0x4c004c00u)};
@@ -526,31 +526,29 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
     const int i = live ? row / a.group : 0;
     const int64_t from = (int64_t)(r.first + i) * a.qs + (int64_t)(head * a.group + (live ? row - i * a.group : 0)) * a.qh;
     off[0] = off[1] = 0;
+    uint4 raw[J];
+    if (!kExact && a.q_vec) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) raw[j] = live ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + from + 32 * j + 8 * t) : make_uint4(0, 0, 0, 0);
+    }
+    if (x == lo) {   // the first tiles, while the first queries are on their way
+      find_batch(0);
+      for (int k = 0; k < kStages; ++k) issue(k, k);
+    }
     float all_v[J][8];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       float (&v)[8] = all_v[j];
+      if (!kExact && a.q_vec) {
+        const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-      if (live) {
-        const int64_t at8 = from + 32 * j + 8 * t;
-        if (a.q_vec && !kExact) {
-          const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at8);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (a.type == EMELB_F16) {
-              v[2 * e] = low_of(w[e]);
-              v[2 * e + 1] = high_of(w[e]);
-            } else {
-              v[2 * e] = __uint_as_float(w[e] << 16);
-              v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = load_query(a, at8 + e);
+        for (int e = 0; e < 4; ++e) {
+          v[2 * e] = kFine ? low_of(w[e]) : __uint_as_float(w[e] << 16);
+          v[2 * e + 1] = kFine ? high_of(w[e]) : __uint_as_float(w[e] & 0xffff0000u);
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = live ? load_query<kind>(a, from + 32 * j + 8 * t + e) : 0.0f;
       }
     }
     // f16 reaches less far than bf16 and f32: the eight rows go in times the power of two (at most 2^60) that takes their largest value
@@ -864,8 +862,8 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
       to[h] = rr < all_rows ? (int64_t)(r.first + i) * a.os + (int64_t)(head * a.group + rr - i * a.group) * a.oh + 2 * g : -1;
     }
     auto put = [&](int i16, const float4& v, float inv0, float inv1) {
-      if (to[0] >= 0) store_pair(a, to[0] + i16 * 16, v.x * inv0, v.z * inv0);
-      if (to[1] >= 0) store_pair(a, to[1] + i16 * 16, v.y * inv1, v.w * inv1);
+      if (to[0] >= 0) store_pair<kind>(a, to[0] + i16 * 16, v.x * inv0, v.z * inv0);
+      if (to[1] >= 0) store_pair<kind>(a, to[1] + i16 * 16, v.y * inv1, v.w * inv1);
     };
     auto inverse = [](float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; };
     const bool all_of_it = step0 == 0 && piece_end == x + r.steps;
@@ -933,8 +931,8 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
         else if (member < D / 16) join(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{});
       }
     }
-    team_barrier(team, team_threads);
     x = piece_end;
+    if (x < hi) team_barrier(team, team_threads);   // before the next piece's results
   }
 }
 
