@@ -1,6 +1,7 @@
 // C-ABI of the backend (include/emelb.h): context, residency table, request
 // guards and op dispatch.  No entry point allocates after emelb_create /
 // emelb_residency_upload / emelb_device_alloc.
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -9,6 +10,7 @@
 
 #include "../../include/emelb.h"
 #include "ctx.h"
+#include "paged.h"
 
 using namespace emelb;
 
@@ -371,7 +373,8 @@ uint32_t emelb_create(int device, emelb_ctx** out) {
   ok = ok && cudaMalloc(&c->part_idx, kMaxArgmaxParts * sizeof(int)) == cudaSuccess;
   ok = ok && cudaMalloc(&c->best_val, sizeof(float)) == cudaSuccess;
   ok = ok && cudaMalloc(&c->best_idx, sizeof(int)) == cudaSuccess;
-  ok = ok && cudaMalloc(&c->fa_part_acc, kFlashPartFloats * sizeof(float)) == cudaSuccess;
+  const uint64_t part_floats = std::max(kFlashPartFloats, c->sm_count * kPackedFoldFloats);
+  ok = ok && cudaMalloc(&c->fa_part_acc, part_floats * sizeof(float)) == cudaSuccess;
   ok = ok && cudaMalloc(&c->fa_part_ml, kFlashPartFloats / 32 * sizeof(float)) == cudaSuccess;
   ok = ok && cudaMalloc(&c->fa_scores, kFlashScoreFloats * sizeof(float)) == cudaSuccess;
   if (!ok) {

@@ -9,6 +9,10 @@
 // taken against follows the true one only when that has passed it by 2^8: only then does O, in TMEM, have to be rescaled.  Weights
 // are rounded to the operands' 16 bits, as the tensor cores take them; the sum is of the f32 ones.
 //
+// The tensor cores cut every sum they add to O off, about 2^-22 of it on average: with O in TMEM all the way one row over 2^20 equal
+// keys came out 0.8 % too small, over 2^25 25 %.  So every kFold tiles of keys O moves to scratch, where f32 additions round to nearest,
+// and starts anew, as does the sum; weights are summed by tiles before a tile's sum joins the row's.  Up to 8192 keys nothing moves.
+//
 // A CTA stays and takes pairs of tiles from a common counter (their walks differ by far): a warp finds the next one and asks for its
 // queries as soon as the last scores against the ones before are done, another asks for keys and values ahead across pairs, another
 // looks at values that not every row may see.  Nothing but the rows' own warps waits while they store results.
@@ -50,6 +54,7 @@ constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(8 * kSoftmaxRegs + 4 * kOtherRegs <= 12 * 168, "registers");
 constexpr float kLowest = -3.0e38f;
 constexpr float kSlack = 8.0f;
+constexpr int kFold = 64;             // key tiles between two moves of O out of TMEM: 512 products, 2^-14 of O
 constexpr int kTmemCols = 512;
 
 struct __align__(64) Map {
@@ -66,7 +71,10 @@ struct PackedArgs {
   int64_t items;
   int* next;           // the next item, CTAs that are done: zero between launches
   int *bad, *status;
+  float* fold;         // of a CTA: kTiles x {dims of O, the maximum that they were taken against, the sum} x kTileRows
 };
+constexpr int kFoldDims = 128;
+static_assert((uint64_t)kTiles * (kFoldDims + 2) * kTileRows == kPackedFoldFloats, "scratch of a CTA");
 
 template <int DP>
 struct Smem {
@@ -182,6 +190,47 @@ __device__ __forceinline__ uint32_t fma_zero(uint32_t z, uint32_t w) {
   if (kBf16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0), "r"(z));
   else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0), "r"(z));
   return r;
+}
+
+// A row's O, its maximum and its sum so far to scratch, on top of what is there but for the first time; and back into TMEM, where
+// results are taken from.  Calls: as code of the loop they cost the 13 prompts 54.6 us, as calls 52.5, which take 51.9 without them
+__device__ __forceinline__ float* fold_row(float* fold, int t, int row) {
+  return fold + ((uint64_t)blockIdx.x * kTiles + t) * ((kFoldDims + 2) * kTileRows) + row;
+}
+template <int DP>
+__device__ __noinline__ void fold_away(float* fold, int t, int row, uint32_t o_col, bool first, float m, float2 sums) {
+  fold = fold_row(fold, t, row);
+  float *at_m = fold + kFoldDims * kTileRows, *at_sum = at_m + kTileRows;
+  const float f = first ? 0.0f : exp2_fast(*at_m - m);
+  *at_sum = sums.x + sums.y + (first ? 0.0f : *at_sum * f);
+  *at_m = m;
+#pragma unroll 1
+  for (int c = 0; c < DP; c += 32) {
+    uint32_t o[32];
+    tmem_ld32(o_col + c, o);
+    wait_ld(o);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      float* to = fold + (c + i) * kTileRows;
+      *to = first ? __uint_as_float(o[i]) : fmaf(*to, f, __uint_as_float(o[i]));
+    }
+  }
+}
+template <int DP>
+__device__ __noinline__ float fold_back(float* fold, int t, int row, uint32_t o_col, float m, float sum) {
+  fold = fold_row(fold, t, row);
+  const float f = exp2_fast(fold[kFoldDims * kTileRows] - m);
+#pragma unroll 1
+  for (int c = 0; c < DP; c += 32) {
+    uint32_t o[32];
+    tmem_ld32(o_col + c, o);
+    wait_ld(o);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(fmaf(fold[(c + i) * kTileRows], f, __uint_as_float(o[i])));
+    tc::tmem_st32(o_col + c, o);
+  }
+  tc::tmem_wait_st();
+  return fmaf(fold[(kFoldDims + 1) * kTileRows], f, sum);
 }
 
 template <int DP, bool kBf16>
@@ -509,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc::fence_after();
 #pragma unroll
                 for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                  mma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, values + (kk * 2048 >> 4), idesc_o, kk > 0 ? 1 : j > 0);
+                  mma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, values + (kk * 2048 >> 4), idesc_o, kk > 0 ? 1 : j % kFold != 0);
               }
               p_parity[t] ^= 1;
               if (alive && j + 1 == n_mine) tc::mma_commit(o_ready(t));
@@ -554,6 +603,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!alive) break;
         s_parity ^= 1;
         tc::fence_after();
+        if (j > 0 && j % kFold == 0) {   // the mix so far is done, as below
+          fold_away<DP>(a.fold, t, row, o_col, j == kFold, m, tc::unpack2(sum2));
+          sum2 = tc::pack2(0.0f, 0.0f);
+        }
         uint32_t s[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(s_col + 32 * c, s + 32 * c);
@@ -576,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           m = next;
           sum2 = tc::mul2(sum2, tc::pack2(f, f));
           // the mix so far: its last product was issued before these scores, so it is done
-          if (j > 0) {
+          if (j % kFold != 0) {
 #pragma unroll 1
             for (int c = 0; c < DP; c += 32) {
               uint32_t o[32];
@@ -589,6 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const tc::f2 minus_m = tc::pack2(-m, -m);
+        tc::f2 tile2 = tc::pack2(0.0f, 0.0f);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t p[32];
@@ -596,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 32; ++i) {
             const float2 x = tc::unpack2(tc::fma2(tc::pack2u(s[64 * half + 2 * i], s[64 * half + 2 * i + 1]), scale2, minus_m));
             const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
-            sum2 = tc::add2(sum2, tc::pack2(e0, e1));
+            tile2 = tc::add2(tile2, tc::pack2(e0, e1));
             p[i] = pack16<kBf16>(e0, e1);
           }
           tc::tmem_st32(s_col + 32 * half, p);
@@ -605,6 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(p_ready(t, half));
         }
+        sum2 = tc::add2(sum2, tile2);
       }
       if (alive && n_mine > 0) {
         alive = __all_sync(kAll, tc::mbar_wait(o_ready(t), o_parity, &gave_up));
@@ -613,7 +668,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!alive) break;
       tc::fence_after();
       const float2 two = tc::unpack2(sum2);
-      const float sum = two.x + two.y, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      float sum = two.x + two.y;
+      if (n_mine > kFold) sum = fold_back<DP>(a.fold, t, row, o_col, m, sum);
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       // 64 dims at a time through shared memory, so that a warp stores 128 bytes of a row at once; addresses are made here, not kept
       // in registers from item to item
       int l = lane;
@@ -730,7 +787,7 @@ cudaError_t launch_one(const PackedArgs& a, const Map& q, const Map& k, const Ma
 
 }  // namespace
 
-cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int* next, int sm_count, int* bad, int* status, bool pdl, cudaStream_t st) {
+cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int* next, float* fold, int sm_count, int* bad, int* status, bool pdl, cudaStream_t st) {
   PackedArgs a{};
   a.q = r.q;
   a.out = r.out;
@@ -759,6 +816,7 @@ cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int* next
   a.next = next;
   a.bad = bad;
   a.status = status;
+  a.fold = fold;
   const bool bf16 = r.type == EMELB_BF16;
   Map q, k, v;
   if (!encode_rows(&q, r.q, bf16, r.head_dim, r.heads, r.queries, r.q_token_stride, r.q_head_stride, a.group, a.tile_tokens) ||

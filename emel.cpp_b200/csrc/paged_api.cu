@@ -281,7 +281,7 @@ uint32_t emelb_attend_packed(emelb_ctx* c, const emelb_attend_packed_request* r)
   if (!c || !r) return EMELB_INVALID_REQUEST;
   if (const uint32_t why = emelb_attend_packed_can_run(r)) return refuse(c, why);
   return dispatch(c, {r->q, r->k, r->v, r->out, r->query_begin, r->key_begin}, 1,
-                  [&] { return launch_attend_packed(*r, c->next_sched(), c->sm_count, c->bad_word(), c->status_word(), c->pdl & 1, c->stream); });
+                  [&] { return launch_attend_packed(*r, c->next_sched(), c->fa_part_acc, c->sm_count, c->bad_word(), c->status_word(), c->pdl & 1, c->stream); });
 }
 
 }  // extern "C"
