@@ -13,6 +13,10 @@
 // takes every tile in turn and joins its warps' results in shared memory.  What a unit has of a (request, head) that others
 // share goes to scratch, and the last to arrive joins the parts in the units' order, so results do not depend on timing.
 //
+// The tensor cores cut every sum that they add to off, about 2^-22 of it on average: a warp's results move to shared memory every kFold
+// steps, by f32 additions that round to nearest.  With one sum all the way, equal values over 131,072 tokens came out 4e-4 too small, over
+// 2^20 0.8 %.
+//
 // 64 requests of 1000 to 8000 tokens, 64 heads on 8 of 128: 139 us with steps of 16 tokens, 131 with 32 (one maximum, one exchange
 // for both), 116 with asynchronous copies in place of bulk ones (no barrier to wait at), 94 since a team takes whole pairs where
 // that costs no more, 90 with joins in the order of the fragments, 85 (3.9 TB/s) with a kernel for each type.  What bounds it is issue:
@@ -42,6 +46,7 @@ constexpr int kJoinSteps = 5;         // what joining the parts of units costs, 
 constexpr int kMostParts = 6;             // parts of a (head, row tile) up to which a team may be smaller
 constexpr int kEach = 4;              // requests a lane in the search that a warp makes alone
 constexpr int kStep = 32;             // tokens a warp takes at a time: two tiles
+constexpr int kFold = 64;             // steps of a warp between two moves of its results: 128 products, 2^-16 of them
 
 struct AttendArgs {
   const uint8_t* data;
@@ -67,7 +72,7 @@ struct Shape {
   static constexpr int kStages = D == 128 ? 2 : D == 32 ? 4 : 3;
   static constexpr int kStage = 2 * Tile<D>::kBytes;
   static constexpr int kRing = kStages * kStage;
-  static constexpr int kSmem = kWarps * kRing + kWarps * kRows * D * 4;
+  static constexpr int kSmem = kWarps * kRing + kWarps * kRows * D * 4 + kWarps * 32 * 16;
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -258,6 +263,7 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
   const uint32_t ring_at = tc::smem_u32(ring) + lane * 16;
   float4* joint = reinterpret_cast<float4*>(smem + kWarps * S::kRing);
   constexpr int kCells = kRows * D / 4;
+  float4* folded = joint + kWarps * kCells;   // maximum and sum of a lane's two rows in what has moved
   bool wrong = false;
 
   // ---- the line: its length, and where each team of this CTA starts
@@ -605,212 +611,249 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
     int scale_exp = -11;
     uint32_t scale_cap = 0x14001400u;                             // 2^-10
     float neg_m[2] = {-kLowest, -kLowest};
+    const int piece_stop = max(taken, (piece_end - lo - member + team_warps - 1) / team_warps);
+    bool moved = false;
 
-    for (; taken < mine_steps; ++taken) {
-      const int pos = lo + member + taken * team_warps;
-      if (pos >= piece_end) break;
-      cp_async_wait<kStages - 1>();
-      __syncwarp();
-      const int token0 = (step0 + pos - x) * kStep;
-      const uint32_t tiles = tc::smem_u32(ring) + stage * S::kStage;
-      const uint32_t at_k = tiles + lane * T::kVecK * 4, at_v = tiles + lane * T::kVecV * 4, at_scale = tiles + g * J * 2, at_own = tiles + own_scale,
-                     at_word = tiles + lane_v * 4, at_dv = tiles + t * J * 8;
-      const bool whole = token0 + kStep <= all_see;
+    for (;;) {
+      for (const int stop = min(piece_stop, taken + kFold); taken < stop; ++taken) {
+        const int pos = lo + member + taken * team_warps;
+        cp_async_wait<kStages - 1>();
+        __syncwarp();
+        const int token0 = (step0 + pos - x) * kStep;
+        const uint32_t tiles = tc::smem_u32(ring) + stage * S::kStage;
+        const uint32_t at_k = tiles + lane * T::kVecK * 4, at_v = tiles + lane * T::kVecV * 4, at_scale = tiles + g * J * 2, at_own = tiles + own_scale,
+                       at_word = tiles + lane_v * 4, at_dv = tiles + t * J * 8;
+        const bool whole = token0 + kStep <= all_see;
 
-      // scores: rows are tokens token0 + 16 u + g and + 8, columns the query rows
-      float score[2][4];
-      uint32_t word[2];                   // this lane's share of the values' scales
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int tile = u * T::kBytes;
-        uint32_t one[1];
-        lds(one, at_word + tile + T::kScaleV);
-        word[u] = one[0] & 0x7fff7fffu;
-        uint32_t kw[2][J];
-        float dk[2][J];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int jv = 0; jv < J / T::kVecK; ++jv) {
-            uint32_t w[T::kVecK];
-            lds(w, at_k + tile + (h * (J / T::kVecK) + jv) * 32 * T::kVecK * 4);
-#pragma unroll
-            for (int e = 0; e < T::kVecK; ++e) kw[h][jv * T::kVecK + e] = w[e];
-          }
-          const uint32_t sc = at_scale + tile + T::key_scale(8 * h, 0);
-          if constexpr (J % 2 == 0) {
-            uint32_t w[J / 2];
-            lds(w, sc);
-#pragma unroll
-            for (int e = 0; e < J / 2; ++e) {
-              dk[h][2 * e] = low_of(w[e]);
-              dk[h][2 * e + 1] = high_of(w[e]);
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < J; ++j) dk[h][j] = lds_half(sc + 2 * j);
-          }
-        }
-        // the scales times what the operands are above q - 8, of all groups at once (k is the groups, twice), then group by group
-        const float d0 = lds_half(at_own + tile + T::key_scale(0, 0)), d1 = lds_half(at_own + tile + T::key_scale(8, 0));
-        mma_tf32(score[u], __float_as_uint(d0), __float_as_uint(d1), off[0], off[1]);
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          uint32_t p0[4], p1[4];
-          if constexpr (kExact) {   // 22 bits of a score's sum of 32 are left below 64 + q, 18 below 1024 + q
-            spread_even(kw[0][j], bases.b64, p0);
-            spread_even(kw[1][j], bases.b64, p1);
-          } else {
-            spread(kw[0][j], bases, p0);
-            spread(kw[1][j], bases, p1);
-          }
-          const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
-          float c[4];
-          mma_first(c, a0, qf[0][j][0], qf[0][j][1]);
-          mma(c, a1, qf[0][j][2], qf[0][j][3]);
-          if constexpr (kExact) {
-            mma(c, a0, qf[kParts - 1][j][0], qf[kParts - 1][j][1]);
-            mma(c, a1, qf[kParts - 1][j][2], qf[kParts - 1][j][3]);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) score[u][e] = fmaf(dk[e >> 1][j], c[e], score[u][e]);
-        }
-      }
-      if (!whole) {
-        // behind the request's tokens a page holds anything: no weight, and no say in the exponent
+        // scores: rows are tokens token0 + 16 u + g and + 8, columns the query rows
+        float score[2][4];
+        uint32_t word[2];                   // this lane's share of the values' scales
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const int t0 = token0 + 16 * u;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (t0 + g + (e >> 1) * 8 >= see[e & 1]) score[u][e] = -INFINITY;
-          const int tok = t0 + lane_v / (2 * J) * 2 + (lane_v & 1) * 8;
-          if (tok >= r.length) word[u] = 0;
-          else if (tok + 1 >= r.length) word[u] &= 0xffffu;
-        }
-      }
-      // a half of `word` that reaches scale_cap keeps the bit above it
-      bool moves = ((((word[0] | 0x80008000u) - scale_cap) | ((word[1] | 0x80008000u) - scale_cap)) & 0x80008000u) != 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        moves |= fmaxf(fmaxf(score[0][h], score[0][h + 2]), fmaxf(score[1][h], score[1][h + 2])) > cap[h];
-      if (__any_sync(kAll, moves)) {
-        int big = (int)max(max(word[0] & 0xffffu, word[0] >> 16), max(word[1] & 0xffffu, word[1] >> 16)) >> 10;
-        big = min(4, __reduce_max_sync(kAll, big) - 15);
-        const int e_new = max(scale_exp, big);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float top = fmaxf(fmaxf(score[0][h], score[0][h + 2]), fmaxf(score[1][h], score[1][h + 2])) * unit_score;
-          top = fmaxf(top, __shfl_xor_sync(kAll, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(kAll, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(kAll, top, 16));
-          top = fmaxf(top, m[h]);
-          const float f = exp2_fast((m[h] - top) + (float)(scale_exp - e_new));
-          m[h] = top;
-          cap[h] = (top + kSlack) / unit_score;
-          neg_m[h] = -(top + (float)e_new);
-          l[h] *= f;
-#pragma unroll
-          for (int i16 = 0; i16 < D / 16; ++i16) {
-            o[i16][h] *= f;
-            o[i16][h + 2] *= f;
-          }
-        }
-        scale_exp = e_new;
-        scale_cap = e_new == 4 ? 0x7c007c00u : (uint32_t)(e_new + 16) * 0x04000400u;
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) score[u][e] = exp2_fast(fmaf(score[u][e], unit_score, neg_m[e & 1]));
-        l[0] += score[u][0] + score[u][2];
-        l[1] += score[u][1] + score[u][3];
-      }
-      constexpr int kVV = T::kVecV;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int tile = u * T::kBytes, t0 = token0 + 16 * u;
-        // scales of this lane's four tokens, and the weights as operands
-        uint32_t dv[J][2], pf[2], low[2];
-        if constexpr (J % 2 == 0) {
-#pragma unroll
-          for (int j = 0; j < J; j += 2) {
-            uint32_t w[4];
-            lds(w, at_dv + tile + T::kScaleV + j * 8);
-            dv[j][0] = w[0]; dv[j][1] = w[1]; dv[j + 1][0] = w[2]; dv[j + 1][1] = w[3];
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < J; ++j) lds(dv[j], at_dv + tile + T::kScaleV + j * 8);
-        }
-        if (!whole) {
-#pragma unroll
-          for (int j = 0; j < J; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int tok = t0 + 2 * t + 8 * h;
-              if (tok >= r.length) dv[j][h] = 0;
-              else if (tok + 1 >= r.length) dv[j][h] &= 0xffffu;
-            }
-        }
-        if constexpr (!kExact) {
+          const int tile = u * T::kBytes;
+          uint32_t one[1];
+          lds(one, at_word + tile + T::kScaleV);
+          word[u] = one[0] & 0x7fff7fffu;
+          uint32_t kw[2][J];
+          float dk[2][J];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t two = half2_of(score[u][2 * h], score[u][2 * h + 1]);
-            pf[h] = turn8x8(two);
-            if constexpr (kFine) low[h] = turn8x8(half2_of(score[u][2 * h] - low_of(two), score[u][2 * h + 1] - high_of(two)));
+#pragma unroll
+            for (int jv = 0; jv < J / T::kVecK; ++jv) {
+              uint32_t w[T::kVecK];
+              lds(w, at_k + tile + (h * (J / T::kVecK) + jv) * 32 * T::kVecK * 4);
+#pragma unroll
+              for (int e = 0; e < T::kVecK; ++e) kw[h][jv * T::kVecK + e] = w[e];
+            }
+            const uint32_t sc = at_scale + tile + T::key_scale(8 * h, 0);
+            if constexpr (J % 2 == 0) {
+              uint32_t w[J / 2];
+              lds(w, sc);
+#pragma unroll
+              for (int e = 0; e < J / 2; ++e) {
+                dk[h][2 * e] = low_of(w[e]);
+                dk[h][2 * e + 1] = high_of(w[e]);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < J; ++j) dk[h][j] = lds_half(sc + 2 * j);
+            }
+          }
+          // the scales times what the operands are above q - 8, of all groups at once (k is the groups, twice), then group by group
+          const float d0 = lds_half(at_own + tile + T::key_scale(0, 0)), d1 = lds_half(at_own + tile + T::key_scale(8, 0));
+          mma_tf32(score[u], __float_as_uint(d0), __float_as_uint(d1), off[0], off[1]);
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            uint32_t p0[4], p1[4];
+            if constexpr (kExact) {   // 22 bits of a score's sum of 32 are left below 64 + q, 18 below 1024 + q
+              spread_even(kw[0][j], bases.b64, p0);
+              spread_even(kw[1][j], bases.b64, p1);
+            } else {
+              spread(kw[0][j], bases, p0);
+              spread(kw[1][j], bases, p1);
+            }
+            const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
+            float c[4];
+            mma_first(c, a0, qf[0][j][0], qf[0][j][1]);
+            mma(c, a1, qf[0][j][2], qf[0][j][3]);
+            if constexpr (kExact) {
+              mma(c, a0, qf[kParts - 1][j][0], qf[kParts - 1][j][1]);
+              mma(c, a1, qf[kParts - 1][j][2], qf[kParts - 1][j][3]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) score[u][e] = fmaf(dk[e >> 1][j], c[e], score[u][e]);
           }
         }
-        uint32_t vw[kVV];
+        if (!whole) {
+          // behind the request's tokens a page holds anything: no weight, and no say in the exponent
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          uint32_t bf[kParts][2];
+          for (int u = 0; u < 2; ++u) {
+            const int t0 = token0 + 16 * u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (t0 + g + (e >> 1) * 8 >= see[e & 1]) score[u][e] = -INFINITY;
+            const int tok = t0 + lane_v / (2 * J) * 2 + (lane_v & 1) * 8;
+            if (tok >= r.length) word[u] = 0;
+            else if (tok + 1 >= r.length) word[u] &= 0xffffu;
+          }
+        }
+        // a half of `word` that reaches scale_cap keeps the bit above it
+        bool moves = ((((word[0] | 0x80008000u) - scale_cap) | ((word[1] | 0x80008000u) - scale_cap)) & 0x80008000u) != 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          moves |= fmaxf(fmaxf(score[0][h], score[0][h + 2]), fmaxf(score[1][h], score[1][h + 2])) > cap[h];
+        if (__any_sync(kAll, moves)) {
+          int big = (int)max(max(word[0] & 0xffffu, word[0] >> 16), max(word[1] & 0xffffu, word[1] >> 16)) >> 10;
+          big = min(4, __reduce_max_sync(kAll, big) - 15);
+          const int e_new = max(scale_exp, big);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float top = fmaxf(fmaxf(score[0][h], score[0][h + 2]), fmaxf(score[1][h], score[1][h + 2])) * unit_score;
+            top = fmaxf(top, __shfl_xor_sync(kAll, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(kAll, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(kAll, top, 16));
+            top = fmaxf(top, m[h]);
+            const float f = exp2_fast((m[h] - top) + (float)(scale_exp - e_new));
+            m[h] = top;
+            cap[h] = (top + kSlack) / unit_score;
+            neg_m[h] = -(top + (float)e_new);
+            l[h] *= f;
+#pragma unroll
+            for (int i16 = 0; i16 < D / 16; ++i16) {
+              o[i16][h] *= f;
+              o[i16][h + 2] *= f;
+            }
+          }
+          scale_exp = e_new;
+          scale_cap = e_new == 4 ? 0x7c007c00u : (uint32_t)(e_new + 16) * 0x04000400u;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) score[u][e] = exp2_fast(fmaf(score[u][e], unit_score, neg_m[e & 1]));
+          l[0] += score[u][0] + score[u][2];
+          l[1] += score[u][1] + score[u][3];
+        }
+        constexpr int kVV = T::kVecV;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int tile = u * T::kBytes, t0 = token0 + 16 * u;
+          // scales of this lane's four tokens, and the weights as operands
+          uint32_t dv[J][2], pf[2], low[2];
+          if constexpr (J % 2 == 0) {
+#pragma unroll
+            for (int j = 0; j < J; j += 2) {
+              uint32_t w[4];
+              lds(w, at_dv + tile + T::kScaleV + j * 8);
+              dv[j][0] = w[0]; dv[j][1] = w[1]; dv[j + 1][0] = w[2]; dv[j + 1][1] = w[3];
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < J; ++j) lds(dv[j], at_dv + tile + T::kScaleV + j * 8);
+          }
+          if (!whole) {
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int tok = t0 + 2 * t + 8 * h;
+                if (tok >= r.length) dv[j][h] = 0;
+                else if (tok + 1 >= r.length) dv[j][h] &= 0xffffu;
+              }
+          }
           if constexpr (!kExact) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const __half2 d = tc::bits_h2(dv[j][h]);
-              const __half2 p = kFine ? __hfma2(tc::bits_h2(pf[h]), d, __hmul2(tc::bits_h2(low[h]), d)) : __hmul2(tc::bits_h2(pf[h]), d);
-              bf[0][h] = tc::h2_bits(p);
-            }
-          } else {
-            // in f32, tokens g and g + 8 a lane, then as two f16
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float d = lds_half(tiles + tile + T::kScaleV + ((g >> 1) * J + j) * 8 + (g & 1) * 2 + 4 * h);
-              if (t0 + g + 8 * h >= r.length) d = 0.0f;
-              const float p0 = score[u][2 * h] * d, p1 = score[u][2 * h + 1] * d;
-              const uint32_t hi2 = half2_of(p0, p1);
-              bf[0][h] = turn8x8(hi2);
-              bf[kParts - 1][h] = turn8x8(half2_of(p0 - low_of(hi2), p1 - high_of(hi2)));
+              const uint32_t two = half2_of(score[u][2 * h], score[u][2 * h + 1]);
+              pf[h] = turn8x8(two);
+              if constexpr (kFine) low[h] = turn8x8(half2_of(score[u][2 * h] - low_of(two), score[u][2 * h + 1] - high_of(two)));
             }
           }
+          uint32_t vw[kVV];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int i16 = 2 * j + half;
-            if (i16 % kVV == 0) lds(vw, at_v + tile + T::kV + i16 / kVV * 32 * kVV * 4);
-            uint32_t av[4];
-            spread(vw[i16 % kVV], bases, av);
-            // centred before the product, exactly: a sum over the tokens would not survive the difference
+          for (int j = 0; j < J; ++j) {
+            uint32_t bf[kParts][2];
+            if constexpr (!kExact) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) av[e] = tc::h2_bits(__hadd2(tc::bits_h2(av[e]), tc::bits_h2(above[e])));
+              for (int h = 0; h < 2; ++h) {
+                const __half2 d = tc::bits_h2(dv[j][h]);
+                const __half2 p = kFine ? __hfma2(tc::bits_h2(pf[h]), d, __hmul2(tc::bits_h2(low[h]), d)) : __hmul2(tc::bits_h2(pf[h]), d);
+                bf[0][h] = tc::h2_bits(p);
+              }
+            } else {
+              // in f32, tokens g and g + 8 a lane, then as two f16
 #pragma unroll
-            for (int part = 0; part < kParts; ++part) mma(o[i16], av, bf[part][0], bf[part][1]);
+              for (int h = 0; h < 2; ++h) {
+                float d = lds_half(tiles + tile + T::kScaleV + ((g >> 1) * J + j) * 8 + (g & 1) * 2 + 4 * h);
+                if (t0 + g + 8 * h >= r.length) d = 0.0f;
+                const float p0 = score[u][2 * h] * d, p1 = score[u][2 * h + 1] * d;
+                const uint32_t hi2 = half2_of(p0, p1);
+                bf[0][h] = turn8x8(hi2);
+                bf[kParts - 1][h] = turn8x8(half2_of(p0 - low_of(hi2), p1 - high_of(hi2)));
+              }
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int i16 = 2 * j + half;
+              if (i16 % kVV == 0) lds(vw, at_v + tile + T::kV + i16 / kVV * 32 * kVV * 4);
+              uint32_t av[4];
+              spread(vw[i16 % kVV], bases, av);
+              // centred before the product, exactly: a sum over the tokens would not survive the difference
+#pragma unroll
+              for (int e = 0; e < 4; ++e) av[e] = tc::h2_bits(__hadd2(tc::bits_h2(av[e]), tc::bits_h2(above[e])));
+#pragma unroll
+              for (int part = 0; part < kParts; ++part) mma(o[i16], av, bf[part][0], bf[part][1]);
+            }
           }
         }
+        __syncwarp();
+        issue(taken + kStages, stage);
+        stage = stage + 1 == kStages ? 0 : stage + 1;
       }
-      __syncwarp();
-      issue(taken + kStages, stage);
-      stage = stage + 1 == kStages ? 0 : stage + 1;
+      if (taken == piece_stop) break;
+      // to where the team's results meet in the end, which is free until then
+      const float4 old = folded[tid];
+      const float m0 = m[0] + (float)scale_exp, m1 = m[1] + (float)scale_exp;
+      const float f0 = moved ? exp2_fast(old.x - m0) : 0.0f, f1 = moved ? exp2_fast(old.z - m1) : 0.0f;
+      folded[tid] = make_float4(m0, moved ? fmaf(old.y, f0, l[0]) : l[0], m1, moved ? fmaf(old.w, f1, l[1]) : l[1]);
+      l[0] = l[1] = 0.0f;
+#pragma unroll
+      for (int i16 = 0; i16 < D / 16; ++i16) {
+        float4& cell = joint[warp * kCells + i16 * 32 + lane];
+        float4 now = make_float4(o[i16][0], o[i16][1], o[i16][2], o[i16][3]);
+        if (moved) {
+          const float4 was = cell;
+          now = make_float4(fmaf(was.x, f0, now.x), fmaf(was.y, f1, now.y), fmaf(was.z, f0, now.z), fmaf(was.w, f1, now.w));
+        }
+        cell = now;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i16][e] = 0.0f;
+      }
+      moved = true;
     }
 
     // ---- the piece's results.  A cell is what a lane holds of 16 dims: rows 2t and 2t + 1, dims 16 i + 2g and the next.  Cells stay in
     // this order all the way: through shared memory, through scratch, until the last sum is made
+    m[0] += (float)scale_exp;
+    m[1] += (float)scale_exp;
+    if (moved) {
+      const float4 old = folded[tid];
+      const float f0 = exp2_fast(old.x - m[0]), f1 = exp2_fast(old.z - m[1]);
+      l[0] = fmaf(old.y, f0, l[0]);
+      l[1] = fmaf(old.w, f1, l[1]);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      m[h] += (float)scale_exp;
+      for (int i16 = 0; i16 < D / 16; ++i16) {
+        const float4 was = joint[warp * kCells + i16 * 32 + lane];
+        o[i16][0] = fmaf(was.x, f0, o[i16][0]);
+        o[i16][1] = fmaf(was.y, f1, o[i16][1]);
+        o[i16][2] = fmaf(was.z, f0, o[i16][2]);
+        o[i16][3] = fmaf(was.w, f1, o[i16][3]);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int s = 4; s < 32; s <<= 1) l[h] += __shfl_xor_sync(kAll, l[h], s);
-    }
     const int w0 = team * team_warps, ttid = tid - w0 * 32;
     if (team_warps > 1) {
       if (g == 0) *reinterpret_cast<float2*>(&join_m[warp][2 * t]) = make_float2(m[0], m[1]);

@@ -7,7 +7,7 @@ import torch
 import emel_cpp_b200 as eb
 from emel_cpp_b200 import paged
 from tests import paged_plain as plain
-from tests.test_gpu_paged import Cache, dev, done, filled, gen
+from tests.test_gpu_paged import Cache, dev, done, filled, gen, slots_of, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,86 @@ def test_packed_planted_keys(be, keys, dim):
     torch.cuda.synchronize()
     done(be, be.attend_packed(paged.packed_request(q, k, v, out, "bf16", *begin, 1, 1, 1, dim, len(at), keys, causal=False)))
     assert torch.equal(out, v[at])
+
+
+# ---------------------------------------------------------------- attention over the pages
+def repeated(be, page_rows, page_tokens=256):
+    """A cache of one page that holds these rows: tables name it as often as they like.  (cache, kept keys, kept values)"""
+    k, v = page_rows
+    c = Cache(1, page_tokens, k.shape[1], k.shape[2])
+    slots = torch.arange(page_tokens, device="cuda")
+    torch.cuda.synchronize()
+    done(be, be.kv_store(paged.store_request(c.pages, k, v, "f32", slots, page_tokens)))
+    return c, plain.kept(k), plain.kept(v)
+
+
+@pytest.mark.parametrize("length,requests,dim,t", [(1 << 17, 1780, 32, "f32"), (1 << 20, 1780, 32, "f16"), (1 << 20, 1200, 64, "f32"), (1 << 18, 1790, 128, "bf16")])
+def test_attend_equal_values_of_many_tokens(be, length, requests, dim, t):
+    """So many requests that a warp walks a whole one, over tokens that are all alike: every rounding goes the same way.  The tensor
+    cores cut a sum's 17 addends (16 products, the result) off at a unit of 2^-23 of the result or less, which grows over 128 such
+    products; a weight has a rounding to f16 (bf16 results: two; f32: one of 22 bits), the result its own, the sums f32 ones: of 128
+    weights, 8 lanes, the moves."""
+    k, v = torch.zeros(256, 1, dim, device="cuda"), torch.linspace(-3, 2, dim, device="cuda").repeat(256, 1, 1)
+    c, _, kept = repeated(be, (k, v))
+    table, lengths = torch.zeros(requests, length // 256, dtype=torch.int32, device="cuda"), dev([length] * requests)
+    q = torch.ones(requests, 8, dim, device="cuda").to(plain.TORCH[t])
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    done(be, be.kv_attend(paged.attend_request(c.pages, q, out, t, table, length // 256, lengths, requests, 8, requests)))
+    want = kept[0]
+    rounding = {"f32": 2.0 ** -22, "f16": 2.0 ** -11, "bf16": 2.0 ** -10}[t] + plain.HALF_STEP[t]
+    rel = rounding + 64 * 17 * 2.0 ** -23 + (128 + 8 + length / 2048) * 2.0 ** -24 + 2.0 ** -21
+    assert ((out.double() - want).abs() <= rel * want.abs() + 1e-30).all(), float(((out.double() - want).abs() / want.abs().clamp_min(1e-9)).max())
+
+
+def weight_step(t, q, k, scale):
+    """What a weight is off by, roundings and (as a fraction of it) scores: a head's scores are sums over groups of 32 of products of
+    (base + q) and a query value, each of four (f32 queries: eight) instructions cutting off about 2^-22 of what stands there."""
+    base = 64.0 if t == "f32" else 1024.0
+    score = (8 if t == "f32" else 4) * 2.0 ** -22 * base * 32 ** 0.5 * rms(q) * rms(k) / 4 * scale * (q.shape[2] / 32) ** 0.5
+    return {"f32": 2.0 ** -22, "f16": 2.0 ** -11, "bf16": 2.0 ** -10}[t], score
+
+
+@pytest.mark.parametrize("lengths,rows,heads,kv,dim,t", [
+    ([20001], [1], 32, 8, 128, "f16"), ([70000], [3], 8, 1, 64, "bf16"), ([30000, 3, 500, 9000], [1, 3, 2, 4], 16, 4, 128, "bf16"),
+    ([12000, 12000], [3, 1], 4, 2, 96, "f16"), ([9000], [5], 8, 1, 128, "f32"), ([40000, 100], [2, 2], 16, 2, 32, "f32"), ([2500] * 40, [1] * 40, 64, 8, 128, "f16"),
+    ([1000 + 37 * i for i in range(150)], [1] * 150, 8, 1, 64, "bf16"), ([5000 + i for i in range(130)], [1 + i % 3 for i in range(130)], 16, 2, 96, "f32"),
+])
+def test_attend_far_errors(be, lengths, rows, heads, kv, dim, t):
+    rng, g = np.random.default_rng(len(lengths)), gen(len(lengths) + dim)
+    c, table, k, v = filled(be, rng, g, lengths, 32, kv, dim)
+    q = torch.randn(sum(rows), heads, dim, generator=g, device="cuda").to(plain.TORCH[t])
+    out, begin, lens = torch.full_like(q, 7.0), dev(np.concatenate([[0], np.cumsum(rows)]).tolist()), dev(lengths)
+    torch.cuda.synchronize()
+    done(be, be.kv_attend(paged.attend_request(c.pages, q, out, t, table, table.shape[1], lens, len(lengths), heads, q.shape[0], query_begin=begin,
+                                               max_queries=max(rows))))
+    at, qa = 0, 0
+    for length, n in zip(lengths, rows):
+        kk, vv, qq = k[at:at + length], v[at:at + length], q[qa:qa + n]
+        want, root = exact(qq, kk, vv, dim ** -0.5)
+        check_rms(out[qa:qa + n], want, root, *weight_step(t, qq, kk, dim ** -0.5)[:1], t, weight_step(t, qq, kk, dim ** -0.5)[1])
+        at, qa = at + length, qa + n
+
+
+@pytest.mark.parametrize("length,rows,group,dim,page,t", [(20000, 200, 1, 64, 16, "f16"), (70001, 100, 8, 32, 256, "bf16"), (3001, 64, 2, 128, 32, "f32"), (9000, 300, 3, 96, 64, "f16")])
+def test_attend_planted_keys(be, length, rows, group, dim, page, t):
+    """One key takes all of a row's weight: at both sides of every kind of border (steps of 32, batches of 32 steps, moves of 64, pages,
+    the ends), and anywhere, so that the borders of shares are among them."""
+    rng, g = np.random.default_rng(length), gen(length)
+    table, pages = tables(rng, [length], page)
+    c = Cache(pages, page, 1, dim, fill=0xff)
+    k = torch.randn(length, 1, dim, generator=g, device="cuda").sign()
+    v = torch.randn(length, 1, dim, generator=g, device="cuda")
+    slots, table = dev(slots_of(table, [0], [length], page).tolist(), torch.int64), torch.from_numpy(table).cuda()
+    torch.cuda.synchronize()
+    done(be, be.kv_store(paged.store_request(c.pages, k, v, "f32", slots, length)))
+    seen = length - rows
+    at = [p for b in (0, 16, 32, 256, 1024, 2048, 4096, seen) for p in (b - 1, b) if 0 <= p < seen]
+    at = np.array((at + rng.integers(0, seen, rows * group).tolist())[:rows * group])
+    q = (4 * k[at, 0]).view(rows, group, dim).to(plain.TORCH[t])     # two signs apart is 15 nats
+    want = plain.kept(v)[at, 0].view(rows, group, dim).double()
+    out, begin, lens = torch.zeros_like(q), dev([0, rows]), dev([length])
+    torch.cuda.synchronize()
+    done(be, be.kv_attend(paged.attend_request(c.pages, q, out, t, table, table.shape[1], lens, 1, group, rows, query_begin=begin, max_queries=rows, scale=1.0)))
+    rounding = {"f32": 2.0 ** -21, "f16": 2.0 ** -11, "bf16": 2.0 ** -10}[t] + plain.HALF_STEP[t]
+    assert ((out.double() - want).abs() <= rounding * want.abs() + 1e-5).all()
