@@ -26,6 +26,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "kernels.h"
@@ -41,7 +42,6 @@ typedef long long i64;
 constexpr unsigned kAll = 0xffffffffu;
 constexpr float kLowest = -3.0e38f;   // running maximum before the first token: finite, below every score
 constexpr float kSlack = 3.0f;        // a score may pass the running maximum by this (log2) before sums are rescaled
-constexpr int kMinShare = 1;          // steps a warp, below which fewer units share the work
 constexpr int kJoinSteps = 5;         // what joining the parts of units costs, in steps of a warp
 constexpr int kMostParts = 6;             // parts of a (head, row tile) up to which a team may be smaller
 constexpr int kEach = 4;              // requests a lane in the search that a warp makes alone
@@ -209,6 +209,18 @@ __device__ __forceinline__ void copy_stage(uint32_t to, const uint8_t* from0, ui
   }
 }
 
+// Places on the line are ints where the request's sizes leave it shorter than 2^30 steps (with 64 bits everywhere one document of
+// 100,001 tokens took 71.3 us for 67.1, calls of few tokens 0.6 to 1 us more).  Sums over the requests that are more than the most are
+// taken for values out of range.  2^40 steps are a quarter of an hour; a unit's share of them still counts in 31 bits, since there are
+// 148 units at least, with 2^26 steps a pair.
+template <class Line>
+constexpr i64 kMostSteps = sizeof(Line) == 4 ? 0x3fffffff : (i64)1 << 40;
+constexpr int kMostPairs = 1 << 30;
+constexpr int kMostTokens = 0x7fffffc0;   // of a request: places up to the end of its last step are ints
+// a / b, mostly of small numbers; a >= 0
+__device__ __forceinline__ int quot(int a, int b) { return a / b; }
+__device__ __forceinline__ i64 quot(i64 a, int b) { return (uint64_t)a >> 32 ? a / b : (i64)((uint32_t)a / (uint32_t)b); }
+
 // one request's part of the line
 struct Request {
   int rows;     // query rows
@@ -224,7 +236,7 @@ __device__ __forceinline__ Request request_at(const AttendArgs& a, int b, bool* 
   r.rows = a.query_begin ? a.query_begin[b + 1] - r.first : 1;
   r.length = a.lengths[b];
   const bool ok = r.rows >= 0 && r.rows <= a.max_queries && r.first >= 0 && r.first <= a.queries - r.rows && r.length >= 0 &&
-                  r.length <= (i64)a.table_width * a.page_tokens;
+                  r.length <= kMostTokens && r.length <= (i64)a.table_width * a.page_tokens;
   if (!ok) {
     *wrong = true;
     r.rows = 0;
@@ -243,7 +255,7 @@ __device__ __forceinline__ void team_barrier(int team, int threads) {
 // kF32: the queries and the weights go in as two f16 operands each.  kF16: a weight's low part goes into its product with the scale,
 // so that there is one rounding to f16 and not two (one document of 100,001 tokens: 3 us of 70, its error against exact results 1.3
 // and not 1.6 times what the results' own rounding makes)
-template <int D, Kind kind>
+template <int D, Kind kind, class Line>
 __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kernel(const __grid_constant__ AttendArgs a) {
   pdl_trigger();
   pdl_wait();
@@ -254,8 +266,18 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
   constexpr int J = T::kGroups, kRows = S::kRows, kStages = S::kStages, kParts = kExact ? 2 : 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ i64 sums[3][kWarps];
-  __shared__ int2 scan[kWarps];
-  __shared__ int4 starts[kWarps];   // a team's request, where that begins, the team's steps
+  constexpr bool kFar = sizeof(Line) == 8;
+  struct Sum {
+    Line steps;
+    int pairs;
+  };
+  struct Start {
+    Line begin, from, to;   // where the request begins, the team's steps
+    int b;
+  };
+  auto line_of = [](const Request& r) { return (Line)r.sides * r.steps; };
+  __shared__ Sum scan[kWarps];
+  __shared__ Start starts[kWarps];
   __shared__ __align__(16) float join_m[kWarps][kRows], join_l[kWarps][kRows];
   __shared__ int last_in[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -273,11 +295,11 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
   // From the sums over the requests (all: steps; sides: (head, row tile) pairs; most: steps of the longest): if a team each can
   // take the pairs whole in about the time that even shares and joining the units' parts (worth about kJoinSteps steps) take,
   // they do; else teams are as small as kMostParts parts a pair allow, since a team waits for its slowest warp at every pair.
-  auto plan = [&](i64 all, int sides, int most) {
-    const int warps = grid * kWarps, line = (int)all;
+  auto plan = [&](Line all, int sides, int most) {
+    const int warps = grid * kWarps;
     split = true;
     for (team_warps = kWarps; team_warps >= 1; --team_warps)
-      if (kWarps % team_warps == 0 && (i64)sides * team_warps <= warps && (most + team_warps - 1) / team_warps <= line / warps + kJoinSteps) {
+      if (kWarps % team_warps == 0 && (i64)sides * team_warps <= warps && (most + team_warps - 1) / team_warps <= quot(all, warps) + kJoinSteps) {
         split = false;
         break;
       }
@@ -287,17 +309,17 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
     }
     team_warps = 1;
     while (team_warps < kWarps && (kWarps % team_warps != 0 || (i64)sides * team_warps * kMostParts < warps)) ++team_warps;
-    units = min(min(warps / team_warps, a.most_units), (line + kMinShare * team_warps - 1) / (kMinShare * team_warps));
-    share = line / units;
-    more = line - share * units;   // the first `more` units take one step more
+    units = (int)min((Line)min(warps / team_warps, a.most_units), quot(all + team_warps - 1, team_warps));
+    share = (int)quot(all, units);
+    more = (int)(all - (Line)share * units);   // the first `more` units take one step more
   };
-  auto start_of = [&](int u) { return u * share + min(u, more); };
-  auto unit_of = [&](int x) {
-    const int edge = more * (share + 1);
-    return x < edge ? x / (share + 1) : more + (x - edge) / share;
+  auto start_of = [&](int u) { return (Line)u * share + min(u, more); };
+  auto unit_of = [&](Line x) {
+    const Line edge = (Line)more * (share + 1);
+    return x < edge ? (int)quot(x, share + 1) : more + (int)quot(x - edge, share);
   };
-  constexpr i64 kMostSteps = 0x3fffffff;   // over a terabyte of cache
-  int team, member, unit, b_start, b_begin, lo, hi;
+  int team, member, unit, b_start;
+  Line b_begin, lo, hi;
   if (a.requests <= 32 * kEach) {
     // every warp for itself, a few requests a lane
     Request each[kEach];
@@ -313,6 +335,7 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
     for (int i = 0; i < kEach; ++i) {
       steps += (i64)each[i].sides * each[i].steps;
       pairs += each[i].sides;
+      if (kFar) pairs = min(pairs, kMostPairs);
       if (each[i].sides) most = max(most, each[i].steps);
     }
     const int my_pairs = pairs;
@@ -323,25 +346,27 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
       const int p = __shfl_up_sync(kAll, pairs, o);
       if (lane >= o) {
         steps += s;
-        pairs += p;
+        pairs = kFar ? (int)min((unsigned)pairs + (unsigned)p, (unsigned)kMostPairs) : pairs + p;
       }
     }
     most = __reduce_max_sync(kAll, most);
     const i64 all = __shfl_sync(kAll, steps, 31);
-    wrong |= all > kMostSteps;
-    if (wrong) *a.bad = 1;
-    if (all == 0 || all > kMostSteps) return;
-    plan(all, __shfl_sync(kAll, pairs, 31), most);
+    const int sides = __shfl_sync(kAll, pairs, 31);
+    const bool much = all > kMostSteps<Line> || (kFar && sides >= kMostPairs);
+    if (wrong || much) *a.bad = 1;
+    if (all == 0 || much) return;
+    plan((Line)all, sides, most);
     team = warp / team_warps;
     unit = team * grid + blockIdx.x;
     if (unit >= units) return;
-    const int from = split ? start_of(unit) : unit;
-    const int owner = __ffs(__ballot_sync(kAll, (split ? (int)steps : pairs) > from)) - 1;
+    const Line from = split ? start_of(unit) : unit;
+    const int owner = __ffs(__ballot_sync(kAll, (split ? (Line)steps : pairs) > from)) - 1;
     // in the owner's few
-    int at = (int)(steps - my_steps), first_pair = pairs - my_pairs, long_pair = 0, i = 0;
+    Line at = (Line)(steps - my_steps);
+    int first_pair = pairs - my_pairs, long_pair = 0, i = 0;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-      const int n = each[k].sides * each[k].steps;
+      const Line n = line_of(each[k]);
       if (i == k) {
         if (split ? at + n <= from : first_pair + each[k].sides <= from) {
           at += n;
@@ -356,11 +381,11 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
     b_begin = __shfl_sync(kAll, at, owner);
     first_pair = __shfl_sync(kAll, first_pair, owner);
     long_pair = __shfl_sync(kAll, long_pair, owner);
-    lo = split ? from : b_begin + (unit - first_pair) * long_pair;
+    lo = split ? from : b_begin + (Line)(unit - first_pair) * long_pair;
     hi = split ? start_of(unit + 1) : lo + long_pair;
   } else {
-    i64 all = 0;
-    int sides = 0, most = 0;
+    i64 all = 0, sides = 0;
+    int most = 0;
     for (int b = tid; b < a.requests; b += kThreads) {
       const Request r = request_at<kRows>(a, b, &wrong);
       all += (i64)r.sides * r.steps;
@@ -379,57 +404,61 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
       sums[2][warp] = most;
     }
     __syncthreads();
-    all = 0;
-    sides = most = 0;
+    all = sides = 0;
+    most = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       all += sums[0][w];
-      sides += (int)sums[1][w];
+      sides += sums[1][w];
       most = max(most, (int)sums[2][w]);
     }
-    wrong |= all > kMostSteps;
-    if (wrong) *a.bad = 1;
-    if (all == 0 || all > kMostSteps) return;
-    plan(all, sides, most);
+    const bool much = all > kMostSteps<Line> || sides >= kMostPairs;
+    if (wrong || much) *a.bad = 1;
+    if (all == 0 || much) return;
+    plan((Line)all, (int)sides, most);
     const int teams = kWarps / team_warps;
-    int carry_s = 0, carry_p = 0;
+    Line carry_s = 0;
+    int carry_p = 0;
     for (int b0 = 0; b0 < a.requests; b0 += kThreads) {
       const int b = b0 + tid;
       bool skip = false;
       Request r{};
       if (b < a.requests) r = request_at<kRows>(a, b, &skip);
-      const int v = r.sides * r.steps;
-      int steps = v, pairs = r.sides;
+      const Line v = line_of(r);
+      Line steps = v;
+      int pairs = r.sides;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int s = __shfl_up_sync(kAll, steps, o), p = __shfl_up_sync(kAll, pairs, o);
+        const Line s = __shfl_up_sync(kAll, steps, o);
+        const int p = __shfl_up_sync(kAll, pairs, o);
         if (lane >= o) {
           steps += s;
           pairs += p;
         }
       }
       if (b0) __syncthreads();
-      if (lane == 31) scan[warp] = make_int2(steps, pairs);
+      if (lane == 31) scan[warp] = Sum{steps, pairs};
       __syncthreads();
-      int before_s = carry_s, before_p = carry_p;
+      Line before_s = carry_s;
+      int before_p = carry_p;
       for (int w = 0; w < kWarps; ++w) {
-        const int2 c = scan[w];
+        const Sum c = scan[w];
         if (w < warp) {
-          before_s += c.x;
-          before_p += c.y;
+          before_s += c.steps;
+          before_p += c.pairs;
         }
-        carry_s += c.x;
-        carry_p += c.y;
+        carry_s += c.steps;
+        carry_p += c.pairs;
       }
       steps += before_s;
       pairs += before_p;
       for (int k = 0; k < teams; ++k) {
         const int u = k * grid + blockIdx.x;
         if (u >= units) break;
-        const int x = split ? start_of(u) : u;
+        const Line x = split ? start_of(u) : u;
         if (split ? x >= steps - v && x < steps : x >= pairs - r.sides && x < pairs) {
-          const int from = split ? x : steps - v + (x - (pairs - r.sides)) * r.steps;
-          starts[k] = make_int4(b, steps - v, from, split ? start_of(u + 1) : from + r.steps);
+          const Line from = split ? x : steps - v + (x - (pairs - r.sides)) * r.steps;
+          starts[k] = Start{steps - v, from, split ? start_of(u + 1) : from + r.steps, b};
         }
       }
     }
@@ -437,35 +466,37 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
     team = warp / team_warps;
     unit = team * grid + blockIdx.x;
     if (unit >= units) return;
-    const int4 s = starts[team];
-    b_start = s.x;
-    b_begin = s.y;
-    lo = s.z;
-    hi = s.w;
+    const Start& s = starts[team];
+    b_start = s.b;
+    b_begin = s.begin;
+    lo = s.from;
+    hi = s.to;
   }
   member = warp % team_warps;
-  const int team_threads = 32 * team_warps;
-  const int mine_steps = (hi - lo - member + team_warps - 1) / team_warps;   // this warp's: lo + member + k * team_warps
+  const int team_threads = 32 * team_warps, span = (int)(hi - lo);   // places in the share count from lo
+  const int mine_steps = (span - member + team_warps - 1) / team_warps;   // this warp's: lo + member + k * team_warps
 
   // ---- copies: lane l of a batch of 32 finds the l-th step of the warp from there, one batch ahead, so that nobody waits for
   // the table
   const int page_tiles = a.page_tokens >> 4;
-  int walk_b = b_start, walk_at = b_begin;    // a request at or before the batch's first step, where it begins
+  int walk_b = b_start;
+  Line walk_at = b_begin;                     // a request at or before the batch's first step, where it begins
   uint32_t ahead[2] = {0, 0}, now[2] = {0, 0};   // tiles of this lane's step, counted through the cache, twice and 1; 0: none
   auto find_batch = [&](int k0) {
-    const int x = lo + member + (k0 + lane) * team_warps;
+    const Line x = lo + member + (k0 + lane) * team_warps;
     const bool mine_too = k0 + lane < mine_steps;
     ahead[0] = ahead[1] = 0;
     if (mine_too) {
       bool skip = false;
-      int b = walk_b, begin = walk_at;
+      int b = walk_b;
+      Line begin = walk_at;
       Request r = request_at<kRows>(a, b, &skip);
-      while (x >= begin + r.sides * r.steps) {
-        begin += r.sides * r.steps;
+      while (x >= begin + line_of(r)) {
+        begin += line_of(r);
         ++b;
         r = request_at<kRows>(a, b, &skip);
       }
-      const int at = x - begin, side = at / r.steps, step = at - side * r.steps, head = side / (r.sides / a.kv_heads);
+      const int side = (int)quot(x - begin, r.steps), step = (int)(x - begin - (Line)side * r.steps), head = side / (r.sides / a.kv_heads);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int tile = 2 * step + h;
@@ -507,20 +538,21 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
   constexpr uint32_t above[4] = {0xe408e408u, 0xd480d480u, 0xdc20dc20u, 0xce00ce00u};   // -1032, -72, -264, -24
 
   // ---- (request, head, row tile) after (request, head, row tile)
-  int b = b_start, begin = b_begin;
+  int b = b_start;
+  Line begin = b_begin;
   bool skip = false;
   Request r = request_at<kRows>(a, b, &skip);
-  int x = lo;
-  while (x < hi) {
-    while (x >= begin + r.sides * r.steps) {
-      begin += r.sides * r.steps;
+  int x = 0;
+  while (x < span) {
+    while (lo + x >= begin + line_of(r)) {
+      begin += line_of(r);
       ++b;
       r = request_at<kRows>(a, b, &skip);
     }
-    const int at = x - begin, side = at / r.steps, step0 = at - side * r.steps;
+    const int side = (int)quot(lo + x - begin, r.steps), step0 = (int)(lo + x - begin - (Line)side * r.steps);
     const int row_tiles = r.sides / a.kv_heads, head = side / row_tiles, row0 = (side - head * row_tiles) * kRows;
     const int all_rows = r.rows * a.group;
-    const int piece_end = min(hi, x - step0 + r.steps);
+    const int piece_end = min(span, x - step0 + r.steps);
 
     // queries: this lane's row g of each tile of 8, dims 8t .. 8t+7 of each group
     uint32_t qf[kParts][J][4];
@@ -537,7 +569,7 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
 #pragma unroll
       for (int j = 0; j < J; ++j) raw[j] = live ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + from + 32 * j + 8 * t) : make_uint4(0, 0, 0, 0);
     }
-    if (x == lo) {   // the first tiles, while the first queries are on their way
+    if (x == 0) {   // the first tiles, while the first queries are on their way
       find_batch(0);
       for (int k = 0; k < kStages; ++k) issue(k, k);
     }
@@ -611,12 +643,12 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
     int scale_exp = -11;
     uint32_t scale_cap = 0x14001400u;                             // 2^-10
     float neg_m[2] = {-kLowest, -kLowest};
-    const int piece_stop = max(taken, (piece_end - lo - member + team_warps - 1) / team_warps);
+    const int piece_stop = max(taken, (piece_end - member + team_warps - 1) / team_warps);
     bool moved = false;
 
     for (;;) {
       for (const int stop = min(piece_stop, taken + kFold); taken < stop; ++taken) {
-        const int pos = lo + member + taken * team_warps;
+        const int pos = member + taken * team_warps;
         cp_async_wait<kStages - 1>();
         __syncwarp();
         const int token0 = (step0 + pos - x) * kStep;
@@ -910,7 +942,8 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
     };
     auto inverse = [](float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; };
     const bool all_of_it = step0 == 0 && piece_end == x + r.steps;
-    const int seg = x - step0, u0 = all_of_it ? unit : unit_of(seg), u1 = all_of_it ? unit : unit_of(seg + r.steps - 1);
+    const Line seg = lo + x - step0;
+    const int u0 = all_of_it ? unit : unit_of(seg), u1 = all_of_it ? unit : unit_of(seg + r.steps - 1);
     auto part_of = [&](int u) { return 2 * (i64)u + (u == u0 ? 1 : 0); };
     float4* acc = reinterpret_cast<float4*>(a.acc);
     float4* stats = reinterpret_cast<float4*>(a.stats);
@@ -975,17 +1008,27 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
       }
     }
     x = piece_end;
-    if (x < hi) team_barrier(team, team_threads);   // before the next piece's results
+    if (x < span) team_barrier(team, team_threads);   // before the next piece's results
   }
 }
 
-template <int D, Kind kind>
-cudaError_t launch_one(const AttendArgs& a, int sm_count, bool pdl, cudaStream_t st) {
+template <int D, Kind kind, class Line>
+cudaError_t launch_line(const AttendArgs& a, int sm_count, bool pdl, cudaStream_t st) {
   using S = Shape<D, kind>;
   const int smem = S::kSmem;
-  cudaError_t e = cudaFuncSetAttribute(kv_attend_kernel<D, kind>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(kv_attend_kernel<D, kind, Line>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kv_attend_kernel<D, kind>, dim3(sm_count), dim3(32 * S::kWarps), smem, st, pdl, a);
+  return launch_kernel(kv_attend_kernel<D, kind, Line>, dim3(sm_count), dim3(32 * S::kWarps), smem, st, pdl, a);
+}
+template <int D, Kind kind>
+cudaError_t launch_one(const AttendArgs& a, int sm_count, bool pdl, cudaStream_t st) {
+  // the most that requests in order may come to: row tiles as each may have them, or as all of the rows do, and whole rows of the table
+  constexpr int kRows = Shape<D, kind>::kRows;
+  const i64 each = ((i64)a.max_queries * a.group + kRows - 1) / kRows;
+  const i64 tiles = std::min<i64>(a.requests * each, (i64)a.queries * a.group / kRows + a.requests);
+  const i64 steps = (std::min<i64>((i64)a.table_width * a.page_tokens, kMostTokens) + kStep - 1) / kStep;
+  const bool far = tiles * a.kv_heads > kMostSteps<int> / steps;
+  return far ? launch_line<D, kind, i64>(a, sm_count, pdl, st) : launch_line<D, kind, int>(a, sm_count, pdl, st);
 }
 template <int D>
 cudaError_t launch_dim(AttendArgs& a, const KvAttendScratch& s, int sm_count, bool pdl, cudaStream_t st) {

@@ -123,7 +123,9 @@ EMELB_API uint32_t emelb_kv_load(emelb_ctx* ctx, const emelb_kv_load_request* re
  * key / value head h.  Queries go in as f16 numbers times a power of two (f32 ones as the sum of two, 22 bits); softmax
  * weights times value scales are rounded to f16 (f32 results: to the sum of two); scores, statistics and sums are f32.
  * Rows of no request are left as they were.  max_queries bounds the rows of a request (more of them are an error that
- * emelb_sync reports, and are not computed); it is fast for few rows, longer chunks belong to emelb_attend_packed.
+ * emelb_sync reports, and are not computed); it is fast for few rows, longer chunks belong to emelb_attend_packed.  Lengths
+ * of more than 2^31 - 64 are out of range, and so is a call as a whole whose requests' tokens / 32 times kv_heads times rows of a
+ * key / value head / 8, each rounded up, come to more than 2^40 or without the tokens to 2^30: nothing of it is computed.
  * heads / kv_heads at most 64; type EMELB_F32, EMELB_F16 or EMELB_BF16 of q and out. */
 typedef struct emelb_kv_attend_request {
   emelb_kv_pages cache;

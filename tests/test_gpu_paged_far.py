@@ -183,3 +183,52 @@ def test_attend_planted_keys(be, length, rows, group, dim, page, t):
     done(be, be.kv_attend(paged.attend_request(c.pages, q, out, t, table, table.shape[1], lens, 1, group, rows, query_begin=begin, max_queries=rows, scale=1.0)))
     rounding = {"f32": 2.0 ** -21, "f16": 2.0 ** -11, "bf16": 2.0 ** -10}[t] + plain.HALF_STEP[t]
     assert ((out.double() - want).abs() <= rounding * want.abs() + 1e-5).all()
+
+
+@pytest.mark.parametrize("requests,rows,heads,kv,length,t", [(1, 4096, 64, 1, 1 << 21, "f16"), (140, 300, 64, 1, 1 << 17, "bf16"), (100, 150, 128, 2, 150001, "f32")])
+def test_attend_long_lines(be, requests, rows, heads, kv, length, t):
+    """More than 2^30 steps of 32 tokens for 8 rows of a key / value head in one call, 2^31 for one request: small caches that many rows
+    walk.  Tokens repeat every 256, so that weights are known by their counts; rounded alike, they are off by as much."""
+    g, dim = gen(rows), 32
+    c, k, v = repeated(be, [torch.randn(256, kv, dim, generator=g, device="cuda") for _ in range(2)])
+    width = -(-length // 256)
+    table, lens = torch.zeros(requests, width, dtype=torch.int32, device="cuda"), dev([length] * requests)
+    q = torch.randn(requests * rows, heads, dim, generator=g, device="cuda").to(plain.TORCH[t])
+    out, begin = torch.full_like(q, 7.0), dev([rows * b for b in range(requests + 1)])
+    torch.cuda.synchronize()
+    done(be, be.kv_attend(paged.attend_request(c.pages, q, out, t, table, width, lens, requests, heads, requests * rows, query_begin=begin, max_queries=rows)))
+    seen = length - rows + 1 + torch.arange(rows, device="cuda")
+    count = (seen[:, None] // 256 + (torch.arange(256, device="cuda")[None] < seen[:, None] % 256)).double()
+    weight, score = weight_step(t, q, k, dim ** -0.5)
+    for b in range(0, requests, max(1, requests // 7)):
+        at = slice(b * rows, (b + 1) * rows)
+        for h in range(heads):
+            s = q[at, h].double() @ k[:, h * kv // heads].double().T * dim ** -0.5
+            p = count * torch.exp(s - s.amax(-1, keepdim=True))
+            p = p / p.sum(-1, keepdim=True)
+            vv = v[:, h * kv // heads].double()
+            want, size = p @ vv, p @ vv.abs()
+            bound = (weight + 40 * score + 64 * 17 * 2.0 ** -23 + 2.0 ** -16) * size + plain.HALF_STEP[t] * want.abs()
+            err = (out[at, h].double() - want).abs()
+            assert (err <= bound).all(), (b, h, float((err / bound).max()))
+
+
+def test_attend_lines_beyond_count_are_reported(be):
+    """More than 2^40 steps, which would take a quarter of an hour, and more tokens than a request may have: not walked, and said."""
+    dim, rows, heads = 32, 4096, 64
+    c, _, _ = repeated(be, [torch.zeros(256, 1, dim, device="cuda") for _ in range(2)])
+    width = 1 << 23
+    table, q = torch.zeros(1, width, dtype=torch.int32, device="cuda"), torch.zeros(rows, heads, dim, dtype=torch.float16, device="cuda")
+    for length, n in ((0x7fffffc0, rows), (0x7fffffc1, 1), (0x7fffffff, 1)):
+        out, begin, lens = torch.full_like(q, 7.0), dev([0, n]), dev([length])
+        torch.cuda.synchronize()
+        assert be.kv_attend(paged.attend_request(c.pages, q, out, "f16", table, width, lens, 1, heads, rows, query_begin=begin, max_queries=rows))
+        assert not be.sync() and be.last_error == eb.INVALID_REQUEST
+        assert be.sync() and (out == 7.0).all()
+    # the longest that there may be, by one row
+    v = torch.linspace(-1, 1, dim, device="cuda").repeat(256, 1, 1)
+    c, _, kept = repeated(be, (torch.zeros_like(v), v))
+    q1, out, lens = torch.ones(1, 8, dim, device="cuda"), torch.zeros(1, 8, dim, device="cuda"), dev([0x7fffffc0])
+    torch.cuda.synchronize()
+    done(be, be.kv_attend(paged.attend_request(c.pages, q1, out, "f32", table, width, lens, 1, 8, 1)))
+    assert ((out[0] - kept[0]).abs() <= 2e-4 * kept[0].abs() + 1e-30).all()
