@@ -42,6 +42,7 @@ typedef long long i64;
 constexpr unsigned kAll = 0xffffffffu;
 constexpr float kLowest = -3.0e38f;   // running maximum before the first token: finite, below every score
 constexpr float kSlack = 3.0f;        // a score may pass the running maximum by this (log2) before sums are rescaled
+constexpr float kFarScore = 0x1p20f;  // from here on an f32 score's own rounding may be more than that
 constexpr int kJoinSteps = 5;         // what joining the parts of units costs, in steps of a warp
 constexpr int kMostParts = 6;             // parts of a (head, row tile) up to which a team may be smaller
 constexpr int kEach = 4;              // requests a lane in the search that a warp makes alone
@@ -638,8 +639,11 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
       for (int e = 0; e < 4; ++e) o[i16][e] = 0.0f;
     const int all_see = r.length - r.rows + row0 / a.group + 1;   // the first row's
     // A weight times a value's scale is rounded to f16, whose range is small: weights are taken times 2^-scale_exp, the running
-    // exponent of the largest scale, as part of the running maximum m.  cap: the score that moves m; scale_cap: the scale that
-    // moves scale_exp.  Neither happens often.
+    // exponent of the largest scale, as part of what scores are taken against, -neg_m.  cap: the score that moves the running maximum m;
+    // scale_cap: the scale that moves scale_exp.  Neither happens often.
+    // A score is rounded to f32 before -neg_m is taken away, as m was when that was made: of far scores the rounding alone, which a fused
+    // multiply-add would leave in, may be so much that weights overflow.  For them cap is the largest, without slack, and -neg_m
+    // is rounded up, since it must not fall behind m by more than scale_exp.
     int scale_exp = -11;
     uint32_t scale_cap = 0x14001400u;                             // 2^-10
     float neg_m[2] = {-kLowest, -kLowest};
@@ -740,15 +744,14 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
           const int e_new = max(scale_exp, big);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float top = fmaxf(fmaxf(score[0][h], score[0][h + 2]), fmaxf(score[1][h], score[1][h + 2])) * unit_score;
+            float top = fmaxf(fmaxf(score[0][h], score[0][h + 2]), fmaxf(score[1][h], score[1][h + 2]));
             top = fmaxf(top, __shfl_xor_sync(kAll, top, 4));
             top = fmaxf(top, __shfl_xor_sync(kAll, top, 8));
             top = fmaxf(top, __shfl_xor_sync(kAll, top, 16));
-            top = fmaxf(top, m[h]);
-            const float f = exp2_fast((m[h] - top) + (float)(scale_exp - e_new));
-            m[h] = top;
-            cap[h] = (top + kSlack) / unit_score;
-            neg_m[h] = -(top + (float)e_new);
+            m[h] = fmaxf(__fmul_rn(top, unit_score), m[h]);
+            cap[h] = fabsf(m[h]) < kFarScore ? (m[h] + kSlack) / unit_score : fmaxf(cap[h], top);
+            const float now = -__fadd_ru(m[h], (float)e_new), f = exp2_fast(now - neg_m[h]);
+            neg_m[h] = now;
             l[h] *= f;
 #pragma unroll
             for (int i16 = 0; i16 < D / 16; ++i16) {
@@ -762,7 +765,11 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) score[u][e] = exp2_fast(fmaf(score[u][e], unit_score, neg_m[e & 1]));
+          for (int e = 0; e < 4; e += 2) {
+            const float2 x = tc::unpack2(tc::mul2(tc::pack2(score[u][e], score[u][e + 1]), tc::pack2(unit_score, unit_score)));
+            score[u][e] = exp2_fast(__fadd_rn(x.x, neg_m[0]));
+            score[u][e + 1] = exp2_fast(__fadd_rn(x.y, neg_m[1]));
+          }
           l[0] += score[u][0] + score[u][2];
           l[1] += score[u][1] + score[u][3];
         }
@@ -845,7 +852,7 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
       if (taken == piece_stop) break;
       // to where the team's results meet in the end, which is free until then
       const float4 old = folded[tid];
-      const float m0 = m[0] + (float)scale_exp, m1 = m[1] + (float)scale_exp;
+      const float m0 = -neg_m[0], m1 = -neg_m[1];
       const float f0 = moved ? exp2_fast(old.x - m0) : 0.0f, f1 = moved ? exp2_fast(old.z - m1) : 0.0f;
       folded[tid] = make_float4(m0, moved ? fmaf(old.y, f0, l[0]) : l[0], m1, moved ? fmaf(old.w, f1, l[1]) : l[1]);
       l[0] = l[1] = 0.0f;
@@ -866,8 +873,8 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
 
     // ---- the piece's results.  A cell is what a lane holds of 16 dims: rows 2t and 2t + 1, dims 16 i + 2g and the next.  Cells stay in
     // this order all the way: through shared memory, through scratch, until the last sum is made
-    m[0] += (float)scale_exp;
-    m[1] += (float)scale_exp;
+    m[0] = -neg_m[0];
+    m[1] = -neg_m[1];
     if (moved) {
       const float4 old = folded[tid];
       const float f0 = exp2_fast(old.x - m[0]), f1 = exp2_fast(old.z - m[1]);

@@ -232,3 +232,26 @@ def test_attend_lines_beyond_count_are_reported(be):
     torch.cuda.synchronize()
     done(be, be.kv_attend(paged.attend_request(c.pages, q1, out, "f32", table, width, lens, 1, 8, 1)))
     assert ((out[0] - kept[0]).abs() <= 2e-4 * kept[0].abs() + 1e-30).all()
+
+
+@pytest.mark.parametrize("t,q_gain,k_gain,scale", [
+    ("bf16", 2.0 ** 30, 1.0, 0.125), ("f32", 2.0 ** 30, 1.0, 0.125), ("f16", 2.0 ** 12, 2.0 ** 12, 0.125), ("bf16", 2.0 ** 60, 2.0 ** 10, 8.0),
+    ("f32", 2.0 ** 80, 1.0, 0.125), ("f16", 1.0, 1.0, 2.0 ** 27), ("bf16", 2.0 ** 26, 1.0, 0.125), ("bf16", 2.0 ** 20, 1.0, 0.125), ("f32", -2.0 ** 30, 1.0, 0.125),
+    ("f16", 1.0, 2.0 ** 18, 1.0),
+])
+def test_attend_far_scores(be, t, q_gain, k_gain, scale):
+    """Scores whose own rounding is far more than one: the largest takes all the weight (the next is far below it)."""
+    dim, heads, lengths = 64, 16, [1500, 1, 40, 700]
+    rng, g = np.random.default_rng(3), gen(3)
+    c, table, k, v = filled(be, rng, g, lengths, 16, 2, dim, gain=(k_gain, 1.0))
+    q = (torch.randn(8, heads, dim, generator=g, device="cuda") * q_gain).to(plain.TORCH[t])
+    out, lens, begin = torch.full_like(q, 7.0), dev(lengths), dev([0, 2, 3, 5, 8])
+    torch.cuda.synchronize()
+    done(be, be.kv_attend(paged.attend_request(c.pages, q, out, t, table, table.shape[1], lens, 4, heads, 8, query_begin=begin, max_queries=3, scale=scale)))
+    at = 0
+    for b, (length, qa, qb) in enumerate(zip(lengths, (0, 2, 3, 5), (2, 3, 5, 8))):
+        want, _ = exact(q[qa:qb], k[at:at + length], v[at:at + length], scale)
+        rounding = weight_step(t, q, k, scale)[0] + 2.0 ** -16 + plain.HALF_STEP[t]
+        err = (out[qa:qb].double() - want).abs()
+        assert (err <= rounding * want.abs() + 1e-30).all(), (b, float(err.max()))
+        at += length
