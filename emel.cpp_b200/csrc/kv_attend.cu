@@ -590,17 +590,22 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
         for (int e = 0; e < 8; ++e) v[e] = live ? load_query<kind>(a, from + 32 * j + 8 * t + e) : 0.0f;
       }
     }
-    // f16 reaches less far than bf16 and f32: the eight rows go in times the power of two (at most 2^60) that takes their largest value
-    // to 2^13 .. 2^14, and the scores come out times the inverse.  Values 2^27 below it are still normal f16 numbers.
+    // f16 reaches less far than bf16 and f32: a row goes in times the power of two (at most 2^126) that takes its largest value to
+    // 2^13 .. 2^14, and its scores come out times the inverse.  Values 2^27 below it are still normal f16 numbers.
     float largest = 0.0f;
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(all_v[j][e]) < INFINITY ? fabsf(all_v[j][e]) : 0.0f);
-    const uint32_t expo = __reduce_max_sync(kAll, __float_as_uint(largest)) >> 23;
-    const int power = expo ? min(60, 140 - (int)expo) : 0;
+    largest = fmaxf(largest, __shfl_xor_sync(kAll, largest, 1));
+    largest = fmaxf(largest, __shfl_xor_sync(kAll, largest, 2));
+    const uint32_t expo = __float_as_uint(largest) >> 23;
+    const int power = expo ? min(126, 140 - (int)expo) : 0;       // of row g
     const float raise = __uint_as_float((uint32_t)(127 + power) << 23);
-    const float unit_score = fminf(fmaxf(a.scale_log2 * __uint_as_float((uint32_t)(127 - power) << 23), 1.2e-38f), 3.0e38f);
+    float unit_score[2];                                          // of rows 2t and 2t + 1
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      unit_score[h] = fminf(fmaxf(a.scale_log2 * __uint_as_float((uint32_t)(127 - __shfl_sync(kAll, power, 8 * t + 4 * h)) << 23), 1.2e-38f), 3.0e38f);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       float (&v)[8] = all_v[j];
@@ -748,8 +753,8 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
             top = fmaxf(top, __shfl_xor_sync(kAll, top, 4));
             top = fmaxf(top, __shfl_xor_sync(kAll, top, 8));
             top = fmaxf(top, __shfl_xor_sync(kAll, top, 16));
-            m[h] = fmaxf(__fmul_rn(top, unit_score), m[h]);
-            cap[h] = fabsf(m[h]) < kFarScore ? (m[h] + kSlack) / unit_score : fmaxf(cap[h], top);
+            m[h] = fmaxf(__fmul_rn(top, unit_score[h]), m[h]);
+            cap[h] = fabsf(m[h]) < kFarScore ? (m[h] + kSlack) / unit_score[h] : fmaxf(cap[h], top);
             const float now = -__fadd_ru(m[h], (float)e_new), f = exp2_fast(now - neg_m[h]);
             neg_m[h] = now;
             l[h] *= f;
@@ -766,7 +771,7 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
           for (int e = 0; e < 4; e += 2) {
-            const float2 x = tc::unpack2(tc::mul2(tc::pack2(score[u][e], score[u][e + 1]), tc::pack2(unit_score, unit_score)));
+            const float2 x = tc::unpack2(tc::mul2(tc::pack2(score[u][e], score[u][e + 1]), tc::pack2(unit_score[0], unit_score[1])));
             score[u][e] = exp2_fast(__fadd_rn(x.x, neg_m[0]));
             score[u][e + 1] = exp2_fast(__fadd_rn(x.y, neg_m[1]));
           }

@@ -255,3 +255,46 @@ def test_attend_far_scores(be, t, q_gain, k_gain, scale):
         err = (out[qa:qb].double() - want).abs()
         assert (err <= rounding * want.abs() + 1e-30).all(), (b, float(err.max()))
         at += length
+
+
+@pytest.mark.parametrize("t,above", [("bf16", 2.0 ** 44), ("f32", 2.0 ** 44), ("f32", 2.0 ** 20), ("f16", 2.0 ** 12), ("bf16", 2.0 ** 100), ("f32", 2.0 ** 100)])
+def test_attend_rows_keep_to_themselves(be, t, above):
+    """Heads and rows of far larger and smaller values in one tile of rows: each as exact as among its like.  (Not the same bits: when
+    a row's running maximum moves, the others of its tile move with it, and weights are rounded against another number.)"""
+    dim, heads, length = 64, 16, 500
+    rng, g = np.random.default_rng(3), gen(3)
+    c, table, k, v = filled(be, rng, g, [length], 16, 2, dim)
+    q = torch.randn(3, heads, dim, generator=g, device="cuda").to(plain.TORCH[t])
+    lens, begin, out = dev([length]), dev([0, 3]), torch.full_like(q, 7.0)
+    weight, score = weight_step(t, q, k, dim ** -0.5)
+    for i, h, by in ((0, 2, above), (1, 5, above), (2, 14, 1 / above), (2, 9, above)):
+        q[i, h] *= by
+    torch.cuda.synchronize()
+    done(be, be.kv_attend(paged.attend_request(c.pages, q, out, t, table, table.shape[1], lens, 1, heads, 3, query_begin=begin, max_queries=3)))
+    want, _ = exact(q, k, v, dim ** -0.5)
+    size, _ = exact(q, k, v.abs(), dim ** -0.5)
+    bound = (weight + 40 * score + 2.0 ** -16) * size + plain.HALF_STEP[t] * want.abs()
+    # Rows `above` times as large: nearly all weight to one key.  Their scores' errors are so many times larger, too: a weight among the
+    # rest, p of the largest one's, is off by a factor of exp(40 * score * above) at most, and cannot pass the largest one's, so the result
+    # by the rest's sum times that (or 1 a key) times the largest value.
+    for i, h in ((0, 2), (1, 5), (2, 9)):
+        s = q[i, h].double() @ k[:, h // 8].double().T * dim ** -0.5
+        gap = (s.max() - s).sort().values[1:]
+        bound[i, h] += torch.exp(torch.clamp(40 * score * above - gap, max=0)).sum() * v[:, h // 8].abs().max()
+    err = (out.double() - want).abs()
+    assert (err <= bound).all(), ((err / bound).amax(-1))
+
+
+@pytest.mark.parametrize("t,small", [("f32", 2.0 ** -100), ("bf16", 2.0 ** -100), ("f32", 2.0 ** 100)])
+def test_attend_scales_and_queries_far_apart(be, t, small):
+    """Queries times a power of two and the scale times its inverse: the same scores, the same bits."""
+    rng, g = np.random.default_rng(4), gen(4)
+    c, table, k, v = filled(be, rng, g, [300], 16, 1, 128)
+    q, lens = torch.randn(1, 8, 128, generator=g, device="cuda").to(plain.TORCH[t]), dev([300])
+    outs = []
+    for by in (1.0, small):
+        x, out = q * by, torch.zeros_like(q)
+        torch.cuda.synchronize()
+        done(be, be.kv_attend(paged.attend_request(c.pages, x, out, t, table, table.shape[1], lens, 1, 8, 1, scale=128 ** -0.5 / by)))
+        outs.append(out)
+    assert torch.equal(*outs)
