@@ -643,14 +643,15 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i16][e] = 0.0f;
     const int all_see = r.length - r.rows + row0 / a.group + 1;   // the first row's
-    // A weight times a value's scale is rounded to f16, whose range is small: weights are taken times 2^-scale_exp, the running
-    // exponent of the largest scale, as part of what scores are taken against, -neg_m.  cap: the score that moves the running maximum m;
-    // scale_cap: the scale that moves scale_exp.  Neither happens often.
+    // A weight times a value's scale is rounded to f16, whose range is small: weights are taken times 2^-scale_exp as part of what scores
+    // are taken against, -neg_m, so that products with the largest scale so far reach 2^15 and f16's grid ends 2^35 below that scale:
+    // scale_exp is its exponent less 11, -11 at least, where weights themselves reach 2^14, and 4 at most.  cap: the score that moves the
+    // running maximum m; scale_cap: the scale that moves scale_exp, 2^(scale_exp + 12).  Neither happens often.
     // A score is rounded to f32 before -neg_m is taken away, as m was when that was made: of far scores the rounding alone, which a fused
     // multiply-add would leave in, may be so much that weights overflow.  For them cap is the largest, without slack, and -neg_m
     // is rounded up, since it must not fall behind m by more than scale_exp.
-    int scale_exp = -11;
-    uint32_t scale_cap = 0x14001400u;                             // 2^-10
+    constexpr auto cap_of = [](int exp) { return (uint32_t)(exp + 27) * 0x04000400u; };   // of 4: infinity
+    uint32_t scale_cap = cap_of(-11);
     float neg_m[2] = {-kLowest, -kLowest};
     const int piece_stop = max(taken, (piece_end - member + team_warps - 1) / team_warps);
     bool moved = false;
@@ -745,8 +746,8 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
           moves |= fmaxf(fmaxf(score[0][h], score[0][h + 2]), fmaxf(score[1][h], score[1][h + 2])) > cap[h];
         if (__any_sync(kAll, moves)) {
           int big = (int)max(max(word[0] & 0xffffu, word[0] >> 16), max(word[1] & 0xffffu, word[1] >> 16)) >> 10;
-          big = min(4, __reduce_max_sync(kAll, big) - 15);
-          const int e_new = max(scale_exp, big);
+          big = min(4, __reduce_max_sync(kAll, big) - 15 - 11);
+          const int e_new = max((int)(scale_cap >> 26) - 27, big);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float top = fmaxf(fmaxf(score[0][h], score[0][h + 2]), fmaxf(score[1][h], score[1][h + 2]));
@@ -764,8 +765,7 @@ __global__ void __launch_bounds__(32 * Shape<D, kind>::kWarps, 1) kv_attend_kern
               o[i16][h + 2] *= f;
             }
           }
-          scale_exp = e_new;
-          scale_cap = e_new == 4 ? 0x7c007c00u : (uint32_t)(e_new + 16) * 0x04000400u;
+          scale_cap = cap_of(e_new);
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {

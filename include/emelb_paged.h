@@ -120,8 +120,11 @@ EMELB_API uint32_t emelb_kv_load(emelb_ctx* ctx, const emelb_kv_load_request* re
 /* ---- attention over the pages.  Request b brings query rows query_begin[b] .. query_begin[b + 1] - 1 (null: row b
  * alone); the last of them is its newest token, so that row i of n sees positions 0 .. lengths[b] - n + i, and none where
  * that is negative (the result is 0).  out = softmax(scale * q k^T) v per head; query heads h * heads / kv_heads .. share
- * key / value head h.  A query row of a head goes in as f16 numbers times a power of two of its own (f32 ones as the sum of two, 22 bits); softmax
- * weights times value scales are rounded to f16 (f32 results: to the sum of two); scores, statistics and sums are f32.
+ * key / value head h.  What is rounded: a query row of a head goes in as f16 numbers times a power of two of its own (f32 ones as
+ * the sum of two, 22 bits).  Its product with 32 dims of a key is an f32 sum that holds quants above a base: 18 bits of what such
+ * products may come to are kept, of f32 queries 22.  A weight times a value's scale is rounded to f16 (bf16 results: the weight
+ * before, too; f32 results: to the sum of two); fewer bits are left below 2^-20 of a row's largest weight, and of products below 2^-20 of
+ * the largest value scale of the head (f32 results: 2^-10), or of 1 where that is larger.  Statistics and sums are f32.
  * Rows of no request are left as they were.  max_queries bounds the rows of a request (more of them are an error that
  * emelb_sync reports, and are not computed); it is fast for few rows, longer chunks belong to emelb_attend_packed.  Lengths
  * of more than 2^31 - 64 are out of range, and so is a call as a whole whose requests' tokens / 32 times kv_heads times rows of a

@@ -42,8 +42,9 @@ def rms(x):
 
 def check_rms(got, want, root, weight_step, t, score=0.0):
     """Roundings of weights are independent of one another: together about weight_step * root; the result has one more.  Twice that, and
-    what errors of the scores make (`score`, relative to root: they are independent, too)."""
-    err, bound = rms(got.double() - want), 2 * ((weight_step + score) * rms(root) + plain.HALF_STEP[t] * rms(want))
+    what errors of the scores make (`score`, relative to root: they are independent, too).  Below 2^-14 f16 results have a fixed step,
+    2^-24, of which a rounding is off by half."""
+    err, bound = rms(got.double() - want), 2 * ((weight_step + score) * rms(root) + plain.HALF_STEP[t] * rms(want)) + 2.0 ** -25 * (t == "f16")
     assert np.isfinite(err) and err <= bound, (err, bound)
 
 
@@ -298,3 +299,31 @@ def test_attend_scales_and_queries_far_apart(be, t, small):
         done(be, be.kv_attend(paged.attend_request(c.pages, x, out, t, table, table.shape[1], lens, 1, 8, 1, scale=128 ** -0.5 / by)))
         outs.append(out)
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("t,dim,scales,tail", [
+    ("f16", 64, (4, -10), -10), ("bf16", 64, (4, -10), -10), ("f32", 64, (4, -6), -4), ("f16", 128, (10, 0, -4, -12), -3), ("f32", 96, (0, -3, -9), -5),
+    ("bf16", 128, (15, 14, 3, 0), -8), ("f16", 32, (-20,), -6), ("f32", 64, (-12, -14), -8),
+])
+def test_attend_values_of_groups_far_apart(be, t, dim, scales, tail):
+    """Groups of 32 dims whose scales are 2^scales, one key 2^-tail above all the others: what the many small weights bring keeps its
+    digits in every group."""
+    g, length, page = gen(dim), 4001, 16
+    rng = np.random.default_rng(dim)
+    table, pages = tables(rng, [length], page)
+    c = Cache(pages, page, 1, dim)
+    k, v = torch.zeros(length, 1, dim, device="cuda"), torch.rand(length, 1, dim, generator=g, device="cuda") * 2 - 1
+    k[700, 0, 0] = -tail
+    for j, e in enumerate(scales):
+        v[..., 32 * j:32 * j + 32] *= 8 * 2.0 ** e * (1 - 2.0 ** -11)
+    slots, table = dev(slots_of(table, [0], [length], page).tolist(), torch.int64), torch.from_numpy(table).cuda()
+    q, lens = torch.zeros(1, 4, dim, device="cuda").to(plain.TORCH[t]), dev([length])
+    q[..., 0] = 1
+    out, scale = torch.zeros_like(q), float(np.log(2))
+    torch.cuda.synchronize()
+    done(be, be.kv_store(paged.store_request(c.pages, k, v, "f32", slots, length)))
+    done(be, be.kv_attend(paged.attend_request(c.pages, q, out, t, table, table.shape[1], lens, 1, 4, 1, scale=scale)))
+    want, root = exact(q, plain.kept(k), plain.kept(v), scale)
+    for j in range(len(scales)):
+        at = slice(32 * j, 32 * j + 32)
+        check_rms(out[..., at], want[..., at], root[..., at], {"f32": 2.0 ** -20, "f16": 2.0 ** -11, "bf16": 2.0 ** -10}[t], t)
