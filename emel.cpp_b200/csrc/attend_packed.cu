@@ -54,6 +54,7 @@ constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(8 * kSoftmaxRegs + 4 * kOtherRegs <= 12 * 168, "registers");
 constexpr float kLowest = -3.0e38f;
 constexpr float kSlack = 8.0f;
+constexpr float kFarScore = 0x1p20f;  // from here on an f32 score's own rounding may be more than that
 constexpr int kFold = 64;             // key tiles between two moves of O out of TMEM: 512 products, 2^-14 of O
 constexpr int kTmemCols = 512;
 
@@ -71,10 +72,11 @@ struct PackedArgs {
   int64_t items;
   int* next;           // the next item, CTAs that are done: zero between launches
   int *bad, *status;
-  float* fold;         // of a CTA: kTiles x {dims of O, the maximum that they were taken against, the sum} x kTileRows
+  float* fold;         // of a CTA: kTiles x {dims of O, the maximum that they were taken against, the sum, far scores' base} x kTileRows
 };
 constexpr int kFoldDims = 128;
-static_assert((uint64_t)kTiles * (kFoldDims + 2) * kTileRows == kPackedFoldFloats, "scratch of a CTA");
+constexpr int kFoldRows = kFoldDims + 3;
+static_assert((uint64_t)kTiles * kFoldRows * kTileRows == kPackedFoldFloats, "scratch of a CTA");
 
 template <int DP>
 struct Smem {
@@ -195,7 +197,7 @@ __device__ __forceinline__ uint32_t fma_zero(uint32_t z, uint32_t w) {
 // A row's O, its maximum and its sum so far to scratch, on top of what is there but for the first time; and back into TMEM, where
 // results are taken from.  Calls: as code of the loop they cost the 13 prompts 54.6 us, as calls 52.5, which take 51.9 without them
 __device__ __forceinline__ float* fold_row(float* fold, int t, int row) {
-  return fold + ((uint64_t)blockIdx.x * kTiles + t) * ((kFoldDims + 2) * kTileRows) + row;
+  return fold + ((uint64_t)blockIdx.x * kTiles + t) * (kFoldRows * kTileRows) + row;
 }
 template <int DP>
 __device__ __noinline__ void fold_away(float* fold, int t, int row, uint32_t o_col, bool first, float m, float2 sums) {
@@ -231,6 +233,41 @@ __device__ __noinline__ float fold_back(float* fold, int t, int row, uint32_t o_
   }
   tc::tmem_wait_st();
   return fmaf(fold[(kFoldDims + 1) * kTileRows], f, sum);
+}
+
+// Far scores.  The loop takes a weight as 2^(score * scale - m) by one multiply-add, while m is a rounded product: of scores beyond
+// 2^27 the rounding alone may be so much that weights overflow.  So scores from kFarScore on are rounded as m is, and put back as
+// differences from a base, the largest of the row so far, over the scale; m, returned, and the maximum in scratch count from the base
+// as well.  `first`: m and scores still count from 0.
+__device__ __noinline__ float rebase(float* fold, int t, int row, uint32_t s_col, int seen, float scale, bool first, float m) {
+  fold = fold_row(fold, t, row);
+  float *fold_m = fold + kFoldDims * kTileRows, *at_base = fold + (kFoldDims + 2) * kTileRows;
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < kTileKeys; c += 32) {
+    uint32_t s[32];
+    tmem_ld32(s_col + c, s);
+    wait_ld(s);
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (c + i < seen) top = max_nan(top, __fmul_rn(__uint_as_float(s[i]), scale));
+  }
+  const float was = first ? m : *at_base;              // kLowest: nothing seen yet
+  if (first && m != kLowest) m = 0.0f;
+  const float base = max_nan(was, top), by = base - was, inv = 1.0f / scale;
+  *at_base = base;
+  *fold_m -= first ? base : by;                        // of nothing moved yet: whatever stands there
+#pragma unroll 1
+  for (int c = 0; c < kTileKeys; c += 32) {
+    uint32_t s[32];
+    tmem_ld32(s_col + c, s);
+    wait_ld(s);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s[i] = __float_as_uint((__fmul_rn(__uint_as_float(s[i]), scale) - base) * inv);
+    tc::tmem_st32(s_col + c, s);
+  }
+  tc::tmem_wait_st();
+  return max_nan(m - by, kLowest);
 }
 
 template <int DP, bool kBf16>
@@ -597,15 +634,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int n_mine = t ? it.n1 : it.n0;
       const int see = sees(it, min(token, it.tokens - 1)), see_all = sees(it, t * a.tile_tokens);   // of the row, of every row
       float m = kLowest;
+      int far = 0;   // 1: scores count from a base, 2: from this tile on, which is taken once more
       tc::f2 sum2 = tc::pack2(0.0f, 0.0f);
       for (int j = 0; j < n_mine; ++j) {
         alive = __all_sync(kAll, tc::mbar_wait(s_ready(t), s_parity, &gave_up));
         if (!alive) break;
         s_parity ^= 1;
         tc::fence_after();
-        if (j > 0 && j % kFold == 0) {   // the mix so far is done, as below
+        if (j > 0 && j % kFold == 0 && far < 2) {   // the mix so far is done, as below
           fold_away<DP>(a.fold, t, row, o_col, j == kFold, m, tc::unpack2(sum2));
           sum2 = tc::pack2(0.0f, 0.0f);
+        }
+        if (far) {
+          m = rebase(a.fold, t, row, s_col, see - j * kTileKeys, a.scale_log2, far == 2, m);
+          far = 1;
         }
         uint32_t s[128];
 #pragma unroll
@@ -626,6 +668,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float now = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * a.scale_log2;
         if (__any_sync(kAll, !(now <= m + kSlack))) {
           const float next = max_nan(m, now), f = exp2_fast(m - next);
+          if (!far && __any_sync(kAll, fabsf(next) >= kFarScore && next != kLowest)) {
+            far = 2;
+            s_parity ^= 1;
+            --j;
+            continue;
+          }
           m = next;
           sum2 = tc::mul2(sum2, tc::pack2(f, f));
           // the mix so far: its last product was issued before these scores, so it is done

@@ -26,7 +26,7 @@ struct KvAttendScratch {
 cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScratch& s, int sm_count, int* bad, bool pdl, cudaStream_t st);
 
 // `next`: two ints, zero between launches; `fold`: kPackedFoldFloats for each SM; `status`: raised to 1 when a bounded wait ran out
-constexpr uint64_t kPackedFoldFloats = 2 * 130 * 128;
+constexpr uint64_t kPackedFoldFloats = 2 * 131 * 128;
 cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int* next, float* fold, int sm_count, int* bad, int* status, bool pdl, cudaStream_t st);
 
 }  // namespace emelb

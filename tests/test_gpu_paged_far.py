@@ -327,3 +327,71 @@ def test_attend_values_of_groups_far_apart(be, t, dim, scales, tail):
     for j in range(len(scales)):
         at = slice(32 * j, 32 * j + 32)
         check_rms(out[..., at], want[..., at], root[..., at], {"f32": 2.0 ** -20, "f16": 2.0 ** -11, "bf16": 2.0 ** -10}[t], t)
+
+
+@pytest.mark.parametrize("t,dim,q_gain,k_gain,scale", [
+    ("f16", 64, 2.0 ** 12, 2.0 ** 12, 0.125), ("bf16", 64, 2.0 ** 30, 1.0, 0.125), ("bf16", 128, 2.0 ** 50, 2.0 ** 30, 1.0), ("f16", 128, 1.0, 1.0, 2.0 ** 26),
+    ("bf16", 40, 2.0 ** 20, 1.0, 1.0), ("f16", 64, 1.0, -1.0, 2.0 ** 24), ("f16", 64, 1.0, 1.0, 2.0 ** 25),
+])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_far_scores(be, t, dim, q_gain, k_gain, scale, causal):
+    """Scores whose own rounding is far more than one: the largest takes all the weight (the next is far below it)."""
+    queries, keys, heads, kv = [300, 1, 40, 7], [700, 1, 200, 7], 4, 2
+    g, dt = gen(dim), plain.TORCH[t]
+    q = (torch.randn(sum(queries), heads, dim, generator=g, device="cuda") * q_gain).to(dt)
+    k = (torch.randn(sum(keys), kv, dim, generator=g, device="cuda") * k_gain).to(dt)
+    v = torch.randn(sum(keys), kv, dim, generator=g, device="cuda").to(dt)
+    out, qb, kb = torch.full_like(q, 7.0), np.concatenate([[0], np.cumsum(queries)]), np.concatenate([[0], np.cumsum(keys)])
+    begin = [dev(qb.tolist()), dev(kb.tolist())]
+    torch.cuda.synchronize()
+    done(be, be.attend_packed(paged.packed_request(q, k, v, out, t, *begin, 4, heads, kv, dim, sum(queries), sum(keys), causal=causal, scale=scale)))
+    near = 0
+    for b in range(4):
+        qs, ks = slice(qb[b], qb[b + 1]), slice(kb[b], kb[b + 1])
+        want, _ = exact(q[qs], k[ks], v[ks], scale, causal)
+        root = exact(q[qs], k[ks], v[ks] * 0 + 1, scale, causal)[1]     # of the weights alone: 1 where one has all
+        sure = (root - 1).abs() < 1e-9
+        near += int((~sure[..., 0]).sum())
+        err = (out[qs].double() - want).abs()
+        assert torch.isfinite(out[qs]).all() and (err <= (2 * plain.HALF_STEP[t] + 2.0 ** -16) * want.abs())[sure].all(), b
+    assert near <= 4                                            # a few rows' two largest scores may lie that near to one another
+
+
+@pytest.mark.parametrize("keys,dim,ramp", [(20000, 64, 4.0), (20000, 128, -4.0), (17000, 40, 0.0)])
+def test_packed_far_scores_of_many_keys(be, keys, dim, ramp):
+    """Far scores that rise, fall or neither over moves of the result, and pairs of alike keys at both ends, which share the weight."""
+    g, heads, scale = gen(keys + dim), 2, 2.0 ** 24
+    k = torch.randn(keys, heads, dim, generator=g, device="cuda").sign()
+    k[..., 0] = torch.linspace(0, ramp, keys, device="cuda")[:, None]
+    v = torch.randn(keys, heads, dim, generator=g, device="cuda")
+    pairs = [(3, keys - 2), (100, 9000), (8191, 8192), (16383, 16384), (128, 129)]
+    for i, j in pairs:
+        k[i] = k[j]
+    q = torch.stack([k[j] for _, j in pairs])
+    q[..., 0] = 0                                          # the two of a pair are the largest, whatever the ramp
+    rising = torch.zeros(1, heads, dim, device="cuda")
+    rising[..., 0] = 1
+    q, k, v = torch.cat([q, rising]).half(), k.half(), v.half()
+    out, begin = torch.full_like(q, 7.0), [dev([0, len(q)]), dev([0, keys])]
+    torch.cuda.synchronize()
+    done(be, be.attend_packed(paged.packed_request(q, k, v, out, "f16", *begin, 1, heads, heads, dim, len(q), keys, causal=False, scale=scale)))
+    want, _ = exact(q, k, v, scale, False)
+    size, _ = exact(q, k, v.abs(), scale, False)
+    rows = slice(0, None if ramp else len(pairs))          # without a ramp the last row's scores are all alike
+    assert ((out.double() - want).abs() <= 2 * plain.HALF_STEP["f16"] * size + plain.HALF_STEP["f16"] * want.abs() + 1e-7)[rows].all()
+
+
+@pytest.mark.parametrize("t,gain", [("f32", 2.0 ** 30), ("bf16", 2.0 ** 40), ("f16", 2.0 ** 13)])
+def test_attend_far_scores_alike(be, t, gain):
+    """The largest of far scores comes back every 256 tokens: in other steps, warps, moves and units, all of which share its weight."""
+    g, dim, heads = gen(5), 64, 8
+    c, k, v = repeated(be, [torch.randn(256, 1, dim, generator=g, device="cuda") for _ in range(2)])
+    lengths = [1 << 20, 256, 70000, 300]
+    table, lens = torch.zeros(4, 4096, dtype=torch.int32, device="cuda"), dev(lengths)
+    q = (torch.randn(4, heads, dim, generator=g, device="cuda") * gain).to(plain.TORCH[t])
+    out, scale = torch.full_like(q, 7.0), 2.0 ** 14
+    torch.cuda.synchronize()
+    done(be, be.kv_attend(paged.attend_request(c.pages, q, out, t, table, 4096, lens, 4, heads, 4, scale=scale)))
+    want, _ = exact(q, k, v, scale, False)
+    rounding = {"f32": 2.0 ** -22, "f16": 2.0 ** -11, "bf16": 2.0 ** -10}[t] + plain.HALF_STEP[t] + 2.0 ** -16 + 64 * 17 * 2.0 ** -23
+    assert ((out.double() - want).abs() <= rounding * want.abs() + 1e-30).all()
