@@ -542,7 +542,9 @@ __global__ void __launch_bounds__(128, 10) kv_load_kernel(const LoadArgs a) {
   __shared__ __align__(16) uint8_t tiles[kLoadHeads][T::kBytes];
   const int tid = threadIdx.x, lane = tid & 31, groups = (a.heads + a.per - 1) / a.per, slot = blockIdx.x / groups, spare = a.first ? 2 : 1;
   const int head0 = blockIdx.x % groups * a.per, heads = min(a.per, a.heads - head0);
-  if (head0 == 0 && tid == 127 && slot < a.requests && (a.row_begin[slot] < 0 || a.row_begin[slot + 1] < a.row_begin[slot])) *a.bad = 1;
+  if (head0 == 0 && tid == 127 && slot < a.requests &&   // there are more slots than requests
+      (a.row_begin[slot] < 0 || a.row_begin[slot + 1] < a.row_begin[slot] || a.lengths[slot] < 0 || (a.first && a.first[slot] < 0)))
+    *a.bad = 1;
   int lo = 0, hi = a.requests;          // the last request whose slots begin at or before this one
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32, b = lo + lane * step;
@@ -554,10 +556,7 @@ __global__ void __launch_bounds__(128, 10) kv_load_kernel(const LoadArgs a) {
   const int b = lo, begin = a.row_begin[b], end = min(a.row_begin[b + 1], a.rows);
   const int64_t length = a.lengths[b], first = a.first ? a.first[b] : 0;
   if (begin < 0 || end <= begin) return;
-  if (first < 0) {
-    if (tid == 0) *a.bad = 1;
-    return;
-  }
+  if (first < 0) return;
   // positions first .. until - 1 go to rows begin and further
   const int64_t until = min(first + (end - begin), length), at = ((first >> 4) + slot - ((begin >> 4) + b * spare)) * kTile;
   const int from = (int)max(first - at, (int64_t)0), to = (int)min(until - at, (int64_t)kTile);

@@ -101,7 +101,8 @@ EMELB_API uint32_t emelb_kv_store_can_run(const emelb_kv_store_request* request)
 EMELB_API uint32_t emelb_kv_store(emelb_ctx* ctx, const emelb_kv_store_request* request);
 
 /* ---- rows back out of the pages, as the values kept (rounded once to `type`): token first[b] + i of request b, up to
- * lengths[b], to row row_begin[b] + i.  Other rows are left as they were.  first null: 0. */
+ * lengths[b], to row row_begin[b] + i.  Other rows are left as they were, and tokens whose row would be `rows` or more are left out
+ * (row_begin may say so without being out of range).  first null: 0. */
 typedef struct emelb_kv_load_request {
   emelb_kv_pages cache;
   void* k;                /* [rows][kv_heads][head_dim] by strides */

@@ -830,3 +830,23 @@ def test_contexts_at_once(be):
     for out in outs[1:]:
         assert torch.equal(out[0], outs[0][0]) and torch.equal(out[1], outs[0][1])
     other.close()
+
+
+@pytest.mark.parametrize("lengths,first", [([10, -1, 10], None), ([10, 10, -7], [0, 0, 0]), ([10, 0, 10], [0, -1, 0]), ([-1, 10, 10], [3, 0, 0])])
+def test_load_reports_negative_lengths(be, lengths, first):
+    """Of requests with rows and without; the others' tokens come back all the same."""
+    rng, g = np.random.default_rng(3), gen(3)
+    c, table, k, v = filled(be, rng, g, [10, 10, 10], 16, 2, 64)
+    for begin in ([0, 10, 20, 30], [0, 10, 10, 20], [5, 5, 5, 5]):
+        out = [torch.full((30, 2, 64), 7.0, device="cuda") for _ in range(2)]
+        keep = [dev(lengths), dev(begin), dev(first) if first else None]
+        torch.cuda.synchronize()
+        assert be.kv_load(paged.load_request(c.pages, *out, "f32", table, table.shape[1], keep[0], keep[1], 3, 30, first=keep[2]))
+        assert not be.sync() and be.last_error == eb.INVALID_REQUEST
+        assert be.sync()
+        for b in range(3):
+            rows = begin[b + 1] - begin[b]
+            sound = lengths[b] == 10 and (not first or first[b] == 0)
+            for got, kept in ((out[0], k), (out[1], v)):
+                at = got[begin[b]:begin[b + 1]]
+                assert torch.equal(at, kept[10 * b:10 * b + rows].float()) if sound else (at == 7.0).all()
