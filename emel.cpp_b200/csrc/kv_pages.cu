@@ -175,8 +175,9 @@ __global__ void __launch_bounds__(512) kv_plan_kernel(const __grid_constant__ Pl
   // what the ended requests gave back and nobody took
   for (i64 x = has_pages ? me : top; x < top - taken - count; x += step) {
     const int e = owner_of(back, n, (int)x);
-    if (count + x < r.pages) r.free_pages[count + x] = r.table[e * r.table_stride + (x - (e ? back[e - 1] : 0))];
-    else wrong = true;
+    const int page = r.table[e * r.table_stride + (x - (e ? back[e - 1] : 0))];
+    if (count + x < r.pages) r.free_pages[count + x] = page;
+    if (count + x >= r.pages || page < 0 || page >= r.pages) wrong = true;
   }
   // slots and positions: four neighbouring rows a thread, of which the first is searched for
   const int total = clip(tok_sum < r.token_capacity ? tok_sum : r.token_capacity);

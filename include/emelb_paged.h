@@ -55,7 +55,8 @@ EMELB_API uint64_t emelb_kv_page_bytes(int32_t head_dim, int32_t kv_heads, int32
  * top of the stack free_pages (free_count entries before) in request and table order; then each request in order takes
  * the pages it lacks from the top and appends them to its row of `table`.  The first request for which they do not suffice
  * gets nothing in this step, nor does any after it that lacks a page: its slots are -1 and its length stays cached[b].
- * A page belongs to one request: one that stands in two rows of the table is given back twice.
+ * A page belongs to one request: one that stands in two rows of the table is given back twice.  A page number out of range is
+ * reported each time it is given back or taken, but passed on as it stands; slots in it are -1, and other calls skip it.
  *
  *   lengths[b]      tokens of the request behind the step (0 when ended)
  *   query_begin[b]  first packed row of the request's fresh tokens; [requests] = all of them (waiting requests included)

@@ -850,3 +850,43 @@ def test_load_reports_negative_lengths(be, lengths, first):
             for got, kept in ((out[0], k), (out[1], v)):
                 at = got[begin[b]:begin[b + 1]]
                 assert torch.equal(at, kept[10 * b:10 * b + rows].float()) if sound else (at == 7.0).all()
+
+
+@pytest.mark.parametrize("n", [4, 1500])
+@pytest.mark.parametrize("where", ["given back", "taken at once", "stack", "unused"])
+def test_plan_reports_pages_out_of_range(be, n, where):
+    """-1 or a number too large in the row of a request that ends, or on the stack, in the step that meets it; not where none does."""
+    page, width = 16, 4
+    pages = 4 * n + 8
+    for bad in (-1, pages, 1 << 30):
+        s = Step(n, width, pages, page, n + 64)
+        cached, fresh = np.full(n, 40), np.ones(n, np.int64)
+        table = np.arange(4 * n, dtype=np.int32).reshape(n, 4)
+        stack = np.full(pages, -77, np.int32)
+        stack[:8] = np.arange(4 * n, 4 * n + 8)
+        fresh[n // 2] = -1
+        if where == "given back":
+            table[n // 2, 0] = bad
+        elif where == "taken at once":                        # the last given back is the first taken
+            table[n // 2, 2] = bad
+            fresh[0] = 9
+        elif where == "stack":
+            stack[7] = bad
+            fresh[0], fresh[n // 2] = 9, 1
+        else:
+            table[n // 2, 3], stack[8] = bad, bad              # behind what the request holds, above the stack's top
+        s.cached.copy_(dev(cached.tolist()))
+        s.fresh.copy_(dev(fresh.tolist()))
+        s.table.copy_(torch.from_numpy(table))
+        s.stack.copy_(torch.from_numpy(stack))
+        s.count.fill_(8)
+        torch.cuda.synchronize()
+        assert be.kv_plan(s.request())
+        ok = be.sync()
+        assert ok == (where == "unused") and (ok or be.last_error == eb.INVALID_REQUEST)
+        assert be.sync()
+        want = plain.plan(cached, fresh, table, stack, 8, page, n + 64)
+        if where in ("taken at once", "stack"):
+            want["slots"][want["slots"] // page == bad] = -1
+            want["slots"][want["slots"] < 0] = -1
+        s.check(want)                                           # passed on as it stands
