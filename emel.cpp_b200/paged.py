@@ -2,7 +2,8 @@
 attention of packed prompts.
 
 The request builders take device memory as torch tensors or addresses.  Strides default to the tensors' own; a row's head_dim
-values are contiguous.  `emel_cpp_b200.Backend` runs the requests: kv_plan, kv_store, kv_load, kv_attend, attend_packed."""
+values are contiguous.  A tensor of another type than the request's (int32 for lengths, tables and sums, int64 for slots), with too few
+values or with gaps inside a row is a ValueError; an address is taken at its word.  `emel_cpp_b200.Backend` runs the requests: kv_plan, kv_store, kv_load, kv_attend, attend_packed."""
 from __future__ import annotations
 
 import ctypes as C
@@ -15,6 +16,7 @@ _I32 = C.c_int32
 
 MAX_REQUESTS = 8192
 TYPES = {"f32": eb.F32, "f16": eb.F16, "bf16": eb.BF16}
+DTYPES = {eb.F32: "float32", eb.F16: "float16", eb.BF16: "bfloat16"}
 
 
 class Pages(C.Structure):
@@ -77,8 +79,53 @@ def page_bytes(head_dim: int, kv_heads: int, page_tokens: int) -> int:
     return eb.lib().emelb_kv_page_bytes(head_dim, kv_heads, page_tokens)
 
 
+def _tensor(x) -> bool:
+    return hasattr(x, "data_ptr") and hasattr(x, "stride")
+
+
+def _fits(name, x, dtype, enough, dense):
+    if str(x.dtype) != f"torch.{dtype}":
+        raise ValueError(f"{name}: {x.dtype}, not {dtype}")
+    if not enough:
+        raise ValueError(f"{name}: a tensor of {tuple(x.shape)} is too small for the request")
+    if not dense:
+        raise ValueError(f"{name}: values that have to be neighbours are {x.stride()} apart")
+
+
+def _array(name, x, count, dtype="int32") -> int:
+    """The address of `count` neighbouring numbers."""
+    if _tensor(x):
+        _fits(name, x, dtype, x.numel() >= count, x.is_contiguous())
+    return eb.ptr(x)
+
+
+def _rows(name, x, given, type, rows, heads, dim):
+    """(token, head) strides of rows: given, a 3-d tensor's own, or those of dense rows."""
+    own = _tensor(x) and x.dim() == 3
+    if _tensor(x):
+        dtype = DTYPES.get(type, str(x.dtype).removeprefix("torch."))     # of a type that nothing takes: refused with the request
+        enough = x.shape[0] >= rows and x.shape[1] >= heads and x.shape[2] >= dim if own else x.numel() >= rows * heads * dim
+        _fits(name, x, dtype, given is not None or enough, x.stride(2) == 1 or dim <= 1 if own else given is not None or x.is_contiguous())
+    if given is not None:
+        return given
+    return (x.stride(0), x.stride(1)) if own else (heads * dim, dim)
+
+
+def _table(x, stride, requests, width):
+    """(address, stride) of a page table."""
+    own = _tensor(x) and x.dim() == 2
+    if stride is None:
+        stride = x.stride(0) if own else width
+    if _tensor(x):
+        enough = x.shape[0] >= requests and x.shape[1] >= width if own else x.numel() >= (requests - 1) * stride + width
+        _fits("table", x, "int32", enough, x.stride(1) == 1 or width <= 1 if own else x.is_contiguous())
+    return eb.ptr(x), stride
+
+
 def pages(data, count: int, page_tokens: int, kv_heads: int, head_dim: int) -> Pages:
     """A cache of `count` pages in device memory of count * page_bytes() bytes."""
+    if _tensor(data):
+        _fits("pages", data, "uint8", data.numel() >= count * page_bytes(head_dim, kv_heads, page_tokens), data.is_contiguous())
     return Pages(eb.ptr(data), count, page_tokens, kv_heads, head_dim)
 
 
@@ -86,49 +133,46 @@ def _type(t) -> int:
     return TYPES[t] if isinstance(t, str) else t
 
 
-def _strides(x, given, heads, dim):
-    """(token, head) strides of rows: given, a 3-d tensor's own, or those of dense rows."""
-    if given is not None:
-        return given
-    if hasattr(x, "stride") and x.dim() == 3:
-        return x.stride(0), x.stride(1)
-    return heads * dim, dim
-
-
 def plan_request(cached, fresh, table, table_width, free_pages, pages, free_count, free_left, lengths, query_begin, key_begin, slots, positions,
                  shortage, requests, page_tokens, token_capacity, table_stride=None) -> PlanRequest:
     """lengths may be cached and free_left free_count: a step in place."""
-    arrays = (cached, fresh, table, free_pages, free_count, free_left, lengths, query_begin, key_begin, slots, positions, shortage)
-    stride = table_stride if table_stride is not None else table.stride(0) if hasattr(table, "stride") and table.dim() == 2 else table_width
-    return PlanRequest(*(eb.ptr(a) for a in arrays), stride, requests, table_width, pages, page_tokens, token_capacity)
+    at, stride = _table(table, table_stride, requests, table_width)
+    return PlanRequest(_array("cached", cached, requests), _array("fresh", fresh, requests), at, _array("free_pages", free_pages, pages),
+                       _array("free_count", free_count, 1), _array("free_left", free_left, 1), _array("lengths", lengths, requests),
+                       _array("query_begin", query_begin, requests + 1), _array("key_begin", key_begin, requests + 1),
+                       _array("slots", slots, token_capacity, "int64"), _array("positions", positions, token_capacity), _array("shortage", shortage, 1),
+                       stride, requests, table_width, pages, page_tokens, token_capacity)
 
 
 def store_request(cache: Pages, k, v, type, slots, tokens, k_strides=None, v_strides=None) -> StoreRequest:
-    h, d = cache.kv_heads, cache.head_dim
-    return StoreRequest(cache, eb.ptr(k), eb.ptr(v), eb.ptr(slots), *_strides(k, k_strides, h, d), *_strides(v, v_strides, h, d), tokens, _type(type))
+    h, d, t = cache.kv_heads, cache.head_dim, _type(type)
+    return StoreRequest(cache, eb.ptr(k), eb.ptr(v), _array("slots", slots, tokens, "int64"), *_rows("k", k, k_strides, t, tokens, h, d),
+                        *_rows("v", v, v_strides, t, tokens, h, d), tokens, t)
 
 
 def load_request(cache: Pages, k, v, type, table, table_width, lengths, row_begin, requests, rows, first=None, table_stride=None, k_strides=None,
                  v_strides=None) -> LoadRequest:
-    h, d = cache.kv_heads, cache.head_dim
-    stride = table_stride if table_stride is not None else table.stride(0) if hasattr(table, "stride") and table.dim() == 2 else table_width
-    return LoadRequest(cache, eb.ptr(k), eb.ptr(v), eb.ptr(table), eb.ptr(first), eb.ptr(lengths), eb.ptr(row_begin), stride,
-                       *_strides(k, k_strides, h, d), *_strides(v, v_strides, h, d), requests, table_width, rows, _type(type))
+    h, d, t = cache.kv_heads, cache.head_dim, _type(type)
+    at, stride = _table(table, table_stride, requests, table_width)
+    return LoadRequest(cache, eb.ptr(k), eb.ptr(v), at, _array("first", first, requests), _array("lengths", lengths, requests),
+                       _array("row_begin", row_begin, requests + 1), stride, *_rows("k", k, k_strides, t, rows, h, d),
+                       *_rows("v", v, v_strides, t, rows, h, d), requests, table_width, rows, t)
 
 
 def attend_request(cache: Pages, q, out, type, table, table_width, lengths, requests, heads, queries, query_begin=None, max_queries=1, scale=None,
                    table_stride=None, q_strides=None, out_strides=None) -> AttendRequest:
-    d = cache.head_dim
-    stride = table_stride if table_stride is not None else table.stride(0) if hasattr(table, "stride") and table.dim() == 2 else table_width
-    return AttendRequest(cache, eb.ptr(q), eb.ptr(out), eb.ptr(table), eb.ptr(lengths), eb.ptr(query_begin), stride, *_strides(q, q_strides, heads, d),
-                         *_strides(out, out_strides, heads, d), requests, table_width, heads, queries, max_queries, max(d, 1) ** -0.5 if scale is None else scale,
-                         _type(type))
+    d, t = cache.head_dim, _type(type)
+    at, stride = _table(table, table_stride, requests, table_width)
+    return AttendRequest(cache, eb.ptr(q), eb.ptr(out), at, _array("lengths", lengths, requests), _array("query_begin", query_begin, requests + 1), stride,
+                         *_rows("q", q, q_strides, t, queries, heads, d), *_rows("out", out, out_strides, t, queries, heads, d), requests, table_width,
+                         heads, queries, max_queries, max(d, 1) ** -0.5 if scale is None else scale, t)
 
 
 def packed_request(q, k, v, out, type, query_begin, key_begin, requests, heads, kv_heads, head_dim, queries, keys, max_queries=None, causal=True,
                    scale=None, q_strides=None, k_strides=None, v_strides=None, out_strides=None) -> PackedRequest:
-    return PackedRequest(eb.ptr(q), eb.ptr(k), eb.ptr(v), eb.ptr(out), eb.ptr(query_begin), eb.ptr(key_begin),
-                         *_strides(q, q_strides, heads, head_dim), *_strides(k, k_strides, kv_heads, head_dim),
-                         *_strides(v, v_strides, kv_heads, head_dim), *_strides(out, out_strides, heads, head_dim), requests, heads, kv_heads, head_dim,
-                         queries, keys, queries if max_queries is None else max_queries, int(causal), max(head_dim, 1) ** -0.5 if scale is None else scale,
-                         _type(type))
+    d, t = head_dim, _type(type)
+    return PackedRequest(eb.ptr(q), eb.ptr(k), eb.ptr(v), eb.ptr(out), _array("query_begin", query_begin, requests + 1),
+                         _array("key_begin", key_begin, requests + 1), *_rows("q", q, q_strides, t, queries, heads, d),
+                         *_rows("k", k, k_strides, t, keys, kv_heads, d), *_rows("v", v, v_strides, t, keys, kv_heads, d),
+                         *_rows("out", out, out_strides, t, queries, heads, d), requests, heads, kv_heads, head_dim, queries, keys,
+                         queries if max_queries is None else max_queries, int(causal), max(head_dim, 1) ** -0.5 if scale is None else scale, t)

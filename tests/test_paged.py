@@ -123,3 +123,48 @@ def test_packed_requests(change, why):
     a = dict(q=at(0), k=at(1), v=at(2), out=at(3), type="f16", query_begin=at(4), key_begin=at(5), requests=3, heads=4, kv_heads=2, head_dim=64, queries=20,
              keys=30)
     assert paged.can_run(paged.packed_request(**{**a, **change})) == why
+
+
+def test_tensors_that_do_not_fit_their_request():
+    """The builders look at a tensor's type, size and innermost stride; at the same values by their address they do not."""
+    import torch
+    z = lambda *shape, t=torch.int32: torch.zeros(*shape, dtype=t)  # noqa: E731
+    c = paged.pages(z(100 * paged.page_bytes(64, 2, 16), t=torch.uint8), 100, 16, 2, 64)
+    half, wide = z(9, 2, 64, t=torch.float16), z(9, 2, 128, t=torch.float16)
+
+    plan = dict(cached=z(7), fresh=z(7), table=z(7, 50)[:, :40], table_width=40, free_pages=z(500), pages=500, free_count=z(1), free_left=z(1), lengths=z(7),
+                query_begin=z(8), key_begin=z(8), slots=z(64, t=torch.int64), positions=z(64), shortage=z(1), requests=7, page_tokens=16, token_capacity=64)
+    store = dict(cache=c, k=half, v=half.clone(), type="f16", slots=z(9, t=torch.int64), tokens=9)
+    load = dict(cache=c, k=half, v=half.clone(), type="f16", table=z(3, 4), table_width=4, lengths=z(3), row_begin=z(4), requests=3, rows=9)
+    attend = dict(cache=c, q=z(3, 4, 64, t=torch.float16), out=z(3, 4, 64, t=torch.float16), type="f16", table=z(3, 4), table_width=4, lengths=z(3), requests=3,
+                  heads=4, queries=3)
+    packed = dict(q=half, k=half, v=half, out=half.clone(), type="f16", query_begin=z(4), key_begin=z(4), requests=3, heads=2, kv_heads=2, head_dim=64, queries=9,
+                  keys=9)
+    builders = {paged.plan_request: plan, paged.store_request: store, paged.load_request: load, paged.attend_request: attend, paged.packed_request: packed}
+    for build, a in builders.items():
+        assert paged.can_run(build(**a)) in (eb.OK, eb.UNSUPPORTED_OP)      # host memory may lie at any address
+    for build, change in (
+            (paged.plan_request, dict(cached=z(7, t=torch.int64))), (paged.plan_request, dict(fresh=z(6))), (paged.plan_request, dict(slots=z(64))),
+            (paged.plan_request, dict(slots=z(63, t=torch.int64))), (paged.plan_request, dict(query_begin=z(7))), (paged.plan_request, dict(lengths=z(14)[::2])),
+            (paged.plan_request, dict(table=z(7, 80)[:, ::2])), (paged.plan_request, dict(table=z(6, 40))), (paged.plan_request, dict(table=z(7, 39))),
+            (paged.plan_request, dict(table=z(7, 40, t=torch.int64))), (paged.plan_request, dict(free_pages=z(499))), (paged.plan_request, dict(table=z(279))),
+            (paged.store_request, dict(k=half.float())), (paged.store_request, dict(v=half.bfloat16())), (paged.store_request, dict(type="f32")),
+            (paged.store_request, dict(k=wide[:, :, ::2])), (paged.store_request, dict(k=half[:8])), (paged.store_request, dict(k=half[:, :1])),
+            (paged.store_request, dict(v=half[..., :32])), (paged.store_request, dict(slots=z(9))), (paged.store_request, dict(k=half.transpose(1, 2))),
+            (paged.store_request, dict(k=z(9 * 2 * 64 - 1, t=torch.float16))), (paged.store_request, dict(k=wide[:, :, ::2], k_strides=(256, 128))),
+            (paged.load_request, dict(lengths=z(3, t=torch.int64))), (paged.load_request, dict(row_begin=z(3))), (paged.load_request, dict(first=z(2))),
+            (paged.load_request, dict(k=half[:8])), (paged.load_request, dict(table=z(2, 4))), (paged.load_request, dict(type="bf16")),
+            (paged.attend_request, dict(q=z(3, 4, 64))), (paged.attend_request, dict(out=z(2, 4, 64, t=torch.float16))), (paged.attend_request, dict(lengths=z(2))),
+            (paged.attend_request, dict(query_begin=z(3))), (paged.attend_request, dict(heads=6)), (paged.attend_request, dict(queries=4)),
+            (paged.packed_request, dict(keys=10)), (paged.packed_request, dict(queries=10)), (paged.packed_request, dict(k=wide[:, :, 1::2])),
+            (paged.packed_request, dict(type="bf16")), (paged.packed_request, dict(key_begin=z(4, t=torch.int64))), (paged.packed_request, dict(head_dim=72))):
+        with pytest.raises(ValueError):
+            build(**{**builders[build], **change})
+    with pytest.raises(ValueError):
+        paged.pages(z(100 * paged.page_bytes(64, 2, 16) - 1, t=torch.uint8), 100, 16, 2, 64)
+    with pytest.raises(ValueError):
+        paged.pages(z(100 * paged.page_bytes(64, 2, 16)), 100, 16, 2, 64)
+    # what fits: more rows, heads and values than asked for, other layouts, addresses
+    paged.store_request(c, wide[..., :64], z(12, 3, 64, t=torch.float16), "f16", z(20, t=torch.int64), 9)
+    paged.store_request(c, half.transpose(0, 1).contiguous().transpose(0, 1), z(9 * 2 * 64, t=torch.float16), "f16", at(1), 9)
+    paged.store_request(c, at(2), at(3), "f16", at(1), 9)
