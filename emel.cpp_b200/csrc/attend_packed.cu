@@ -63,10 +63,10 @@ struct __align__(64) Map {
 };
 
 struct PackedArgs {
-  const void *q, *v;
+  const void* v;
   void* out;
   const int32_t *query_begin, *key_begin;
-  int64_t qs, qh, vs, vh, os, oh;
+  int64_t vs, vh, os, oh;
   int requests, kv_heads, group, group_inv, tile_tokens, head_dim, queries, keys, max_queries, causal;
   float scale_log2;
   int64_t items;
@@ -837,15 +837,12 @@ cudaError_t launch_one(const PackedArgs& a, const Map& q, const Map& k, const Ma
 
 cudaError_t launch_attend_packed(const emelb_attend_packed_request& r, int* next, float* fold, int sm_count, int* bad, int* status, bool pdl, cudaStream_t st) {
   PackedArgs a{};
-  a.q = r.q;
   a.out = r.out;
   a.query_begin = r.query_begin;
   a.key_begin = r.key_begin;
   a.v = r.v;
   a.vs = r.v_token_stride;
   a.vh = r.v_head_stride;
-  a.qs = r.q_token_stride;
-  a.qh = r.q_head_stride;
   a.os = r.out_token_stride;
   a.oh = r.out_head_stride;
   a.requests = r.requests;

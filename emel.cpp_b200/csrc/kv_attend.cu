@@ -54,8 +54,8 @@ struct AttendArgs {
   const void* q;
   void* out;
   const int32_t *table, *lengths, *query_begin;
-  int64_t table_stride, qs, qh, os, oh, page_bytes;
-  int requests, table_width, kv_heads, group, queries, max_queries, pages, page_tokens, page_shift, type, q_vec, out_pairs;
+  int64_t table_stride, qs, qh, os, oh;
+  int requests, table_width, kv_heads, group, queries, max_queries, pages, page_tokens, page_shift, q_vec, out_pairs;
   float scale_log2;
   float *acc, *stats;
   int* arrived;
@@ -1043,14 +1043,14 @@ cudaError_t launch_one(const AttendArgs& a, int sm_count, bool pdl, cudaStream_t
   return far ? launch_line<D, kind, i64>(a, sm_count, pdl, st) : launch_line<D, kind, int>(a, sm_count, pdl, st);
 }
 template <int D>
-cudaError_t launch_dim(AttendArgs& a, const KvAttendScratch& s, int sm_count, bool pdl, cudaStream_t st) {
+cudaError_t launch_dim(AttendArgs& a, int type, const KvAttendScratch& s, int sm_count, bool pdl, cudaStream_t st) {
   constexpr uint64_t rows = 8;
   uint64_t units = s.acc_floats / (2 * rows * D);
   units = units < s.stats_floats / (4 * rows) ? units : s.stats_floats / (4 * rows);
   units = units < s.arrived_ints ? units : s.arrived_ints;
   a.most_units = (int)units;
-  if (a.type == EMELB_F32) return launch_one<D, kF32>(a, sm_count, pdl, st);
-  return a.type == EMELB_F16 ? launch_one<D, kF16>(a, sm_count, pdl, st) : launch_one<D, kBf16>(a, sm_count, pdl, st);
+  if (type == EMELB_F32) return launch_one<D, kF32>(a, sm_count, pdl, st);
+  return type == EMELB_F16 ? launch_one<D, kF16>(a, sm_count, pdl, st) : launch_one<D, kBf16>(a, sm_count, pdl, st);
 }
 
 }  // namespace
@@ -1068,7 +1068,6 @@ cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScr
   a.qh = r.q_head_stride;
   a.os = r.out_token_stride;
   a.oh = r.out_head_stride;
-  a.page_bytes = (int64_t)emelb_kv_page_bytes(r.cache.head_dim, r.cache.kv_heads, r.cache.page_tokens);
   a.requests = r.requests;
   a.table_width = r.table_width;
   a.kv_heads = r.cache.kv_heads;
@@ -1078,7 +1077,6 @@ cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScr
   a.pages = r.cache.pages;
   a.page_tokens = r.cache.page_tokens;
   while ((1 << a.page_shift) < a.page_tokens) ++a.page_shift;
-  a.type = r.type;
   const int64_t size = r.type == EMELB_F32 ? 4 : 2;
   a.q_vec = reinterpret_cast<uintptr_t>(r.q) % 16 == 0 && a.qs * size % 16 == 0 && a.qh * size % 16 == 0;
   a.out_pairs = reinterpret_cast<uintptr_t>(r.out) % 4 == 0 && a.os % 2 == 0 && a.oh % 2 == 0;
@@ -1088,10 +1086,10 @@ cudaError_t launch_kv_attend(const emelb_kv_attend_request& r, const KvAttendScr
   a.arrived = s.arrived;
   a.bad = bad;
   switch (r.cache.head_dim) {
-    case 32: return launch_dim<32>(a, s, sm_count, pdl, st);
-    case 64: return launch_dim<64>(a, s, sm_count, pdl, st);
-    case 96: return launch_dim<96>(a, s, sm_count, pdl, st);
-    default: return launch_dim<128>(a, s, sm_count, pdl, st);
+    case 32: return launch_dim<32>(a, r.type, s, sm_count, pdl, st);
+    case 64: return launch_dim<64>(a, r.type, s, sm_count, pdl, st);
+    case 96: return launch_dim<96>(a, r.type, s, sm_count, pdl, st);
+    default: return launch_dim<128>(a, r.type, s, sm_count, pdl, st);
   }
 }
 

@@ -13,7 +13,6 @@
 namespace emelb {
 namespace {
 
-using kv::kGroup;
 using kv::kTile;
 using kv::Tile;
 typedef long long i64;
