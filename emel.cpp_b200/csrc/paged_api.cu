@@ -156,7 +156,7 @@ uint32_t emelb_kv_store_can_run(const emelb_kv_store_request* r) {
       !apart(cache, rows_span(r->v, r->v_token_stride, r->v_head_stride, D, r->tokens, H, size)) ||
       !apart(cache, Span{r->slots, (uint64_t)r->tokens * 8}))
     return EMELB_INVALID_REQUEST;
-  if (((int64_t)r->tokens + 15) / 16 * H > 0x3fffffff) return EMELB_UNSUPPORTED_OP;   // CTAs
+  if (r->tokens > 0x7ffffff0 || ((int64_t)r->tokens + 15) / 16 * H > 0x3fffffff) return EMELB_UNSUPPORTED_OP;   // places in a last tile, CTAs
   return EMELB_OK;
 }
 

@@ -54,7 +54,9 @@ EMELB_API uint64_t emelb_kv_page_bytes(int32_t head_dim, int32_t kv_heads, int32
  * fresh[b] tokens join the cached[b] of request b; fresh[b] = -1: the request has ended.  The ended requests' pages go on
  * top of the stack free_pages (free_count entries before) in request and table order; then each request in order takes
  * the pages it lacks from the top and appends them to its row of `table`.  The first request for which they do not suffice
- * gets nothing in this step, nor does any after it that lacks a page: its slots are -1 and its length stays cached[b].
+ * gets nothing in this step, nor does any after it that lacks a page: its slots are -1 and its length stays cached[b].  Its
+ * rows count in query_begin all the same: attention computes them, against the last of its cached tokens, and a slot of -1 is the
+ * sign to drop the result.
  * A page belongs to one request: one that stands in two rows of the table is given back twice.  A page number out of range is
  * reported each time it is given back or taken, but passed on as it stands; slots in it are -1, and other calls skip it.
  *
@@ -88,7 +90,7 @@ EMELB_API uint32_t emelb_kv_plan(emelb_ctx* ctx, const emelb_kv_plan_request* re
 
 /* ---- keys and values of `tokens` packed rows into their slots; rows with a negative slot are skipped.  type EMELB_F32,
  * EMELB_F16 or EMELB_BF16.  The slots of one call are distinct (which of two rows a slot named twice holds is not
- * specified, nor whether it holds one of them whole). */
+ * specified, nor whether it holds one of them whole).  tokens at most 2^31 - 16. */
 typedef struct emelb_kv_store_request {
   emelb_kv_pages cache;
   const void* k;          /* [tokens][kv_heads][head_dim] by strides */
@@ -125,8 +127,9 @@ EMELB_API uint32_t emelb_kv_load(emelb_ctx* ctx, const emelb_kv_load_request* re
  * key / value head h.  What is rounded: a query row of a head goes in as f16 numbers times a power of two of its own (f32 ones as
  * the sum of two, 22 bits).  Its product with 32 dims of a key is an f32 sum that holds quants above a base: 18 bits of what such
  * products may come to are kept, of f32 queries 22.  A weight times a value's scale is rounded to f16 (bf16 results: the weight
- * before, too; f32 results: to the sum of two); fewer bits are left below 2^-20 of a row's largest weight, and of products below 2^-20 of
- * the largest value scale of the head (f32 results: 2^-10), or of 1 where that is larger.  Statistics and sums are f32.
+ * before, too; f32 results: to the sum of two).  With S the largest value scale of the head, or 1 where that is larger, and the largest
+ * weight of a row as 1, fewer bits are left of weights below 2^-25 S (16-bit results) and of such products below 2^-25 S (f32
+ * results: 2^-14 S).  Statistics and sums are f32.
  * Rows of no request are left as they were.  max_queries bounds the rows of a request (more of them are an error that
  * emelb_sync reports, and are not computed); it is fast for few rows, longer chunks belong to emelb_attend_packed.  Lengths
  * of more than 2^31 - 64 are out of range, and so is a call as a whole whose requests' tokens / 32 times kv_heads times rows of a

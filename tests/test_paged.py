@@ -168,3 +168,10 @@ def test_tensors_that_do_not_fit_their_request():
     paged.store_request(c, wide[..., :64], z(12, 3, 64, t=torch.float16), "f16", z(20, t=torch.int64), 9)
     paged.store_request(c, half.transpose(0, 1).contiguous().transpose(0, 1), z(9 * 2 * 64, t=torch.float16), "f16", at(1), 9)
     paged.store_request(c, at(2), at(3), "f16", at(1), 9)
+
+
+@pytest.mark.parametrize("tokens,why", [(0x7ffffff0, eb.OK), (0x7ffffff1, eb.UNSUPPORTED_OP), (0x7fffffff, eb.UNSUPPORTED_OP)])
+def test_store_of_the_most_rows(tokens, why):
+    """Places of a last tile of 16 rows are ints."""
+    c = cache(head_dim=32, kv_heads=1, data=at(10000000))
+    assert paged.can_run(paged.store_request(c, at(0), at(0), "f16", at(5000), tokens)) == why
