@@ -81,6 +81,7 @@ _SIGNATURES = {
     "emelb_set_attention_mode": [_P, C.c_int],
     "emelb_set_upload_route": [_P, C.c_int32, C.c_int32],
     "emelb_set_peer_wait_ms": [_P, C.c_uint32],
+    "emelb_set_upload_wait_ms": [_P, C.c_uint32],
     "emelb_selftest_wait_timeout": [_P, C.c_uint32],
     "emelb_residency_upload": [_P, C.c_int32, _P, C.c_uint64, C.c_int32, C.POINTER(_P)],
     "emelb_residency_evict": [_P, C.c_int32],
@@ -338,6 +339,10 @@ class Backend:
         """route: "ring" (page-locked staging ring, the default), "plain" or "register"; threads 0 = automatic."""
         code = {"ring": 0, "plain": 1, "register": 2}[route]
         return self._ret(lib().emelb_set_upload_route(self._h, code, threads))
+
+    def set_upload_wait_ms(self, limit_ms: int) -> bool:
+        """How long an upload waits for the device each time it has to (120,000 ms by default)."""
+        return self._ret(lib().emelb_set_upload_wait_ms(self._h, limit_ms))
 
     # -- residency
     def upload(self, tensor_id: int, host, nbytes: int | None = None, tensor_type: int = 0) -> int:

@@ -394,6 +394,7 @@ uint32_t emelb_destroy(emelb_ctx* c) {
   if (c->stream) cudaStreamSynchronize(c->stream);
   comm_release(c);
   upload_ring_release(c);
+  upload_unlock(c);
   for (auto& kv : c->residents)
     if (kv.second.dev) cudaFree(kv.second.dev);
   for (void* p : c->owned) cudaFree(p);
@@ -447,6 +448,12 @@ uint32_t emelb_set_upload_route(emelb_ctx* c, int32_t route, int32_t threads) {
   return EMELB_OK;
 }
 
+uint32_t emelb_set_upload_wait_ms(emelb_ctx* c, uint32_t limit_ms) {
+  if (!c || limit_ms == 0) return EMELB_INVALID_REQUEST;
+  c->upload_wait_ms = limit_ms;
+  return EMELB_OK;
+}
+
 uint32_t emelb_set_attention_mode(emelb_ctx* c, int mode) {
   if (!c || mode < 0 || mode > 2) return EMELB_INVALID_REQUEST;
   c->attention_mode = mode;
@@ -488,8 +495,12 @@ uint32_t emelb::residency_upload_many(emelb_ctx* c, UploadSpan* spans, size_t co
       return EMELB_INTERNAL_ERROR;
     }
   }
-  if (!cuda_ok(c, upload_spans(c, spans, count, fd))) {
-    release(count);
+  const cudaError_t copied = upload_spans(c, spans, count, fd);
+  if (!cuda_ok(c, copied)) {
+    // copies that may still be under way keep their memory until emelb_destroy
+    if (copied == cudaErrorTimeout)
+      for (size_t i = 0; i < count; ++i) c->owned.insert(spans[i].dev);
+    else release(count);
     return EMELB_INTERNAL_ERROR;
   }
   for (size_t i = 0; i < count; ++i) {

@@ -52,6 +52,7 @@ struct UploadSpan {
 // staging ring in one pipeline over all of them; fd >= 0 names the file the spans map (read by pread).
 cudaError_t upload_spans(emelb_ctx* c, const UploadSpan* spans, size_t count, int fd);
 void upload_ring_release(emelb_ctx* c);
+void upload_unlock(emelb_ctx* c);  // behind the stream's end
 // emelb_residency_upload for several tensors at once: all or nothing
 uint32_t residency_upload_many(emelb_ctx* c, UploadSpan* spans, size_t count, int fd);
 }  // namespace emelb
@@ -116,6 +117,8 @@ struct emelb_ctx {
   std::vector<emelb::UploadLane> upload_lanes;  // created by the first large residency upload
   int upload_route = 0;    // EMELB_UPLOAD_RING / _PLAIN / _REGISTER (emelb_set_upload_route)
   int upload_threads = 0;  // 0: one per host core, at most 16
+  std::vector<void*> upload_locked;  // spans that an upload whose wait ran out left page-locked, until the stream is idle
+  uint32_t upload_wait_ms = 120000;  // of one wait for the device (emelb_set_upload_wait_ms)
   // row-shard exchange (comm.cu): one communicator per context, one rank per GPU
   void* comm = nullptr;  // ncclComm_t
   int comm_rank = 0;

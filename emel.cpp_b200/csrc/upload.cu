@@ -11,12 +11,14 @@
 //     is filled by pread() when the caller names the file the span maps (the
 //     kernel copies out of the page cache without touching this process's page
 //     tables), else by memcpy from the span (one page fault per fresh page).
-// Bytes arrive unchanged; the call returns when the whole span is in HBM.
+// Bytes arrive unchanged; the call returns when the whole span is in HBM.  Waits for the device end after the context's limit
+// with cudaErrorTimeout (what the driver does inside of a call, page-locking or a copy of pageable memory, has none).
 #include <unistd.h>
 
 #include <algorithm>
 #include <atomic>
 #include <cerrno>
+#include <chrono>
 #include <cstdlib>
 #include <cstring>
 #include <thread>
@@ -47,8 +49,28 @@ bool page_locked(const void* p) {
   return a.type == cudaMemoryTypeHost;
 }
 
-// the read-only in-place route; false = not available here, nothing was copied
-bool upload_registered(emelb_ctx* c, void* dev, const void* host, uint64_t bytes) {
+// the end of what a stream or an event stands for, by asking again and again
+template <class Query>
+cudaError_t wait_until(const emelb_ctx* c, Query&& query) {
+  const auto start = std::chrono::steady_clock::now();
+  for (int turn = 0;; ++turn) {
+    const cudaError_t e = query();
+    if (e != cudaErrorNotReady) return e;
+    if (turn < 256) {
+      std::this_thread::yield();
+      continue;
+    }
+    if (std::chrono::steady_clock::now() - start > std::chrono::milliseconds(c->upload_wait_ms)) return cudaErrorTimeout;
+    std::this_thread::sleep_for(std::chrono::microseconds(20));
+  }
+}
+cudaError_t wait_stream(const emelb_ctx* c, cudaStream_t st) {
+  return wait_until(c, [&] { return cudaStreamQuery(st); });
+}
+
+// the read-only in-place route; false = not available here, nothing was copied.  `*timeout`: the copy may still be under way, so
+// the span stays page-locked
+bool upload_registered(emelb_ctx* c, void* dev, const void* host, uint64_t bytes, bool* timeout) {
   if (bytes < kDirectBelow) return false;
   const uintptr_t page = uintptr_t(sysconf(_SC_PAGESIZE));
   const uintptr_t lo = uintptr_t(host) & ~(page - 1);
@@ -58,7 +80,12 @@ bool upload_registered(emelb_ctx* c, void* dev, const void* host, uint64_t bytes
     return false;
   }
   cudaError_t e = cudaMemcpyAsync(dev, host, bytes, cudaMemcpyHostToDevice, c->stream);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
+  if (e == cudaSuccess) e = wait_stream(c, c->stream);
+  if (e == cudaErrorTimeout) {
+    *timeout = true;
+    c->upload_locked.push_back(reinterpret_cast<void*>(lo));
+    return false;
+  }
   cudaHostUnregister(reinterpret_cast<void*>(lo));
   if (e != cudaSuccess) c->last_cuda_error = int(e);
   return e == cudaSuccess;
@@ -94,8 +121,15 @@ void upload_ring_release(emelb_ctx* c) {
   c->upload_lanes.clear();
 }
 
+void upload_unlock(emelb_ctx* c) {
+  for (void* p : c->upload_locked) cudaHostUnregister(p);
+  c->upload_locked.clear();
+  cudaGetLastError();
+}
+
 cudaError_t upload_spans(emelb_ctx* c, const UploadSpan* spans, size_t count, int fd) {
   const bool want_register = c->upload_route == EMELB_UPLOAD_REGISTER;
+  if (!c->upload_locked.empty() && cudaStreamQuery(c->stream) == cudaSuccess) upload_unlock(c);
   const bool want_plain = c->upload_route == EMELB_UPLOAD_PLAIN;
   // spans that go in one copy; the rest is cut into chunks for the lanes
   struct Chunk {
@@ -108,10 +142,12 @@ cudaError_t upload_spans(emelb_ctx* c, const UploadSpan* spans, size_t count, in
     const UploadSpan& sp = spans[i];
     if (sp.bytes == 0) continue;
     const bool direct = want_plain || page_locked(sp.host) || (sp.bytes < kDirectBelow && count == 1);
-    if (want_register && upload_registered(c, sp.dev, sp.host, sp.bytes)) continue;
+    bool timeout = false;
+    if (want_register && upload_registered(c, sp.dev, sp.host, sp.bytes, &timeout)) continue;
+    if (timeout) return cudaErrorTimeout;
     if (direct) {
       cudaError_t e = cudaMemcpyAsync(sp.dev, sp.host, sp.bytes, cudaMemcpyHostToDevice, c->stream);
-      if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
+      if (e == cudaSuccess) e = wait_stream(c, c->stream);
       if (e != cudaSuccess) return e;
       continue;
     }
@@ -145,7 +181,7 @@ cudaError_t upload_spans(emelb_ctx* c, const UploadSpan* spans, size_t count, in
     // chunk i belongs to lane i % threads: neighbouring chunks are read concurrently
     for (size_t i = size_t(t); i < chunks.size() && e == cudaSuccess; i += size_t(threads), turn ^= 1) {
       const Chunk& ch = chunks[i];
-      e = cudaEventSynchronize(lane.drained[turn]);  // the DMA that last read this buffer (done at once the first time)
+      e = wait_until(c, [&] { return cudaEventQuery(lane.drained[turn]); });  // the DMA that last read this buffer (done at once the first time)
       if (e != cudaSuccess) break;
       if (!fill(lane.pinned[turn], ch)) {
         e = cudaErrorUnknown;  // the file ended or failed under the mapping
@@ -154,11 +190,11 @@ cudaError_t upload_spans(emelb_ctx* c, const UploadSpan* spans, size_t count, in
       e = cudaMemcpyAsync(ch.dev, lane.pinned[turn], ch.bytes, cudaMemcpyHostToDevice, lane.stream);
       if (e == cudaSuccess) e = cudaEventRecord(lane.drained[turn], lane.stream);
     }
-    const cudaError_t done = cudaStreamSynchronize(lane.stream);
-    if (e == cudaSuccess) e = done;
+    const cudaError_t done = e == cudaErrorTimeout ? e : wait_stream(c, lane.stream);
+    if (e == cudaSuccess || done == cudaErrorTimeout) e = done;
     if (e != cudaSuccess) {
       int expected = int(cudaSuccess);
-      first_error.compare_exchange_strong(expected, int(e));
+      if (!first_error.compare_exchange_strong(expected, int(e)) && e == cudaErrorTimeout) first_error.store(int(e));   // above others
     }
   };
   std::vector<std::thread> workers;

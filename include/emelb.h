@@ -172,6 +172,10 @@ EMELB_API uint32_t emelb_residency_evict(emelb_ctx* ctx, int32_t tensor_id);
  * without a host copy. */
 enum { EMELB_UPLOAD_RING = 0, EMELB_UPLOAD_PLAIN = 1, EMELB_UPLOAD_REGISTER = 2 };
 EMELB_API uint32_t emelb_set_upload_route(emelb_ctx* ctx, int32_t route, int32_t threads);
+/* how long an upload waits for the device each time it has to (default two
+ * minutes).  One that runs out is EMELB_INTERNAL_ERROR: nothing is resident, and
+ * the host span has to stay until the context's stream is idle. */
+EMELB_API uint32_t emelb_set_upload_wait_ms(emelb_ctx* ctx, uint32_t limit_ms);
 
 EMELB_API uint32_t emelb_residency_state(const emelb_ctx* ctx, int32_t tensor_id,
                                emelb_tensor_state* out);
