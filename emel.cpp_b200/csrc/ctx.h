@@ -53,6 +53,9 @@ struct UploadSpan {
 cudaError_t upload_spans(emelb_ctx* c, const UploadSpan* spans, size_t count, int fd);
 void upload_ring_release(emelb_ctx* c);
 void upload_unlock(emelb_ctx* c);  // behind the stream's end
+// whether any of [lo, hi) maps a file.  Such memory is not page-locked in place: pinning pages of a file just written has kept a call in
+// the kernel for good
+bool maps_file(uintptr_t lo, uintptr_t hi);
 // emelb_residency_upload for several tensors at once: all or nothing
 uint32_t residency_upload_many(emelb_ctx* c, UploadSpan* spans, size_t count, int fd);
 }  // namespace emelb

@@ -3,8 +3,8 @@
 // A weight span usually lies in a file mapping (page cache), which the copy
 // engines cannot read directly.  Three routes, picked per call:
 //   * spans that are already page-locked, and small spans: one cudaMemcpyAsync;
-//   * EMELB_UPLOAD_MODE=register: page-lock the span read-only in place, one DMA
-//     straight from the page cache, unlock (no intermediate copy at all);
+//   * EMELB_UPLOAD_REGISTER: page-lock the span read-only in place, one DMA, unlock
+//     (no intermediate copy at all); not for spans that map a file, see maps_file;
 //   * default: several threads each walk their share of the span in 4 MB chunks
 //     through two page-locked buffers of their own -- filling one chunk overlaps
 //     the DMA of the previous one, and the threads overlap each other.  A chunk
@@ -19,6 +19,7 @@
 #include <atomic>
 #include <cerrno>
 #include <chrono>
+#include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <thread>
@@ -75,6 +76,7 @@ bool upload_registered(emelb_ctx* c, void* dev, const void* host, uint64_t bytes
   const uintptr_t page = uintptr_t(sysconf(_SC_PAGESIZE));
   const uintptr_t lo = uintptr_t(host) & ~(page - 1);
   const uintptr_t hi = (uintptr_t(host) + bytes + page - 1) & ~(page - 1);
+  if (maps_file(lo, hi)) return false;
   if (cudaHostRegister(reinterpret_cast<void*>(lo), hi - lo, cudaHostRegisterReadOnly) != cudaSuccess) {
     cudaGetLastError();
     return false;
@@ -119,6 +121,21 @@ void upload_ring_release(emelb_ctx* c) {
     if (lane.stream) cudaStreamDestroy(lane.stream);
   }
   c->upload_lanes.clear();
+}
+
+bool maps_file(uintptr_t lo, uintptr_t hi) {
+  std::FILE* f = std::fopen("/proc/self/maps", "re");
+  if (!f) return true;
+  bool found = false;
+  char line[512];
+  bool head = true;   // of a line: names may be longer than the buffer
+  while (!found && std::fgets(line, sizeof(line), f)) {
+    unsigned long long from = 0, to = 0, inode = 0;
+    if (head && std::sscanf(line, "%llx-%llx %*s %*s %*s %llu", &from, &to, &inode) == 3) found = inode != 0 && from < hi && lo < to;
+    head = std::strchr(line, '\n') != nullptr;
+  }
+  std::fclose(f);
+  return found;
 }
 
 void upload_unlock(emelb_ctx* c) {

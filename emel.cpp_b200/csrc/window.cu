@@ -3,7 +3,7 @@
 // The plan arithmetic, the order of the bind decisions and the ring rules restate the reference's
 // model::tensor::window (src/emel/model/tensor/window/detail.hpp:128-183, guards.hpp:13-186 and 296-470,
 // actions.hpp:218-227 and 394-406).  A slot load is a device matter:
-//   * source page-locked (tried at bind): a load is one asynchronous copy per extent on the window's own stream.
+//   * source page-locked (tried at bind, but for mapped files): a load is one asynchronous copy per extent on the window's own stream.
 //     The copy waits for the event that marks the end of the slot's previous readers on the compute stream, and the
 //     compute stream waits for the event behind the copy: the host thread never blocks;
 //   * otherwise one I/O thread stages each extent in chunks through two page-locked buffers; an acquire of a layer that
@@ -165,10 +165,11 @@ bool lock_source(emelb_window* w) {
   const uintptr_t page = uintptr_t(sysconf(_SC_PAGESIZE));
   const uintptr_t a = (uintptr_t(w->source) + lo) & ~(page - 1);
   const uintptr_t b = (uintptr_t(w->source) + hi + page - 1) & ~(page - 1);
+  if (emelb::maps_file(a, b)) return false;
   // read-only first (the only form a PROT_READ mapping takes), then the plain form for ordinary memory
   if (cudaHostRegister(reinterpret_cast<void*>(a), b - a, cudaHostRegisterReadOnly) != cudaSuccess) {
     cudaGetLastError();
-    if (w->mapped_here || cudaHostRegister(reinterpret_cast<void*>(a), b - a, cudaHostRegisterDefault) != cudaSuccess) {
+    if (cudaHostRegister(reinterpret_cast<void*>(a), b - a, cudaHostRegisterDefault) != cudaSuccess) {
       cudaGetLastError();
       return false;
     }

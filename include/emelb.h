@@ -169,7 +169,8 @@ EMELB_API uint32_t emelb_residency_evict(emelb_ctx* ctx, int32_t tensor_id);
  * page-locked staging ring fed by `threads` host threads (0 = one per core, at
  * most 16; pread-fed when the span maps a file).  PLAIN: one pageable copy per
  * span.  REGISTER: the span is page-locked in place (read-only) and copied
- * without a host copy. */
+ * without a host copy; one that maps a file goes through the ring, since page-locking
+ * a mapped file can keep the call in the kernel for good. */
 enum { EMELB_UPLOAD_RING = 0, EMELB_UPLOAD_PLAIN = 1, EMELB_UPLOAD_REGISTER = 2 };
 EMELB_API uint32_t emelb_set_upload_route(emelb_ctx* ctx, int32_t route, int32_t threads);
 /* how long an upload waits for the device each time it has to (default two
