@@ -23,9 +23,9 @@
 // a pair of tiles about 5,000 besides (first scores, last mix, results).
 //
 // us, two prompts of 4100 and 8190 tokens / 13 of 17 to 600, 32 heads of 128: 756 with weights handed over at once and an arrival a
-// thread; 659 / 95 by halves and with registers split; 578 / 61 with queries by asynchronous copies; 544 (1,263 TFLOP/s) / 52 since
-// CTAs stay (640 when repeated for seconds: the chip is at 990 W then, at 1.58 GHz).  One prompt of 8192 and heads of 64: 394 (698
-// TFLOP/s; its exponentials alone take 252).
+// thread; 659 / 95 by halves and with registers split; 578 / 61 with queries by asynchronous copies; 544 / 52 since CTAs stay.
+// Repeated for seconds, at 990 W and 1.58 GHz, the long ones took 640 then; 655 (1,050 TFLOP/s) / 53 since sums keep their digits and far
+// scores are looked for.  One prompt of 8192 and heads of 64: 393 (699 TFLOP/s; its exponentials alone take 252).
 //
 // Measured and left out: an issuer of products for each row tile 613 / - (they fall into step and wait for the same pipes); scores
 // of 64 keys in two buffers a row tile, so that none waits for a mix, 588 (products with 64 columns take longer); weights against a

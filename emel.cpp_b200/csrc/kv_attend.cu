@@ -1,7 +1,7 @@
 // Attention of a few query rows a request over the pages of the 4-bit key / value cache.
 //
-// The cache is read once: 18 bytes for 32 values, so HBM bounds it, with about 25 instructions of a warp to each token of a head
-// at that rate.  What keeps it near them: the cache is the A operand of mma.sync.m16n8k16 (16 tokens, or 16 dims, a side), the query
+// The cache is read once: 18 bytes for 32 values, so HBM bounds it: at its rate the SMs could issue about 25 instructions of a
+// warp to each token of a head, and take 19.  What keeps them that few: the cache is the A operand of mma.sync.m16n8k16 (16 tokens, or 16 dims, a side), the query
 // rows of a group of heads the other (8 of them, none of a tile wasted on a group of 8), so tokens and not heads fill the
 // tiles; quants become f16 by one lop3 a pair, as a power of two + q, and what that is above q - 8 leaves the scores through the
 // tensor cores too (one tf32 product a tile), the values by an addition, since sums over tokens would not survive it; a key's scale
@@ -19,9 +19,10 @@
 //
 // 64 requests of 1000 to 8000 tokens, 64 heads on 8 of 128: 139 us with steps of 16 tokens, 131 with 32 (one maximum, one exchange
 // for both), 116 with asynchronous copies in place of bulk ones (no barrier to wait at), 94 since a team takes whole pairs where
-// that costs no more, 90 with joins in the order of the fragments, 85 (3.9 TB/s) with a kernel for each type.  What bounds it is issue:
+// that costs no more, 90 with joins in the order of the fragments, 86.5 with a kernel for each type, 89 (3.75 TB/s) since results move to
+// shared memory, far scores are rounded and rows have powers of two of their own.  What bounds it is issue:
 // about 300 instructions to 16 tokens of a head, two of the four that an SM could issue a cycle.  One document of 100,001 tokens and 16
-// rows reads as two tiles of rows, each unpacked for itself: 68 us, 78 with both in one warp (registers).  12 warps with 168 registers do better than 16 with
+// rows reads as two tiles of rows, each unpacked for itself: 69 us; both in one warp (registers) 78 for 68 then.  12 warps with 168 registers do better than 16 with
 // 128 (105 us).  Small calls are a chain: the line from the lengths, the first tiles from memory, the joins.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -43,8 +44,10 @@ constexpr unsigned kAll = 0xffffffffu;
 constexpr float kLowest = -3.0e38f;   // running maximum before the first token: finite, below every score
 constexpr float kSlack = 3.0f;        // a score may pass the running maximum by this (log2) before sums are rescaled
 constexpr float kFarScore = 0x1p20f;  // from here on an f32 score's own rounding may be more than that
-constexpr int kJoinSteps = 5;         // what joining the parts of units costs, in steps of a warp
-constexpr int kMostParts = 6;             // parts of a (head, row tile) up to which a team may be smaller
+constexpr int kJoinSteps = 5;         // what joining the parts of units costs, in steps of a warp: with 0, 16 requests
+                                      // of 120 to 600 tokens take 24 us for 11, with 20 as long
+constexpr int kMostParts = 6;         // parts of a (head, row tile) up to which a team may be smaller: with 3 the 64 requests above
+                                      // take 92 us for 89, with 12 as long
 constexpr int kEach = 4;              // requests a lane in the search that a warp makes alone
 constexpr int kStep = 32;             // tokens a warp takes at a time: two tiles
 constexpr int kFold = 64;             // steps of a warp between two moves of its results: 128 products, 2^-16 of them
