@@ -54,6 +54,9 @@ constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(8 * kSoftmaxRegs + 4 * kOtherRegs <= 12 * 168, "registers");
 constexpr float kLowest = -3.0e38f;
 constexpr float kSlack = 8.0f;
+// f16 weights are taken times 2^7, so that with the slack they reach 2^15 and keep 11 bits down to 2^-21 of the largest; bf16 has range
+template <bool kBf16>
+constexpr float kRaise = kBf16 ? 0.0f : 7.0f;
 constexpr float kFarScore = 0x1p20f;  // from here on an f32 score's own rounding may be more than that
 constexpr int kFold = 64;             // key tiles between two moves of O out of TMEM: 512 products, 2^-14 of O
 constexpr int kTmemCols = 512;
@@ -689,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const tc::f2 minus_m = tc::pack2(-m, -m);
+        const tc::f2 minus_m = tc::pack2(kRaise<kBf16> - m, kRaise<kBf16> - m);
         tc::f2 tile2 = tc::pack2(0.0f, 0.0f);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {

@@ -157,8 +157,8 @@ EMELB_API uint32_t emelb_kv_attend(emelb_ctx* ctx, const emelb_kv_attend_request
  * rows that see it in its head and dim alone.  max_queries bounds the rows of a request (more of them are an error that
  * emelb_sync reports, and are not computed).
  * type EMELB_F16 or EMELB_BF16 of all four tensors; head_dim a multiple of 8 up to 128; heads / kv_heads at most 128; keys at most 2^25; every
- * row 16-byte aligned (base, strides), strides of q, k and v below 2^39, else EMELB_UNSUPPORTED_OP.  Scores, statistics and sums are f32, softmax weights are
- * rounded to `type` for the second product. */
+ * row 16-byte aligned (base, strides), strides of q, k and v below 2^39, else EMELB_UNSUPPORTED_OP.  Scores, statistics and sums
+ * are f32, softmax weights are rounded to `type` for the second product (f16 ones with fewer bits below 2^-21 of a row's largest). */
 typedef struct emelb_attend_packed_request {
   const void* q;          /* [queries][heads][head_dim] by strides */
   const void* k;          /* [keys][kv_heads][head_dim] */

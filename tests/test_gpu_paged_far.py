@@ -395,3 +395,25 @@ def test_attend_far_scores_alike(be, t, gain):
     want, _ = exact(q, k, v, scale, False)
     rounding = {"f32": 2.0 ** -22, "f16": 2.0 ** -11, "bf16": 2.0 ** -10}[t] + plain.HALF_STEP[t] + 2.0 ** -16 + 64 * 17 * 2.0 ** -23
     assert ((out.double() - want).abs() <= rounding * want.abs() + 1e-30).all()
+
+
+@pytest.mark.parametrize("t,keys,lift", [("f16", 1 << 20, 22.58), ("f16", 120001, 18.6), ("bf16", 1 << 20, 22.58), ("f16", 30000, 14.3)])
+def test_packed_many_small_weights(be, t, keys, lift):
+    """One key 2^lift above all the others, which together still count: the first by 1, in the sum, the others by keys * 2^-lift.  A weight
+    has a rounding to the type's bits, in f16 to a grid of 2^-31 of the largest at least (2^-24 over 2^7), for all of them the same."""
+    dim, dt = 64, plain.TORCH[t]
+    q, k = torch.zeros(2, 1, dim, device="cuda", dtype=dt), torch.zeros(keys, 1, dim, device="cuda", dtype=dt)
+    q[0, 0, 0], q[1, 0, 1] = 1, 1
+    k[700, 0, 0], k[keys - 3, 0, 1] = lift, lift
+    v = torch.empty(keys, 1, dim, device="cuda", dtype=dt).copy_(torch.linspace(-3, 2, dim, device="cuda").to(dt))
+    v[700], v[keys - 3] = -v[700], -v[keys - 3]
+    out, begin, scale = torch.zeros_like(q), [dev([0, 2]), dev([0, keys])], float(np.log(2))
+    torch.cuda.synchronize()
+    done(be, be.attend_packed(paged.packed_request(q, k, v, out, t, *begin, 1, 1, 1, dim, 2, keys, causal=False, scale=scale)))
+    want, _ = exact(q, k, v, scale, False)
+    size = v[0].double().abs()
+    up = float(k[700, 0, 0])
+    rest = (keys - 1) * 2.0 ** -up / (1 + (keys - 1) * 2.0 ** -up)
+    weight = plain.HALF_STEP[t] if t == "bf16" else max(2.0 ** -11, 2.0 ** (up - 32))
+    rel = plain.HALF_STEP[t] + weight * rest + 2.0 ** -18
+    assert ((out.double() - want).abs() <= rel * size + plain.HALF_STEP[t] * want.abs() + 256 * 17 * 2.0 ** -23 * rest * size).all()
