@@ -3,7 +3,7 @@
 // The plan arithmetic, the order of the bind decisions and the ring rules restate the reference's
 // model::tensor::window (src/emel/model/tensor/window/detail.hpp:128-183, guards.hpp:13-186 and 296-470,
 // actions.hpp:218-227 and 394-406).  A slot load is a device matter:
-//   * source page-locked (tried at bind, but for mapped files): a load is one asynchronous copy per extent on the window's own stream.
+//   * source page-locked, or its layers copied to page-locked memory where it maps a file (tried at bind): a load is one asynchronous copy per extent on the window's own stream.
 //     The copy waits for the event that marks the end of the slot's previous readers on the compute stream, and the
 //     compute stream waits for the event behind the copy: the host thread never blocks;
 //   * otherwise one I/O thread stages each extent in chunks through two page-locked buffers; an acquire of a layer that
@@ -14,7 +14,10 @@
 #include <sys/stat.h>
 #include <unistd.h>
 
+#include <algorithm>
+#include <atomic>
 #include <condition_variable>
+#include <cstdio>
 #include <cstring>
 #include <deque>
 #include <mutex>
@@ -56,6 +59,9 @@ struct emelb_window {
   bool mapped_here = false;      // the window mapped the file itself
   bool page_locked = false;      // the copy engines can read the source in place
   void* locked_base = nullptr;   // start of the range this window page-locked itself (null: none)
+  void* copy = nullptr;          // page-locked memory with a mapped file's layers (null: none)
+  uint64_t copy_bytes = 0;
+  const uint8_t* locked = nullptr;   // where the copy engines find the source's first byte (of the layers' bytes, no others need be there)
   bool staged_only = false;
   uint32_t prefetch_depth = 0;
   uint64_t chunk = EMELB_WINDOW_DEFAULT_CHUNK_BYTES;
@@ -143,17 +149,70 @@ bool map_source(emelb_window* w, const emelb_window_request& r) {
 
 void release_source(emelb_window* w) {
   if (w->locked_base) cudaHostUnregister(w->locked_base);
+  if (w->copy) {
+    cudaHostUnregister(w->copy);
+    ::munmap(w->copy, size_t(w->copy_bytes));
+  }
   if (w->mapped_here && w->source) ::munmap(const_cast<uint8_t*>(w->source), size_t(w->source_bytes));
   cudaGetLastError();
   w->page_locked = false;
   w->locked_base = nullptr;
+  w->copy = nullptr;
+  w->locked = nullptr;
   w->mapped_here = false;
   w->source = nullptr;
   w->source_bytes = 0;
 }
 
+// bytes that the host can give without taking them from others' memory; 0 where it does not say
+uint64_t host_room() {
+  std::FILE* f = std::fopen("/proc/meminfo", "re");
+  if (!f) return 0;
+  unsigned long long kb = 0;
+  char line[256];
+  while (std::fgets(line, sizeof(line), f))
+    if (std::sscanf(line, "MemAvailable: %llu", &kb) == 1) break;
+  std::fclose(f);
+  return kb * 1024;
+}
+
+// A mapped file's bytes lo .. hi - 1 to memory that is page-locked then, by several threads, which touch its pages first: the same memory as
+// the file's pages would take if they were locked where they are, while these can go.
+bool copy_source(emelb_window* w, uint64_t lo, uint64_t hi) {
+  const uint64_t bytes = hi - lo;
+  if (bytes + bytes / 8 + (1ull << 30) > host_room()) return false;
+  void* to = ::mmap(nullptr, size_t(bytes), PROT_READ | PROT_WRITE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0);
+  if (to == MAP_FAILED) return false;
+  ::madvise(to, size_t(bytes), MADV_HUGEPAGE);
+  constexpr uint64_t kPiece = 8ull << 20;
+  std::atomic<uint64_t> next{0};
+  auto body = [&] {
+    for (uint64_t at = next.fetch_add(kPiece); at < bytes; at = next.fetch_add(kPiece))
+      std::memcpy(static_cast<uint8_t*>(to) + at, w->source + lo + at, size_t(bytes - at < kPiece ? bytes - at : kPiece));
+  };
+  std::vector<std::thread> others;
+  const unsigned count = std::min(16u, std::max(1u, std::thread::hardware_concurrency()));
+  try {
+    for (unsigned i = 1; i < count && i * kPiece < bytes; ++i) others.emplace_back(body);
+  } catch (...) {
+    // no more threads to be had: those that there are share the work
+  }
+  body();
+  for (std::thread& t : others) t.join();
+  if (cudaHostRegister(to, bytes, cudaHostRegisterDefault) != cudaSuccess) {
+    cudaGetLastError();
+    ::munmap(to, size_t(bytes));
+    return false;
+  }
+  w->copy = to;
+  w->copy_bytes = bytes;
+  w->locked = reinterpret_cast<const uint8_t*>(uintptr_t(w->copy) - lo);
+  return true;
+}
+
 // page-lock the pages the extents lie in, read-only: the copy engines then read the source in place
 bool lock_source(emelb_window* w) {
+  w->locked = w->source;
   cudaPointerAttributes at{};
   if (cudaPointerGetAttributes(&at, w->source) == cudaSuccess && at.type == cudaMemoryTypeHost) return true;   // already is: nothing to undo
   cudaGetLastError();
@@ -165,7 +224,7 @@ bool lock_source(emelb_window* w) {
   const uintptr_t page = uintptr_t(sysconf(_SC_PAGESIZE));
   const uintptr_t a = (uintptr_t(w->source) + lo) & ~(page - 1);
   const uintptr_t b = (uintptr_t(w->source) + hi + page - 1) & ~(page - 1);
-  if (emelb::maps_file(a, b)) return false;
+  if (emelb::maps_file(a, b)) return copy_source(w, lo, hi);
   // read-only first (the only form a PROT_READ mapping takes), then the plain form for ordinary memory
   if (cudaHostRegister(reinterpret_cast<void*>(a), b - a, cudaHostRegisterReadOnly) != cudaSuccess) {
     cudaGetLastError();
@@ -256,7 +315,7 @@ void submit_load(emelb_window* w, int layer) {
   uint64_t copied = 0;
   for (uint32_t i = 0; ok && i < d.weight_count; ++i) {
     const emelb_window_extent& e = d.weights[i];
-    ok = cudaMemcpyAsync(slot.storage + e.slot_offset, w->source + e.file_offset, size_t(e.byte_size), cudaMemcpyHostToDevice,
+    ok = cudaMemcpyAsync(slot.storage + e.slot_offset, w->locked + e.file_offset, size_t(e.byte_size), cudaMemcpyHostToDevice,
                          w->copy_stream) == cudaSuccess;
     copied += e.byte_size;
   }

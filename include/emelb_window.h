@@ -14,10 +14,11 @@
  * layer, slot of layer l = l % window_slots), same decisions in the same order
  * and the same error bits (src/emel/model/tensor/window/errors.hpp:9-21).
  * What differs is what a slot load is:
- *   - the window first tries to page-lock the source read-only, unless it maps
- *     a file (page-locking that can keep the call in the kernel for good); loads
- *     are then asynchronous copies on a stream of the window, ordered against
- *     the compute stream by events only (the host never waits);
+ *   - the window first tries to page-lock the source read-only, or, where that maps
+ *     a file (page-locking that can keep the call in the kernel for good), to
+ *     copy the layers' part of it to page-locked memory, if the host has room for
+ *     it; loads are then asynchronous copies on a stream of the window, ordered
+ *     against the compute stream by events only (the host never waits);
  *   - where the source is not page-locked, one I/O thread copies chunk by
  *     chunk (stage_chunk_bytes) through two page-locked buffers, and an acquire
  *     of a layer whose load is still running waits for it on the host.

@@ -1,9 +1,10 @@
-"""Sources that map files: never page-locked in place, whatever route is asked for; other memory is."""
+"""Sources that map files: never page-locked in place, whatever route is asked for (a window copies them); other memory is."""
 import mmap
 import os
 
 import numpy as np
 import pytest
+import torch
 
 import emel_cpp_b200 as eb
 from emel_cpp_b200 import window as ew
@@ -26,14 +27,17 @@ def test_a_window_page_locks_memory_but_not_files(be, how, tmp_path):
     image.tofile(path)
     source = path if how == "path" else image
     if how == "memmap":
-        source = np.memmap(path, dtype=np.uint8, mode="r")
+        source = np.memmap(path, dtype=np.uint8, mode="c")
     elif how == "anonymous":
         source = np.frombuffer(mmap.mmap(-1, image.nbytes, flags=mmap.MAP_PRIVATE | mmap.MAP_ANONYMOUS), dtype=np.uint8)
         source[:] = image
     win = ew.LayerWindow(be)
     try:
         assert win.bind(source, layers, STREAMING_BUDGET, 4, 2), win.last_error
-        assert win.bound["source_page_locked"] == (how in ("anonymous", "array"))
+        assert win.bound["source_page_locked"]
+        if how != "path":
+            first = np.asarray(source)[layers[0][0][1]:]          # the header in front of the layers stays as it is
+            assert torch.frombuffer(first, dtype=torch.uint8).is_pinned() == (how != "memmap")
         for l in range(LAYERS):
             got = win.acquire(l)
             assert got is not None and slot_content_matches(be, got, l)
