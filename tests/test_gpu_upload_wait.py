@@ -24,7 +24,7 @@ def test_upload_behind_a_busy_stream_ends_at_the_limit(route, pinned):
         t0 = time.perf_counter()
         with pytest.raises(eb.BackendError):
             be.upload(2, host.numpy(), tensor_type=24)
-        assert time.perf_counter() - t0 < 0.5 and be.last_error == eb.INTERNAL_ERROR
+        assert time.perf_counter() - t0 < 2.0 and be.last_error == eb.INTERNAL_ERROR
         assert eb.LIFECYCLE[be.state(2).lifecycle_state] != "resident"
         assert be.sync()
         assert be.set_upload_wait_ms(60000)
